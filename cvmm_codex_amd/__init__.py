@@ -5,14 +5,18 @@ projections -- as hand-written HIP kernels behind the reference's Python API.
 """
 from .api import (  # noqa: F401
     CVMM,
+    CVMMMx4,
     CVMMSel,
     create_kernels,
     cvmm,
     cvmm_expert_offsets,
     cvmm_gate_logits,
     cvmm_gelu,
+    cvmm_mx4,
+    cvmm_mx4_quantize,
     cvmm_prepare_sel,
     cvmm_prepare_sel2,
+    cvmm_route_scored,
     cvmm_route_topk,
     cvmm_triton_call,
     dtype_to_type_id,

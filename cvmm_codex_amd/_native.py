@@ -24,6 +24,7 @@ FLAG_ROWS_SCALED = 64
 # host-only flag of the extension's backward (never passed to the C ABI):
 # the weight gradient on a second stream, concurrent with the grad-input
 HOST_OVERLAP_BACKWARD = 1 << 48
+SCORES = {"softmax": 0, "sigmoid": 1}
 CAST_T_INTERLEAVED = 1
 CAST_N_INTERLEAVED = 2
 TUNE_PANEL_TILES_PER_WG = 1
@@ -72,6 +73,10 @@ _SIGS = {
     "cvmm_route_topk": (ctypes.c_int, [_P, _I32, _I64, _I64, _I32, _I64, _I32, _P, _P,
                                        _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "cvmm_route_topk_backward": (ctypes.c_int, [_P, _I32, _I64, _I64, _I32, _I64, _I32, _P, _P, _P, _I64, _P]),
+    "cvmm_route_scored": (ctypes.c_int, [_P, _I32, _I64, _I64, _I32, _I64, _P, _I32, _I32, _I32, _I32,
+                                         ctypes.c_double, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "cvmm_route_scored_backward": (ctypes.c_int, [_P, _I32, _I64, _I64, _I32, _I64, _I32, _I32, ctypes.c_double,
+                                                  _P, _P, _P, _I64, _P]),
     "cvmm_fwd_workspace_bytes": (_SZ, [_I64, _I32, _I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32]),
     "cvmm_fwd": (ctypes.c_int, [
         _P, _I32, _I64, _I64,                 # x, dtype, rows, ld
@@ -131,6 +136,29 @@ _SIGS = {
         _P, _I32, _I64, _I32,                 # rw, rw dtype, top_k, op
         _P, _I32, _I64, _I64, _I64,           # grad_keys, dtype, strides
         _I32, _P, _SZ, _P, _SZ, _P]),         # flags, rows, workspace, stream
+    "cvmm_mx4_rows_bytes": (_SZ, [_I64, _I64, _I32]),
+    "cvmm_mx4_keys_bytes": (_SZ, [_I64, _I64, _I64, _I32]),
+    "cvmm_mx4_quantize_rows": (ctypes.c_int, [_P, _I32, _I64, _I64, _I64, _P, _P, _P]),
+    "cvmm_mx4_quantize_keys": (ctypes.c_int, [_P, _I32, _I32, _I64, _I64, _I64, _I64, _I64, _P, _P, _P]),
+    "cvmm_mx4_dequantize_rows": (ctypes.c_int, [_P, _P, _I64, _I64, _P, _I32, _P]),
+    "cvmm_mx4_dequantize_keys": (ctypes.c_int, [_P, _P, _I32, _I64, _I64, _P, _I32, _P]),
+    "cvmm_mx4_fwd_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I32, _I32, _I32, _I32]),
+    "cvmm_mx4_fwd": (ctypes.c_int, [
+        _P, _I32, _I64, _I64,                 # x, dtype, rows, ld
+        _P, _P, _I32, _I64, _I64,             # codes, scales, E, d_in, d_out
+        _P, _P, _I64, _P, _P,                 # sel_index, out_index, R, offsets, route_pos
+        _P, _I64, _I32,                       # rw (fp32), reduce_k, quantize_input
+        _P, _I64, _I64,                       # out, out rows, out ld
+        _P, _SZ, _P]),                        # ws, ws bytes, stream
+    "cvmm_mx4_bwd_x_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I32, _I32, _I32, _I32, _I32]),
+    "cvmm_mx4_bwd_x": (ctypes.c_int, [
+        _P, _I32, _I64, _I64,                 # grad, op dtype, rows, ld
+        _P, _P, _I32, _I64, _I64,             # codes, scales, E, d_in, d_out
+        _P, _P, _I64, _P, _P,                 # sel_index, out_index, R, offsets, route_pos
+        _P, _I64,                             # rw (fp32), top_k
+        _P, _I32, _I64, _I64,                 # x, dtype, rows, ld
+        _P, _I32, _I64, _I64,                 # grad_x, dtype, rows, ld
+        _P, _P, _SZ, _P]),                    # grad_rw, ws, ws bytes, stream
 }
 
 EXPORTED = tuple(_SIGS)

@@ -48,7 +48,7 @@ def _compiling() -> bool:
 __all__ = [
     "CVMMSel", "cvmm_prepare_sel", "cvmm_prepare_sel2", "cvmm", "CVMM", "get_dtype",
     "dtype_to_type_id", "create_kernels", "cvmm_expert_offsets", "cvmm_triton_call", "cvmm_route_topk",
-    "cvmm_gelu",
+    "cvmm_gelu", "cvmm_route_scored", "CVMMMx4", "cvmm_mx4_quantize", "cvmm_mx4",
 ]
 
 
@@ -632,6 +632,75 @@ def cvmm_route_topk(logits: torch.Tensor, k: int, renormalize: bool = True):
     return w.view(*lead, k), sel, CVMMSel._deferred(sel, routing, False, None)
 
 
+class _RouteScored(torch.autograd.Function):
+    """Eager path of cvmm_route_scored: as _RouteTopK.  The bias enters the
+    choice alone and has no gradient."""
+
+    @staticmethod
+    def forward(ctx, logits, top_k, bias, scores, groups, topk_groups, renormalize, scale):
+        w, sel, ssel, perm, tok, offsets, route_pos = N.host().route_scored(
+            logits, top_k, bias, scores, groups, topk_groups, renormalize, scale, N.stream_of(logits.device))
+        ctx.save_for_backward(logits, sel)
+        ctx.args = (top_k, scores, renormalize, scale)
+        ctx.mark_non_differentiable(sel, ssel, perm, tok, offsets, route_pos)
+        ctx.set_materialize_grads(False)
+        return w, sel, ssel, perm, tok, offsets, route_pos
+
+    @staticmethod
+    def backward(ctx, grad_w, *_):
+        if grad_w is None:
+            return (None,) * 8
+        logits, sel = ctx.saved_tensors
+        g = N.host().route_scored_backward(logits, sel, grad_w.contiguous(), *ctx.args, N.stream_of(logits.device))
+        return (g,) + (None,) * 7
+
+
+def cvmm_route_scored(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None, scores: str = "softmax",
+                      groups: int = 1, topk_groups: Optional[int] = None, renormalize: bool = True,
+                      scale: float = 1.0):
+    """The router of balanced MoE models, with the selection sorted for
+    ``cvmm`` / ``cvmm_mx4`` in the same call:
+
+        s = torch.sigmoid(logits)  or  torch.softmax(logits, -1)      # scores
+        c = s + bias                                                   # the choice alone
+        # the experts stand in `groups` runs; the topk_groups with the greatest
+        # sum of their two best c stay
+        sel = the k best c of the experts that stay (ties to the lower id, NaN lowest)
+        weights = s[sel];  weights = scale * weights / weights.sum(-1)    # renormalize
+
+    Scores, sums and comparisons are 64-bit.  Returns ``(weights, sel,
+    sel_up)`` as ``cvmm_route_topk``: fp32 weights ``[..., k]`` (gradient flows
+    to ``logits``, not to ``bias``), int64 ids ``[..., k]`` by falling c and the
+    sorted token-input selector.  At most 1024 experts, k <= 64 and, where some
+    groups are left out (``topk_groups < groups``), 64 groups."""
+    _require_device(logits, "logits")
+    if scores not in N.SCORES:
+        raise ValueError(f"cvmm_route_scored: scores must be 'softmax' or 'sigmoid', not {scores!r}")
+    if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        logits = logits.float()
+    E = logits.shape[-1]
+    kept = groups if topk_groups is None else topk_groups
+    if groups <= 0 or E % groups:
+        raise ValueError(f"cvmm_route_scored: {E} experts do not split into {groups} groups")
+    if not (0 < kept <= groups):
+        raise ValueError(f"cvmm_route_scored: topk_groups={kept} outside 1..{groups}")
+    if not (0 < k <= kept * (E // groups)):
+        raise ValueError(f"cvmm_route_scored: k={k} outside 1..{kept * (E // groups)}")
+    lead = logits.shape[:-1]
+    args = (logits, k, None if bias is None else bias.detach(), N.SCORES[scores], groups, kept, bool(renormalize),
+            float(scale))
+    if _compiling():
+        w, sel, ssel, perm, tok, offsets, route_pos = _ops.route_scored(*args)
+    else:
+        w, sel, ssel, perm, tok, offsets, route_pos = _apply(_RouteScored, *args)
+        perm._cvmm_route_pos = route_pos
+    sel = sel.view(*lead, k)
+    routing = _Routing(sel.reshape(-1), k)
+    routing.by_e[E] = (ssel, perm, tok, offsets)
+    routing.first_e = E
+    return w.view(*lead, k), sel, CVMMSel._deferred(sel, routing, False, None)
+
+
 def _gate_grad_chunks(n_tokens: int, d_in: int, n_experts: int) -> int:
     """Token chunks of the gate gradient's product: enough [E x D] output
     tiles to fill the GPU (a single [D x T] @ [T x E] product has D*E/8192
@@ -982,3 +1051,117 @@ def _cvmm_eager(x: torch.Tensor, sel: Union[torch.Tensor, CVMMSel], keys: torch.
 
 
 _DTYPE_IDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+# ----------------------------------------------------------------------------
+# microscaled 4-bit weights
+# ----------------------------------------------------------------------------
+
+@dataclass
+class CVMMMx4:
+    """A tensor in microscaled 4-bit values (cvmm_mx4_quantize): blocks of 32
+    along ``dim`` share a power of two, the values stand on the grid +-{0, .5, 1,
+    1.5, 2, 3, 4, 6} times it.  ``codes`` and ``scales`` are uint8 buffers in the
+    layout the kernels read: rows (``dim`` the last) or expert weights (``dim`` 1
+    of ``[E, d_in, d_out]``)."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    shape: torch.Size
+    dim: int
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+    def to(self, device) -> "CVMMMx4":
+        return CVMMMx4(self.codes.to(device), self.scales.to(device), self.shape, self.dim)
+
+    def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
+        """The values, contiguous, in ``dtype`` (exact in fp32 and bf16; fp16
+        rounds below 2^-14 and overflows from 65520 on)."""
+        _require_device(self.codes, "codes")
+        if _compiling():
+            return _ops.mx4_dequantize(self.codes, self.scales, list(self.shape), self._keys, dtype)
+        return N.host().mx4_dequantize(self.codes, self.scales, list(self.shape), self._keys, N.dtype_id(dtype),
+                                       N.stream_of(self.codes.device))
+
+    @property
+    def _keys(self) -> bool:
+        return self.dim != len(self.shape) - 1
+
+
+def cvmm_mx4_quantize(t: torch.Tensor, dim: int = -1) -> CVMMMx4:
+    """``t`` in microscaled 4-bit values, blocks of 32 along ``dim``: the last
+    dimension (activations), or dimension 1 of expert weights ``[E, d_in, d_out]``
+    (their contraction, as ``cvmm_mx4`` reads them).  A block's scale is 2^s, s =
+    floor(log2 max|v|) - 2; each value becomes the nearest of the grid, ties to
+    the even code, the largest where it lies beyond.  A block with a NaN or an
+    infinity comes back as NaN.  No gradient."""
+    _require_device(t, "t")
+    if not t.is_floating_point():
+        raise TypeError(f"cvmm_mx4_quantize: {t.dtype} is no floating-point type")
+    if not (-t.dim() <= dim < t.dim()):
+        raise ValueError(f"cvmm_mx4_quantize: dim {dim} outside a tensor of {t.dim()} dimensions")
+    d = dim % t.dim()
+    last = d == t.dim() - 1
+    if not last and not (t.dim() == 3 and d == 1):
+        raise ValueError("cvmm_mx4_quantize: dim must be the last, or 1 of [E, d_in, d_out]")
+    if t.shape[d] == 0 or (not last and t.numel() == 0):
+        raise ValueError(f"cvmm_mx4_quantize: no values along dim {dim} of {tuple(t.shape)}")
+    t = t.detach()
+    if _compiling():
+        codes, scales = _ops.mx4_quantize(t, not last)
+    elif last:
+        codes, scales = N.host().mx4_quantize_rows(t, N.stream_of_tensor(t))
+    else:
+        codes, scales = N.host().mx4_quantize_keys(t, N.stream_of_tensor(t))
+    return CVMMMx4(codes, scales, t.shape, d)
+
+
+def cvmm_mx4(x: torch.Tensor, sel: Union[torch.Tensor, CVMMSel], keys: CVMMMx4,
+             quantize_input: bool = False) -> torch.Tensor:
+    """``cvmm`` with expert weights in 4 bits (``cvmm_mx4_quantize(keys, dim=1)``),
+    frozen: gradients flow to ``x`` and to the selection's routing weights, as in
+    fine-tuning around a quantised model.  The op type is the autocast dtype, or
+    ``x``'s where autocast is off, and must be 16-bit; the weights' values are
+    exact in bf16 (and in fp16 within its range), products and the weighted sum
+    over a token's routes are fp32, routes' rows of a weighted sum rounded once to
+    the op type.
+
+    ``quantize_input``: the rows are quantised to 4-bit values as well and
+    multiplied as such (four times the matrix rate); for inference, without
+    gradients."""
+    if not isinstance(keys, CVMMMx4) or not keys._keys:
+        raise TypeError("cvmm_mx4: keys must be cvmm_mx4_quantize(weights, dim=1)")
+    _require_device(x, "x")
+    _require_device(keys.codes, "keys")
+    op = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
+    if op not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"cvmm_mx4: the op type must be bfloat16 or float16, not {op} (autocast, or the rows' type)")
+    E, d_in, d_out = keys.shape
+    if x.shape[-1] != d_in:
+        raise ValueError(f"cvmm_mx4: x has {x.shape[-1]} columns, the weights {d_in} rows")
+    if not isinstance(sel, CVMMSel):
+        sel = cvmm_prepare_sel(sel, E)
+    rw = sel.reduction_weight
+    grad = torch.is_grad_enabled() and (x.requires_grad or (rw is not None and rw.requires_grad))
+    if grad and quantize_input:
+        raise RuntimeError("cvmm_mx4: quantize_input is for inference (rounding to 4 bits has no gradient)")
+    raw = sel._raw_shape_tensor()
+    top_k = raw.shape[-1] if raw.ndim > 0 else 1
+    sel._resolve(E)
+    s, sel_index, out_index = sel._sel, sel._sel_index, sel._out_index
+    _require_device(s, "sel")
+    shape = [*rw.shape[:-1], d_out] if rw is not None else [*s.shape, d_out]
+    offsets = _offsets_for(s, E)
+    if _compiling():
+        return _ops.mx4_product(x, rw, keys.codes, keys.scales, d_in, d_out, sel_index, out_index, offsets, top_k, op,
+                                quantize_input).view(shape)
+    pos = _route_pos(out_index if out_index is not None else sel_index, s.numel())
+    return N.host().mx4_apply(x, rw, keys.codes, keys.scales, d_in, d_out, sel_index, out_index, offsets, pos, top_k,
+                              _DTYPE_IDS[op], quantize_input, grad, shape)

@@ -203,3 +203,145 @@ def _route_backward(ctx, grad_w, *_):
 
 
 route_topk.register_autograd(_route_backward, setup_context=_route_setup)
+
+
+# ---------------------------------------------------------------------------
+# router of balanced models (api.cvmm_route_scored): outputs as route_topk's
+# ---------------------------------------------------------------------------
+@torch.library.custom_op(f"{NS}::route_scored", mutates_args=())
+def route_scored(logits: torch.Tensor, top_k: int, bias: Optional[torch.Tensor], scores: int, groups: int,
+                 topk_groups: int, renormalize: bool, scale: float) -> Tuple[torch.Tensor, torch.Tensor,
+                                                                           torch.Tensor, torch.Tensor,
+                                                                           torch.Tensor, torch.Tensor,
+                                                                           torch.Tensor]:
+    out = N.host().route_scored(logits, top_k, bias, scores, groups, topk_groups, renormalize, scale,
+                                N.stream_of(logits.device))
+    return tuple(t.clone() for t in out)
+
+
+@route_scored.register_fake
+def _(logits, top_k, bias, scores, groups, topk_groups, renormalize, scale):
+    T = logits.numel() // logits.shape[-1]
+    E = logits.shape[-1]
+    R = T * top_k
+    return (logits.new_empty((T, top_k), dtype=torch.float32), logits.new_empty((T, top_k), dtype=torch.int64),
+            logits.new_empty((R,), dtype=torch.int32), logits.new_empty((R,), dtype=torch.int64),
+            logits.new_empty((R,), dtype=torch.int64), logits.new_empty((E,), dtype=torch.int64),
+            logits.new_empty((R,), dtype=torch.int32))
+
+
+@torch.library.custom_op(f"{NS}::route_scored_backward", mutates_args=())
+def route_scored_backward(logits: torch.Tensor, sel: torch.Tensor, grad_weights: torch.Tensor, top_k: int,
+                          scores: int, renormalize: bool, scale: float) -> torch.Tensor:
+    return N.host().route_scored_backward(logits, sel, grad_weights, top_k, scores, renormalize, scale,
+                                          N.stream_of(logits.device))
+
+
+@route_scored_backward.register_fake
+def _(logits, sel, grad_weights, top_k, scores, renormalize, scale):
+    return torch.empty_like(logits, memory_format=torch.contiguous_format)
+
+
+def _scored_setup(ctx, inputs, output):
+    logits, top_k, _, scores, _, _, renormalize, scale = inputs
+    ctx.save_for_backward(logits, output[1])
+    ctx.args = (top_k, scores, renormalize, scale)
+
+
+def _scored_backward(ctx, grad_w, *_):
+    if grad_w is None:
+        return (None,) * 8
+    logits, sel = ctx.saved_tensors
+    return (route_scored_backward(logits, sel, grad_w.contiguous(), *ctx.args),) + (None,) * 7
+
+
+route_scored.register_autograd(_scored_backward, setup_context=_scored_setup)
+
+
+# ---------------------------------------------------------------------------
+# microscaled 4-bit values (api.cvmm_mx4_quantize, CVMMMx4.dequantize, cvmm_mx4)
+# ---------------------------------------------------------------------------
+def _mx4_bytes(shape, keys: bool) -> Tuple[List[int], List[int]]:
+    """Shapes of the codes and scales (layouts: csrc/cvmm_mx4.h)."""
+    if keys:
+        E, K, n = shape
+        panels = ((n + 63) // 64) * ((K + 127) // 128)
+        return [E, panels * 4096], [E, panels * 256]
+    rows = 1
+    for s in shape[:-1]:
+        rows = rows * s
+    K = shape[-1]
+    return [rows, (K + 127) // 128 * 64], [rows, (K + 511) // 512 * 16]
+
+
+@torch.library.custom_op(f"{NS}::mx4_quantize", mutates_args=())
+def mx4_quantize(t: torch.Tensor, keys: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    host = N.host()
+    return (host.mx4_quantize_keys if keys else host.mx4_quantize_rows)(t, N.stream_of(t.device))
+
+
+@mx4_quantize.register_fake
+def _(t, keys):
+    codes, scales = _mx4_bytes(t.shape, keys)
+    return t.new_empty(codes, dtype=torch.uint8), t.new_empty(scales, dtype=torch.uint8)
+
+
+@torch.library.custom_op(f"{NS}::mx4_dequantize", mutates_args=())
+def mx4_dequantize(codes: torch.Tensor, scales: torch.Tensor, shape: List[int], keys: bool,
+                   dtype: torch.dtype) -> torch.Tensor:
+    return N.host().mx4_dequantize(codes, scales, shape, keys, N.dtype_id(dtype), N.stream_of(codes.device))
+
+
+@mx4_dequantize.register_fake
+def _(codes, scales, shape, keys, dtype):
+    return codes.new_empty(shape, dtype=dtype)
+
+
+@torch.library.custom_op(f"{NS}::mx4_product", mutates_args=())
+def mx4_product(x: torch.Tensor, rw: Optional[torch.Tensor], codes: torch.Tensor, scales: torch.Tensor, d_in: int,
+                d_out: int, sel_index: torch.Tensor, out_index: Optional[torch.Tensor], offsets: torch.Tensor,
+                top_k: int, op_dtype: torch.dtype, quantize_input: bool) -> torch.Tensor:
+    return N.host().mx4_forward(x, codes, scales, d_in, d_out, sel_index, out_index, offsets, None, rw,
+                                N.dtype_id(op_dtype), quantize_input, N.stream_of(x.device))
+
+
+@mx4_product.register_fake
+def _(x, rw, codes, scales, d_in, d_out, sel_index, out_index, offsets, top_k, op_dtype, quantize_input):
+    R = sel_index.numel()
+    rows = R if rw is None else R // rw.shape[-1]
+    return x.new_empty((rows, d_out), dtype=op_dtype)
+
+
+@torch.library.custom_op(f"{NS}::mx4_product_backward", mutates_args=())
+def mx4_product_backward(grad: torch.Tensor, x: torch.Tensor, rw: Optional[torch.Tensor], codes: torch.Tensor,
+                         scales: torch.Tensor, d_in: int, d_out: int, sel_index: torch.Tensor,
+                         out_index: Optional[torch.Tensor], offsets: torch.Tensor, top_k: int,
+                         op_dtype: torch.dtype, need_x: bool, need_rw: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    gx, grw = N.host().mx4_backward(grad, x, codes, scales, d_in, d_out, sel_index, out_index, offsets, None, rw,
+                                    top_k, N.dtype_id(op_dtype), need_x, need_rw, N.stream_of(x.device))
+    return gx if gx is not None else _empty(x), grw if grw is not None else _empty(x)
+
+
+@mx4_product_backward.register_fake
+def _(grad, x, rw, codes, scales, d_in, d_out, sel_index, out_index, offsets, top_k, op_dtype, need_x, need_rw):
+    gx = x.new_empty(x.shape) if need_x else _empty(x)
+    grw = (torch.empty_like(rw, memory_format=torch.contiguous_format) if need_rw and rw is not None else _empty(x))
+    return gx, grw
+
+
+def _mx4_setup(ctx, inputs, output):
+    x, rw, codes, scales, d_in, d_out, sel_index, out_index, offsets, top_k, op_dtype, _ = inputs
+    ctx.save_for_backward(x, rw, codes, scales, sel_index, out_index, offsets)
+    ctx.args = (d_in, d_out, top_k, op_dtype)
+
+
+def _mx4_backward(ctx, grad):
+    x, rw, codes, scales, sel_index, out_index, offsets = ctx.saved_tensors
+    d_in, d_out, top_k, op_dtype = ctx.args
+    need_x, need_rw = bool(ctx.needs_input_grad[0]), bool(ctx.needs_input_grad[1]) and rw is not None
+    gx, grw = mx4_product_backward(grad.contiguous(), x, rw, codes, scales, d_in, d_out, sel_index, out_index,
+                                   offsets, top_k, op_dtype, need_x, need_rw)
+    return (gx if need_x else None, grw if need_rw else None) + (None,) * 10
+
+
+mx4_product.register_autograd(_mx4_backward, setup_context=_mx4_setup)

@@ -10,6 +10,7 @@
 
 #include "cvmm_common.h"
 #include "cvmm_internal.h"
+#include "cvmm_mx4.h"
 #include "../../include/cvmm_hip.h"
 
 namespace cvmm {
@@ -711,6 +712,59 @@ int cvmm_route_topk_backward(const void* logits, int32_t logits_dtype, int64_t n
                                                                         top_k, renormalize, sel, grad_weights,
                                                                         grad_logits, grad_ld, s); }),
                       "cvmm_route_topk_backward");
+}
+
+static int scored_args_ok(const char* what, int32_t logits_dtype, int64_t n_tokens, int64_t logits_ld,
+                          int32_t n_experts, int64_t top_k, int32_t scores) {
+  int r = route_args_ok(what, logits_dtype, n_tokens, logits_ld, n_experts, top_k);
+  if (r) return r;
+  if (scores != CVMM_SCORES_SOFTMAX && scores != CVMM_SCORES_SIGMOID)
+    return fail(CVMM_ERR_INVALID, "%s: unknown scores %d", what, scores);
+  return CVMM_OK;
+}
+
+int cvmm_route_scored(const void* logits, int32_t logits_dtype, int64_t n_tokens, int64_t logits_ld,
+                      int32_t n_experts, int64_t top_k, const float* bias, int32_t scores, int32_t groups,
+                      int32_t topk_groups, int32_t renormalize, double scale, float* weights, int64_t* sel,
+                      int32_t* sorted_sel, int64_t* perm, int64_t* token_index, int64_t* offsets,
+                      int32_t* route_pos, void* workspace, size_t workspace_bytes, void* stream) {
+  int r = scored_args_ok("cvmm_route_scored", logits_dtype, n_tokens, logits_ld, n_experts, top_k, scores);
+  if (r) return r;
+  if (groups <= 0 || n_experts % groups != 0 || topk_groups <= 0 || topk_groups > groups ||
+      top_k > (int64_t)topk_groups * (n_experts / groups))
+    return fail(CVMM_ERR_INVALID, "cvmm_route_scored: bad groups (E=%d, groups=%d, kept=%d, k=%lld)", n_experts, groups,
+                topk_groups, (long long)top_k);
+  if (topk_groups < groups && groups > kRouteMaxGroups)
+    return fail(CVMM_ERR_UNSUPPORTED, "cvmm_route_scored: at most %d groups", kRouteMaxGroups);
+  const size_t need = route_workspace_bytes(n_tokens, n_experts, top_k);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(CVMM_ERR_WORKSPACE, "cvmm_route_scored: workspace too small (%zu < %zu)", workspace_bytes, need);
+  if (n_tokens == 0) return CVMM_OK;
+  if (!logits || !weights || !sel || !sorted_sel || !perm || !offsets)
+    return fail(CVMM_ERR_INVALID, "cvmm_route_scored: NULL pointer");
+  hipStream_t s = (hipStream_t)stream;
+  return check_launch(timed(CVMM_KC_ROUTE, s, [&] { return launch_route_scored(logits, logits_dtype, n_tokens, logits_ld, n_experts, top_k,
+                                                                 bias, scores, groups, topk_groups, renormalize, scale,
+                                                                 weights, sel, sorted_sel, perm, token_index, offsets,
+                                                                 route_pos, workspace, s); }),
+                      "cvmm_route_scored");
+}
+
+int cvmm_route_scored_backward(const void* logits, int32_t logits_dtype, int64_t n_tokens, int64_t logits_ld,
+                               int32_t n_experts, int64_t top_k, int32_t scores, int32_t renormalize, double scale,
+                               const int64_t* sel, const float* grad_weights, void* grad_logits, int64_t grad_ld,
+                               void* stream) {
+  int r = scored_args_ok("cvmm_route_scored_backward", logits_dtype, n_tokens, logits_ld, n_experts, top_k, scores);
+  if (r) return r;
+  if (grad_ld < n_experts) return fail(CVMM_ERR_INVALID, "cvmm_route_scored_backward: grad row stride too small");
+  if (n_tokens == 0) return CVMM_OK;
+  if (!logits || !sel || !grad_weights || !grad_logits)
+    return fail(CVMM_ERR_INVALID, "cvmm_route_scored_backward: NULL pointer");
+  hipStream_t s = (hipStream_t)stream;
+  return check_launch(timed(CVMM_KC_ROUTE, s, [&] { return launch_route_scored_backward(logits, logits_dtype, n_tokens, logits_ld, n_experts,
+                                                                          top_k, scores, renormalize, scale, sel,
+                                                                          grad_weights, grad_logits, grad_ld, s); }),
+                      "cvmm_route_scored_backward");
 }
 
 // ---------------------------------------------------------------------------
@@ -1577,6 +1631,295 @@ int cvmm_bwd_w_rows(const void* x, int32_t x_dtype, int64_t x_rows, int64_t x_ld
                     sel_index, out_index, n_routes, offsets, rw, rw_dtype, top_k, op_dtype, grad_keys,
                     grad_keys_dtype, gk_se, gk_si, gk_sj, flags, rows, rows_bytes, workspace, workspace_bytes,
                     stream);
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// microscaled 4-bit weights
+// ---------------------------------------------------------------------------
+namespace {
+
+bool mx4_sizes_ok(int64_t E, int64_t K, int64_t N) {
+  constexpr int64_t kMax = int64_t(1) << 31;
+  return E > 0 && E < kMax && K > 0 && K < kMax && N > 0 && N < kMax &&
+         E <= (int64_t(1) << 46) / (mx4_panels_n(N) * mx4_panels_k(K));
+}
+
+// Rows the products cannot read in aligned 16-byte pieces are copied.
+bool mx4_rows_copied(const void* p, int64_t ld, int64_t width) {
+  return width % 8 != 0 || ld % 8 != 0 || !aligned16(p);
+}
+
+size_t mx4_fwd_bytes(int64_t n_routes, int64_t d_in, int64_t d_out, int64_t x_rows, bool weighted, bool have_pos,
+                     bool copied, bool quantize) {
+  size_t b = 0;
+  if (weighted) {
+    b += align_up((size_t)n_routes * pad8(d_out) * 2, 256);
+    if (!have_pos) b += align_up((size_t)n_routes * 4, 256);
+  }
+  if (quantize)
+    b += align_up((size_t)x_rows * mx4_row_code_bytes(d_in), 256) + align_up((size_t)x_rows * mx4_row_scale_bytes(d_in), 256);
+  else if (copied)
+    b += align_up((size_t)x_rows * pad8(d_in) * 2, 256);
+  return b;
+}
+
+size_t mx4_bwd_bytes(int64_t n_routes, int64_t d_in, int64_t d_out, int64_t grad_rows, bool reduce, bool have_pos,
+                     bool copied, bool need_rw, int32_t gx_dtype) {
+  size_t b = 0;
+  if (reduce) {
+    b += align_up((size_t)n_routes * pad8(d_in) * dtype_size(gx_dtype), 256);
+    if (!have_pos) b += align_up((size_t)n_routes * 4, 256);
+  }
+  if (need_rw) b += align_up((size_t)n_routes * ((d_in + 63) / 64) * 4, 256);
+  if (copied) b += align_up((size_t)grad_rows * pad8(d_out) * 2, 256);
+  return b;
+}
+
+struct Mx4Carve {
+  char* p;
+  void* take(size_t bytes) {
+    char* r = p;
+    p += align_up(bytes, 256);
+    return r;
+  }
+};
+
+}  // namespace
+
+extern "C" {
+
+size_t cvmm_mx4_rows_bytes(int64_t rows, int64_t d, int32_t scales) {
+  if (rows < 0 || d <= 0) return 0;
+  return (size_t)rows * (scales ? mx4_row_scale_bytes(d) : mx4_row_code_bytes(d));
+}
+
+size_t cvmm_mx4_keys_bytes(int64_t n_experts, int64_t d_in, int64_t d_out, int32_t scales) {
+  if (!mx4_sizes_ok(n_experts, d_in, d_out)) return 0;
+  return (size_t)n_experts * mx4_panels_n(d_out) * mx4_panels_k(d_in) * (scales ? kMx4PanelScales : kMx4PanelCodes);
+}
+
+int cvmm_mx4_quantize_rows(const void* src, int32_t dtype, int64_t ld, int64_t rows, int64_t d, void* codes,
+                           void* scales, void* stream) {
+  if (!valid_dtype(dtype)) return fail(CVMM_ERR_INVALID, "cvmm_mx4_quantize_rows: invalid dtype");
+  if (rows < 0 || d <= 0 || (rows > 1 && ld < d))
+    return fail(CVMM_ERR_INVALID, "cvmm_mx4_quantize_rows: bad sizes (rows=%lld, d=%lld, ld=%lld)", (long long)rows,
+                (long long)d, (long long)ld);
+  if (rows == 0) return CVMM_OK;
+  if (!src || !codes || !scales) return fail(CVMM_ERR_INVALID, "cvmm_mx4_quantize_rows: NULL pointer");
+  hipStream_t s = (hipStream_t)stream;
+  return check_launch(timed_combine(s, [&] { return launch_mx4_quantize_rows(src, dtype, ld, rows, d, codes, scales, s); }),
+                      "cvmm_mx4_quantize_rows");
+}
+
+int cvmm_mx4_quantize_keys(const void* keys, int32_t keys_dtype, int32_t n_experts, int64_t d_in, int64_t d_out,
+                           int64_t k_se, int64_t k_si, int64_t k_sj, void* codes, void* scales, void* stream) {
+  if (!valid_dtype(keys_dtype)) return fail(CVMM_ERR_INVALID, "cvmm_mx4_quantize_keys: invalid dtype");
+  if (!mx4_sizes_ok(n_experts, d_in, d_out))
+    return fail(CVMM_ERR_INVALID, "cvmm_mx4_quantize_keys: bad sizes (E=%d, d_in=%lld, d_out=%lld)", n_experts,
+                (long long)d_in, (long long)d_out);
+  if (!keys || !codes || !scales) return fail(CVMM_ERR_INVALID, "cvmm_mx4_quantize_keys: NULL pointer");
+  hipStream_t s = (hipStream_t)stream;
+  return check_launch(timed(CVMM_KC_CAST_KEYS, s, [&] { return launch_mx4_quantize_keys(keys, keys_dtype, k_se, k_si, k_sj, n_experts,
+                                                                            d_in, d_out, codes, scales, s); }),
+                      "cvmm_mx4_quantize_keys");
+}
+
+int cvmm_mx4_dequantize_rows(const void* codes, const void* scales, int64_t rows, int64_t d, void* out, int32_t dtype,
+                             void* stream) {
+  if (!valid_dtype(dtype)) return fail(CVMM_ERR_INVALID, "cvmm_mx4_dequantize_rows: invalid dtype");
+  if (rows < 0 || d <= 0) return fail(CVMM_ERR_INVALID, "cvmm_mx4_dequantize_rows: bad sizes");
+  if (rows == 0) return CVMM_OK;
+  if (!codes || !scales || !out) return fail(CVMM_ERR_INVALID, "cvmm_mx4_dequantize_rows: NULL pointer");
+  hipStream_t s = (hipStream_t)stream;
+  return check_launch(timed_combine(s, [&] { return launch_mx4_dequantize_rows(codes, scales, rows, d, out, dtype, s); }),
+                      "cvmm_mx4_dequantize_rows");
+}
+
+int cvmm_mx4_dequantize_keys(const void* codes, const void* scales, int32_t n_experts, int64_t d_in, int64_t d_out,
+                             void* out, int32_t dtype, void* stream) {
+  if (!valid_dtype(dtype)) return fail(CVMM_ERR_INVALID, "cvmm_mx4_dequantize_keys: invalid dtype");
+  if (!mx4_sizes_ok(n_experts, d_in, d_out)) return fail(CVMM_ERR_INVALID, "cvmm_mx4_dequantize_keys: bad sizes");
+  if (!codes || !scales || !out) return fail(CVMM_ERR_INVALID, "cvmm_mx4_dequantize_keys: NULL pointer");
+  hipStream_t s = (hipStream_t)stream;
+  return check_launch(timed(CVMM_KC_CAST_KEYS, s, [&] { return launch_mx4_dequantize_keys(codes, scales, n_experts, d_in, d_out, out, dtype, s); }),
+                      "cvmm_mx4_dequantize_keys");
+}
+
+size_t cvmm_mx4_fwd_workspace_bytes(int64_t n_routes, int64_t d_in, int64_t d_out, int64_t x_rows, int32_t weighted,
+                                    int32_t have_route_pos, int32_t x_copied, int32_t quantize_input) {
+  if (n_routes < 0 || d_in <= 0 || d_out <= 0 || x_rows < 0) return 0;
+  return mx4_fwd_bytes(n_routes, d_in, d_out, x_rows, weighted != 0, have_route_pos != 0, x_copied != 0,
+                       quantize_input != 0);
+}
+
+int cvmm_mx4_fwd(const void* x, int32_t x_dtype, int64_t x_rows, int64_t x_ld, const void* codes, const void* scales,
+                 int32_t n_experts, int64_t d_in, int64_t d_out, const int64_t* sel_index, const int64_t* out_index,
+                 int64_t n_routes, const int64_t* offsets, const int32_t* route_pos, const float* reduction_weight,
+                 int64_t reduce_k, int32_t quantize_input, void* out, int64_t out_rows, int64_t out_ld,
+                 void* workspace, size_t workspace_bytes, void* stream) {
+  if (x_dtype != CVMM_DTYPE_F16 && x_dtype != CVMM_DTYPE_BF16)
+    return fail(CVMM_ERR_INVALID, "cvmm_mx4_fwd: rows must be 16-bit");
+  const bool weighted = reduction_weight != nullptr;
+  if (!mx4_sizes_ok(n_experts, d_in, d_out) || n_routes < 0 || n_routes > 0x7fffffff || x_rows < 0 ||
+      (x_rows > 1 && x_ld < d_in) || (out_rows > 1 && out_ld < d_out) || (weighted && reduce_k <= 0) ||
+      out_rows * (weighted ? reduce_k : 1) != n_routes)
+    return fail(CVMM_ERR_INVALID, "cvmm_mx4_fwd: bad sizes (E=%d, d_in=%lld, d_out=%lld, R=%lld, rows %lld -> %lld)",
+                n_experts, (long long)d_in, (long long)d_out, (long long)n_routes, (long long)x_rows,
+                (long long)out_rows);
+  if (n_routes == 0) return CVMM_OK;
+  const bool quantize = quantize_input != 0;
+  const bool copied = !quantize && mx4_rows_copied(x, x_ld, d_in);
+  const size_t need = mx4_fwd_bytes(n_routes, d_in, d_out, x_rows, weighted, route_pos != nullptr, copied, quantize);
+  if (workspace_bytes < need || (need > 0 && workspace == nullptr))
+    return fail(CVMM_ERR_WORKSPACE, "cvmm_mx4_fwd: workspace too small (%zu < %zu)", workspace_bytes, need);
+  if (!x || !codes || !scales || !sel_index || !offsets || !out)
+    return fail(CVMM_ERR_INVALID, "cvmm_mx4_fwd: NULL pointer");
+  hipStream_t s = (hipStream_t)stream;
+  Mx4Carve c{(char*)workspace};
+  const int64_t* rp = out_index ? out_index : sel_index;
+  GemmParams g{};
+  g.a = x; g.a_dtype = x_dtype; g.a_ld = x_ld; g.a_rows = x_rows; g.a_idx = sel_index; g.a_div = 1;
+  g.K = d_in; g.N = g.n_out = d_out;
+  g.offsets = offsets; g.n_experts = n_experts; g.n_routes = n_routes;
+  g.o_idx = rp; g.o_div = 1; g.w_idx = rp;
+  g.val_dtype = g.out_dtype = x_dtype; g.prod_dtype = -1;
+  g.zero_unrouted = 1;
+  g.out = out; g.out_ld = out_ld; g.out_rows = out_rows;
+  const int32_t* inv = route_pos;
+  int r = 0;
+  if (weighted) {
+    // row q of the buffer is sorted route q, rounded to the rows' type once,
+    // as an unweighted call returns it; the sum per token is fp32
+    const int64_t w8 = pad8(d_out);
+    g.out = c.take((size_t)n_routes * w8 * 2);
+    g.out_ld = w8; g.out_rows = n_routes; g.o_idx = nullptr;
+    g.N = g.n_out = w8;  // (columns past d_out are products of zero codes)
+    g.zero_unrouted = 0;
+    if (!inv) {
+      int32_t* ws = (int32_t*)c.take((size_t)n_routes * 4);
+      r = check_launch(timed_combine(s, [&] { return launch_invert_rows(rp, n_routes, ws, s); }), "cvmm_mx4_fwd(invert)");
+      if (r) return r;
+      inv = ws;
+    }
+  }
+  const void* a_scales = nullptr;
+  if (quantize) {
+    void* qc = c.take((size_t)x_rows * mx4_row_code_bytes(d_in));
+    void* qs = c.take((size_t)x_rows * mx4_row_scale_bytes(d_in));
+    r = check_launch(timed_combine(s, [&] { return launch_mx4_quantize_rows(x, x_dtype, x_ld, x_rows, d_in, qc, qs, s); }),
+                     "cvmm_mx4_fwd(quantize)");
+    if (r) return r;
+    g.a = qc;
+    a_scales = qs;
+  } else if (copied) {
+    void* xp = c.take((size_t)x_rows * pad8(d_in) * 2);
+    r = check_launch(timed_combine(s, [&] { return launch_pad_rows(x, x_dtype, x_ld, x_rows, d_in, nullptr, 0, x_dtype, xp, s); }),
+                     "cvmm_mx4_fwd(pad rows)");
+    if (r) return r;
+    g.a = xp; g.a_ld = pad8(d_in); g.K = pad8(d_in);
+  }
+  r = check_launch(timed(CVMM_KC_GEMM_FWD, s, [&] { return launch_mx4_fwd(g, codes, scales, a_scales, x_dtype, s); }), "cvmm_mx4_fwd(gemm)");
+  if (r || !weighted) return r;
+  return check_launch(timed_combine(s, [&] { return launch_combine_rows(g.out, x_dtype, g.out_ld, inv, rp, offsets + (n_experts - 1), reduction_weight,
+                                          kF32, kF32, out_rows, reduce_k, d_out, -1, out, x_dtype, out_ld, s); }),
+                      "cvmm_mx4_fwd(combine)");
+}
+
+size_t cvmm_mx4_bwd_x_workspace_bytes(int64_t n_routes, int64_t d_in, int64_t d_out, int64_t grad_rows,
+                                      int32_t token_input, int32_t have_route_pos, int32_t grad_copied,
+                                      int32_t need_grad_rw, int32_t grad_x_dtype) {
+  if (n_routes < 0 || d_in <= 0 || d_out <= 0 || grad_rows < 0 || !valid_dtype(grad_x_dtype)) return 0;
+  return mx4_bwd_bytes(n_routes, d_in, d_out, grad_rows, token_input != 0, have_route_pos != 0, grad_copied != 0,
+                       need_grad_rw != 0, grad_x_dtype);
+}
+
+int cvmm_mx4_bwd_x(const void* grad, int32_t op_dtype, int64_t grad_rows, int64_t grad_ld, const void* codes,
+                   const void* scales, int32_t n_experts, int64_t d_in, int64_t d_out, const int64_t* sel_index,
+                   const int64_t* out_index, int64_t n_routes, const int64_t* offsets, const int32_t* route_pos,
+                   const float* reduction_weight, int64_t top_k, const void* x, int32_t x_dtype, int64_t x_rows,
+                   int64_t x_ld, void* grad_x, int32_t grad_x_dtype, int64_t grad_x_rows, int64_t grad_x_ld,
+                   float* grad_rw, void* workspace, size_t workspace_bytes, void* stream) {
+  if ((op_dtype != CVMM_DTYPE_F16 && op_dtype != CVMM_DTYPE_BF16) || !valid_dtype(x_dtype) ||
+      (grad_x_dtype != op_dtype && grad_x_dtype != CVMM_DTYPE_F32) || (x_dtype != op_dtype && x_dtype != CVMM_DTYPE_F32))
+    return fail(CVMM_ERR_INVALID, "cvmm_mx4_bwd_x: invalid dtypes");
+  const bool weighted = reduction_weight != nullptr, reduce = out_index != nullptr && grad_x != nullptr;
+  if (!mx4_sizes_ok(n_experts, d_in, d_out) || n_routes < 0 || n_routes > 0x7fffffff || top_k <= 0 ||
+      grad_rows * (weighted ? top_k : 1) != n_routes || (grad_rows > 1 && grad_ld < d_out) ||
+      (grad_x != nullptr && (grad_x_rows * (out_index != nullptr ? top_k : 1) != n_routes ||
+                             (grad_x_rows > 1 && grad_x_ld < d_in))) ||
+      (grad_rw != nullptr && (!weighted || x_rows < 0 || (x_rows > 1 && x_ld < d_in))))
+    return fail(CVMM_ERR_INVALID, "cvmm_mx4_bwd_x: bad sizes (E=%d, d_in=%lld, d_out=%lld, R=%lld, grad rows %lld)",
+                n_experts, (long long)d_in, (long long)d_out, (long long)n_routes, (long long)grad_rows);
+  if (n_routes == 0 || (!grad_x && !grad_rw)) return CVMM_OK;
+  const bool copied = mx4_rows_copied(grad, grad_ld, d_out);
+  const size_t need = mx4_bwd_bytes(n_routes, d_in, d_out, grad_rows, reduce, route_pos != nullptr, copied,
+                                    grad_rw != nullptr, grad_x_dtype);
+  if (workspace_bytes < need || (need > 0 && workspace == nullptr))
+    return fail(CVMM_ERR_WORKSPACE, "cvmm_mx4_bwd_x: workspace too small (%zu < %zu)", workspace_bytes, need);
+  if (!grad || !codes || !scales || !sel_index || !offsets || (grad_rw && !x))
+    return fail(CVMM_ERR_INVALID, "cvmm_mx4_bwd_x: NULL pointer");
+  hipStream_t s = (hipStream_t)stream;
+  Mx4Carve c{(char*)workspace};
+  const int64_t* rp = out_index ? out_index : sel_index;
+  GemmParams g{};
+  g.a = grad; g.a_dtype = op_dtype; g.a_ld = grad_ld; g.a_rows = grad_rows;
+  g.a_idx = rp; g.a_div = weighted ? top_k : 1;
+  g.K = d_out; g.N = g.n_out = d_in;
+  g.offsets = offsets; g.n_experts = n_experts; g.n_routes = n_routes;
+  g.o_idx = rp; g.o_div = 1; g.w_idx = rp;
+  g.val_dtype = g.out_dtype = grad_x_dtype; g.prod_dtype = -1;
+  g.role = 1;
+  const int32_t* inv = route_pos;
+  int r = 0;
+  if (reduce) {
+    const int64_t w8 = pad8(d_in);
+    g.out = c.take((size_t)n_routes * w8 * dtype_size(grad_x_dtype));
+    g.out_ld = w8; g.out_rows = n_routes; g.o_idx = nullptr;
+    g.N = g.n_out = w8;
+    if (!inv) {
+      int32_t* ws = (int32_t*)c.take((size_t)n_routes * 4);
+      r = check_launch(timed_combine(s, [&] { return launch_invert_rows(rp, n_routes, ws, s); }), "cvmm_mx4_bwd_x(invert)");
+      if (r) return r;
+      inv = ws;
+    }
+  } else if (grad_x != nullptr) {
+    g.out = grad_x; g.out_ld = grad_x_ld; g.out_rows = grad_x_rows;
+    g.zero_unrouted = 1;
+    if (weighted) {
+      g.w = reduction_weight; g.w_dtype = kF32; g.w_round = kF32;
+    }
+  }
+  const int32_t nt = (int32_t)((d_in + 63) / 64);
+  if (grad_rw != nullptr) {
+    // one 64-column piece: its partial is the gradient
+    float* part = (float*)c.take((size_t)n_routes * nt * 4);
+    g.dg = nt == 1 ? grad_rw : part;
+    g.dg_ntiles = nt;
+    g.dg_x = x; g.dg_x_dtype = x_dtype; g.dg_x_ld = x_ld; g.dg_x_rows = x_rows; g.dg_x_idx = sel_index;
+    g.dg_n = d_in;
+    g.dg_val_dtype = kF32;
+  }
+  if (copied) {
+    void* gp = c.take((size_t)grad_rows * pad8(d_out) * 2);
+    r = check_launch(timed_combine(s, [&] { return launch_pad_rows(grad, op_dtype, grad_ld, grad_rows, d_out, nullptr, 0, op_dtype, gp, s); }),
+                     "cvmm_mx4_bwd_x(pad rows)");
+    if (r) return r;
+    g.a = gp; g.a_ld = pad8(d_out); g.K = pad8(d_out);
+  }
+  r = check_launch(timed(CVMM_KC_GEMM_BWDX, s, [&] { return launch_mx4_bwd_x(g, codes, scales, op_dtype, s); }), "cvmm_mx4_bwd_x(gemm)");
+  if (r) return r;
+  if (reduce) {
+    r = check_launch(timed_combine(s, [&] { return launch_combine_rows(g.out, grad_x_dtype, g.out_ld, inv, rp, offsets + (n_experts - 1), reduction_weight,
+                                         kF32, kF32, grad_x_rows, top_k, d_in, -1, grad_x, grad_x_dtype, grad_x_ld, s); }),
+                     "cvmm_mx4_bwd_x(combine)");
+    if (r) return r;
+  }
+  if (grad_rw != nullptr && nt > 1)
+    r = check_launch(timed_combine(s, [&] { return launch_sum_partials(g.dg, n_routes, nt, grad_rw, kF32, s); }),
+                     "cvmm_mx4_bwd_x(dgate)");
+  return r;
 }
 
 }  // extern "C"

@@ -282,6 +282,43 @@ hipError_t launch_route_topk_backward(const void* logits, int32_t logits_dtype, 
                                       const float* grad_weights, void* grad_logits, int64_t grad_ld,
                                       hipStream_t stream);
 
+// The router of balanced models (cvmm_router_scored.hip): sigmoid or softmax
+// scores, a bias in the choice, groups of experts, renormalised and scaled
+// weights.  The workspace is route_workspace_bytes.
+constexpr int32_t kRouteMaxGroups = 64;
+hipError_t launch_route_scored(const void* logits, int32_t logits_dtype, int64_t n_tokens, int64_t logits_ld,
+                               int32_t n_experts, int64_t top_k, const float* bias, int32_t sigmoid, int32_t groups,
+                               int32_t topk_groups, int32_t renormalize, double scale, float* weights, int64_t* sel,
+                               int32_t* sorted_sel, int64_t* perm, int64_t* token_index, int64_t* offsets,
+                               int32_t* route_pos, void* workspace, hipStream_t stream);
+hipError_t launch_route_scored_backward(const void* logits, int32_t logits_dtype, int64_t n_tokens,
+                                        int64_t logits_ld, int32_t n_experts, int64_t top_k, int32_t sigmoid,
+                                        int32_t renormalize, double scale, const int64_t* sel,
+                                        const float* grad_weights, void* grad_logits, int64_t grad_ld,
+                                        hipStream_t stream);
+
+// ---------------------------------------------------------------------------
+// microscaled 4-bit values (cvmm_mx4.h: format and layouts)
+// ---------------------------------------------------------------------------
+hipError_t launch_mx4_quantize_rows(const void* src, int32_t dtype, int64_t ld, int64_t rows, int64_t K, void* codes,
+                                    void* scales, hipStream_t stream);
+hipError_t launch_mx4_quantize_keys(const void* src, int32_t dtype, int64_t se, int64_t sk, int64_t sn, int64_t E,
+                                    int64_t K, int64_t N, void* codes, void* scales, hipStream_t stream);
+hipError_t launch_mx4_dequantize_rows(const void* codes, const void* scales, int64_t rows, int64_t K, void* out,
+                                      int32_t dtype, hipStream_t stream);
+hipError_t launch_mx4_dequantize_keys(const void* codes, const void* scales, int64_t E, int64_t K, int64_t N,
+                                      void* out, int32_t dtype, hipStream_t stream);
+
+// Routed products with 4-bit weights in the keys layout (cvmm_mx4_gemm.h).  g:
+// A rows, routes and epilogue as launch_routed_gemm's, without b; A in the op
+// type (16-byte aligned rows, K % 8 == 0), or, with a_scales, codes of the rows
+// layout.  bwd_x: g.K = d_out, g.N = d_in, the output scaled by g.w in fp32,
+// the routing-weight gradient's partials one per 64 columns.
+hipError_t launch_mx4_fwd(const GemmParams& g, const void* codes, const void* scales, const void* a_scales,
+                          int32_t op_dtype, hipStream_t stream);
+hipError_t launch_mx4_bwd_x(const GemmParams& g, const void* codes, const void* scales, int32_t op_dtype,
+                            hipStream_t stream);
+
 // Op-dtype copies padded with zeros to multiples of 8 (cvmm_pad.hip): rows
 // (with w: scaled by their rounded weight, one per row), and the expert
 // matrices keys[e][i][j] as [E][i8][j8] or, transposed, [E][j8][i8].

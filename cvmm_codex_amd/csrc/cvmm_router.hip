@@ -14,56 +14,12 @@
 
 #include "cvmm_common.h"
 #include "cvmm_internal.h"
+#include "cvmm_router.h"
 
 namespace cvmm {
 
 constexpr int kRouteThreads = 256;
 constexpr int kRouteHistThreads = 512;  // two waves per SIMD: the selection rounds are latency-bound
-
-// Segments of LPT lanes (4..64) each route one token: lane i of a segment
-// holds experts i + LPT * v, v < MAXV.  Reductions over a segment use DPP
-// (quad permutes, half-row and row mirrors) and, past 16 lanes, shuffles; every
-// lane of the segment ends with the same result.
-template <int CTRL>
-__device__ __forceinline__ float dpp_f(float v) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
-}
-template <int CTRL>
-__device__ __forceinline__ int32_t dpp_i(int32_t v) {
-  return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, true);
-}
-constexpr int kDppXor1 = 0xB1, kDppXor2 = 0x4E, kDppHalfMirror = 0x141, kDppMirror = 0x140;
-
-template <int LPT>
-__device__ __forceinline__ float seg_max(float v) {
-  v = fmaxf(v, dpp_f<kDppXor1>(v));
-  v = fmaxf(v, dpp_f<kDppXor2>(v));
-  if constexpr (LPT >= 8) v = fmaxf(v, dpp_f<kDppHalfMirror>(v));
-  if constexpr (LPT >= 16) v = fmaxf(v, dpp_f<kDppMirror>(v));
-  if constexpr (LPT >= 32) v = fmaxf(v, __shfl_xor(v, 16, 64));
-  if constexpr (LPT >= 64) v = fmaxf(v, __shfl_xor(v, 32, 64));
-  return v;
-}
-template <int LPT>
-__device__ __forceinline__ float seg_sum(float v) {  // same two partials per step: same total in every lane
-  v = v + dpp_f<kDppXor1>(v);
-  v = v + dpp_f<kDppXor2>(v);
-  if constexpr (LPT >= 8) v = v + dpp_f<kDppHalfMirror>(v);
-  if constexpr (LPT >= 16) v = v + dpp_f<kDppMirror>(v);
-  if constexpr (LPT >= 32) v = v + __shfl_xor(v, 16, 64);
-  if constexpr (LPT >= 64) v = v + __shfl_xor(v, 32, 64);
-  return v;
-}
-template <int LPT>
-__device__ __forceinline__ int32_t seg_min_i(int32_t v) {
-  v = min(v, dpp_i<kDppXor1>(v));
-  v = min(v, dpp_i<kDppXor2>(v));
-  if constexpr (LPT >= 8) v = min(v, dpp_i<kDppHalfMirror>(v));
-  if constexpr (LPT >= 16) v = min(v, dpp_i<kDppMirror>(v));
-  if constexpr (LPT >= 32) v = min(v, __shfl_xor(v, 16, 64));
-  if constexpr (LPT >= 64) v = min(v, __shfl_xor(v, 32, 64));
-  return v;
-}
 
 // Softmax of one token's logits in its segment.
 template <typename LT, int LPT, int MAXV>
@@ -90,23 +46,6 @@ __device__ __forceinline__ void route_softmax(const LT* __restrict__ row, int32_
   *m_out = m;
   *s_out = s;
 }
-
-// The sort's outputs, written by the router's own launch where one workgroup
-// holds every route (ONE).
-struct RouteSortOut {
-  int32_t* sorted_sel;
-  int64_t* perm;
-  int64_t* token_index;  // or NULL
-  int64_t* offsets;
-  int32_t* route_pos;    // or NULL
-};
-
-// Routes that a single router workgroup sorts itself, at most.  Beyond them
-// its ranking outlasts a second launch: 64 tokens, top-8, 128 / 256 / 512
-// experts 26 / 42 / 76 us per call in one launch, 23 / 38 / 73 in two; 32
-// tokens 14 / 22 / 39 and 20 / 23 / 41.
-constexpr int kRouteOneMax = 256;
-static_assert(kRouteOneMax % 64 == 0, "whole waves of ids");
 
 // ONE: a single workgroup routes every token (a decode step: up to 256
 // routes) and sorts the routes itself -- the histogram's scan in LDS, then
@@ -193,47 +132,7 @@ __global__ __launch_bounds__(kRouteHistThreads) void route_topk_hist_kernel(
   }
   __syncthreads();
   if constexpr (ONE) {
-    // hist -> first output position of each expert (exclusive scan, wave 0)
-    if (threadIdx.x < 64) {
-      int32_t carry = 0;
-      for (int base = 0; base < E; base += 64) {
-        const int e = base + (int)threadIdx.x;
-        const int32_t c = e < E ? hist[e] : 0;
-        const int32_t incl = wave_incl_scan(c) + carry;
-        if (e < E) {
-          hist[e] = incl - c;
-          so.offsets[e] = incl;
-        }
-        carry = __builtin_amdgcn_readlane(incl, 63);
-      }
-    }
-    __syncthreads();
-    const int n = (int)(n_tokens * k);
-    for (int i = threadIdx.x; i < n; i += kRouteHistThreads) {
-      const int32_t e = ids[i];
-      // routes before i on the same expert, 16 ids per step (a wave's lanes
-      // share their reads and the bound)
-      int rank = 0;
-      const int end = (i | 63) + 1;
-      for (int j = 0; j < end; j += 16) {
-        int4 o[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) o[q] = *reinterpret_cast<const int4*>(ids + j + 4 * q);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int at = j + 4 * q;
-          rank += (o[q].x == e && at < i) ? 1 : 0;
-          rank += (o[q].y == e && at + 1 < i) ? 1 : 0;
-          rank += (o[q].z == e && at + 2 < i) ? 1 : 0;
-          rank += (o[q].w == e && at + 3 < i) ? 1 : 0;
-        }
-      }
-      const int p = hist[e] + rank;
-      so.sorted_sel[p] = e;
-      so.perm[p] = i;
-      if (so.token_index != nullptr) so.token_index[p] = i / k;
-      if (so.route_pos != nullptr) so.route_pos[i] = p;
-    }
+    route_sort_one<kRouteHistThreads>(hist, ids, (int)(n_tokens * k), E, k, so);
     return;
   }
   for (int e = threadIdx.x; e <= E; e += kRouteHistThreads) counts[b * (int64_t)(E + 1) + e] = hist[e];

@@ -271,6 +271,58 @@ Tensor route_topk_backward(const Tensor& logits, const Tensor& sel, const Tensor
   return out.view(logits.sizes());
 }
 
+// The router of balanced models: outputs as route_topk's.
+std::vector<Tensor> route_scored(const Tensor& logits, int64_t top_k, const OptT& bias, int64_t scores,
+                                 int64_t groups, int64_t topk_groups, bool renormalize, double scale,
+                                 int64_t stream) {
+  require_device(logits, "logits");
+  Tensor l = logits.reshape({-1, logits.size(-1)});
+  if (l.stride(-1) != 1 || (l.size(0) > 1 && l.stride(0) < l.size(1))) l = l.contiguous();
+  const int64_t T = l.size(0), E = l.size(1);
+  const int64_t R = T * top_k;
+  OptT b;
+  if (bias.has_value()) {
+    require_device(*bias, "bias");
+    if (bias->dim() != 1 || bias->numel() != E)
+      throw py::value_error("cvmm_route_scored: bias must hold one value per expert");
+    b = bias->to(at::kFloat).contiguous();
+  }
+  Tensor w = at::empty({T, top_k}, opts(l, at::kFloat));
+  Tensor sel = at::empty({T, top_k}, opts(l, at::kLong));
+  Tensor i32 = at::empty({2 * R}, opts(l, at::kInt));
+  // (no tokens: no launch writes the offsets)
+  Tensor i64 = T > 0 ? at::empty({2 * R + E}, opts(l, at::kLong)) : at::zeros({E}, opts(l, at::kLong));
+  Tensor ssel = i32.narrow(0, 0, R), pos = i32.narrow(0, R, R);
+  Tensor perm = i64.narrow(0, 0, R), tok = i64.narrow(0, R, R), off = i64.narrow(0, 2 * R, E);
+  const size_t ws_bytes = cvmm_route_topk_workspace_bytes(T, (int32_t)E, top_k);
+  Tensor ws = sort_workspace(l, stream, ws_bytes);
+  check(cvmm_route_scored(ptr(l), dtype_id(l.scalar_type()), T, std::max(l.stride(0), E), (int32_t)E, top_k,
+                          tptr<float>(b), (int32_t)scores, (int32_t)groups, (int32_t)topk_groups, renormalize ? 1 : 0,
+                          scale, tptr<float>(w), tptr<int64_t>(sel), tptr<int32_t>(ssel), tptr<int64_t>(perm),
+                          tptr<int64_t>(tok), tptr<int64_t>(off), tptr<int32_t>(pos), ptr(ws), (size_t)ws.numel(),
+                          (void*)stream),
+        "cvmm_route_scored");
+  return {w, sel, ssel, perm, tok, off, pos};
+}
+
+Tensor route_scored_backward(const Tensor& logits, const Tensor& sel, const Tensor& grad_weights, int64_t top_k,
+                             int64_t scores, bool renormalize, double scale, int64_t stream) {
+  require_device(logits, "logits");
+  Tensor l = logits.reshape({-1, logits.size(-1)});
+  if (l.stride(-1) != 1 || (l.size(0) > 1 && l.stride(0) < l.size(1))) l = l.contiguous();
+  const int64_t T = l.size(0), E = l.size(1);
+  Tensor s = sel.reshape({-1}).contiguous();
+  Tensor g = grad_weights.reshape({-1}).to(at::kFloat).contiguous();
+  if (s.numel() != T * top_k || g.numel() != T * top_k)
+    throw py::value_error("cvmm_route_scored: sel / grad have the wrong size");
+  Tensor out = at::empty({T, E}, opts(l, l.scalar_type()));
+  check(cvmm_route_scored_backward(ptr(l), dtype_id(l.scalar_type()), T, std::max(l.stride(0), E), (int32_t)E, top_k,
+                                   (int32_t)scores, renormalize ? 1 : 0, scale, tptr<int64_t>(s), tptr<float>(g),
+                                   ptr(out), E, (void*)stream),
+        "cvmm_route_scored_backward");
+  return out.view(logits.sizes());
+}
+
 // The int32 copy of the ids cvmm_prepare_sel2 takes (cvmm.py:1796), in the
 // ids' shape.
 Tensor copy_ids(const Tensor& sel, int64_t stream) {
@@ -771,6 +823,202 @@ struct CvmmFunction : public torch::autograd::Function<CvmmFunction> {
   }
 };
 
+// ---------------------------------------------------------------------------
+// microscaled 4-bit values (no counterpart in cvmm.py)
+// ---------------------------------------------------------------------------
+// Float tensors other than fp32, fp16 and bf16 are widened to fp32.
+Tensor mx4_source(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: case at::kHalf: case at::kBFloat16: return t;
+    default: return t.to(at::kFloat);
+  }
+}
+
+// Blocks along the last dimension: (codes [rows, bytes], scales [rows, bytes]).
+std::tuple<Tensor, Tensor> mx4_quantize_rows(const Tensor& t, int64_t stream) {
+  require_device(t, "t");
+  const int64_t d = t.size(-1);
+  Tensor f = rows_of(mx4_source(t), d);
+  const int64_t rows = f.size(0);
+  Tensor codes = at::empty({rows, (int64_t)cvmm_mx4_rows_bytes(1, d, 0)}, opts(t, at::kByte));
+  Tensor scales = at::empty({rows, (int64_t)cvmm_mx4_rows_bytes(1, d, 1)}, opts(t, at::kByte));
+  check(cvmm_mx4_quantize_rows(ptr(f), dtype_id(f.scalar_type()), f.stride(0), rows, d, ptr(codes), ptr(scales),
+                               (void*)stream),
+        "cvmm_mx4_quantize");
+  return {codes, scales};
+}
+
+// Expert weights [E, d_in, d_out] of any strides, blocks along d_in.
+std::tuple<Tensor, Tensor> mx4_quantize_keys(const Tensor& t, int64_t stream) {
+  require_device(t, "t");
+  const int64_t E = t.size(0), d_in = t.size(1), d_out = t.size(2);
+  Tensor k = mx4_source(t);
+  Tensor codes = at::empty({E, (int64_t)cvmm_mx4_keys_bytes(1, d_in, d_out, 0)}, opts(t, at::kByte));
+  Tensor scales = at::empty({E, (int64_t)cvmm_mx4_keys_bytes(1, d_in, d_out, 1)}, opts(t, at::kByte));
+  check(cvmm_mx4_quantize_keys(ptr(k), dtype_id(k.scalar_type()), (int32_t)E, d_in, d_out, k.stride(0), k.stride(1),
+                               k.stride(2), ptr(codes), ptr(scales), (void*)stream),
+        "cvmm_mx4_quantize");
+  return {codes, scales};
+}
+
+Tensor mx4_dequantize(const Tensor& codes, const Tensor& scales, const std::vector<int64_t>& shape, bool keys,
+                      int64_t dtype, int64_t stream) {
+  require_device(codes, "codes");
+  require_device(scales, "scales");
+  Tensor out = at::empty(shape, opts(codes, dtype_of(dtype)));
+  if (out.numel() == 0) return out;
+  if (keys)
+    check(cvmm_mx4_dequantize_keys(ptr(codes), ptr(scales), (int32_t)shape[0], shape[1], shape[2], ptr(out),
+                                   (int32_t)dtype, (void*)stream),
+          "cvmm_mx4_dequantize");
+  else
+    check(cvmm_mx4_dequantize_rows(ptr(codes), ptr(scales), out.numel() / shape.back(), shape.back(), ptr(out),
+                                   (int32_t)dtype, (void*)stream),
+          "cvmm_mx4_dequantize");
+  return out;
+}
+
+bool mx4_copied(const Tensor& rows, int64_t width) {
+  return width % 8 != 0 || rows.stride(0) % 8 != 0 || (reinterpret_cast<uintptr_t>(rows.data_ptr()) & 15) != 0;
+}
+
+// The 4-bit weights of a call: buffers of the sizes the library lays out.
+void mx4_check_keys(const Tensor& codes, const Tensor& scales, int64_t E, int64_t d_in, int64_t d_out) {
+  require_device(codes, "keys");
+  require_device(scales, "keys");
+  if (codes.scalar_type() != at::kByte || scales.scalar_type() != at::kByte || !codes.is_contiguous() ||
+      !scales.is_contiguous() || (size_t)codes.numel() != cvmm_mx4_keys_bytes(E, d_in, d_out, 0) ||
+      (size_t)scales.numel() != cvmm_mx4_keys_bytes(E, d_in, d_out, 1) ||
+      (reinterpret_cast<uintptr_t>(codes.data_ptr()) & 15) != 0 || (reinterpret_cast<uintptr_t>(scales.data_ptr()) & 3) != 0)
+    throw py::value_error("cvmm_mx4: codes and scales are not those of the weights' shape");
+}
+
+// y (cvmm_forward_impl with 4-bit weights): [R or R / k, d_out] in the op dtype.
+Tensor mx4_forward(const Tensor& x, const Tensor& codes, const Tensor& scales, int64_t d_in, int64_t d_out,
+                   const Tensor& sel_index, const OptT& out_index, const Tensor& offsets, const OptT& route_pos,
+                   const OptT& rw, int64_t op_id, bool quantize_input, int64_t stream) {
+  require_device(x, "x");
+  require_device(sel_index, "sel_index");
+  const auto op = dtype_of(op_id);
+  const int64_t E = offsets.numel();
+  mx4_check_keys(codes, scales, E, d_in, d_out);
+  if (x.size(-1) != d_in) throw py::value_error("cvmm_mx4: x.shape[-1] must equal the weights' d_in");
+  Tensor xf = rows_of(x.scalar_type() == op ? x : x.to(op), d_in);
+  Tensor si = as_i64(sel_index);
+  OptT oi = as_i64(out_index);
+  const int64_t R = si.numel();
+  if (oi.has_value() && oi->numel() != R)
+    throw py::value_error("cvmm_mx4: sel_index/out_index must have one entry per route");
+  OptT rwf;
+  int64_t k = 1;
+  if (rw.has_value()) {
+    require_device(*rw, "reduction_weight");
+    if (rw->numel() != R || rw->dim() < 1)
+      throw py::value_error("cvmm_mx4: reduction_weight must have one entry per route");
+    k = std::max<int64_t>(rw->size(-1), 1);
+    rwf = rw->reshape({-1}).to(at::kFloat).contiguous();
+  }
+  const int64_t rows = R / k;
+  Tensor out = at::empty({rows, d_out}, opts(x, op));
+  if (R == 0) return out;
+  const size_t ws_bytes = cvmm_mx4_fwd_workspace_bytes(R, d_in, d_out, xf.size(0), rwf.has_value() ? 1 : 0,
+                                                       route_pos.has_value() ? 1 : 0, mx4_copied(xf, d_in) ? 1 : 0,
+                                                       quantize_input ? 1 : 0);
+  OptT ws;
+  if (ws_bytes) ws = at::empty({(int64_t)ws_bytes}, opts(x, at::kByte));
+  check(cvmm_mx4_fwd(ptr(xf), (int32_t)op_id, xf.size(0), xf.stride(0), ptr(codes), ptr(scales), (int32_t)E, d_in,
+                     d_out, tptr<int64_t>(si), tptr<int64_t>(oi), R, tptr<int64_t>(offsets),
+                     tptr<int32_t>(route_pos), tptr<float>(rwf), k, quantize_input ? 1 : 0, ptr(out), rows, d_out,
+                     ptr(ws), ws_bytes, (void*)stream),
+        "cvmm_mx4");
+  return out;
+}
+
+// (grad_x, grad_reduction_weight) for frozen 4-bit weights.
+std::tuple<OptT, OptT> mx4_backward(const Tensor& grad_output, const Tensor& x, const Tensor& codes,
+                                    const Tensor& scales, int64_t d_in, int64_t d_out, const Tensor& sel_index,
+                                    const OptT& out_index, const Tensor& offsets, const OptT& route_pos,
+                                    const OptT& rw, int64_t top_k, int64_t op_id, bool need_grad_x,
+                                    bool need_grad_rw, int64_t stream) {
+  const auto op = dtype_of(op_id);
+  const int64_t E = offsets.numel(), R = sel_index.numel();
+  const int64_t k = rw.has_value() ? std::max<int64_t>(rw->size(-1), 1) : std::max<int64_t>(top_k, 1);
+  Tensor g = rows_of(grad_output.scalar_type() == op ? grad_output : grad_output.to(op), d_out);
+  Tensor si = as_i64(sel_index);
+  OptT oi = as_i64(out_index);
+  OptT rwf, gx, grw;
+  if (rw.has_value()) rwf = rw->reshape({-1}).to(at::kFloat).contiguous();
+  // x in fp32 or the op type (the product's own rows are x in the op type)
+  Tensor xr = rows_of(x.scalar_type() == op ? x : x.to(op), d_in);
+  const auto gx_type = x.scalar_type() == op ? op : at::kFloat;
+  if (need_grad_x) gx = at::empty(xr.sizes(), opts(x, gx_type));
+  if (need_grad_rw) grw = at::empty({R}, opts(x, at::kFloat));
+  if (R > 0) {
+    const size_t ws_bytes = cvmm_mx4_bwd_x_workspace_bytes(R, d_in, d_out, g.size(0), need_grad_x && oi.has_value() ? 1 : 0,
+                                                           route_pos.has_value() ? 1 : 0, mx4_copied(g, d_out) ? 1 : 0,
+                                                           need_grad_rw ? 1 : 0, dtype_id(gx_type));
+    OptT ws;
+    if (ws_bytes) ws = at::empty({(int64_t)ws_bytes}, opts(x, at::kByte));
+    check(cvmm_mx4_bwd_x(ptr(g), (int32_t)op_id, g.size(0), g.stride(0), ptr(codes), ptr(scales), (int32_t)E, d_in,
+                         d_out, tptr<int64_t>(si), tptr<int64_t>(oi), R, tptr<int64_t>(offsets),
+                         tptr<int32_t>(route_pos), tptr<float>(rwf), k, ptr(xr), (int32_t)op_id, xr.size(0),
+                         xr.stride(0), ptr(gx), dtype_id(gx_type), gx.has_value() ? gx->size(0) : 0, d_in,
+                         tptr<float>(grw), ptr(ws), ws_bytes, (void*)stream),
+          "cvmm_mx4 backward");
+  } else if (gx.has_value()) {
+    gx->zero_();
+  }
+  if (gx.has_value()) gx = gx->to(x.scalar_type()).view(x.sizes());
+  if (grw.has_value()) grw = grw->to(rw->scalar_type()).view(rw->sizes());
+  return {gx, grw};
+}
+
+struct CvmmMx4Function : public torch::autograd::Function<CvmmMx4Function> {
+  // x and reduction_weight (optional) are the differentiable inputs
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const OptT& rw, const Tensor& codes,
+                        const Tensor& scales, int64_t d_in, int64_t d_out, const Tensor& sel_index,
+                        const OptT& out_index, const Tensor& offsets, const OptT& route_pos, int64_t top_k,
+                        int64_t op_id, const std::vector<int64_t>& out_shape) {
+    const bool need_x = x.requires_grad(), need_rw = rw.has_value() && rw->requires_grad();
+    ctx->saved_data["d_in"] = d_in;
+    ctx->saved_data["d_out"] = d_out;
+    ctx->saved_data["top_k"] = top_k;
+    ctx->saved_data["op_id"] = op_id;
+    ctx->saved_data["need"] = (int64_t)((need_x ? 1 : 0) | (need_rw ? 2 : 0));
+    Tensor out = mx4_forward(x, codes, scales, d_in, d_out, sel_index, out_index, offsets, route_pos, rw, op_id, false,
+                             current_stream(x));
+    ctx->save_for_backward({x, opt_or_undef(rw), codes, scales, sel_index, opt_or_undef(out_index), offsets,
+                            opt_or_undef(route_pos)});
+    return at::_unsafe_view(out, out_shape);
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto v = ctx->get_saved_variables();
+    const int64_t need = ctx->saved_data["need"].toInt();
+    auto [gx, grw] = mx4_backward(grads[0], v[0], v[2], v[3], ctx->saved_data["d_in"].toInt(),
+                                  ctx->saved_data["d_out"].toInt(), v[4], undef_or_opt(v[5]), v[6],
+                                  undef_or_opt(v[7]), undef_or_opt(v[1]), ctx->saved_data["top_k"].toInt(),
+                                  ctx->saved_data["op_id"].toInt(), (need & 1) != 0, (need & 2) != 0,
+                                  current_stream(v[0]));
+    // one entry per forward argument
+    return {opt_or_undef(gx), opt_or_undef(grw), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(),
+            Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor mx4_apply(const Tensor& x, const OptT& rw, const Tensor& codes, const Tensor& scales, int64_t d_in,
+                 int64_t d_out, const Tensor& sel_index, const OptT& out_index, const Tensor& offsets,
+                 const OptT& route_pos, int64_t top_k, int64_t op_id, bool quantize_input, bool grad,
+                 const std::vector<int64_t>& out_shape) {
+  if (!grad)
+    return mx4_forward(x, codes, scales, d_in, d_out, sel_index, out_index, offsets, route_pos, rw, op_id,
+                       quantize_input, current_stream(x))
+        .view(out_shape);
+  return CvmmMx4Function::apply(x, rw, codes, scales, d_in, d_out, sel_index, out_index, offsets, route_pos, top_k,
+                                op_id, out_shape);
+}
+
 // The Python-facing forward and backward (torch.compile's ops): no kept rows.
 Tensor forward_py(const Tensor& x, const Tensor& keys, const OptT& keys_op, bool keys_op_is_t, const Tensor& sel,
                   const Tensor& sel_index, const OptT& out_index, const Tensor& offsets, const OptT& route_pos,
@@ -809,6 +1057,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("route_topk", &route_topk, py::arg("logits"), py::arg("top_k"), py::arg("renormalize"), py::arg("stream"));
   m.def("route_topk_backward", &route_topk_backward, py::arg("logits"), py::arg("sel"), py::arg("grad_weights"),
         py::arg("top_k"), py::arg("renormalize"), py::arg("stream"));
+  m.def("route_scored", &route_scored, py::arg("logits"), py::arg("top_k"), py::arg("bias"), py::arg("scores"),
+        py::arg("groups"), py::arg("topk_groups"), py::arg("renormalize"), py::arg("scale"), py::arg("stream"));
+  m.def("route_scored_backward", &route_scored_backward, py::arg("logits"), py::arg("sel"), py::arg("grad_weights"),
+        py::arg("top_k"), py::arg("scores"), py::arg("renormalize"), py::arg("scale"), py::arg("stream"));
   m.def("sort_routes_cast", &sort_routes_cast, py::arg("raw"), py::arg("n_experts"), py::arg("top_k"),
         py::arg("keys"), py::arg("op_id"), py::arg("want_t"), py::arg("want_n"), py::arg("layout"),
         py::arg("stream"), py::arg("counted_ws") = py::none());
@@ -820,6 +1072,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gelu_backward", &gelu_backward, py::arg("grad"), py::arg("pre_act"), py::arg("stream"));
   m.def("backward", &backward_py);
   m.def("cvmm_apply", &cvmm_apply);
+  m.def("mx4_quantize_rows", &mx4_quantize_rows);
+  m.def("mx4_quantize_keys", &mx4_quantize_keys);
+  m.def("mx4_dequantize", &mx4_dequantize);
+  m.def("mx4_forward", &mx4_forward);
+  m.def("mx4_backward", &mx4_backward);
+  m.def("mx4_apply", &mx4_apply);
   // operand rules, exposed for tests
   m.def("storage_for", [](const Tensor& t, int64_t op_id) { return storage_for(t, dtype_of(op_id)); });
   m.def("keys_view", &keys_view);

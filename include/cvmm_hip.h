@@ -274,6 +274,28 @@ int cvmm_route_topk_backward(const void* logits, int32_t logits_dtype, int64_t n
                              int32_t n_experts, int64_t top_k, int32_t renormalize, const int64_t* sel,
                              const float* grad_weights, void* grad_logits, int64_t grad_ld, void* stream);
 
+/* Router of balanced MoE models (no counterpart in cvmm.py).  scores s =
+ * sigmoid(logits) or softmax(logits); the choice goes by s + bias (bias: fp32
+ * [E], or NULL); the experts stand in `groups` runs of E / groups, of which the
+ * topk_groups with the greatest sum of their two best biased scores stay; the
+ * top_k best remaining experts are chosen (ties to the lower id).  weights =
+ * scale * s at the chosen experts, divided by their sum if renormalize.  Scores
+ * and comparisons are 64-bit.  Outputs and workspace as cvmm_route_topk's
+ * (cvmm_route_topk_workspace_bytes); at most 64 groups unless all stay. */
+#define CVMM_SCORES_SOFTMAX 0
+#define CVMM_SCORES_SIGMOID 1
+int cvmm_route_scored(const void* logits, int32_t logits_dtype, int64_t n_tokens, int64_t logits_ld,
+                      int32_t n_experts, int64_t top_k, const float* bias, int32_t scores, int32_t groups,
+                      int32_t topk_groups, int32_t renormalize, double scale, float* weights, int64_t* sel,
+                      int32_t* sorted_sel, int64_t* perm, int64_t* token_index, int64_t* offsets,
+                      int32_t* route_pos, void* workspace, size_t workspace_bytes, void* stream);
+/* Its backward: the logits' gradient (logits dtype) of the weights' gradient
+ * (the choice itself has none, nor has the bias). */
+int cvmm_route_scored_backward(const void* logits, int32_t logits_dtype, int64_t n_tokens, int64_t logits_ld,
+                               int32_t n_experts, int64_t top_k, int32_t scores, int32_t renormalize, double scale,
+                               const int64_t* sel, const float* grad_weights, void* grad_logits, int64_t grad_ld,
+                               void* stream);
+
 /* out[i] = the int32 value of id i (int64 ids: their low 32 bits), n ids:
  * the `fsel = sel.flatten().to(torch.int32)` copy cvmm_prepare_sel2 takes
  * (cvmm.py:1796), which fixes the routing when the selector is prepared. */
@@ -485,6 +507,55 @@ int cvmm_bwd_w_rows(const void* x, int32_t x_dtype, int64_t x_rows, int64_t x_ld
                     int32_t op_dtype, void* grad_keys, int32_t grad_keys_dtype, int64_t gk_se, int64_t gk_si,
                     int64_t gk_sj, int32_t flags, void* rows, size_t rows_bytes, void* workspace,
                     size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Microscaled 4-bit values: blocks of 32 share a scale 2^s, s = floor(log2
+ * max|v|) - 2 (a byte s + 127; 255: the block holds a NaN or an infinity and
+ * comes back as NaN), each value the nearest of +-{0, .5, 1, 1.5, 2, 3, 4, 6}
+ * * 2^s, ties to the even code, the largest beyond.  Two layouts, both opaque
+ * to the caller: rows [rows][d] in blocks along d (activations), keys
+ * [E][d_in][d_out] in blocks along d_in (expert weights).  The *_bytes queries
+ * give the sizes of the codes (scales = 0) and of the scales (scales = 1). */
+size_t cvmm_mx4_rows_bytes(int64_t rows, int64_t d, int32_t scales);
+size_t cvmm_mx4_keys_bytes(int64_t n_experts, int64_t d_in, int64_t d_out, int32_t scales);
+int cvmm_mx4_quantize_rows(const void* src, int32_t dtype, int64_t ld, int64_t rows, int64_t d, void* codes,
+                           void* scales, void* stream);
+int cvmm_mx4_quantize_keys(const void* keys, int32_t keys_dtype, int32_t n_experts, int64_t d_in, int64_t d_out,
+                           int64_t k_se, int64_t k_si, int64_t k_sj, void* codes, void* scales, void* stream);
+/* Back to values: out is contiguous, [rows][d] or [E][d_in][d_out]. */
+int cvmm_mx4_dequantize_rows(const void* codes, const void* scales, int64_t rows, int64_t d, void* out, int32_t dtype,
+                             void* stream);
+int cvmm_mx4_dequantize_keys(const void* codes, const void* scales, int32_t n_experts, int64_t d_in, int64_t d_out,
+                             void* out, int32_t dtype, void* stream);
+
+/* cvmm_fwd with 4-bit weights in the keys layout.  x: 16-bit rows, which is
+ * also the output's type; quantize_input != 0: the rows are quantised to 4-bit
+ * values first (rows layout, in the workspace) and multiplied as such.
+ * reduction_weight (fp32, or NULL): the weighted sum over each token's
+ * reduce_k routes, summed in fp32.  Rows of routes with an expert id outside
+ * [0, E) are zero.  x_copied of the workspace query: the rows are not made of
+ * aligned 16-byte pieces (d_in or x_ld no multiple of 8, or x not aligned). */
+size_t cvmm_mx4_fwd_workspace_bytes(int64_t n_routes, int64_t d_in, int64_t d_out, int64_t x_rows, int32_t weighted,
+                                    int32_t have_route_pos, int32_t x_copied, int32_t quantize_input);
+int cvmm_mx4_fwd(const void* x, int32_t x_dtype, int64_t x_rows, int64_t x_ld, const void* codes, const void* scales,
+                 int32_t n_experts, int64_t d_in, int64_t d_out, const int64_t* sel_index, const int64_t* out_index,
+                 int64_t n_routes, const int64_t* offsets, const int32_t* route_pos, const float* reduction_weight,
+                 int64_t reduce_k, int32_t quantize_input, void* out, int64_t out_rows, int64_t out_ld,
+                 void* workspace, size_t workspace_bytes, void* stream);
+
+/* Its backward for frozen weights: grad_x (op dtype or fp32; NULL: not
+ * wanted) and grad_rw (fp32, one per route; NULL: not wanted).  grad: one row
+ * per route, or per token of a weighted selection, in the op dtype.  With
+ * out_index (token input) grad_x sums each token's top_k routes. */
+size_t cvmm_mx4_bwd_x_workspace_bytes(int64_t n_routes, int64_t d_in, int64_t d_out, int64_t grad_rows,
+                                      int32_t token_input, int32_t have_route_pos, int32_t grad_copied,
+                                      int32_t need_grad_rw, int32_t grad_x_dtype);
+int cvmm_mx4_bwd_x(const void* grad, int32_t op_dtype, int64_t grad_rows, int64_t grad_ld, const void* codes,
+                   const void* scales, int32_t n_experts, int64_t d_in, int64_t d_out, const int64_t* sel_index,
+                   const int64_t* out_index, int64_t n_routes, const int64_t* offsets, const int32_t* route_pos,
+                   const float* reduction_weight, int64_t top_k, const void* x, int32_t x_dtype, int64_t x_rows,
+                   int64_t x_ld, void* grad_x, int32_t grad_x_dtype, int64_t grad_x_rows, int64_t grad_x_ld,
+                   float* grad_rw, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
