@@ -39,9 +39,61 @@ struct Mx4Params {
   const uint8_t* a_scales;  // 4-bit rows: 16 bytes per 512 values
   int64_t a_bytes;          // 4-bit rows: code bytes of a row
   int64_t a_groups;
+  int32_t passes;           // 4-bit rows: column tiles per workgroup
+  FastDiv a_div;            // input gradient: routes per row of A
   int32_t pieces;           // output rows not made of whole aligned 16-byte pieces
   int32_t dg_vec;           // x rows of the routing-weight gradient in 8-byte pieces
 };
+
+// The tile's rows: A row and output row of each, -1 for none (indices below
+// 2^31; the general metadata divides in 64 bits).
+template <int BM, int NT>
+__device__ __forceinline__ void mx4_route_meta(const Mx4Params& p, RouteMeta<BM>& m) {
+  const GemmParams& g = p.g;
+  for (int r = threadIdx.x; r < BM; r += NT) {
+    int64_t a = -1, o = -1, wi = -1, d = -1;
+    float w = 1.f;
+    if (r < m.rows) {
+      const int64_t q = m.row0 + r;
+      a = g.a_idx[q];
+      o = g.o_idx != nullptr ? g.o_idx[q] : q;
+      wi = g.w_idx[q];
+      if (g.dg != nullptr) d = g.dg_x_idx[q];
+      a = a < 0 || a >= g.n_routes ? -1 : p.a_div.div(a);
+      if (a >= g.a_rows) a = -1;
+      if (o < 0 || o >= g.out_rows) o = -1;
+      if (wi < 0 || wi >= g.n_routes) wi = -1;
+      if (d < 0 || d >= g.dg_x_rows) d = -1;
+      if (g.w != nullptr && wi >= 0) w = static_cast<const float*>(g.w)[wi];
+    }
+    m.arow[r] = a;
+    m.orow[r] = o;
+    m.widx[r] = wi;
+    m.dgrow[r] = d;
+    m.w[r] = w;
+  }
+  __syncthreads();
+}
+template <int BM>
+struct Mx4Rows {
+  int32_t a[BM], o[BM];
+};
+template <int BM, int NT>
+__device__ __forceinline__ void mx4_rows(const GemmParams& g, const RouteMeta<BM>& m, Mx4Rows<BM>& rows) {
+  for (int r = threadIdx.x; r < BM; r += NT) {
+    int64_t a = -1, o = -1;
+    if (r < m.rows) {
+      const int64_t q = m.row0 + r;
+      a = g.a_idx[q];
+      o = g.o_idx != nullptr ? g.o_idx[q] : q;
+      if (a < 0 || a >= g.a_rows) a = -1;
+      if (o < 0 || o >= g.out_rows) o = -1;
+    }
+    rows.a[r] = (int32_t)a;
+    rows.o[r] = (int32_t)o;
+  }
+  __syncthreads();
+}
 
 // acc[i][j] of lane (fr, fq): row j * 16 + fr, columns 16 i + 4 fq .. + 4 of
 // the wave's 64.  Two lane swaps make 8 consecutive columns, one 16-byte store.
@@ -124,30 +176,33 @@ __global__ __launch_bounds__(NW * 64, OCC) void mx4_gemm_kernel(const Mx4Params 
   __shared__ __attribute__((aligned(1024))) char stage0[Cfg::A_BYTES];
   __shared__ __attribute__((aligned(1024))) char stage1[Cfg::A_BYTES];
   __shared__ RouteMeta<BM> meta;
+  __shared__ Mx4Rows<BM> rows;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t n_ntiles = (g.N + BN - 1) / BN;
-  const bool tiled = gemm_schedule<BM, Cfg::NT>(g, n_ntiles, meta);
+  const bool tiled = gemm_schedule_tile<BM>(g, n_ntiles, meta);
   const int64_t n0 = (int64_t)uniform_i32(meta.group) * BN;
   if (!tiled) {
     zero_unrouted_cols<BM, Cfg::NT>(g, meta, gridDim.x / n_ntiles, n0, n0 + BN, -1);
     return;
   }
+  mx4_rows<BM, Cfg::NT>(g, meta, rows);
   const int32_t expert = uniform_i32(meta.expert);
   const char* zero = reinterpret_cast<const char*>(g_cvmm_zero_page);
-  const char* src[Cfg::D];
-  int kc[Cfg::D];
+  // DMA instruction j of this wave fills 4 rows of 16 pieces
+  const int r0 = wave * Cfg::D * 4 + (lane >> 4), kl = (lane & 15) ^ (lane >> 4);
+  auto issue = [&](int s, char* buf) {
+    int l = kl, rr = r0;
+    asm volatile("" : "+v"(l), "+v"(rr));  // (addresses made here, not kept over the loop)
+    int32_t ar[Cfg::D];
 #pragma unroll
-  for (int j = 0; j < Cfg::D; ++j) {
-    const int q = (wave * Cfg::D + j) * 64 + lane, row = q / 16;
-    kc[j] = ((q % 16) ^ (row & 15)) * 8;
-    const int64_t ar = meta.arow[row];
-    src[j] = ar >= 0 ? reinterpret_cast<const char*>(g.a) + (ar * g.a_ld + kc[j]) * 2 : nullptr;
-  }
-  auto issue = [&](int64_t s, char* buf) {
-    const int64_t k0 = s * 128;
+    for (int j = 0; j < Cfg::D; ++j) ar[j] = rows.a[rr + 4 * j];
 #pragma unroll
-    for (int j = 0; j < Cfg::D; ++j)
-      dma16(src[j] != nullptr && k0 + kc[j] < g.K ? src[j] + k0 * 2 : zero, buf + (wave * Cfg::D + j) * 1024);
+    for (int j = 0; j < Cfg::D; ++j) {
+      // piece (lane & 15) ^ (row & 15), row = r0 + 4 j
+      const int64_t k = (int64_t)s * 128 + (l ^ ((4 * (wave * Cfg::D + j)) & 15)) * 8;
+      const char* row = reinterpret_cast<const char*>(g.a) + ((int64_t)ar[j] * g.a_ld + k) * 2;
+      dma16(ar[j] >= 0 && k < g.K ? row : zero, buf + (wave * Cfg::D + j) * 1024);
+    }
   };
   const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
   const int fr = lane & 15, fq = lane >> 4;
@@ -164,74 +219,97 @@ __global__ __launch_bounds__(NW * 64, OCC) void mx4_gemm_kernel(const Mx4Params 
     for (int j = 0; j < MB; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   uint4 w0[4], w1[4];
   uint32_t s0, s1;
-  auto load_w = [&](int64_t s, uint4 (&w)[4], uint32_t& sc) {
+  auto load_w = [&](uint4 (&w)[4], uint32_t& sc) {  // the next panel
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint4*>(cp + s * kMx4PanelCodes + i * 1024);
-    sc = *reinterpret_cast<const uint32_t*>(sp + s * kMx4PanelScales);
+    for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint4*>(cp + i * 1024);
+    sc = *reinterpret_cast<const uint32_t*>(sp);
+    cp += kMx4PanelCodes;
+    sp += kMx4PanelScales;
+    issue_fence();
   };
+  // row wm * WR + 16 j + fr, chunk 4 fq + m, at chunk ^ fr
+  const int a_at = (wm * Cfg::WR + fr) * 256 + (((4 * fq) ^ fr) << 4);
   auto multiply = [&](const char* buf, const uint4 (&w)[4], uint32_t sc) {
     float scale[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) scale[i] = mx4_scale((sc >> (8 * i)) & 255u);
+    int at = a_at;
+    asm volatile("" : "+v"(at));
+    uint4 a[2][MB];
+    auto read = [&](int m) {
+#pragma unroll
+      for (int j = 0; j < MB; ++j) a[m & 1][j] = *reinterpret_cast<const uint4*>(buf + (at ^ (m << 4)) + j * 16 * 256);
+    };
+    read(0);
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
-      uint4 a[MB];
-#pragma unroll
-      for (int j = 0; j < MB; ++j) {
-        const int ra = wm * Cfg::WR + j * 16 + fr;
-        a[j] = *reinterpret_cast<const uint4*>(buf + ra * 256 + (((4 * fq + m) ^ (ra & 15)) << 4));
-      }
+      if (m < 3) read(m + 1);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t c = m == 0 ? w[i].x : m == 1 ? w[i].y : m == 2 ? w[i].z : w[i].w;
         const uint4 b = mx4_unpack8<OpT>(c, scale[i]);
 #pragma unroll
-        for (int j = 0; j < MB; ++j) MfmaOp<OpT>::step(acc[i][j], b, a[j]);
+        for (int j = 0; j < MB; ++j) MfmaOp<OpT>::step(acc[i][j], b, a[m & 1][j]);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
-  // slice s: everything it needs was requested a whole slice ago
-  issue(0, stage0);
-  load_w(0, w0, s0);
-  for (int64_t s = 0; s < p.kp; s += 2) {
+  // slice s: everything it needs was requested a whole slice ago.  Slices go in
+  // pairs, an odd one first: a loop left in the middle held two sets of sums.
+  const int kp = (int)p.kp;
+  int s = kp & 1;
+  if (s) {
+    issue(0, stage1);
+    load_w(w1, s1);
     vm_wait<0>();
     wg_barrier();
-    if (s + 1 < p.kp) {
-      issue(s + 1, stage1);
-      load_w(s + 1, w1, s1);
+    if (kp > 1) {
+      issue(1, stage0);
+      load_w(w0, s0);
     }
-    multiply(stage0, w0, s0);
-    if (s + 1 >= p.kp) break;
+    multiply(stage1, w1, s1);
+  } else {
+    issue(0, stage0);
+    load_w(w0, s0);
+  }
+  for (; s < kp; s += 2) {
     vm_wait<0>();
     wg_barrier();
-    if (s + 2 < p.kp) {
+    issue(s + 1, stage1);
+    load_w(w1, s1);
+    multiply(stage0, w0, s0);
+    vm_wait<0>();
+    wg_barrier();
+    if (s + 2 < kp) {
       issue(s + 2, stage0);
-      load_w(s + 2, w0, s0);
+      load_w(w0, s0);
     }
     multiply(stage1, w1, s1);
   }
   mx4_store<OpT, MB>(p, acc, nwave, fr, fq, [&](int j, float& w) {
     w = 1.f;
-    return meta.orow[wm * Cfg::WR + j * 16 + fr];
+    return (int64_t)rows.o[wm * Cfg::WR + j * 16 + fr];
   });
 }
 
-// Few routes per expert: 16-row tiles of one panel column, K split over the
-// waves, every operand straight to registers; the partial tiles are added in
-// wave order through LDS (deterministic).
+// Few tiles: 16 rows x 64 columns, every operand straight to registers.  Each of
+// the NW waves takes a part of K; the partial tiles are added in wave order
+// through LDS (deterministic).  A wave requests its first four panels before the
+// route rows are known, and each further one as soon as its registers are free.
 template <typename OpT, int NW>
 __global__ __launch_bounds__(NW * 64) void mx4_decode_kernel(const Mx4Params p) {
-  constexpr int NT = NW * 64;
+  constexpr int NT = NW * 64, BN = 64;
   const GemmParams& g = p.g;
   __shared__ __attribute__((aligned(16))) float part[NW][16][68];
   __shared__ RouteMeta<16> meta;
+  __shared__ Mx4Rows<16> rows;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int fr = lane & 15, fq = lane >> 4;
   const int64_t n_ntiles = p.np;
   const bool tiled = gemm_schedule_tile<16>(g, n_ntiles, meta);
-  const int64_t pn = uniform_i32(meta.group), n0 = pn * 64;
+  const int64_t pn = uniform_i32(meta.group), n0 = pn * BN;
   if (!tiled) {
-    zero_unrouted_cols<16, NT>(g, meta, gridDim.x / n_ntiles, n0, n0 + 64, -1);
+    zero_unrouted_cols<16, NT>(g, meta, gridDim.x / n_ntiles, n0, n0 + BN, -1);
     return;
   }
   const int32_t expert = uniform_i32(meta.expert);
@@ -241,53 +319,47 @@ __global__ __launch_bounds__(NW * 64) void mx4_decode_kernel(const Mx4Params p) 
   // this wave's panels
   const int kp = (int)p.kp, per = (kp + NW - 1) / NW;
   const int b0 = wave * per, b1 = b0 + per < kp ? b0 + per : kp;
-  auto load_w = [&](int s, uint4 (&w)[4], uint32_t& sc) {
+  uint4 w[4][4], a[2][4];
+  uint32_t sc[4];
+  auto load_w = [&](int k, int set) {
+    if (k >= b1) return;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint4*>(cp + s * kMx4PanelCodes + i * 1024);
-    sc = *reinterpret_cast<const uint32_t*>(sp + s * kMx4PanelScales);
+    for (int i = 0; i < 4; ++i) w[set][i] = *reinterpret_cast<const uint4*>(cp + (int64_t)k * kMx4PanelCodes + i * 1024);
+    sc[set] = *reinterpret_cast<const uint32_t*>(sp + (int64_t)k * kMx4PanelScales);
   };
-  uint4 w0[4], w1[4], a0[4], a1[4];
-  uint32_t s0 = 0, s1 = 0;
-  // the first weights are requested before the route rows are known
-  if (b0 < b1) load_w(b0, w0, s0);
-  gemm_route_meta<16, NT>(g, meta);
-  const int64_t ar = meta.arow[fr];
-  const char* arow = ar >= 0 ? static_cast<const char*>(g.a) + ar * g.a_ld * 2 : nullptr;
-  auto load_a = [&](int s, uint4 (&a)[4]) {
+#pragma unroll
+  for (int u = 0; u < 4; ++u) load_w(b0 + u, u);
+  mx4_rows<16, NT>(g, meta, rows);
+  const int32_t ar = rows.a[fr];
+  const char* arow = static_cast<const char*>(g.a) + ((int64_t)(ar >= 0 ? ar : 0) * g.a_ld + fq * 32) * 2;
+  auto load_a = [&](int k, int set) {
 #pragma unroll
     for (int m = 0; m < 4; ++m) {
-      const int64_t k = (int64_t)s * 128 + fq * 32 + m * 8;
-      a[m] = arow != nullptr && k < g.K ? *reinterpret_cast<const uint4*>(arow + k * 2) : make_uint4(0, 0, 0, 0);
+      const int64_t k0 = (int64_t)k * 128 + m * 8;
+      a[set][m] = ar >= 0 && k < b1 && k0 + fq * 32 < g.K ? *reinterpret_cast<const uint4*>(arow + k0 * 2)
+                                                          : make_uint4(0, 0, 0, 0);
     }
   };
   f32x4_t acc[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) acc[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  auto multiply = [&](const uint4 (&w)[4], uint32_t sc, const uint4 (&a)[4]) {
+  load_a(b0, 0);
+  for (int k = b0; k < b1; k += 4) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float scale = mx4_scale((sc >> (8 * i)) & 255u);
+    for (int u = 0; u < 4; ++u) {
+      if (k + u < b1) {
+        load_a(k + u + 1, (u + 1) & 1);
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        const uint32_t c = m == 0 ? w[i].x : m == 1 ? w[i].y : m == 2 ? w[i].z : w[i].w;
-        MfmaOp<OpT>::step(acc[i], mx4_unpack8<OpT>(c, scale), a[m]);
+        for (int i = 0; i < 4; ++i) {
+          const float scale = mx4_scale((sc[u] >> (8 * i)) & 255u);
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            const uint32_t c = m == 0 ? w[u][i].x : m == 1 ? w[u][i].y : m == 2 ? w[u][i].z : w[u][i].w;
+            MfmaOp<OpT>::step(acc[i], mx4_unpack8<OpT>(c, scale), a[u & 1][m]);
+          }
+        }
+        load_w(k + u + 4, u);
       }
-    }
-  };
-  if (b0 < b1) {
-    load_a(b0, a0);
-    for (int s = b0; s < b1; s += 2) {
-      if (s + 1 < b1) {
-        load_w(s + 1, w1, s1);
-        load_a(s + 1, a1);
-      }
-      multiply(w0, s0, a0);
-      if (s + 1 >= b1) break;
-      if (s + 2 < b1) {
-        load_w(s + 2, w0, s0);
-        load_a(s + 2, a0);
-      }
-      multiply(w1, s1, a1);
     }
   }
 #pragma unroll
@@ -296,15 +368,15 @@ __global__ __launch_bounds__(NW * 64) void mx4_decode_kernel(const Mx4Params p) 
   __syncthreads();
   for (int pc = tid; pc < 128; pc += NT) {
     const int r = pc / 8, c = (pc % 8) * 8;
-    const int64_t orow = meta.orow[r], n = n0 + c;
+    const int64_t orow = rows.o[r], n = n0 + c;
     if (orow < 0 || n >= g.N) continue;
     float v[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[q] = 0.f;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
+    for (int s = 0; s < NW; ++s) {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) v[q] += part[w][r][c + q];
+      for (int q = 0; q < 8; ++q) v[q] += part[s][r][c + q];
     }
     union { uint32_t d[4]; OpT e[8]; } h;
 #pragma unroll
@@ -327,128 +399,136 @@ __device__ __forceinline__ void mx4_mfma(f32x4_t& c, const uint4& w, uint32_t sw
   c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(vw, va, c, 4, 4, OpselW, (int)sw, OpselA, (int)sa);
 }
 
-// A slice is 512 k: 256 bytes of codes per row, chunk 4 s + q block q of its
-// s-th 128 k, with the swizzle of the 16-bit rows' slices.
-template <typename OutT, int BM, int BN, int NW, int OCC>
-__global__ __launch_bounds__(NW * 64, OCC) void mx4_gemm4_kernel(const Mx4Params p) {
-  using Cfg = Mx4Cfg<BM, BN, NW>;
-  constexpr int MB = Cfg::MB;
+// Four waves, each all BM rows x 64 columns of the tile's 256.  The rows' codes
+// of up to 1024 k (512 bytes of every row) sit in LDS, chunk 4 s + q block
+// q of the s-th 128 k, at c ^ (row & 15) of each 16 chunks; with them the rows'
+// scales.  The weights stream past them straight into registers, RING sets of
+// one panel in turn, so the loop over panels and column tiles holds no barrier
+// and no DMA: the waits for the weights are the compiler's own counts.  A tile
+// of K <= 1024 is loaded once for all of the workgroup's `passes` column tiles.
+constexpr int kMx4ChunkK = 1024;
+template <typename OutT, int BM, int OCC>
+__global__ __launch_bounds__(256, OCC) void mx4_gemm4_kernel(const Mx4Params p) {
+  constexpr int BN = 256, NW = 4, NT = 256, MB = BM / 16, RING = 2, PD = RING - 1;
+  constexpr int STEPS = kMx4ChunkK / 128;  // panels per chunk
+  constexpr int ROWB = kMx4ChunkK / 2, D = BM * ROWB / (NW * 1024);
+  static_assert(STEPS % RING == 0, "sets by the panel's place in its chunk");
   const GemmParams& g = p.g;
-  __shared__ __attribute__((aligned(1024))) char stage0[Cfg::A_BYTES];
-  __shared__ __attribute__((aligned(1024))) char stage1[Cfg::A_BYTES];
+  __shared__ __attribute__((aligned(1024))) char codes[BM * ROWB];
+  __shared__ __attribute__((aligned(16))) uint32_t row_scales[BM][kMx4ChunkK / 512 * 4];
   __shared__ RouteMeta<BM> meta;
+  __shared__ Mx4Rows<BM> rows;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t n_ntiles = (g.N + BN - 1) / BN;
-  const bool tiled = gemm_schedule<BM, Cfg::NT>(g, n_ntiles, meta);
-  const int64_t n0 = (int64_t)uniform_i32(meta.group) * BN;
+  const int64_t n_ntiles = (g.N + BN - 1) / BN, n_groups = (n_ntiles + p.passes - 1) / p.passes;
+  const bool tiled = gemm_schedule_tile<BM>(g, n_groups, meta);
+  const int64_t t0 = (int64_t)uniform_i32(meta.group) * p.passes;
+  const int64_t t1 = t0 + p.passes < n_ntiles ? t0 + p.passes : n_ntiles;
   if (!tiled) {
-    zero_unrouted_cols<BM, Cfg::NT>(g, meta, gridDim.x / n_ntiles, n0, n0 + BN, -1);
+    zero_unrouted_cols<BM, NT>(g, meta, gridDim.x / n_groups, t0 * BN, t1 * BN, -1);
     return;
   }
+  mx4_rows<BM, NT>(g, meta, rows);
   const int32_t expert = uniform_i32(meta.expert);
   const char* zero = reinterpret_cast<const char*>(g_cvmm_zero_page);
-  const char* src[Cfg::D];
-  int bc[Cfg::D];
-#pragma unroll
-  for (int j = 0; j < Cfg::D; ++j) {
-    const int q = (wave * Cfg::D + j) * 64 + lane, row = q / 16;
-    bc[j] = ((q % 16) ^ (row & 15)) * 16;
-    const int64_t ar = meta.arow[row];
-    src[j] = ar >= 0 ? reinterpret_cast<const char*>(g.a) + ar * p.a_bytes + bc[j] : nullptr;
-  }
-  auto issue = [&](int64_t s, char* buf) {
-    const int64_t b = s * 256;
-#pragma unroll
-    for (int j = 0; j < Cfg::D; ++j)
-      dma16(src[j] != nullptr && b + bc[j] < p.a_bytes ? src[j] + b : zero, buf + (wave * Cfg::D + j) * 1024);
-  };
-  const int wm = wave / Cfg::WN, wn = wave % Cfg::WN;
+  const int kp = (int)p.kp, chunks = (kp + STEPS - 1) / STEPS;
   const int fr = lane & 15, fq = lane >> 4;
-  const int64_t nwave = n0 + wn * 64;
-  const int64_t pn = nwave / 64 < p.np ? nwave / 64 : p.np - 1;
-  const int64_t panel0 = ((int64_t)expert * p.np + pn) * p.kp;
-  const uint8_t* cp = p.codes + panel0 * kMx4PanelCodes + lane * 16;
-  const uint8_t* sp = p.scales + panel0 * kMx4PanelScales + lane * 4;
-  const uint8_t* asp[MB];
+  auto load_rows = [&](int c) {
+    // instruction j of this wave: 2 rows of 32 16-byte pieces
+    int l = lane;
+    asm volatile("" : "+v"(l));  // (addresses made here, not kept over the tile)
+    const int r0 = wave * D * 2 + (l >> 5);
+    int32_t ar[D];
 #pragma unroll
-  for (int j = 0; j < MB; ++j) {
-    const int64_t ar = meta.arow[wm * Cfg::WR + j * 16 + fr];
-    asp[j] = p.a_scales + (ar >= 0 ? ar : 0) * p.a_groups * 16 + fq * 4;  // (no row: zero codes)
-  }
+    for (int j = 0; j < D; ++j) ar[j] = rows.a[r0 + 2 * j];
+#pragma unroll
+    for (int j = 0; j < D; ++j) {
+      const int64_t b = (int64_t)c * ROWB + (((l & 31) ^ ((r0 + 2 * j) & 15)) << 4);
+      const char* sp_ = reinterpret_cast<const char*>(g.a) + ((int64_t)ar[j] * p.a_bytes + b);
+      dma16(ar[j] >= 0 && b < p.a_bytes ? sp_ : zero, codes + (wave * D + j) * 1024);
+    }
+    // one 16-byte scale group per thread: row tid / 2, group tid % 2
+    if (tid >= 2 * BM) return;
+    const int64_t sr = rows.a[tid >> 1], gr = (int64_t)c * (kMx4ChunkK / 512) + (tid & 1);
+    uint4 s = make_uint4(0, 0, 0, 0);
+    if (sr >= 0 && gr < p.a_groups) s = *reinterpret_cast<const uint4*>(p.a_scales + (sr * p.a_groups + gr) * 16);
+    *reinterpret_cast<uint4*>(&row_scales[tid >> 1][(tid & 1) * 4]) = s;
+  };
+  const int a_at = fr * ROWB + ((fq ^ fr) << 4);
   f32x4_t acc[4][MB];
+  uint4 w[RING][4];
+  uint32_t sc[RING];
+  const uint8_t *cp, *sp;
+  auto load_w = [&](int k, int set) {  // (past the last panel: the last again, unused)
+    k = k < kp ? k : kp - 1;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < MB; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  const int64_t slices = (p.kp + 3) / 4;
-  uint32_t sa0[MB], sa1[MB];
-  auto load_sa = [&](int64_t s, uint32_t (&sa)[MB]) {
-#pragma unroll
-    for (int j = 0; j < MB; ++j) sa[j] = *reinterpret_cast<const uint32_t*>(asp[j] + s * 16);
+    for (int i = 0; i < 4; ++i) w[set][i] = *reinterpret_cast<const uint4*>(cp + (int64_t)k * kMx4PanelCodes + i * 1024);
+    sc[set] = *reinterpret_cast<const uint32_t*>(sp + (int64_t)k * kMx4PanelScales);
   };
-  uint4 w0[4], w1[4];
-  uint32_t c0 = 0, c1 = 0;
-  auto load_w = [&](int64_t s, uint4 (&w)[4], uint32_t& sc) {
-    if (s >= p.kp) return;
+  auto step = [&](auto mc, int k) {
+    constexpr int m = decltype(mc)::value, set = m % RING;
+    load_w(k + PD, (m + PD) % RING);
+    issue_fence();
+    // chunk (4 m + fq) ^ fr of row 16 j + fr
+    int at = a_at;
+    asm volatile("" : "+v"(at));  // (one address, not one per panel)
+    const char* ap = codes + (at ^ (m << 6));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = *reinterpret_cast<const uint4*>(cp + s * kMx4PanelCodes + i * 1024);
-    sc = *reinterpret_cast<const uint32_t*>(sp + s * kMx4PanelScales);
-  };
-  // step m of a slice
-  auto step = [&](auto mc, const char* buf, const uint4 (&w)[4], uint32_t sc, const uint32_t (&sa)[MB]) {
-    constexpr int m = decltype(mc)::value;
-    uint4 a[MB];
+    for (int h = 0; h < 2; ++h) {
+      uint4 a[MB / 2];
+      uint32_t sa[MB / 2];
 #pragma unroll
-    for (int j = 0; j < MB; ++j) {
-      const int ra = wm * Cfg::WR + j * 16 + fr;
-      a[j] = *reinterpret_cast<const uint4*>(buf + ra * 256 + (((4 * m + fq) ^ (ra & 15)) << 4));
-    }
+      for (int j = 0; j < MB / 2; ++j) {
+        a[j] = *reinterpret_cast<const uint4*>(ap + (h * (MB / 2) + j) * 16 * ROWB);
+        sa[j] = row_scales[(h * (MB / 2) + j) * 16 + fr][m / 4 * 4 + fq];
+      }
 #pragma unroll
-    for (int j = 0; j < MB; ++j) {
-      mx4_mfma<0, m>(acc[0][j], w[0], sc, a[j], sa[j]);
-      mx4_mfma<1, m>(acc[1][j], w[1], sc, a[j], sa[j]);
-      mx4_mfma<2, m>(acc[2][j], w[2], sc, a[j], sa[j]);
-      mx4_mfma<3, m>(acc[3][j], w[3], sc, a[j], sa[j]);
+      for (int j = 0; j < MB / 2; ++j) {
+        mx4_mfma<0, m % 4>(acc[0][h * (MB / 2) + j], w[set][0], sc[set], a[j], sa[j]);
+        mx4_mfma<1, m % 4>(acc[1][h * (MB / 2) + j], w[set][1], sc[set], a[j], sa[j]);
+        mx4_mfma<2, m % 4>(acc[2][h * (MB / 2) + j], w[set][2], sc[set], a[j], sa[j]);
+        mx4_mfma<3, m % 4>(acc[3][h * (MB / 2) + j], w[set][3], sc[set], a[j], sa[j]);
+      }
     }
   };
-  auto slice = [&](int64_t s, const char* buf, const uint32_t (&sa)[MB]) {
-    const int64_t k = s * 4;
-    load_w(k + 1, w1, c1);
-    step(std::integral_constant<int, 0>(), buf, w0, c0, sa);
-    if (k + 1 >= p.kp) return;
-    load_w(k + 2, w0, c0);
-    step(std::integral_constant<int, 1>(), buf, w1, c1, sa);
-    if (k + 2 >= p.kp) return;
-    load_w(k + 3, w1, c1);
-    step(std::integral_constant<int, 2>(), buf, w0, c0, sa);
-    if (k + 3 >= p.kp) return;
-    load_w(k + 4, w0, c0);
-    step(std::integral_constant<int, 3>(), buf, w1, c1, sa);
+  auto start = [&](int64_t t) {
+    const int64_t nwave = t * BN + wave * 64;
+    const int64_t pn = nwave / 64 < p.np ? nwave / 64 : p.np - 1;
+    const int64_t panel0 = ((int64_t)expert * p.np + pn) * p.kp;
+    cp = p.codes + panel0 * kMx4PanelCodes + lane * 16;
+    sp = p.scales + panel0 * kMx4PanelScales + lane * 4;
+#pragma unroll
+    for (int k = 0; k < PD; ++k) load_w(k, k);
   };
-  issue(0, stage0);
-  load_w(0, w0, c0);
-  load_sa(0, sa0);
-  for (int64_t s = 0; s < slices; s += 2) {
-    vm_wait<0>();
-    wg_barrier();
-    if (s + 1 < slices) {
-      issue(s + 1, stage1);
-      load_sa(s + 1, sa1);
+  for (int64_t t = t0; t < t1; ++t) {
+    const int64_t nwave = t * BN + wave * 64;
+    start(t);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < MB; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < chunks; ++c) {
+      const int k0 = c * STEPS;
+      if (chunks > 1 || t == t0) {
+        if (c > 0 || t > t0) wg_barrier();  // every wave is past the chunk before
+        load_rows(c);
+        vm_wait<0>();
+        lds_barrier();
+      }
+      const int left = kp - k0;
+      step(std::integral_constant<int, 0>(), k0);
+      if (left > 1) step(std::integral_constant<int, 1>(), k0 + 1);
+      if (left > 2) step(std::integral_constant<int, 2>(), k0 + 2);
+      if (left > 3) step(std::integral_constant<int, 3>(), k0 + 3);
+      if (left > 4) step(std::integral_constant<int, 4>(), k0 + 4);
+      if (left > 5) step(std::integral_constant<int, 5>(), k0 + 5);
+      if (left > 6) step(std::integral_constant<int, 6>(), k0 + 6);
+      if (left > 7) step(std::integral_constant<int, 7>(), k0 + 7);
     }
-    slice(s, stage0, sa0);
-    if (s + 1 >= slices) break;
-    vm_wait<0>();
-    wg_barrier();
-    if (s + 2 < slices) {
-      issue(s + 2, stage0);
-      load_sa(s + 2, sa0);
-    }
-    slice(s + 1, stage1, sa1);
+    mx4_store<OutT, MB>(p, acc, nwave, fr, fq, [&](int j, float& wt) {
+      wt = 1.f;
+      return (int64_t)rows.o[j * 16 + fr];
+    });
   }
-  mx4_store<OutT, MB>(p, acc, nwave, fr, fq, [&](int j, float& w) {
-    w = 1.f;
-    return meta.orow[wm * Cfg::WR + j * 16 + fr];
-  });
 }
 
 // ---------------------------------------------------------------------------
@@ -461,7 +541,7 @@ __device__ __forceinline__ uint2 mx4_read_tr(const char* p) {
   return __builtin_bit_cast(uint2, v);
 }
 
-template <typename OpT, typename OutT, int BM, int OCC>
+template <typename OpT, typename OutT, int BM, int OCC, bool DG>
 __global__ __launch_bounds__(256, OCC) void mx4_gemm_t_kernel(const Mx4Params p) {
   constexpr int NW = 4, NT = 256, BN = 128, MB = BM / 2 / 16;
   constexpr int A_BYTES = BM * 128, B_BYTES = 64 * 256, D = A_BYTES / (NW * 1024);
@@ -472,7 +552,7 @@ __global__ __launch_bounds__(256, OCC) void mx4_gemm_t_kernel(const Mx4Params p)
   __shared__ RouteMeta<BM> meta;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t n_ntiles = (g.N + BN - 1) / BN;
-  const bool tiled = gemm_schedule<BM, NT>(g, n_ntiles, meta);
+  const bool tiled = gemm_schedule_tile<BM>(g, n_ntiles, meta);
   const int64_t ntile = uniform_i32(meta.group), n0 = ntile * BN;
   if (!tiled) {
     // (the routing-weight gradient's partials: one per 64 columns)
@@ -480,40 +560,39 @@ __global__ __launch_bounds__(256, OCC) void mx4_gemm_t_kernel(const Mx4Params p)
                                2 * ntile + 1 < g.dg_ntiles ? 2 : 1);
     return;
   }
+  mx4_route_meta<BM, NT>(p, meta);
   const int32_t expert = uniform_i32(meta.expert);
   const char* zero = reinterpret_cast<const char*>(g_cvmm_zero_page);
-  const char* src[D];
-  int kc[D];
+  // DMA instruction j of this wave fills 8 rows of 8 pieces
+  const int r0 = wave * D * 8 + (lane >> 3), kl = (lane & 7) ^ (lane >> 3);
+  int32_t ar[D];
 #pragma unroll
-  for (int j = 0; j < D; ++j) {
-    const int q = (wave * D + j) * 64 + lane, row = q / 8;
-    kc[j] = ((q % 8) ^ (row & 7)) * 8;
-    const int64_t ar = meta.arow[row];
-    src[j] = ar >= 0 ? reinterpret_cast<const char*>(g.a) + (ar * g.a_ld + kc[j]) * 2 : nullptr;
-  }
-  auto issue = [&](int64_t s, char* buf) {
-    const int64_t k0 = s * 64;
+  for (int j = 0; j < D; ++j) ar[j] = (int32_t)meta.arow[r0 + 8 * j];
+  auto issue = [&](int s, char* buf) {
+    const int64_t k = (int64_t)s * 64 + kl * 8;
 #pragma unroll
-    for (int j = 0; j < D; ++j)
-      dma16(src[j] != nullptr && k0 + kc[j] < g.K ? src[j] + k0 * 2 : zero, buf + (wave * D + j) * 1024);
+    for (int j = 0; j < D; ++j) {
+      const char* row = reinterpret_cast<const char*>(g.a) + ((int64_t)ar[j] * g.a_ld + k) * 2;
+      dma16(ar[j] >= 0 && k < g.K ? row : zero, buf + (wave * D + j) * 1024);
+    }
   };
   // this thread's part of a panel: column (of W) 16 wave + lane % 16, the 32 k of block lane / 16
   const uint8_t* cp = p.codes + ((int64_t)expert * p.np * p.kp + ntile) * kMx4PanelCodes + wave * 1024 + lane * 16;
   const uint8_t* sp = p.scales + ((int64_t)expert * p.np * p.kp + ntile) * kMx4PanelScales + lane * 4 + wave;
   uint4 w;
   uint32_t sb;
-  auto load_w = [&](int64_t s) {
-    w = *reinterpret_cast<const uint4*>(cp + s * p.kp * kMx4PanelCodes);
-    sb = sp[s * p.kp * kMx4PanelScales];
+  auto load_w = [&](int s) {
+    w = *reinterpret_cast<const uint4*>(cp + (int64_t)s * p.kp * kMx4PanelCodes);
+    sb = sp[(int64_t)s * p.kp * kMx4PanelScales];
   };
-  auto put_w = [&](char* buf) {  // LDS row (of 128 k) of this n, chunks 4 (lane / 16) .. + 4
-    const int r = wave * 16 + (lane & 15);
+  // LDS row (of 128 k) of this n, chunks 4 (lane / 16) .. + 4; the swizzle is even
+  const int w_at = A_BYTES + (wave * 16 + (lane & 15)) * 256 +
+                   (((4 * (lane >> 4)) ^ tr_row_swz<16>(wave * 16 + (lane & 15))) << 4);
+  auto put_w = [&](char* buf) {
     const float scale = mx4_scale(sb);
     const uint32_t c[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
-      *reinterpret_cast<uint4*>(buf + A_BYTES + r * 256 + (((4 * (lane >> 4) + m) ^ tr_row_swz<16>(r)) << 4)) =
-          mx4_unpack8<OpT>(c[m], scale);
+    for (int m = 0; m < 4; ++m) *reinterpret_cast<uint4*>(buf + (w_at ^ (m << 4))) = mx4_unpack8<OpT>(c[m], scale);
   };
   const int wm = wave >> 1, wn = wave & 1;
   const int fr = lane & 15, fq = lane >> 4;
@@ -522,50 +601,66 @@ __global__ __launch_bounds__(256, OCC) void mx4_gemm_t_kernel(const Mx4Params p)
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < MB; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  // A row wm * BM / 2 + 16 j + fr, chunk 4 kk + fq at chunk ^ (fr & 7); W rows
+  // 32 kk + 8 fq + fr / 4 (+ 4) of the slice, 4 of 16 columns
+  const int a_at = (wm * (BM / 2) + fr) * 128 + ((fq ^ (fr & 7)) << 4);
+  const int wr = fq * 8 + (fr >> 2);  // (the swizzle of row + 32 is the row's)
+  const int b_at = A_BYTES + wr * 256 + ((fr & 1) << 3) + (((fr >> 1) & 1) << 4) + (((wn * 8) ^ tr_row_swz<16>(wr)) << 4);
   auto multiply = [&](const char* buf) {
+    int aa = a_at, ba = b_at;
+    asm volatile("" : "+v"(aa), "+v"(ba));
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
       uint4 a[MB];
 #pragma unroll
-      for (int j = 0; j < MB; ++j) {
-        const int ra = wm * (BM / 2) + j * 16 + fr;
-        a[j] = *reinterpret_cast<const uint4*>(buf + ra * 128 + (((kk * 4 + fq) ^ (ra & 7)) << 4));
-      }
-      // rows kk * 32 + 8 fq + fr / 4 (+ 4) of the slice, 4 of the 16 columns
-      const int r = kk * 32 + fq * 8 + (fr >> 2);
-      const int lane_lo = ((fr & 1) << 3) + (((fr >> 1) & 1) << 4);
+      for (int j = 0; j < MB; ++j) a[j] = *reinterpret_cast<const uint4*>(buf + (aa ^ (kk << 6)) + j * 16 * 128);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const char* at = buf + A_BYTES + r * 256 + lane_lo + (((wn * 8 + 2 * i) ^ tr_row_swz<16>(r)) << 4);
+        const char* at = buf + (ba ^ (i << 5)) + kk * 32 * 256;
         const uint2 lo = mx4_read_tr(at), hi = mx4_read_tr(at + 4 * 256);
         const uint4 b = make_uint4(lo.x, lo.y, hi.x, hi.y);
 #pragma unroll
         for (int j = 0; j < MB; ++j) MfmaOp<OpT>::step(acc[i][j], b, a[j]);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
-  const int64_t slices = p.np;
-  // slice s is converted into its buffer while slice s - 1 is multiplied
-  issue(0, stage0);
-  load_w(0);
-  put_w(stage0);
-  if (slices > 1) load_w(1);
-  for (int64_t s = 0; s < slices; s += 2) {
+  // slice s is converted into its buffer while slice s - 1 is multiplied, an odd
+  // one first, then pairs
+  const int np = (int)p.np;
+  int s = np & 1;
+  if (s) {
+    issue(0, stage1);
+    load_w(0);
+    put_w(stage1);
+    if (np > 1) load_w(1);
     vm_wait<0>();
     lds_barrier();
-    if (s + 1 < slices) {
-      issue(s + 1, stage1);
-      put_w(stage1);
-      if (s + 2 < slices) load_w(s + 2);
+    if (np > 1) {
+      issue(1, stage0);
+      put_w(stage0);
+      load_w(2);
     }
-    multiply(stage0);
-    if (s + 1 >= slices) break;
+    multiply(stage1);
+  } else {
+    issue(0, stage0);
+    load_w(0);
+    put_w(stage0);
+    load_w(1);
+  }
+  for (; s < np; s += 2) {
     vm_wait<0>();
     lds_barrier();
-    if (s + 2 < slices) {
+    issue(s + 1, stage1);
+    put_w(stage1);
+    if (s + 2 < np) load_w(s + 2);
+    multiply(stage0);
+    vm_wait<0>();
+    lds_barrier();
+    if (s + 2 < np) {
       issue(s + 2, stage0);
       put_w(stage0);
-      if (s + 3 < slices) load_w(s + 3);
+      load_w(s + 3);
     }
     multiply(stage1);
   }
@@ -576,7 +671,7 @@ __global__ __launch_bounds__(256, OCC) void mx4_gemm_t_kernel(const Mx4Params p)
       wt = meta.w[m];
       return meta.orow[m];
     });
-  if (g.dg != nullptr && nwave < g.dg_n) {
+  if (DG && nwave < g.dg_n) {
     // routing-weight gradient: sum over the wave's 64 columns of acc * x, in
     // the order of the lane's 16 columns, then the row's 4 lanes
 #pragma unroll

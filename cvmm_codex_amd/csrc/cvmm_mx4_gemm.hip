@@ -11,24 +11,88 @@ static hipError_t launch(K kernel, const Mx4Params& p, int64_t grid, int threads
   return hipGetLastError();
 }
 
+template <typename OpT, int BM, int BN, int NW, int OCC>
+static hipError_t tile16(const Mx4Params& p, hipStream_t s) {
+  return launch(mx4_gemm_kernel<OpT, BM, BN, NW, OCC>, p, mx4_grid<BM>(p.g, (p.g.N + BN - 1) / BN), NW * 64, s);
+}
+
+// 16-bit rows.  Times of bf16 launches, 128 experts of 2048 x 512 (512 x 2048):
+//   routes per expert     2           8           16          32          125        1024
+//   16-row tiles      14.1 (14.6)  16.3        17.0 (18.7)  21.8 (24.3)   53         423
+//   32-row            15.5 (15.5)  16.5        19.6 (19.7)  21.3 (22.9)   46 (50)    323
+//   64-row            21.2 (20.3)  21.7        22.2 (23.9)  29.5 (25.9)   44 (48)    295
+// 256-column tiles, 4 waves of 64 columns; 128-column ones where the columns
+// end there (64 experts of 1024 x 128, 250 routes: 18.1 -> 14.1 us) or
+// where they leave less than four fifths of the wide tiles filled.  A launch
+// of fewer than 256 16-row tiles splits K over the waves of a workgroup
+// instead: 8 tokens, top-8, 128 experts of 2048 x 512: 11.3 -> 8.1 us; 16
+// tokens, 64 experts of 1024 x 128: 7.0 -> 4.6.
 template <typename OpT>
 static hipError_t fwd16(const Mx4Params& p, hipStream_t s) {
   const GemmParams& g = p.g;
-  if (g.n_routes <= 16 * (int64_t)g.n_experts)
+  const int64_t E = g.n_experts < g.n_routes ? g.n_experts : g.n_routes, R = g.n_routes;
+  if (((R + 15) / 16 + E) * ((g.N + 255) / 256) < 256 && p.kp >= 4) {
+    // eight parts of K where four leave CUs idle (4 tokens, 1024 x 128: 5.0 -> 4.5 us; 8, 2048 x 512: 8.1 -> 9.9)
+    if (E * p.np <= 256 && p.kp >= 8)
+      return launch(mx4_decode_kernel<OpT, 8>, p, mx4_grid<16>(g, p.np), 512, s);
     return launch(mx4_decode_kernel<OpT, 4>, p, mx4_grid<16>(g, p.np), 256, s);
-  return launch(mx4_gemm_kernel<OpT, 128, 128, 4, 2>, p, mx4_grid<128>(g, (g.N + 127) / 128), 256, s);
+  }
+  const int64_t w128 = (g.N + 127) / 128 * 128, w256 = (g.N + 255) / 256 * 256;
+  const bool narrow = 5 * w128 < 4 * w256;
+  if (R <= 24 * E) return narrow ? tile16<OpT, 16, 128, 2, 4>(p, s) : tile16<OpT, 16, 256, 4, 4>(p, s);
+  if (R <= 128 * E) return narrow ? tile16<OpT, 32, 128, 2, 4>(p, s) : tile16<OpT, 32, 256, 4, 4>(p, s);
+  return narrow ? tile16<OpT, 64, 128, 4, 4>(p, s) : tile16<OpT, 64, 256, 4, 3>(p, s);
+}
+
+// 4-bit rows.  A tile of K <= 1024 keeps its rows for two column tiles: 16384
+// tokens, top-8 of 128 experts of 512 x 2048 take 240 / 218 / 228 us with 1 / 2
+// / 4 tiles per workgroup; past that the rows are read again either way, and
+// one tile each fills the GPU better (2048 x 512: 106 / 122 us with 1 / 2).
+template <typename OutT, int BM, int OCC>
+static hipError_t tile4(Mx4Params p, hipStream_t s) {
+  const int64_t tiles = (p.g.N + 255) / 256;
+  p.passes = p.g.K <= kMx4ChunkK && tiles > 1 ? 2 : 1;
+  return launch(mx4_gemm4_kernel<OutT, BM, OCC>, p, mx4_grid<BM>(p.g, (tiles + p.passes - 1) / p.passes), 256, s);
 }
 
 template <typename OutT>
 static hipError_t fwd4(const Mx4Params& p, hipStream_t s) {
-  return launch(mx4_gemm4_kernel<OutT, 128, 128, 4, 2>, p, mx4_grid<128>(p.g, (p.g.N + 127) / 128), 256, s);
+  const GemmParams& g = p.g;
+  const int64_t E = g.n_experts < g.n_routes ? g.n_experts : g.n_routes;
+  if (g.n_routes <= 64 * E) return tile4<OutT, 32, 4>(p, s);
+  return tile4<OutT, 128, 2>(p, s);
+}
+
+// Input gradient: 160-row tiles unless they cost over 5 % more than 128-row ones
+// in rounds of 512 tiles x tile height (65536 routes of 64 experts, 1024 -> 128:
+// 32.4 / 46.4 us, one round against two; 512 x 2048: 248 / 270); 64-row ones
+// where the average expert fills no more.
+static int bwd_rows(const GemmParams& g) {
+  const int64_t E = g.n_experts < g.n_routes ? g.n_experts : g.n_routes, nt = (g.N + 127) / 128;
+  if (g.n_routes <= 64 * E) return 64;
+  auto rounds = [&](int64_t bm) { return (((g.n_routes + bm - 1) / bm + E / 2) * nt + 511) / 512; };
+  return 20 * 160 * rounds(160) <= 21 * 128 * rounds(128) ? 160 : 128;
+}
+
+template <typename OpT, typename OutT, int BM, int OCC>
+static hipError_t tile_t(const Mx4Params& p, hipStream_t s) {
+  const int64_t grid = mx4_grid<BM>(p.g, (p.g.N + 127) / 128);
+  if (p.g.dg != nullptr) return launch(mx4_gemm_t_kernel<OpT, OutT, BM, OCC, true>, p, grid, 256, s);
+  return launch(mx4_gemm_t_kernel<OpT, OutT, BM, OCC, false>, p, grid, 256, s);
+}
+
+template <typename OpT, typename OutT>
+static hipError_t bwd_out(const Mx4Params& p, hipStream_t s) {
+  switch (bwd_rows(p.g)) {
+    case 64: return tile_t<OpT, OutT, 64, 3>(p, s);
+    case 160: return tile_t<OpT, OutT, 160, 2>(p, s);
+    default: return tile_t<OpT, OutT, 128, 2>(p, s);
+  }
 }
 
 template <typename OpT>
 static hipError_t bwd(const Mx4Params& p, hipStream_t s) {
-  const int64_t grid = mx4_grid<128>(p.g, (p.g.N + 127) / 128);
-  if (p.g.out_dtype == kF32) return launch(mx4_gemm_t_kernel<OpT, float, 128, 2>, p, grid, 256, s);
-  return launch(mx4_gemm_t_kernel<OpT, OpT, 128, 2>, p, grid, 256, s);
+  return p.g.out_dtype == kF32 ? bwd_out<OpT, float>(p, s) : bwd_out<OpT, OpT>(p, s);
 }
 
 // Output rows in whole aligned 16-byte pieces?
@@ -65,6 +129,7 @@ hipError_t launch_mx4_bwd_x(const GemmParams& g, const void* codes, const void* 
   p.scales = (const uint8_t*)scales;
   p.np = mx4_panels_n(g.K);
   p.kp = mx4_panels_k(g.N);
+  p.a_div = make_fast_div(g.a_div);
   finish(p);
   return op_dtype == kBF16 ? bwd<bf16_t>(p, stream) : bwd<f16_t>(p, stream);
 }

@@ -106,6 +106,15 @@ SIZES = [  # T, d_in, d_out, E, k
     (300, 1000, 312, 7, 4),
     (130, 64, 513, 2, 1),
     (257, 384, 320, 16, 8),
+    # each tile height and width of the products on either side of its rule
+    (30, 256, 128, 8, 2),        # K split over waves
+    (260, 640, 320, 64, 4),      # 16-row tiles, narrow and (next) wide
+    (260, 320, 640, 64, 4),
+    (400, 136, 320, 8, 1),       # 32-row
+    (400, 320, 256, 8, 1),
+    (900, 130, 72, 3, 2),        # 64-row
+    (900, 264, 520, 3, 2),
+    (2100, 1100, 96, 2, 2),      # more than one chunk of 4-bit rows
 ]
 MODES = ["up", "down", "token_weighted"]
 
