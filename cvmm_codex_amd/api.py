@@ -632,29 +632,6 @@ def cvmm_route_topk(logits: torch.Tensor, k: int, renormalize: bool = True):
     return w.view(*lead, k), sel, CVMMSel._deferred(sel, routing, False, None)
 
 
-class _RouteScored(torch.autograd.Function):
-    """Eager path of cvmm_route_scored: as _RouteTopK.  The bias enters the
-    choice alone and has no gradient."""
-
-    @staticmethod
-    def forward(ctx, logits, top_k, bias, scores, groups, topk_groups, renormalize, scale):
-        w, sel, ssel, perm, tok, offsets, route_pos = N.host().route_scored(
-            logits, top_k, bias, scores, groups, topk_groups, renormalize, scale, N.stream_of(logits.device))
-        ctx.save_for_backward(logits, sel)
-        ctx.args = (top_k, scores, renormalize, scale)
-        ctx.mark_non_differentiable(sel, ssel, perm, tok, offsets, route_pos)
-        ctx.set_materialize_grads(False)
-        return w, sel, ssel, perm, tok, offsets, route_pos
-
-    @staticmethod
-    def backward(ctx, grad_w, *_):
-        if grad_w is None:
-            return (None,) * 8
-        logits, sel = ctx.saved_tensors
-        g = N.host().route_scored_backward(logits, sel, grad_w.contiguous(), *ctx.args, N.stream_of(logits.device))
-        return (g,) + (None,) * 7
-
-
 def cvmm_route_scored(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor] = None, scores: str = "softmax",
                       groups: int = 1, topk_groups: Optional[int] = None, renormalize: bool = True,
                       scale: float = 1.0):
@@ -687,12 +664,14 @@ def cvmm_route_scored(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor]
     if not (0 < k <= kept * (E // groups)):
         raise ValueError(f"cvmm_route_scored: k={k} outside 1..{kept * (E // groups)}")
     lead = logits.shape[:-1]
+    # (the bias enters the choice alone)
     args = (logits, k, None if bias is None else bias.detach(), N.SCORES[scores], groups, kept, bool(renormalize),
             float(scale))
     if _compiling():
         w, sel, ssel, perm, tok, offsets, route_pos = _ops.route_scored(*args)
     else:
-        w, sel, ssel, perm, tok, offsets, route_pos = _apply(_RouteScored, *args)
+        w, sel, ssel, perm, tok, offsets, route_pos = N.host().route_scored_apply(
+            *args, torch.is_grad_enabled() and logits.requires_grad)
         perm._cvmm_route_pos = route_pos
     sel = sel.view(*lead, k)
     routing = _Routing(sel.reshape(-1), k)

@@ -8,7 +8,7 @@ namespace cvmm {
 
 // Segments of LPT lanes (4..64) each route one token: lane i of a segment
 // holds experts i + LPT * v, v < MAXV.  Reductions over a segment use DPP
-// (quad permutes, half-row and row mirrors) and, past 16 lanes, shuffles; every
+// (quad permutes, half-row and row mirrors) and, past 16 lanes, lane swaps; every
 // lane of the segment ends with the same result.
 template <int CTRL>
 __device__ __forceinline__ float dpp_f(float v) {
@@ -20,14 +20,34 @@ __device__ __forceinline__ int32_t dpp_i(int32_t v) {
 }
 constexpr int kDppXor1 = 0xB1, kDppXor2 = 0x4E, kDppHalfMirror = 0x141, kDppMirror = 0x140;
 
+// The values of the lane and of the one 16 (32) lanes across, in the same order
+// for both.
+__device__ __forceinline__ void across16(uint32_t v, uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  a = r[0];
+  b = r[1];
+}
+__device__ __forceinline__ void across32(uint32_t v, uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  a = r[0];
+  b = r[1];
+}
+
 template <int LPT>
 __device__ __forceinline__ float seg_max(float v) {
   v = fmaxf(v, dpp_f<kDppXor1>(v));
   v = fmaxf(v, dpp_f<kDppXor2>(v));
   if constexpr (LPT >= 8) v = fmaxf(v, dpp_f<kDppHalfMirror>(v));
   if constexpr (LPT >= 16) v = fmaxf(v, dpp_f<kDppMirror>(v));
-  if constexpr (LPT >= 32) v = fmaxf(v, __shfl_xor(v, 16, 64));
-  if constexpr (LPT >= 64) v = fmaxf(v, __shfl_xor(v, 32, 64));
+  uint32_t a, b;
+  if constexpr (LPT >= 32) {
+    across16(__float_as_uint(v), a, b);
+    v = fmaxf(__uint_as_float(a), __uint_as_float(b));
+  }
+  if constexpr (LPT >= 64) {
+    across32(__float_as_uint(v), a, b);
+    v = fmaxf(__uint_as_float(a), __uint_as_float(b));
+  }
   return v;
 }
 template <int LPT>
@@ -36,8 +56,15 @@ __device__ __forceinline__ float seg_sum(float v) {  // same two partials per st
   v = v + dpp_f<kDppXor2>(v);
   if constexpr (LPT >= 8) v = v + dpp_f<kDppHalfMirror>(v);
   if constexpr (LPT >= 16) v = v + dpp_f<kDppMirror>(v);
-  if constexpr (LPT >= 32) v = v + __shfl_xor(v, 16, 64);
-  if constexpr (LPT >= 64) v = v + __shfl_xor(v, 32, 64);
+  uint32_t a, b;
+  if constexpr (LPT >= 32) {
+    across16(__float_as_uint(v), a, b);
+    v = __uint_as_float(a) + __uint_as_float(b);
+  }
+  if constexpr (LPT >= 64) {
+    across32(__float_as_uint(v), a, b);
+    v = __uint_as_float(a) + __uint_as_float(b);
+  }
   return v;
 }
 template <int LPT>
@@ -46,8 +73,50 @@ __device__ __forceinline__ int32_t seg_min_i(int32_t v) {
   v = min(v, dpp_i<kDppXor2>(v));
   if constexpr (LPT >= 8) v = min(v, dpp_i<kDppHalfMirror>(v));
   if constexpr (LPT >= 16) v = min(v, dpp_i<kDppMirror>(v));
-  if constexpr (LPT >= 32) v = min(v, __shfl_xor(v, 16, 64));
-  if constexpr (LPT >= 64) v = min(v, __shfl_xor(v, 32, 64));
+  uint32_t a, b;
+  if constexpr (LPT >= 32) {
+    across16((uint32_t)v, a, b);
+    v = min((int32_t)a, (int32_t)b);
+  }
+  if constexpr (LPT >= 64) {
+    across32((uint32_t)v, a, b);
+    v = min((int32_t)a, (int32_t)b);
+  }
+  return v;
+}
+template <int LPT>
+__device__ __forceinline__ int32_t seg_max_i(int32_t v) {
+  v = max(v, dpp_i<kDppXor1>(v));
+  v = max(v, dpp_i<kDppXor2>(v));
+  if constexpr (LPT >= 8) v = max(v, dpp_i<kDppHalfMirror>(v));
+  if constexpr (LPT >= 16) v = max(v, dpp_i<kDppMirror>(v));
+  uint32_t a, b;
+  if constexpr (LPT >= 32) {
+    across16((uint32_t)v, a, b);
+    v = max((int32_t)a, (int32_t)b);
+  }
+  if constexpr (LPT >= 64) {
+    across32((uint32_t)v, a, b);
+    v = max((int32_t)a, (int32_t)b);
+  }
+  return v;
+}
+
+template <int LPT>
+__device__ __forceinline__ uint32_t seg_or(uint32_t v) {
+  v |= (uint32_t)dpp_i<kDppXor1>((int32_t)v);
+  v |= (uint32_t)dpp_i<kDppXor2>((int32_t)v);
+  if constexpr (LPT >= 8) v |= (uint32_t)dpp_i<kDppHalfMirror>((int32_t)v);
+  if constexpr (LPT >= 16) v |= (uint32_t)dpp_i<kDppMirror>((int32_t)v);
+  uint32_t a, b;
+  if constexpr (LPT >= 32) {
+    across16(v, a, b);
+    v = a | b;
+  }
+  if constexpr (LPT >= 64) {
+    across32(v, a, b);
+    v = a | b;
+  }
   return v;
 }
 

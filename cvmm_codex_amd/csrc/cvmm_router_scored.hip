@@ -11,14 +11,14 @@
 // sort chunk and leaves its histogram to the scatter launch, or sorts all
 // routes itself where it holds them.
 //
-// The scores, the biased scores and the group sums are computed and compared
-// in 64 bits: the choice is part of the answer, and between neighbours that
-// 32 bits cannot tell apart it would depend on how exp was rounded (131072
-// choices of 128 experts see about one such pair per call).
-//
-// A selection round compares in two steps: the segment's maximum of the
-// 32-bit roundings (rounding keeps the order, so the winner is among the
-// lanes that attain it), and only where several lanes do, the 64-bit values.
+// The choice is that of 64-bit scores: it is part of the answer, and between
+// neighbours that 32 bits cannot tell apart it would depend on how exp was
+// rounded (131072 choices of 128 experts see about one such pair per call).  It
+// is made in 32 bits, with the candidates that are within the error of the ones
+// before them ranked by their 64-bit scores, and in 64 bits throughout for the
+// few tokens where that is not enough; without a bias and groups the logits
+// themselves are compared.  (64-bit exps for all: 32 tokens of 256 experts, on
+// one CU, 33 us.)
 #include <cmath>
 
 #include "cvmm_common.h"
@@ -27,7 +27,9 @@
 
 namespace cvmm {
 
-constexpr int kScoredThreads = 512;
+// Threads of a workgroup: one pass over a chunk's 64 tokens (top-8) with up to
+// 128 experts.
+template <int LPT> constexpr int scored_threads(bool one) { return one || LPT >= 16 ? 1024 : 512; }
 constexpr int kScoredBwdThreads = 256;
 
 template <int LPT>
@@ -49,8 +51,6 @@ __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
-__device__ __forceinline__ double sigmoid64(double l) { return 1.0 / (1.0 + exp(-l)); }
-
 struct ScoredParams {
   int64_t ld, n_tokens;
   int32_t E, k;
@@ -59,139 +59,283 @@ struct ScoredParams {
   double scale;
 };
 
-template <typename LT, int LPT, int MAXV, bool ONE, bool GROUPED>
-__global__ __launch_bounds__(kScoredThreads) void route_scored_kernel(
+// A chosen expert's score, and for the sigmoid 1 minus it, from its logit: one
+// inlined exp and division for both kinds.
+__device__ __forceinline__ double score64(double x, bool sigmoid, double m, double total) {
+  const double e = exp(sigmoid ? -x : x - m);
+  return (sigmoid ? 1.0 : e) / (sigmoid ? 1.0 + e : total);
+}
+
+// The groups that stay, by one wave's lanes for its segments: the sum of the two
+// best of the scores ct of each group, ranked.  Returns the experts of this lane
+// that go, as bits of v; gap (32 bits): the distance between the last group that
+// stays and the first that goes.
+template <typename T, int LPT, int MAXV>
+__device__ __forceinline__ uint32_t groups_out(const T* ct, T* gt, const ScoredParams& p, int li, T* gap) {
+  const int32_t G = p.groups, per = p.E / G;
+  wave_lds_fence();
+#pragma unroll 1
+  for (int g = li; g < G; g += LPT) {
+    T b1 = ct[g * per], b2 = -INFINITY;
+#pragma unroll 8
+    for (int i = 1; i < per; ++i) {
+      const T x = ct[g * per + i];
+      b2 = fmax(b2, fmin(b1, x));
+      b1 = fmax(b1, x);
+    }
+    const T s = per > 1 ? b1 + b2 : b1;
+    gt[g] = isnan(s) ? -INFINITY : s;  // (+inf and -inf)
+  }
+  wave_lds_fence();
+  T last = INFINITY, first = -INFINITY;
+  uint32_t lo = 0, hi = 0;  // the groups that stay, as bits
+#pragma unroll 1
+  for (int g = li; g < G; g += LPT) {
+    const T mine = gt[g];
+    int rank = 0;  // groups ahead of this one
+#pragma unroll 8
+    for (int h = 0; h < G; ++h) {
+      const T x = gt[h];
+      rank += x > mine || (x == mine && h < g) ? 1 : 0;
+    }
+    if (rank < p.topk_groups) {
+      last = fmin(last, mine);
+      if (g < 32) lo |= 1u << g;
+      else hi |= 1u << (g - 32);
+    } else {
+      first = fmax(first, mine);
+    }
+  }
+  lo = seg_or<LPT>(lo);
+  hi = seg_or<LPT>(hi);
+  uint32_t out = 0;
+  const float inv = 1.f / (float)per;  // e / per: exact for e + 0.5 (e < 1024)
+#pragma unroll
+  for (int v = 0; v < MAXV; ++v) {
+    const int e = li + LPT * v, g = (int)(((float)e + 0.5f) * inv);
+    const uint32_t stays = ((g < 32 ? lo : hi) >> (g & 31)) & 1u;
+    if (e < p.E) out |= (stays ^ 1u) << v;
+  }
+  if constexpr (sizeof(T) == 4) *gap = -seg_max<LPT>(-last) - seg_max<LPT>(first);
+  else *gap = 0;
+  return out;
+}
+
+template <typename LT, int LPT, int MAXV, bool ONE, bool GROUPED, int THREADS>
+__global__ __launch_bounds__(THREADS) void route_scored_kernel(
     const LT* __restrict__ logits, const ScoredParams p, int64_t tpc, float* __restrict__ weights,
     int64_t* __restrict__ sel, int32_t* __restrict__ counts, const RouteSortOut so) {
-  constexpr int SEGS = kScoredThreads / LPT;  // tokens per workgroup pass
-  constexpr int SLOTS = 64 / LPT;             // results j held by lane j % LPT, slot j / LPT
-  constexpr int PER = LPT * MAXV;             // expert slots per token
+  constexpr int SEGS = THREADS / LPT;  // tokens per workgroup pass
+  constexpr int SLOTS = 64 / LPT;      // results j held by lane j % LPT, slot j / LPT
+  constexpr int PER = LPT * MAXV;      // expert slots per token
   constexpr int GMAX = PER < kRouteMaxGroups ? PER : kRouteMaxGroups;
-  // grouped: per segment the biased scores, then the group scores
+  // per segment the biased scores, then (grouped) the groups'
   __shared__ double cs[GROUPED ? SEGS * (PER + GMAX) : 1];
   __shared__ int32_t hist[PER + 1];
   __shared__ __attribute__((aligned(16))) int32_t ids[ONE ? kRouteOneMax : 1];
   const int32_t E = p.E, k = p.k;
   const int64_t b = blockIdx.x;
-  for (int e = threadIdx.x; e <= E; e += kScoredThreads) hist[e] = 0;
+  for (int e = threadIdx.x; e <= E; e += THREADS) hist[e] = 0;
   __syncthreads();
   const int lane = threadIdx.x & 63;
   const int li = threadIdx.x % LPT, seg = threadIdx.x / LPT;
   const uint64_t seg_mask = (LPT == 64 ? ~0ull : ((1ull << (LPT & 63)) - 1)) << (lane - li);
+  double* const ct = cs + (GROUPED ? seg * (PER + GMAX) : 0);
+  const bool by_logit = !GROUPED && p.bias == nullptr;
   const int64_t t_lo = b * tpc, t_hi = t_lo + tpc < p.n_tokens ? t_lo + tpc : p.n_tokens;
-  // every lane runs every pass (segment reductions need the whole wave)
-  for (int64_t t0 = t_lo; t0 < t_hi; t0 += SEGS) {
+  // every lane runs every pass (segment reductions need the whole wave); waves
+  // of no token have none to run
+  for (int64_t t0 = t_lo; t0 < t_hi && t0 + (threadIdx.x & ~63) / LPT < t_hi; t0 += SEGS) {
     const int64_t t = t0 + seg;
     const bool active = t < t_hi;
     const LT* row = logits + (active ? t : t_lo) * p.ld;
-    double c[MAXV];
-    double m = 0.0, sum = 1.0;
-    if (p.sigmoid) {
-#pragma unroll
-      for (int v = 0; v < MAXV; ++v) {
-        const int e = li + LPT * v;
-        c[v] = e < E ? sigmoid64((double)(float)row[e]) : 0.0;
-      }
-    } else {
-      float l[MAXV], mf = -INFINITY;
-#pragma unroll
-      for (int v = 0; v < MAXV; ++v) {
-        const int e = li + LPT * v;
-        l[v] = e < E ? (float)row[e] : -INFINITY;
-        mf = fmaxf(mf, l[v]);
-      }
-      m = (double)seg_max<LPT>(mf);
-      double s = 0.0;
-#pragma unroll
-      for (int v = 0; v < MAXV; ++v) {
-        c[v] = li + LPT * v < E ? exp((double)l[v] - m) : 0.0;
-        s += c[v];
-      }
-      sum = seg_sum_f64<LPT>(s);
-#pragma unroll
-      for (int v = 0; v < MAXV; ++v) c[v] = c[v] / sum;
-    }
-    uint32_t taken = 0;  // experts out of the choice
+    // ---- 32 bits.  exp: |x| 2^-24 by its argument and an ulp, so a sigmoid is off
+    // by at most 0.6 * 2^-24 + two roundings < 2^-22, a softmax score by that
+    // part of the largest; the sum with the bias by half an ulp of itself.
+    // (Loads at clamped places: a guard around each made them
+    // wait for one another.)
+    float l[MAXV], c[MAXV];
 #pragma unroll
     for (int v = 0; v < MAXV; ++v) {
       const int e = li + LPT * v;
-      if (e < E && p.bias != nullptr) c[v] += (double)p.bias[e];
-      if (e >= E) taken |= 1u << v;
-      c[v] = e >= E || isnan(c[v]) ? -INFINITY : c[v];
+      l[v] = (float)row[e < E ? e : E - 1];
+      c[v] = 0.f;
     }
-    if constexpr (GROUPED) {
-      const int32_t G = p.groups, per = E / G;
-      double* ct = cs + seg * (PER + GMAX);
-      double* gt = ct + PER;
+    if (p.bias != nullptr) {
 #pragma unroll
-      for (int v = 0; v < MAXV; ++v) ct[li + LPT * v] = c[v];
-      wave_lds_fence();
-      for (int g = li; g < G; g += LPT) {
-        double b1 = ct[g * per], b2 = -INFINITY;
-        for (int i = 1; i < per; ++i) {
-          const double x = ct[g * per + i];
-          b2 = fmax(b2, fmin(b1, x));
-          b1 = fmax(b1, x);
-        }
-        const double s = per > 1 ? b1 + b2 : b1;
-        gt[g] = isnan(s) ? -INFINITY : s;  // (+inf and -inf)
-      }
-      wave_lds_fence();
+      for (int v = 0; v < MAXV; ++v) c[v] = p.bias[li + LPT * v < E ? li + LPT * v : E - 1];
+    }
+    float m = -INFINITY, sum = 1.f, err = 0x1p-21f;  // of a score, both sides (below)
+    bool unsure = false;                             // NaN, or groups within the error
+    if (p.sigmoid) {
+#pragma unroll
+      for (int v = 0; v < MAXV; ++v) c[v] += __frcp_rn(1.f + __expf(-l[v]));
+    } else {
+#pragma unroll
+      for (int v = 0; v < MAXV; ++v) m = fmaxf(m, l[v]);  // (a repeated last one changes nothing)
+      m = seg_max<LPT>(m);
+      float s = 0.f, x[MAXV];
 #pragma unroll
       for (int v = 0; v < MAXV; ++v) {
-        const int e = li + LPT * v;
-        if (e >= E) continue;
-        const int g = e / per;
-        const double mine = gt[g];
-        int rank = 0;  // groups ahead of this one
-        for (int h = 0; h < G; ++h) {
-          const double x = gt[h];
-          rank += x > mine || (x == mine && h < g) ? 1 : 0;
-        }
-        if (rank >= p.topk_groups) taken |= 1u << v;
+        x[v] = __expf(l[v] - m);
+        s += li + LPT * v < E ? x[v] : 0.f;
       }
+      sum = seg_sum<LPT>(s);
+      unsure = isnan(sum);
+      const float inv = 1.f / sum;
+      err *= inv;  // of the largest score, 1 / sum
+#pragma unroll
+      for (int v = 0; v < MAXV; ++v) c[v] += x[v] * inv;
     }
+    // the scores as integers of the same order, the smallest for experts out of
+    // the choice: one maximum finds the lane's best
+    constexpr int32_t kOut = INT32_MIN;
+    int32_t key[MAXV];
+    float top = 0.f;
+#pragma unroll
+    for (int v = 0; v < MAXV; ++v) {
+      const bool in = li + LPT * v < E;
+      if (by_logit) c[v] = l[v];
+      unsure |= in && isnan(c[v]);
+      const int32_t i = __float_as_int(c[v] + 0.f);  // (-0 and 0 tie)
+      key[v] = in ? i ^ ((i >> 31) & 0x7fffffff) : kOut;
+      top = fmaxf(top, in ? fabsf(c[v]) : 0.f);
+    }
+    if constexpr (GROUPED) {
+      float gap, *cf = reinterpret_cast<float*>(ct);
+#pragma unroll
+      for (int v = 0; v < MAXV; ++v) cf[li + LPT * v] = c[v];
+      const uint32_t out = groups_out<float, LPT, MAXV>(cf, reinterpret_cast<float*>(ct + PER), p, li, &gap);
+#pragma unroll
+      for (int v = 0; v < MAXV; ++v) key[v] = (out >> v) & 1u ? kOut : key[v];
+      // sums of two scores of size up to top, each rounded with its bias
+      top = seg_max<LPT>(top);
+      unsure |= !(gap > 2.f * err + 0x1p-21f * top);
+    }
+    // candidates by falling score: the k best, and those after them that the
+    // error does not part from the one before
     int32_t res_e[SLOTS];
 #pragma unroll
     for (int q = 0; q < SLOTS; ++q) res_e[q] = 0;
-    for (int j = 0; j < k; ++j) {
-      // the lane's best, then the segment's
-      double bv = -INFINITY;
-      int32_t bi = E;
+    float before = INFINITY;
+    int n = 0;
+    bool near = false;
+#pragma unroll 1
+    for (; n < 64; ++n) {
+      if (n == k && by_logit) break;
+      int32_t bv = key[0];
 #pragma unroll
-      for (int v = 0; v < MAXV; ++v) {
-        const bool in = !((taken >> v) & 1u);
-        // (a lane's experts rise with v: the first of equals is the lower id)
-        if (in && (c[v] > bv || bi == E)) {
-          bv = c[v];
-          bi = li + LPT * v;
-        }
-      }
-      const float hi = bi < E ? (float)bv : -INFINITY;
-      const float mv = seg_max<LPT>(hi);
-      bool cand = bi < E && hi == mv;
-      const uint64_t ball = __ballot(cand) & seg_mask;
-      if (__any(active && __popcll(ball) > 1)) {
-        const double top = seg_max_f64<LPT>(cand ? bv : -INFINITY);
-        cand = cand && bv == top;
-      }
-      const int32_t win = seg_min_i<LPT>(cand ? bi : E);
-      if (win == bi) taken |= 1u << (win / LPT);
+      for (int v = 1; v < MAXV; ++v) bv = max(bv, key[v]);
+      const int32_t mv = seg_max_i<LPT>(bv);
+      if (mv == kOut) break;  // none is left
+      int32_t bi = E;  // the lane's first of that score (its experts rise with v)
+#pragma unroll
+      for (int v = MAXV - 1; v >= 0; --v) bi = key[v] == mv ? li + LPT * v : bi;
+      const int32_t win = seg_min_i<LPT>(bi);
+      const float now = __int_as_float(mv ^ ((mv >> 31) & 0x7fffffff));
+      const bool apart = by_logit || n == 0 || before - now > err + 0x1p-23f * (fabsf(before) + fabsf(now));
+      if (n >= k && apart) break;
+      near |= !apart;
+      before = now;
+#pragma unroll
+      for (int v = 0; v < MAXV; ++v) key[v] = win == li + LPT * v ? kOut : key[v];
 #pragma unroll
       for (int q = 0; q < SLOTS; ++q)
-        if (j == q * LPT + li) res_e[q] = win;
+        if (n == q * LPT + li) res_e[q] = win;
     }
-    // the winners' scores, by the lanes that hold them
+    unsure |= n > k + 8 || n < k || (near && n == 64);
+    // ---- all scores in 64 bits, for a wave with an unsure token: NaN, groups within
+    // the error, or a crowd of candidates
+    const bool again = active && (__ballot(unsure) & seg_mask) != 0;
+    if (__any(again)) {
+      double d[MAXV], den = 1.0;
+#pragma unroll
+      for (int v = 0; v < MAXV; ++v) d[v] = exp(p.sigmoid ? -(double)l[v] : (double)l[v] - (double)m);
+      if (!p.sigmoid) {
+        double s = 0.0;
+#pragma unroll
+        for (int v = 0; v < MAXV; ++v) s += li + LPT * v < E ? d[v] : 0.0;
+        den = seg_sum_f64<LPT>(s);
+      }
+      uint32_t taken = 0;
+#pragma unroll
+      for (int v = 0; v < MAXV; ++v) {
+        const int e = li + LPT * v;
+        d[v] = (p.sigmoid ? 1.0 : d[v]) / (p.sigmoid ? 1.0 + d[v] : den);
+        if (e < E && p.bias != nullptr) d[v] += (double)p.bias[e];
+        if (e >= E) taken |= 1u << v;
+        if (e >= E || isnan(d[v])) d[v] = -INFINITY;
+      }
+      if constexpr (GROUPED) {
+#pragma unroll
+        for (int v = 0; v < MAXV; ++v) ct[li + LPT * v] = d[v];
+        double gap;
+        taken |= groups_out<double, LPT, MAXV>(ct, ct + PER, p, li, &gap);
+      }
+#pragma unroll 1
+      for (int j = 0; j < k; ++j) {
+        double bv = -INFINITY;
+        int32_t bi = E;
+#pragma unroll
+        for (int v = 0; v < MAXV; ++v)
+          if (!((taken >> v) & 1u) && (d[v] > bv || bi == E)) {
+            bv = d[v];
+            bi = li + LPT * v;
+          }
+        const double mv = seg_max_f64<LPT>(bi < E ? bv : -INFINITY);
+        const int32_t win = seg_min_i<LPT>(bi < E && bv == mv ? bi : E);
+        if (win == bi) taken |= 1u << (win / LPT);
+#pragma unroll
+        for (int q = 0; q < SLOTS; ++q)
+          if (again && j == q * LPT + li) res_e[q] = win;
+      }
+      if (again) {
+        n = k;
+        near = false;
+      }
+    }
+    // the candidates' scores in 64 bits, by the lanes that hold them; a softmax's
+    // sum is 64-bit where it does not cancel
+    double total = (double)sum;
+    const bool rank = __any(active && near);
+    if (!p.sigmoid && (rank || !p.renorm)) {
+      double s = 0.0;
+#pragma unroll 1
+      for (int e = li; e < E; e += LPT) s += exp((double)(float)row[e] - (double)m);
+      total = seg_sum_f64<LPT>(s);
+    }
     double w[SLOTS], part = 0.0;
+    int at[SLOTS];  // place among the chosen
 #pragma unroll
     for (int q = 0; q < SLOTS; ++q) {
       w[q] = 0.0;
-      if (q * LPT + li < k) {
-        const double l = (double)(float)row[res_e[q]];
-        w[q] = p.sigmoid ? sigmoid64(l) : exp(l - m) / sum;
-        part += w[q];
+      at[q] = q * LPT + li;
+      if (q * LPT + li < n) w[q] = score64((double)(float)row[res_e[q]], p.sigmoid, (double)m, total);
+    }
+    if (rank) {
+      // ranked among the candidates, which hold the k best in some order
+      double d[SLOTS];
+#pragma unroll
+      for (int q = 0; q < SLOTS; ++q) {
+        d[q] = w[q] + (p.bias != nullptr && q * LPT + li < n ? (double)p.bias[res_e[q]] : 0.0);
+        if (near) at[q] = q * LPT + li < n ? 0 : 64;
+      }
+      const int most = (int)seg_max<64>((float)(near ? n : 0));
+#pragma unroll
+      for (int q2 = 0; q2 < SLOTS; ++q2) {
+#pragma unroll 1
+        for (int i = 0; i < LPT && q2 * LPT + i < most; ++i) {
+          const int from = lane - li + i;
+          const double x = __shfl(d[q2], from, 64);
+          const int32_t e = __shfl(res_e[q2], from, 64);
+#pragma unroll
+          for (int q = 0; q < SLOTS; ++q)
+            at[q] += near && q2 * LPT + i < n && (x > d[q] || (x == d[q] && e < res_e[q])) ? 1 : 0;
+        }
       }
     }
+#pragma unroll
+    for (int q = 0; q < SLOTS; ++q) part += at[q] < k ? w[q] : 0.0;
     double f = p.scale;
     if (p.renorm) {
       const double den = seg_sum_f64<LPT>(part);
@@ -200,7 +344,7 @@ __global__ __launch_bounds__(kScoredThreads) void route_scored_kernel(
     if (active) {
 #pragma unroll
       for (int q = 0; q < SLOTS; ++q) {
-        const int j = q * LPT + li;
+        const int j = at[q];
         if (j < k) {
           sel[t * k + j] = res_e[q];
           weights[t * k + j] = (float)(w[q] * f);
@@ -212,10 +356,10 @@ __global__ __launch_bounds__(kScoredThreads) void route_scored_kernel(
   }
   __syncthreads();
   if constexpr (ONE) {
-    route_sort_one<kScoredThreads>(hist, ids, (int)(p.n_tokens * k), E, k, so);
+    route_sort_one<THREADS>(hist, ids, (int)(p.n_tokens * k), E, k, so);
     return;
   }
-  for (int e = threadIdx.x; e <= E; e += kScoredThreads) counts[b * (int64_t)(E + 1) + e] = hist[e];
+  for (int e = threadIdx.x; e <= E; e += THREADS) counts[b * (int64_t)(E + 1) + e] = hist[e];
 }
 
 // d logits.  With gw the weights' gradient, S = sum of the chosen scores:
@@ -271,8 +415,11 @@ __global__ __launch_bounds__(kScoredBwdThreads) void route_scored_bwd_kernel(
       if (id >= 0 && id < E) {
         sj[q] = (int32_t)id;
         const double x = (double)(float)row[id];
-        pj[q] = p.sigmoid ? sigmoid64(x) : exp(x - (double)mf) / (double)sum;
-        sg[q] = p.sigmoid ? sigmoid64(-x) : 0.0;
+        const double e = exp(p.sigmoid ? -x : x - (double)mf);
+        const double r = 1.0 / (p.sigmoid ? 1.0 + e : (double)sum);
+        pj[q] = p.sigmoid ? r : e * r;
+        // 1 - s = e / (1 + e), 1 where e overflows
+        sg[q] = !p.sigmoid ? 0.0 : r > 0.0 ? e * r : 1.0;
         dw[q] = (double)gw[t * k + j] * p.scale;
       }
     }
@@ -310,11 +457,11 @@ template <typename LT, int LPT, int MAXV, bool GROUPED>
 static void launch_scored(const LT* logits, const ScoredParams& p, int64_t tpc, int64_t n_chunks, float* w,
                           int64_t* sel, int32_t* counts, const RouteSortOut& so, hipStream_t s) {
   if (n_chunks == 1 && p.n_tokens * p.k <= kRouteOneMax)
-    hipLaunchKernelGGL((route_scored_kernel<LT, LPT, MAXV, true, GROUPED>), dim3(1), dim3(kScoredThreads), 0, s,
-                       logits, p, tpc, w, sel, counts, so);
+    hipLaunchKernelGGL((route_scored_kernel<LT, LPT, MAXV, true, GROUPED, scored_threads<LPT>(true)>), dim3(1),
+                       dim3(scored_threads<LPT>(true)), 0, s, logits, p, tpc, w, sel, counts, so);
   else
-    hipLaunchKernelGGL((route_scored_kernel<LT, LPT, MAXV, false, GROUPED>), dim3((unsigned)n_chunks),
-                       dim3(kScoredThreads), 0, s, logits, p, tpc, w, sel, counts, so);
+    hipLaunchKernelGGL((route_scored_kernel<LT, LPT, MAXV, false, GROUPED, scored_threads<LPT>(false)>), dim3((unsigned)n_chunks),
+                       dim3(scored_threads<LPT>(false)), 0, s, logits, p, tpc, w, sel, counts, so);
 }
 
 // Segment width: 8 experts per lane up to 512 experts, then 16.

@@ -973,6 +973,44 @@ std::tuple<OptT, OptT> mx4_backward(const Tensor& grad_output, const Tensor& x, 
   return {gx, grw};
 }
 
+// cvmm_route_scored as a C++ autograd function, like CvmmFunction: the logits
+// are the differentiable input, the weights the differentiable output.
+struct RouteScoredFunction : public torch::autograd::Function<RouteScoredFunction> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits,
+                                                int64_t top_k, const OptT& bias, int64_t scores, int64_t groups,
+                                                int64_t topk_groups, bool renormalize, double scale) {
+    auto out = route_scored(logits, top_k, bias, scores, groups, topk_groups, renormalize, scale,
+                            current_stream(logits));
+    ctx->saved_data["top_k"] = top_k;
+    ctx->saved_data["scores"] = scores;
+    ctx->saved_data["renormalize"] = renormalize;
+    ctx->saved_data["scale"] = scale;
+    ctx->save_for_backward({logits, out[1]});
+    ctx->mark_non_differentiable({out[1], out[2], out[3], out[4], out[5], out[6]});
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    torch::autograd::variable_list res(8);
+    if (!grads[0].defined()) return res;
+    const auto v = ctx->get_saved_variables();
+    res[0] = route_scored_backward(v[0], v[1], grads[0], ctx->saved_data["top_k"].toInt(),
+                                   ctx->saved_data["scores"].toInt(), ctx->saved_data["renormalize"].toBool(),
+                                   ctx->saved_data["scale"].toDouble(), current_stream(v[0]));
+    return res;
+  }
+};
+
+std::vector<Tensor> route_scored_apply(const Tensor& logits, int64_t top_k, const OptT& bias, int64_t scores,
+                                       int64_t groups, int64_t topk_groups, bool renormalize, double scale,
+                                       bool grad) {
+  require_device(logits, "logits");
+  if (grad) return RouteScoredFunction::apply(logits, top_k, bias, scores, groups, topk_groups, renormalize, scale);
+  return route_scored(logits, top_k, bias, scores, groups, topk_groups, renormalize, scale, current_stream(logits));
+}
+
 struct CvmmMx4Function : public torch::autograd::Function<CvmmMx4Function> {
   // x and reduction_weight (optional) are the differentiable inputs
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const OptT& rw, const Tensor& codes,
@@ -1072,6 +1110,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gelu_backward", &gelu_backward, py::arg("grad"), py::arg("pre_act"), py::arg("stream"));
   m.def("backward", &backward_py);
   m.def("cvmm_apply", &cvmm_apply);
+  m.def("route_scored_apply", &route_scored_apply);
   m.def("mx4_quantize_rows", &mx4_quantize_rows);
   m.def("mx4_quantize_keys", &mx4_quantize_keys);
   m.def("mx4_dequantize", &mx4_dequantize);
