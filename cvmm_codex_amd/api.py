@@ -327,18 +327,36 @@ class _Routing:
         self.by_e: Dict[int, Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]] = {}
         self.first_e: Optional[int] = None
         self.counted = counted
+        # expert count -> the sort's two buffers (int32, int64), views of which
+        # make a by_e entry where one is asked for
+        self.buffers: Dict[int, Tuple[torch.Tensor, torch.Tensor]] = {}
+
+    def counts(self, n_experts: int) -> Optional[torch.Tensor]:
+        """The sort workspace that holds the ids' histogram for this expert
+        count, and a note of the count for the next selection of this size."""
+        ws = None
+        if self.counted is not None:   # one use: the sort turns the counts into prefixes
+            ws = self.counted[1] if self.counted[0] == n_experts else None
+            self.counted = None
+        if not _compiling():
+            if len(_expert_guess) > 64:
+                _expert_guess.clear()
+            _expert_guess[(self.raw.numel(), self.k)] = n_experts
+        return ws
+
+    def keep(self, n_experts: int, i32: torch.Tensor, i64: torch.Tensor) -> None:
+        self.buffers[n_experts] = (i32, i64)
+        if self.first_e is None:
+            self.first_e = n_experts
 
     def get(self, n_experts: int, cast=None):
         hit = self.by_e.get(n_experts)
+        if hit is None and n_experts in self.buffers:
+            ssel, perm, tok, offsets, route_pos = N.host().routing_views(*self.buffers[n_experts])
+            perm._cvmm_route_pos = route_pos
+            hit = self.by_e[n_experts] = (ssel, perm, tok, offsets)
         if hit is None:
-            ws = None
-            if self.counted is not None:   # one use: the sort turns the counts into prefixes
-                ws = self.counted[1] if self.counted[0] == n_experts else None
-                self.counted = None
-            if not _compiling():
-                if len(_expert_guess) > 64:
-                    _expert_guess.clear()
-                _expert_guess[(self.raw.numel(), self.k)] = n_experts
+            ws = self.counts(n_experts)
             hit = (_sort_routes_cast(self.raw, n_experts, self.k, cast, ws) if cast is not None
                    else _sort_routes(self.raw, n_experts, self.k, ws))
             self.by_e[n_experts] = hit
@@ -350,7 +368,7 @@ class _Routing:
         if self.first_e is None:
             n = int(self.raw.max().item()) + 1 if self.raw.numel() else 1   # host sync
             self.get(max(n, 1))
-        return self.by_e[self.first_e]
+        return self.get(self.first_e)
 
 
 @dataclass(init=False)
@@ -668,16 +686,18 @@ def cvmm_route_scored(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor]
     args = (logits, k, None if bias is None else bias.detach(), N.SCORES[scores], groups, kept, bool(renormalize),
             float(scale))
     if _compiling():
-        w, sel, ssel, perm, tok, offsets, route_pos = _ops.route_scored(*args)
+        w, sel, *sort = _ops.route_scored(*args)
     else:
-        w, sel, ssel, perm, tok, offsets, route_pos = N.host().route_scored_apply(
-            *args, torch.is_grad_enabled() and logits.requires_grad)
-        perm._cvmm_route_pos = route_pos
-    sel = sel.view(*lead, k)
-    routing = _Routing(sel.reshape(-1), k)
-    routing.by_e[E] = (ssel, perm, tok, offsets)
-    routing.first_e = E
-    return w.view(*lead, k), sel, CVMMSel._deferred(sel, routing, False, None)
+        w, sel, *sort = N.host().route_scored_apply(*args, torch.is_grad_enabled() and logits.requires_grad)
+    if len(lead) != 1:
+        w, sel = w.view(*lead, k), sel.view(*lead, k)
+    routing = _Routing(sel.view(-1), k)
+    if _compiling():
+        routing.by_e[E] = tuple(sort[:4])
+        routing.first_e = E
+    else:
+        routing.keep(E, *sort)
+    return w, sel, CVMMSel._deferred(sel, routing, False, None)
 
 
 def _gate_grad_chunks(n_tokens: int, d_in: int, n_experts: int) -> int:
@@ -1133,6 +1153,18 @@ def cvmm_mx4(x: torch.Tensor, sel: Union[torch.Tensor, CVMMSel], keys: CVMMMx4,
         raise RuntimeError("cvmm_mx4: quantize_input is for inference (rounding to 4 bits has no gradient)")
     raw = sel._raw_shape_tensor()
     top_k = raw.shape[-1] if raw.ndim > 0 else 1
+    if not _compiling() and sel._pending() and E not in sel._routing.by_e:
+        # a recorded selection: its sort (if still to be made) and the product in
+        # one host call
+        r = sel._routing
+        bufs = r.buffers.get(E)
+        shape = [*rw.shape[:-1], d_out] if rw is not None else [*raw.shape, d_out]
+        y, i32, i64 = N.host().mx4_apply_recorded(
+            x, rw, keys.codes, keys.scales, E, d_in, d_out, r.raw, r.k, r.counts(E) if bufs is None else None,
+            *(bufs or (None, None)), sel._route_mode, _DTYPE_IDS[op], quantize_input, grad, shape)
+        if bufs is None:
+            r.keep(E, i32, i64)
+        return y
     sel._resolve(E)
     s, sel_index, out_index = sel._sel, sel._sel_index, sel._out_index
     _require_device(s, "sel")

@@ -214,9 +214,9 @@ def route_scored(logits: torch.Tensor, top_k: int, bias: Optional[torch.Tensor],
                                                                            torch.Tensor, torch.Tensor,
                                                                            torch.Tensor, torch.Tensor,
                                                                            torch.Tensor]:
-    out = N.host().route_scored(logits, top_k, bias, scores, groups, topk_groups, renormalize, scale,
-                                N.stream_of(logits.device))
-    return tuple(t.clone() for t in out)
+    w, sel, i32, i64 = N.host().route_scored_apply(logits, top_k, bias, scores, groups, topk_groups, renormalize,
+                                                   scale, False)
+    return (w, sel, *(t.clone() for t in N.host().routing_views(i32, i64)))
 
 
 @route_scored.register_fake

@@ -38,13 +38,13 @@ __device__ __forceinline__ uint32_t mx4_abs_bits(float v) { return __float_as_ui
 template <typename T>
 __global__ __launch_bounds__(kMx4Threads) void mx4_quantize_rows_kernel(const T* __restrict__ src, int64_t ld,
                                                                         int64_t rows, int64_t K, int64_t k128,
-                                                                        int64_t groups, bool vec,
+                                                                        int64_t groups, FastDiv by_groups, bool vec,
                                                                         uint8_t* __restrict__ codes,
                                                                         uint8_t* __restrict__ scales) {
   const int lane = threadIdx.x & 63;
   const int64_t item = (int64_t)blockIdx.x * (kMx4Threads / 64) + (threadIdx.x >> 6);
   if (item >= rows * groups) return;
-  const int64_t r = item / groups, g = item - r * groups;
+  const int64_t r = by_groups.div(item), g = item - r * groups;
   const int64_t k = g * 512 + lane * 8;
   float v[8];
   mx4_load8<T>(src + r * ld, k, K, vec, v);
@@ -108,26 +108,31 @@ __device__ __forceinline__ void mx4_unpack_to(uint32_t c, float scale, T (&v)[8]
   }
 }
 
-// Rows back: 8 values per thread into contiguous rows of K values.
+// Rows back, into contiguous rows of K values: a wave takes 512 values of a row,
+// as above.
 template <typename T>
 __global__ __launch_bounds__(kMx4Threads) void mx4_dequantize_rows_kernel(const uint8_t* __restrict__ codes,
                                                                           const uint8_t* __restrict__ scales,
                                                                           int64_t rows, int64_t K, int64_t k128,
-                                                                          int64_t groups, T* __restrict__ out) {
-  const int64_t per = (K + 7) / 8;
-  const int64_t item = (int64_t)blockIdx.x * kMx4Threads + threadIdx.x;
-  if (item >= rows * per) return;
-  const int64_t r = item / per, k = (item - r * per) * 8;
+                                                                          int64_t groups, FastDiv by_groups,
+                                                                          T* __restrict__ out) {
+  const int lane = threadIdx.x & 63;
+  const int64_t item = (int64_t)blockIdx.x * (kMx4Threads / 64) + (threadIdx.x >> 6);
+  if (item >= rows * groups) return;
+  const int64_t r = by_groups.div(item), g = item - r * groups;
+  const int64_t k = g * 512 + lane * 8;
+  if (k >= K) return;
   const uint32_t c = *reinterpret_cast<const uint32_t*>(codes + r * (k128 / 2) + k / 2);
-  const int b = (int)(k % 512) / 32;
-  const uint32_t sb = scales[(r * groups + k / 512) * 16 + (b & 3) * 4 + (b >> 2)];
+  const int b = lane >> 2;
   T v[8];
-  mx4_unpack_to<T>(c, mx4_scale(sb), v);
+  mx4_unpack_to<T>(c, mx4_scale(scales[(r * groups + g) * 16 + (b & 3) * 4 + (b >> 2)]), v);
   T* dst = out + r * K + k;
-  if (k + 8 <= K) {
-    __builtin_memcpy(dst, v, 8 * sizeof(T));
+  if (K % 8 == 0) {  // (rows and out 16-byte aligned)
+    __builtin_memcpy(__builtin_assume_aligned(dst, 16), v, 8 * sizeof(T));
   } else {
-    for (int i = 0; k + i < K; ++i) dst[i] = v[i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (k + i < K) dst[i] = v[i];
   }
 }
 
@@ -170,12 +175,13 @@ hipError_t launch_mx4_quantize_rows(const void* src, int32_t dtype, int64_t ld, 
   if (rows <= 0 || K <= 0) return hipSuccess;
   const int64_t groups = (K + 511) / 512;
   const int64_t blocks = (rows * groups + kMx4Threads / 64 - 1) / (kMx4Threads / 64);
-  if (blocks > 0x7fffffffll) return hipErrorInvalidValue;
+  if (rows * groups > 0x7fffffffll) return hipErrorInvalidValue;
   const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0 && (ld * (int64_t)dtype_size(dtype)) % 16 == 0;
   by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     hipLaunchKernelGGL((mx4_quantize_rows_kernel<T>), dim3((unsigned)blocks), dim3(kMx4Threads), 0, stream,
-                       (const T*)src, ld, rows, K, mx4_k128(K), groups, vec, (uint8_t*)codes, (uint8_t*)scales);
+                       (const T*)src, ld, rows, K, mx4_k128(K), groups, make_fast_div(groups), vec, (uint8_t*)codes,
+                       (uint8_t*)scales);
   });
   return hipGetLastError();
 }
@@ -196,12 +202,14 @@ hipError_t launch_mx4_quantize_keys(const void* src, int32_t dtype, int64_t se, 
 hipError_t launch_mx4_dequantize_rows(const void* codes, const void* scales, int64_t rows, int64_t K, void* out,
                                       int32_t dtype, hipStream_t stream) {
   if (rows <= 0 || K <= 0) return hipSuccess;
-  const int64_t items = rows * ((K + 7) / 8), blocks = (items + kMx4Threads - 1) / kMx4Threads;
-  if (blocks > 0x7fffffffll) return hipErrorInvalidValue;
+  const int64_t groups = (K + 511) / 512;
+  const int64_t blocks = (rows * groups + kMx4Threads / 64 - 1) / (kMx4Threads / 64);
+  if (rows * groups > 0x7fffffffll) return hipErrorInvalidValue;
   by_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     hipLaunchKernelGGL((mx4_dequantize_rows_kernel<T>), dim3((unsigned)blocks), dim3(kMx4Threads), 0, stream,
-                       (const uint8_t*)codes, (const uint8_t*)scales, rows, K, mx4_k128(K), (K + 511) / 512, (T*)out);
+                       (const uint8_t*)codes, (const uint8_t*)scales, rows, K, mx4_k128(K), groups, make_fast_div(groups),
+                       (T*)out);
   });
   return hipGetLastError();
 }

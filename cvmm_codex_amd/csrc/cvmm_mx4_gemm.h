@@ -415,7 +415,8 @@ __global__ __launch_bounds__(256, OCC) void mx4_gemm4_kernel(const Mx4Params p) 
   static_assert(STEPS % RING == 0, "sets by the panel's place in its chunk");
   const GemmParams& g = p.g;
   __shared__ __attribute__((aligned(1024))) char codes[BM * ROWB];
-  __shared__ __attribute__((aligned(16))) uint32_t row_scales[BM][kMx4ChunkK / 512 * 4];
+  // [512 k][16 rows][q][row]: a fragment's 64 scales are 64 consecutive dwords
+  __shared__ __attribute__((aligned(16))) uint32_t row_scales[kMx4ChunkK / 512][BM / 16][4][16];
   __shared__ RouteMeta<BM> meta;
   __shared__ Mx4Rows<BM> rows;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -451,7 +452,8 @@ __global__ __launch_bounds__(256, OCC) void mx4_gemm4_kernel(const Mx4Params p) 
     const int64_t sr = rows.a[tid >> 1], gr = (int64_t)c * (kMx4ChunkK / 512) + (tid & 1);
     uint4 s = make_uint4(0, 0, 0, 0);
     if (sr >= 0 && gr < p.a_groups) s = *reinterpret_cast<const uint4*>(p.a_scales + (sr * p.a_groups + gr) * 16);
-    *reinterpret_cast<uint4*>(&row_scales[tid >> 1][(tid & 1) * 4]) = s;
+    uint32_t* d = &row_scales[tid & 1][tid >> 5][0][(tid >> 1) & 15];
+    d[0] = s.x; d[16] = s.y; d[32] = s.z; d[48] = s.w;
   };
   const int a_at = fr * ROWB + ((fq ^ fr) << 4);
   f32x4_t acc[4][MB];
@@ -479,7 +481,7 @@ __global__ __launch_bounds__(256, OCC) void mx4_gemm4_kernel(const Mx4Params p) 
 #pragma unroll
       for (int j = 0; j < MB / 2; ++j) {
         a[j] = *reinterpret_cast<const uint4*>(ap + (h * (MB / 2) + j) * 16 * ROWB);
-        sa[j] = row_scales[(h * (MB / 2) + j) * 16 + fr][m / 4 * 4 + fq];
+        sa[j] = row_scales[m / 4][h * (MB / 2) + j][fq][fr];
       }
 #pragma unroll
       for (int j = 0; j < MB / 2; ++j) {

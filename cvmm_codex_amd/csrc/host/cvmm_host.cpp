@@ -177,6 +177,35 @@ std::vector<Tensor> sort_routes(const Tensor& raw, int64_t n_experts, int64_t to
   return {ssel, perm, tok, off, pos};
 }
 
+// The sort's outputs as its two buffers: int32 [2 R] (sorted ids, route_pos) and
+// int64 [2 R + E] (perm, perm // top_k, offsets).
+std::vector<Tensor> routing_views(const Tensor& i32, const Tensor& i64) {
+  const int64_t R = i32.numel() / 2, E = i64.numel() - 2 * R;
+  return {i32.narrow(0, 0, R), i64.narrow(0, 0, R), i64.narrow(0, R, R), i64.narrow(0, 2 * R, E),
+          i32.narrow(0, R, R)};
+}
+
+std::pair<Tensor, Tensor> sort_routes_buffers(const Tensor& raw, int64_t n_experts, int64_t top_k, int64_t stream,
+                                              const OptT& counted_ws) {
+  require_device(raw, "sel");
+  Tensor flat = raw;
+  if (flat.scalar_type() != at::kInt && flat.scalar_type() != at::kLong) flat = flat.to(at::kInt);
+  if (!flat.is_contiguous()) flat = flat.contiguous();
+  const int64_t R = flat.numel();
+  Tensor i32 = at::empty({2 * R}, opts(flat, at::kInt));
+  Tensor i64 = at::empty({2 * R + n_experts}, opts(flat, at::kLong));
+  const size_t ws_bytes = cvmm_sort_workspace_bytes(R, (int32_t)n_experts);
+  Tensor ws = counted_ws.has_value() ? *counted_ws : sort_workspace(flat, stream, ws_bytes);
+  int32_t* a = tptr<int32_t>(i32);
+  int64_t* b = tptr<int64_t>(i64);
+  check(cvmm_sort_routes_cast_keys_ex(ptr(flat), flat.scalar_type() == at::kLong ? 1 : 0, R, (int32_t)n_experts,
+                                      std::max<int64_t>(top_k, 1), a, b, b + R, b + 2 * R, a + R, nullptr, ptr(ws),
+                                      (size_t)ws.numel(), nullptr, 0, 0, 0, 0, 0, 0, 0, nullptr, nullptr, 0,
+                                      counted_ws.has_value() ? CVMM_FLAG_COUNTS_READY : 0, (void*)stream),
+        "cvmm_sort_routes");
+  return {i32, i64};
+}
+
 // The op-dtype weight copies of a cast (`layout`: CVMM_CAST_* bits): kt
 // [E, d_out, d_in] or, interleaved, [d_out, E, d_in]; kn [E, d_in, d_out] or
 // [d_in, E, d_out].
@@ -271,7 +300,7 @@ Tensor route_topk_backward(const Tensor& logits, const Tensor& sel, const Tensor
   return out.view(logits.sizes());
 }
 
-// The router of balanced models: outputs as route_topk's.
+// The router of balanced models: (weights, sel, and the sort's two buffers).
 std::vector<Tensor> route_scored(const Tensor& logits, int64_t top_k, const OptT& bias, int64_t scores,
                                  int64_t groups, int64_t topk_groups, bool renormalize, double scale,
                                  int64_t stream) {
@@ -292,17 +321,16 @@ std::vector<Tensor> route_scored(const Tensor& logits, int64_t top_k, const OptT
   Tensor i32 = at::empty({2 * R}, opts(l, at::kInt));
   // (no tokens: no launch writes the offsets)
   Tensor i64 = T > 0 ? at::empty({2 * R + E}, opts(l, at::kLong)) : at::zeros({E}, opts(l, at::kLong));
-  Tensor ssel = i32.narrow(0, 0, R), pos = i32.narrow(0, R, R);
-  Tensor perm = i64.narrow(0, 0, R), tok = i64.narrow(0, R, R), off = i64.narrow(0, 2 * R, E);
+  int32_t* a = tptr<int32_t>(i32);
+  int64_t* b64 = tptr<int64_t>(i64);
   const size_t ws_bytes = cvmm_route_topk_workspace_bytes(T, (int32_t)E, top_k);
   Tensor ws = sort_workspace(l, stream, ws_bytes);
   check(cvmm_route_scored(ptr(l), dtype_id(l.scalar_type()), T, std::max(l.stride(0), E), (int32_t)E, top_k,
                           tptr<float>(b), (int32_t)scores, (int32_t)groups, (int32_t)topk_groups, renormalize ? 1 : 0,
-                          scale, tptr<float>(w), tptr<int64_t>(sel), tptr<int32_t>(ssel), tptr<int64_t>(perm),
-                          tptr<int64_t>(tok), tptr<int64_t>(off), tptr<int32_t>(pos), ptr(ws), (size_t)ws.numel(),
-                          (void*)stream),
+                          scale, tptr<float>(w), tptr<int64_t>(sel), a, b64, b64 + R, b64 + 2 * R, a + R, ptr(ws),
+                          (size_t)ws.numel(), (void*)stream),
         "cvmm_route_scored");
-  return {w, sel, ssel, perm, tok, off, pos};
+  return {w, sel, i32, i64};
 }
 
 Tensor route_scored_backward(const Tensor& logits, const Tensor& sel, const Tensor& grad_weights, int64_t top_k,
@@ -893,84 +921,120 @@ void mx4_check_keys(const Tensor& codes, const Tensor& scales, int64_t E, int64_
     throw py::value_error("cvmm_mx4: codes and scales are not those of the weights' shape");
 }
 
+// A sorted selection: pointers into the sort's buffers, or into a selector's own
+// tensors (both kept by the caller).
+struct Mx4Routes {
+  const int64_t *sel_index, *out_index, *offsets;
+  const int32_t* pos;
+  int64_t R, E;
+};
+
+Mx4Routes routes_of_buffers(const Tensor& i32, const Tensor& i64, bool route_input) {
+  const int64_t R = i32.numel() / 2;
+  const int64_t* p = tptr<int64_t>(i64);
+  return {route_input ? p : p + R, route_input ? nullptr : p, p + 2 * R, tptr<int32_t>(i32) + R, R,
+          i64.numel() - 2 * R};
+}
+
 // y (cvmm_forward_impl with 4-bit weights): [R or R / k, d_out] in the op dtype.
-Tensor mx4_forward(const Tensor& x, const Tensor& codes, const Tensor& scales, int64_t d_in, int64_t d_out,
-                   const Tensor& sel_index, const OptT& out_index, const Tensor& offsets, const OptT& route_pos,
-                   const OptT& rw, int64_t op_id, bool quantize_input, int64_t stream) {
+Tensor mx4_forward_impl(const Tensor& x, const Tensor& codes, const Tensor& scales, int64_t d_in, int64_t d_out,
+                        const Mx4Routes& r, const OptT& rw, int64_t op_id, bool quantize_input, int64_t stream,
+                        at::IntArrayRef shape) {
   require_device(x, "x");
-  require_device(sel_index, "sel_index");
   const auto op = dtype_of(op_id);
-  const int64_t E = offsets.numel();
-  mx4_check_keys(codes, scales, E, d_in, d_out);
-  if (x.size(-1) != d_in) throw py::value_error("cvmm_mx4: x.shape[-1] must equal the weights' d_in");
+  mx4_check_keys(codes, scales, r.E, d_in, d_out);
+  if (x.dim() < 1 || x.size(-1) != d_in) throw py::value_error("cvmm_mx4: x.shape[-1] must equal the weights' d_in");
   Tensor xf = rows_of(x.scalar_type() == op ? x : x.to(op), d_in);
-  Tensor si = as_i64(sel_index);
-  OptT oi = as_i64(out_index);
-  const int64_t R = si.numel();
-  if (oi.has_value() && oi->numel() != R)
-    throw py::value_error("cvmm_mx4: sel_index/out_index must have one entry per route");
   OptT rwf;
   int64_t k = 1;
   if (rw.has_value()) {
     require_device(*rw, "reduction_weight");
-    if (rw->numel() != R || rw->dim() < 1)
+    if (rw->numel() != r.R || rw->dim() < 1)
       throw py::value_error("cvmm_mx4: reduction_weight must have one entry per route");
     k = std::max<int64_t>(rw->size(-1), 1);
-    rwf = rw->reshape({-1}).to(at::kFloat).contiguous();
+    rwf = rw->scalar_type() == at::kFloat && rw->is_contiguous() ? *rw : rw->to(at::kFloat).contiguous();
   }
-  const int64_t rows = R / k;
-  Tensor out = at::empty({rows, d_out}, opts(x, op));
-  if (R == 0) return out;
-  const size_t ws_bytes = cvmm_mx4_fwd_workspace_bytes(R, d_in, d_out, xf.size(0), rwf.has_value() ? 1 : 0,
-                                                       route_pos.has_value() ? 1 : 0, mx4_copied(xf, d_in) ? 1 : 0,
+  const int64_t rows = r.R / k;
+  Tensor out = at::empty(shape, opts(x, op));
+  if (out.numel() != rows * d_out) throw py::value_error("cvmm_mx4: the output's shape does not hold the routes");
+  if (r.R == 0) return out;
+  const size_t ws_bytes = cvmm_mx4_fwd_workspace_bytes(r.R, d_in, d_out, xf.size(0), rwf.has_value() ? 1 : 0,
+                                                       r.pos != nullptr ? 1 : 0, mx4_copied(xf, d_in) ? 1 : 0,
                                                        quantize_input ? 1 : 0);
   OptT ws;
   if (ws_bytes) ws = at::empty({(int64_t)ws_bytes}, opts(x, at::kByte));
-  check(cvmm_mx4_fwd(ptr(xf), (int32_t)op_id, xf.size(0), xf.stride(0), ptr(codes), ptr(scales), (int32_t)E, d_in,
-                     d_out, tptr<int64_t>(si), tptr<int64_t>(oi), R, tptr<int64_t>(offsets),
-                     tptr<int32_t>(route_pos), tptr<float>(rwf), k, quantize_input ? 1 : 0, ptr(out), rows, d_out,
-                     ptr(ws), ws_bytes, (void*)stream),
+  check(cvmm_mx4_fwd(ptr(xf), (int32_t)op_id, xf.size(0), xf.stride(0), ptr(codes), ptr(scales), (int32_t)r.E, d_in,
+                     d_out, r.sel_index, r.out_index, r.R, r.offsets, r.pos, tptr<float>(rwf), k,
+                     quantize_input ? 1 : 0, ptr(out), rows, d_out, ptr(ws), ws_bytes, (void*)stream),
         "cvmm_mx4");
   return out;
 }
 
 // (grad_x, grad_reduction_weight) for frozen 4-bit weights.
-std::tuple<OptT, OptT> mx4_backward(const Tensor& grad_output, const Tensor& x, const Tensor& codes,
-                                    const Tensor& scales, int64_t d_in, int64_t d_out, const Tensor& sel_index,
-                                    const OptT& out_index, const Tensor& offsets, const OptT& route_pos,
-                                    const OptT& rw, int64_t top_k, int64_t op_id, bool need_grad_x,
-                                    bool need_grad_rw, int64_t stream) {
+std::tuple<OptT, OptT> mx4_backward_impl(const Tensor& grad_output, const Tensor& x, const Tensor& codes,
+                                         const Tensor& scales, int64_t d_in, int64_t d_out, const Mx4Routes& r,
+                                         const OptT& rw, int64_t top_k, int64_t op_id, bool need_grad_x,
+                                         bool need_grad_rw, int64_t stream) {
   const auto op = dtype_of(op_id);
-  const int64_t E = offsets.numel(), R = sel_index.numel();
   const int64_t k = rw.has_value() ? std::max<int64_t>(rw->size(-1), 1) : std::max<int64_t>(top_k, 1);
   Tensor g = rows_of(grad_output.scalar_type() == op ? grad_output : grad_output.to(op), d_out);
-  Tensor si = as_i64(sel_index);
-  OptT oi = as_i64(out_index);
   OptT rwf, gx, grw;
-  if (rw.has_value()) rwf = rw->reshape({-1}).to(at::kFloat).contiguous();
-  // x in fp32 or the op type (the product's own rows are x in the op type)
-  Tensor xr = rows_of(x.scalar_type() == op ? x : x.to(op), d_in);
+  if (rw.has_value()) rwf = rw->to(at::kFloat).contiguous();
+  // the rows the product saw: x in the op type (for the routing weights' gradient alone)
+  Tensor xr = rows_of(need_grad_rw && x.scalar_type() != op ? x.to(op) : x, d_in);
   const auto gx_type = x.scalar_type() == op ? op : at::kFloat;
-  if (need_grad_x) gx = at::empty(xr.sizes(), opts(x, gx_type));
-  if (need_grad_rw) grw = at::empty({R}, opts(x, at::kFloat));
-  if (R > 0) {
-    const size_t ws_bytes = cvmm_mx4_bwd_x_workspace_bytes(R, d_in, d_out, g.size(0), need_grad_x && oi.has_value() ? 1 : 0,
-                                                           route_pos.has_value() ? 1 : 0, mx4_copied(g, d_out) ? 1 : 0,
+  if (need_grad_x) gx = at::empty({xr.size(0), d_in}, opts(x, gx_type));
+  if (need_grad_rw) grw = at::empty(rw->sizes(), opts(x, at::kFloat));
+  if (r.R > 0) {
+    const bool copied = mx4_copied(g, d_out);
+    const size_t ws_bytes = cvmm_mx4_bwd_x_workspace_bytes(r.R, d_in, d_out, g.size(0),
+                                                           need_grad_x && r.out_index != nullptr ? 1 : 0,
+                                                           r.pos != nullptr ? 1 : 0, copied ? 1 : 0,
                                                            need_grad_rw ? 1 : 0, dtype_id(gx_type));
     OptT ws;
     if (ws_bytes) ws = at::empty({(int64_t)ws_bytes}, opts(x, at::kByte));
-    check(cvmm_mx4_bwd_x(ptr(g), (int32_t)op_id, g.size(0), g.stride(0), ptr(codes), ptr(scales), (int32_t)E, d_in,
-                         d_out, tptr<int64_t>(si), tptr<int64_t>(oi), R, tptr<int64_t>(offsets),
-                         tptr<int32_t>(route_pos), tptr<float>(rwf), k, ptr(xr), (int32_t)op_id, xr.size(0),
-                         xr.stride(0), ptr(gx), dtype_id(gx_type), gx.has_value() ? gx->size(0) : 0, d_in,
-                         tptr<float>(grw), ptr(ws), ws_bytes, (void*)stream),
+    check(cvmm_mx4_bwd_x(ptr(g), (int32_t)op_id, g.size(0), g.stride(0), ptr(codes), ptr(scales), (int32_t)r.E, d_in,
+                         d_out, r.sel_index, r.out_index, r.R, r.offsets, r.pos, tptr<float>(rwf), k, ptr(xr),
+                         need_grad_rw ? (int32_t)op_id : dtype_id(gx_type), xr.size(0), xr.stride(0), ptr(gx),
+                         dtype_id(gx_type), gx.has_value() ? gx->size(0) : 0, d_in, tptr<float>(grw), ptr(ws), ws_bytes,
+                         (void*)stream),
           "cvmm_mx4 backward");
   } else if (gx.has_value()) {
     gx->zero_();
   }
   if (gx.has_value()) gx = gx->to(x.scalar_type()).view(x.sizes());
-  if (grw.has_value()) grw = grw->to(rw->scalar_type()).view(rw->sizes());
+  if (grw.has_value()) grw = grw->to(rw->scalar_type());
   return {gx, grw};
+}
+
+// The same over a selector's own tensors.
+Mx4Routes routes_of_tensors(Tensor& sel_index, OptT& out_index, const Tensor& offsets, const OptT& route_pos) {
+  require_device(sel_index, "sel_index");
+  require_device(offsets, "offsets");
+  sel_index = as_i64(sel_index);
+  out_index = as_i64(out_index);
+  if (out_index.has_value() && out_index->numel() != sel_index.numel())
+    throw py::value_error("cvmm_mx4: sel_index/out_index must have one entry per route");
+  return {tptr<int64_t>(sel_index), tptr<int64_t>(out_index), tptr<int64_t>(offsets), tptr<int32_t>(route_pos),
+          sel_index.numel(), offsets.numel()};
+}
+
+Tensor mx4_forward(const Tensor& x, const Tensor& codes, const Tensor& scales, int64_t d_in, int64_t d_out,
+                   Tensor sel_index, OptT out_index, const Tensor& offsets, const OptT& route_pos, const OptT& rw,
+                   int64_t op_id, bool quantize_input, int64_t stream) {
+  const Mx4Routes r = routes_of_tensors(sel_index, out_index, offsets, route_pos);
+  const int64_t k = rw.has_value() && rw->dim() > 0 ? std::max<int64_t>(rw->size(-1), 1) : 1;
+  return mx4_forward_impl(x, codes, scales, d_in, d_out, r, rw, op_id, quantize_input, stream, {r.R / k, d_out});
+}
+
+std::tuple<OptT, OptT> mx4_backward(const Tensor& grad_output, const Tensor& x, const Tensor& codes,
+                                    const Tensor& scales, int64_t d_in, int64_t d_out, Tensor sel_index,
+                                    OptT out_index, const Tensor& offsets, const OptT& route_pos, const OptT& rw,
+                                    int64_t top_k, int64_t op_id, bool need_grad_x, bool need_grad_rw,
+                                    int64_t stream) {
+  const Mx4Routes r = routes_of_tensors(sel_index, out_index, offsets, route_pos);
+  return mx4_backward_impl(grad_output, x, codes, scales, d_in, d_out, r, rw, top_k, op_id, need_grad_x,
+                           need_grad_rw, stream);
 }
 
 // cvmm_route_scored as a C++ autograd function, like CvmmFunction: the logits
@@ -986,7 +1050,7 @@ struct RouteScoredFunction : public torch::autograd::Function<RouteScoredFunctio
     ctx->saved_data["renormalize"] = renormalize;
     ctx->saved_data["scale"] = scale;
     ctx->save_for_backward({logits, out[1]});
-    ctx->mark_non_differentiable({out[1], out[2], out[3], out[4], out[5], out[6]});
+    ctx->mark_non_differentiable({out[1], out[2], out[3]});
     ctx->set_materialize_grads(false);
     return out;
   }
@@ -1012,49 +1076,86 @@ std::vector<Tensor> route_scored_apply(const Tensor& logits, int64_t top_k, cons
 }
 
 struct CvmmMx4Function : public torch::autograd::Function<CvmmMx4Function> {
-  // x and reduction_weight (optional) are the differentiable inputs
+  // x and reduction_weight (optional) are the differentiable inputs.  The
+  // selection: the sort's buffers i32 and i64, or (i32 undefined) sel_index in
+  // i64's place with out_index, offsets and route_pos.
+  static Mx4Routes routes(Tensor& i32, Tensor& i64, OptT& out_index, const OptT& offsets, const OptT& pos,
+                          bool route_input) {
+    if (i32.defined()) return routes_of_buffers(i32, i64, route_input);
+    return routes_of_tensors(i64, out_index, *offsets, pos);
+  }
+
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const OptT& rw, const Tensor& codes,
-                        const Tensor& scales, int64_t d_in, int64_t d_out, const Tensor& sel_index,
-                        const OptT& out_index, const Tensor& offsets, const OptT& route_pos, int64_t top_k,
-                        int64_t op_id, const std::vector<int64_t>& out_shape) {
+                        const Tensor& scales, int64_t d_in, int64_t d_out, Tensor i32, Tensor i64, OptT out_index,
+                        const OptT& offsets, const OptT& route_pos, bool route_input, int64_t top_k, int64_t op_id,
+                        const std::vector<int64_t>& out_shape) {
     const bool need_x = x.requires_grad(), need_rw = rw.has_value() && rw->requires_grad();
     ctx->saved_data["d_in"] = d_in;
     ctx->saved_data["d_out"] = d_out;
     ctx->saved_data["top_k"] = top_k;
     ctx->saved_data["op_id"] = op_id;
-    ctx->saved_data["need"] = (int64_t)((need_x ? 1 : 0) | (need_rw ? 2 : 0));
-    Tensor out = mx4_forward(x, codes, scales, d_in, d_out, sel_index, out_index, offsets, route_pos, rw, op_id, false,
-                             current_stream(x));
-    ctx->save_for_backward({x, opt_or_undef(rw), codes, scales, sel_index, opt_or_undef(out_index), offsets,
-                            opt_or_undef(route_pos)});
-    return at::_unsafe_view(out, out_shape);
+    ctx->saved_data["need"] = (int64_t)((need_x ? 1 : 0) | (need_rw ? 2 : 0) | (route_input ? 4 : 0));
+    const Mx4Routes r = routes(i32, i64, out_index, offsets, route_pos, route_input);
+    Tensor out = mx4_forward_impl(x, codes, scales, d_in, d_out, r, rw, op_id, false, current_stream(x), out_shape);
+    ctx->save_for_backward({x, opt_or_undef(rw), codes, scales, i32, i64, opt_or_undef(out_index),
+                            opt_or_undef(offsets), opt_or_undef(route_pos)});
+    return out;
   }
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
-    const auto v = ctx->get_saved_variables();
+    auto v = ctx->get_saved_variables();
     const int64_t need = ctx->saved_data["need"].toInt();
-    auto [gx, grw] = mx4_backward(grads[0], v[0], v[2], v[3], ctx->saved_data["d_in"].toInt(),
-                                  ctx->saved_data["d_out"].toInt(), v[4], undef_or_opt(v[5]), v[6],
-                                  undef_or_opt(v[7]), undef_or_opt(v[1]), ctx->saved_data["top_k"].toInt(),
-                                  ctx->saved_data["op_id"].toInt(), (need & 1) != 0, (need & 2) != 0,
-                                  current_stream(v[0]));
+    OptT out_index = undef_or_opt(v[6]);
+    const Mx4Routes r = routes(v[4], v[5], out_index, undef_or_opt(v[7]), undef_or_opt(v[8]), (need & 4) != 0);
+    auto [gx, grw] = mx4_backward_impl(grads[0], v[0], v[2], v[3], ctx->saved_data["d_in"].toInt(),
+                                       ctx->saved_data["d_out"].toInt(), r, undef_or_opt(v[1]),
+                                       ctx->saved_data["top_k"].toInt(), ctx->saved_data["op_id"].toInt(),
+                                       (need & 1) != 0, (need & 2) != 0, current_stream(v[0]));
     // one entry per forward argument
-    return {opt_or_undef(gx), opt_or_undef(grw), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(),
-            Tensor(), Tensor(), Tensor(), Tensor()};
+    torch::autograd::variable_list res(15);
+    res[0] = opt_or_undef(gx);
+    res[1] = opt_or_undef(grw);
+    return res;
   }
 };
 
 Tensor mx4_apply(const Tensor& x, const OptT& rw, const Tensor& codes, const Tensor& scales, int64_t d_in,
-                 int64_t d_out, const Tensor& sel_index, const OptT& out_index, const Tensor& offsets,
-                 const OptT& route_pos, int64_t top_k, int64_t op_id, bool quantize_input, bool grad,
-                 const std::vector<int64_t>& out_shape) {
-  if (!grad)
-    return mx4_forward(x, codes, scales, d_in, d_out, sel_index, out_index, offsets, route_pos, rw, op_id,
-                       quantize_input, current_stream(x))
-        .view(out_shape);
-  return CvmmMx4Function::apply(x, rw, codes, scales, d_in, d_out, sel_index, out_index, offsets, route_pos, top_k,
-                                op_id, out_shape);
+                 int64_t d_out, Tensor sel_index, OptT out_index, const Tensor& offsets, const OptT& route_pos,
+                 int64_t top_k, int64_t op_id, bool quantize_input, bool grad, const std::vector<int64_t>& out_shape) {
+  require_device(x, "x");
+  if (grad)
+    return CvmmMx4Function::apply(x, rw, codes, scales, d_in, d_out, Tensor(), sel_index, out_index, OptT(offsets),
+                                  route_pos, !out_index.has_value(), top_k, op_id, out_shape);
+  const Mx4Routes r = routes_of_tensors(sel_index, out_index, offsets, route_pos);
+  return mx4_forward_impl(x, codes, scales, d_in, d_out, r, rw, op_id, quantize_input, current_stream(x), out_shape);
+}
+
+// A recorded selection in one call: sorted here unless its buffers are given.
+// Returns (y, i32, i64).
+std::tuple<Tensor, Tensor, Tensor> mx4_apply_recorded(const Tensor& x, const OptT& rw, const Tensor& codes,
+                                                      const Tensor& scales, int64_t n_experts, int64_t d_in,
+                                                      int64_t d_out, const Tensor& raw, int64_t top_k,
+                                                      const OptT& counted_ws, const OptT& i32_in, const OptT& i64_in,
+                                                      bool route_input, int64_t op_id, bool quantize_input, bool grad,
+                                                      const std::vector<int64_t>& out_shape) {
+  require_device(x, "x");
+  const int64_t stream = current_stream(x);
+  Tensor i32, i64;
+  if (i32_in.has_value()) {
+    i32 = *i32_in;
+    i64 = *i64_in;
+  } else {
+    std::tie(i32, i64) = sort_routes_buffers(raw, n_experts, top_k, stream, counted_ws);
+  }
+  Tensor y;
+  if (grad)
+    y = CvmmMx4Function::apply(x, rw, codes, scales, d_in, d_out, i32, i64, OptT(), OptT(), OptT(), route_input, top_k,
+                               op_id, out_shape);
+  else
+    y = mx4_forward_impl(x, codes, scales, d_in, d_out, routes_of_buffers(i32, i64, route_input), rw, op_id,
+                         quantize_input, stream, out_shape);
+  return {y, i32, i64};
 }
 
 // The Python-facing forward and backward (torch.compile's ops): no kept rows.
@@ -1095,8 +1196,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("route_topk", &route_topk, py::arg("logits"), py::arg("top_k"), py::arg("renormalize"), py::arg("stream"));
   m.def("route_topk_backward", &route_topk_backward, py::arg("logits"), py::arg("sel"), py::arg("grad_weights"),
         py::arg("top_k"), py::arg("renormalize"), py::arg("stream"));
-  m.def("route_scored", &route_scored, py::arg("logits"), py::arg("top_k"), py::arg("bias"), py::arg("scores"),
-        py::arg("groups"), py::arg("topk_groups"), py::arg("renormalize"), py::arg("scale"), py::arg("stream"));
   m.def("route_scored_backward", &route_scored_backward, py::arg("logits"), py::arg("sel"), py::arg("grad_weights"),
         py::arg("top_k"), py::arg("scores"), py::arg("renormalize"), py::arg("scale"), py::arg("stream"));
   m.def("sort_routes_cast", &sort_routes_cast, py::arg("raw"), py::arg("n_experts"), py::arg("top_k"),
@@ -1117,6 +1216,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mx4_forward", &mx4_forward);
   m.def("mx4_backward", &mx4_backward);
   m.def("mx4_apply", &mx4_apply);
+  m.def("mx4_apply_recorded", &mx4_apply_recorded);
+  m.def("routing_views", &routing_views);
   // operand rules, exposed for tests
   m.def("storage_for", [](const Tensor& t, int64_t op_id) { return storage_for(t, dtype_of(op_id)); });
   m.def("keys_view", &keys_view);
