@@ -73,6 +73,7 @@ _SIGS = {
     "cvmm_route_topk": (ctypes.c_int, [_P, _I32, _I64, _I64, _I32, _I64, _I32, _P, _P,
                                        _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "cvmm_route_topk_backward": (ctypes.c_int, [_P, _I32, _I64, _I64, _I32, _I64, _I32, _P, _P, _P, _I64, _P]),
+    "cvmm_route_scored_workspace_bytes": (_SZ, [_I64, _I32, _I64]),
     "cvmm_route_scored": (ctypes.c_int, [_P, _I32, _I64, _I64, _I32, _I64, _P, _I32, _I32, _I32, _I32,
                                          ctypes.c_double, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "cvmm_route_scored_backward": (ctypes.c_int, [_P, _I32, _I64, _I64, _I32, _I64, _I32, _I32, ctypes.c_double,

@@ -723,6 +723,11 @@ static int scored_args_ok(const char* what, int32_t logits_dtype, int64_t n_toke
   return CVMM_OK;
 }
 
+size_t cvmm_route_scored_workspace_bytes(int64_t n_tokens, int32_t n_experts, int64_t top_k) {
+  if (n_tokens < 0 || n_experts <= 0 || top_k <= 0) return 0;
+  return scored_workspace_bytes(n_tokens, n_experts, top_k);
+}
+
 int cvmm_route_scored(const void* logits, int32_t logits_dtype, int64_t n_tokens, int64_t logits_ld,
                       int32_t n_experts, int64_t top_k, const float* bias, int32_t scores, int32_t groups,
                       int32_t topk_groups, int32_t renormalize, double scale, float* weights, int64_t* sel,
@@ -736,7 +741,7 @@ int cvmm_route_scored(const void* logits, int32_t logits_dtype, int64_t n_tokens
                 topk_groups, (long long)top_k);
   if (topk_groups < groups && groups > kRouteMaxGroups)
     return fail(CVMM_ERR_UNSUPPORTED, "cvmm_route_scored: at most %d groups", kRouteMaxGroups);
-  const size_t need = route_workspace_bytes(n_tokens, n_experts, top_k);
+  const size_t need = scored_workspace_bytes(n_tokens, n_experts, top_k);
   if (workspace == nullptr || workspace_bytes < need)
     return fail(CVMM_ERR_WORKSPACE, "cvmm_route_scored: workspace too small (%zu < %zu)", workspace_bytes, need);
   if (n_tokens == 0) return CVMM_OK;
@@ -1641,7 +1646,7 @@ int cvmm_bwd_w_rows(const void* x, int32_t x_dtype, int64_t x_rows, int64_t x_ld
 namespace {
 
 bool mx4_sizes_ok(int64_t E, int64_t K, int64_t N) {
-  constexpr int64_t kMax = int64_t(1) << 31;
+  constexpr int64_t kMax = int64_t(1) << 30;  // (row bytes in 32 bits)
   return E > 0 && E < kMax && K > 0 && K < kMax && N > 0 && N < kMax &&
          E <= (int64_t(1) << 46) / (mx4_panels_n(N) * mx4_panels_k(K));
 }
@@ -1763,7 +1768,8 @@ int cvmm_mx4_fwd(const void* x, int32_t x_dtype, int64_t x_rows, int64_t x_ld, c
     return fail(CVMM_ERR_INVALID, "cvmm_mx4_fwd: rows must be 16-bit");
   const bool weighted = reduction_weight != nullptr;
   if (!mx4_sizes_ok(n_experts, d_in, d_out) || n_routes < 0 || n_routes > 0x7fffffff || x_rows < 0 ||
-      (x_rows > 1 && x_ld < d_in) || (out_rows > 1 && out_ld < d_out) || (weighted && reduce_k <= 0) ||
+      (x_rows > 1 && x_ld < d_in) || (out_rows > 1 && out_ld < d_out) || out_ld >= int64_t(1) << 30 ||
+      (weighted && reduce_k <= 0) ||
       out_rows * (weighted ? reduce_k : 1) != n_routes)
     return fail(CVMM_ERR_INVALID, "cvmm_mx4_fwd: bad sizes (E=%d, d_in=%lld, d_out=%lld, R=%lld, rows %lld -> %lld)",
                 n_experts, (long long)d_in, (long long)d_out, (long long)n_routes, (long long)x_rows,
@@ -1848,7 +1854,7 @@ int cvmm_mx4_bwd_x(const void* grad, int32_t op_dtype, int64_t grad_rows, int64_
   if (!mx4_sizes_ok(n_experts, d_in, d_out) || n_routes < 0 || n_routes > 0x7fffffff || top_k <= 0 ||
       grad_rows * (weighted ? top_k : 1) != n_routes || (grad_rows > 1 && grad_ld < d_out) ||
       (grad_x != nullptr && (grad_x_rows * (out_index != nullptr ? top_k : 1) != n_routes ||
-                             (grad_x_rows > 1 && grad_x_ld < d_in))) ||
+                             (grad_x_rows > 1 && grad_x_ld < d_in) || grad_x_ld >= int64_t(1) << 30)) ||
       (grad_rw != nullptr && (!weighted || x_rows < 0 || (x_rows > 1 && x_ld < d_in))))
     return fail(CVMM_ERR_INVALID, "cvmm_mx4_bwd_x: bad sizes (E=%d, d_in=%lld, d_out=%lld, R=%lld, grad rows %lld)",
                 n_experts, (long long)d_in, (long long)d_out, (long long)n_routes, (long long)grad_rows);

@@ -284,8 +284,9 @@ hipError_t launch_route_topk_backward(const void* logits, int32_t logits_dtype, 
 
 // The router of balanced models (cvmm_router_scored.hip): sigmoid or softmax
 // scores, a bias in the choice, groups of experts, renormalised and scaled
-// weights.  The workspace is route_workspace_bytes.
+// weights.
 constexpr int32_t kRouteMaxGroups = 64;
+size_t scored_workspace_bytes(int64_t n_tokens, int32_t n_experts, int64_t top_k);
 hipError_t launch_route_scored(const void* logits, int32_t logits_dtype, int64_t n_tokens, int64_t logits_ld,
                                int32_t n_experts, int64_t top_k, const float* bias, int32_t sigmoid, int32_t groups,
                                int32_t topk_groups, int32_t renormalize, double scale, float* weights, int64_t* sel,

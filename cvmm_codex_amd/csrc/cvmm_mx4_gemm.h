@@ -97,27 +97,31 @@ __device__ __forceinline__ void mx4_rows(const GemmParams& g, const RouteMeta<BM
 
 // acc[i][j] of lane (fr, fq): row j * 16 + fr, columns 16 i + 4 fq .. + 4 of
 // the wave's 64.  Two lane swaps make 8 consecutive columns, one 16-byte store.
-template <typename OutT, int MB, typename Row>
+// row(j, w): the output row, or -1, and its scale.
+template <typename OutT, int MB, bool SCALED, typename Row>
 __device__ __forceinline__ void mx4_store(const Mx4Params& p, const f32x4_t (&acc)[4][MB], int64_t nwave, int fr,
                                           int fq, Row&& row) {
   const GemmParams& g = p.g;
+  const uint32_t ldb = (uint32_t)(g.out_ld * (int64_t)sizeof(OutT));  // (columns below 2^30)
+  const int64_t left = g.N - nwave;                                   // columns from the wave's first on
 #pragma unroll
   for (int j = 0; j < MB; ++j) {
-    float w;
-    const int64_t orow = row(j, w);
-    char* rowp = orow >= 0 ? reinterpret_cast<char*>(g.out) + orow * g.out_ld * (int64_t)sizeof(OutT) : nullptr;
+    float w = 1.f;
+    const int32_t orow = row(j, w);
+    char* rowp = reinterpret_cast<char*>(g.out) + nwave * (int64_t)sizeof(OutT) + (uint64_t)(uint32_t)orow * ldb;
+    auto val = [&](int i, int q) { return SCALED ? acc[i][j][q] * w : acc[i][j][q]; };
     if constexpr (sizeof(OutT) == 4) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int64_t n = nwave + i * 16 + 4 * fq;
-        if (rowp == nullptr) continue;
+        const int n = i * 16 + 4 * fq;
         float* d = reinterpret_cast<float*>(rowp) + n;
-        if (!p.pieces && n + 4 <= g.N) {
-          *reinterpret_cast<float4*>(d) = make_float4(acc[i][j][0] * w, acc[i][j][1] * w, acc[i][j][2] * w, acc[i][j][3] * w);
+        if (orow < 0) continue;
+        if (!p.pieces && n + 4 <= left) {
+          *reinterpret_cast<float4*>(d) = make_float4(val(i, 0), val(i, 1), val(i, 2), val(i, 3));
         } else {
 #pragma unroll
           for (int q = 0; q < 4; ++q)
-            if (n + q < g.N) d[q] = acc[i][j][q] * w;
+            if (n + q < left) d[q] = val(i, q);
         }
       }
     } else {
@@ -127,10 +131,10 @@ __device__ __forceinline__ void mx4_store(const Mx4Params& p, const f32x4_t (&ac
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           union { uint32_t u; OutT e[2]; } pa, pb;
-          pa.e[0] = (OutT)(acc[2 * pr][j][2 * h] * w);
-          pa.e[1] = (OutT)(acc[2 * pr][j][2 * h + 1] * w);
-          pb.e[0] = (OutT)(acc[2 * pr + 1][j][2 * h] * w);
-          pb.e[1] = (OutT)(acc[2 * pr + 1][j][2 * h + 1] * w);
+          pa.e[0] = (OutT)val(2 * pr, 2 * h);
+          pa.e[1] = (OutT)val(2 * pr, 2 * h + 1);
+          pb.e[0] = (OutT)val(2 * pr + 1, 2 * h);
+          pb.e[1] = (OutT)val(2 * pr + 1, 2 * h + 1);
           a[h] = pa.u;
           b[h] = pb.u;
         }
@@ -138,13 +142,13 @@ __device__ __forceinline__ void mx4_store(const Mx4Params& p, const f32x4_t (&ac
         const auto s1 = __builtin_amdgcn_permlane32_swap(a[1], b[1], false, false);
         const auto t0 = __builtin_amdgcn_permlane16_swap(s0[0], s0[1], false, false);
         const auto t1 = __builtin_amdgcn_permlane16_swap(s1[0], s1[1], false, false);
-        const int64_t n = nwave + pr * 32 + 8 * fq;
-        if (rowp == nullptr || n >= g.N) continue;
+        const int n = pr * 32 + 8 * fq;
+        if (orow < 0 || n >= left) continue;
         if (!p.pieces) {  // N % 8 == 0
           *reinterpret_cast<uint4*>(rowp + n * 2) = make_uint4(t0[0], t1[0], t0[1], t1[1]);
         } else {
           const uint32_t d[4] = {t0[0], t1[0], t0[1], t1[1]};
-          store_piece16(rowp + n * 2, d, g.N - n);
+          store_piece16(rowp + n * 2, d, left - n);
         }
       }
     }
@@ -286,10 +290,8 @@ __global__ __launch_bounds__(NW * 64, OCC) void mx4_gemm_kernel(const Mx4Params 
     }
     multiply(stage1, w1, s1);
   }
-  mx4_store<OpT, MB>(p, acc, nwave, fr, fq, [&](int j, float& w) {
-    w = 1.f;
-    return (int64_t)rows.o[wm * Cfg::WR + j * 16 + fr];
-  });
+  mx4_store<OpT, MB, false>(p, acc, nwave, fr, fq,
+                            [&](int j, float&) { return rows.o[wm * Cfg::WR + j * 16 + fr]; });
 }
 
 // Few tiles: 16 rows x 64 columns, every operand straight to registers.  Each of
@@ -526,10 +528,7 @@ __global__ __launch_bounds__(256, OCC) void mx4_gemm4_kernel(const Mx4Params p) 
       if (left > 6) step(std::integral_constant<int, 6>(), k0 + 6);
       if (left > 7) step(std::integral_constant<int, 7>(), k0 + 7);
     }
-    mx4_store<OutT, MB>(p, acc, nwave, fr, fq, [&](int j, float& wt) {
-      wt = 1.f;
-      return (int64_t)rows.o[j * 16 + fr];
-    });
+    mx4_store<OutT, MB, false>(p, acc, nwave, fr, fq, [&](int j, float&) { return rows.o[j * 16 + fr]; });
   }
 }
 
@@ -668,10 +667,10 @@ __global__ __launch_bounds__(256, OCC) void mx4_gemm_t_kernel(const Mx4Params p)
   }
   const int64_t nwave = n0 + wn * 64;
   if (g.out != nullptr)
-    mx4_store<OutT, MB>(p, acc, nwave, fr, fq, [&](int j, float& wt) {
+    mx4_store<OutT, MB, true>(p, acc, nwave, fr, fq, [&](int j, float& wt) {
       const int m = wm * (BM / 2) + j * 16 + fr;
       wt = meta.w[m];
-      return meta.orow[m];
+      return (int32_t)meta.orow[m];
     });
   if (DG && nwave < g.dg_n) {
     // routing-weight gradient: sum over the wave's 64 columns of acc * x, in

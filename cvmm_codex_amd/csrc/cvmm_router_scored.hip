@@ -482,17 +482,45 @@ static void by_dtype(int32_t dt, F&& f) {
   else f(f16_t());
 }
 
+// Tokens per workgroup (= per sort chunk).  Up to 128 routes one workgroup chooses
+// and sorts them; past that its CU's instruction rate is the bound and a second
+// launch to sort costs less (32 tokens, top-8 of 256 experts in 8 groups 22.1 ->
+// 17.5 us in chunks of 8, of 64 experts 14.4 -> 12.5; but 16 tokens of 128
+// experts 9.4 -> 12.3).  Then a workgroup per CU, of at most 64 tokens and at
+// least 8, 32 or 64 (the tokens that a workgroup's lanes hold, by the experts):
+// 500 / 4096 tokens of 256 experts 23 / 33 us, 35 / 47 in chunks of 64; 16384
+// tokens, top-1 of 128, 17 in chunks of 64, 38 in chunks of 512.  Shorter ones
+// cost the sort more than they save (16384 tokens, top-8: 27 / 33 / 47 us at 64
+// / 32 / 16).  The count matrix stays within 64K entries.
+static int64_t scored_chunk_tokens(int64_t n_tokens, int32_t n_experts, int64_t top_k) {
+  const int64_t routes = n_tokens * top_k;
+  if (routes <= 128 && n_tokens <= 64) return n_tokens > 0 ? n_tokens : 1;
+  if (routes <= kRouteOneMax) return 8;
+  const int64_t least = n_experts <= 64 ? 64 : n_experts <= 128 ? 32 : 8;
+  int64_t tpc = (n_tokens + 255) / 256;
+  tpc = tpc < least ? least : tpc > 64 ? 64 : tpc;
+  const int64_t counts = (n_tokens * (int64_t)(n_experts + 1) + 65535) / 65536;
+  return tpc > counts ? tpc : counts;
+}
+
+size_t scored_workspace_bytes(int64_t n_tokens, int32_t n_experts, int64_t top_k) {
+  const int64_t tpc = scored_chunk_tokens(n_tokens, n_experts, top_k);
+  const int64_t n_chunks = n_tokens > 0 ? (n_tokens + tpc - 1) / tpc : 1;
+  // counts, bucket totals for the column scan, 256 bytes ending in n_invalid
+  return sort_counts_bytes(n_chunks, n_experts) + align_up((size_t)(n_experts + 1) * sizeof(int32_t), 256) + 256;
+}
+
 hipError_t launch_route_scored(const void* logits, int32_t logits_dtype, int64_t n_tokens, int64_t logits_ld,
                                int32_t n_experts, int64_t top_k, const float* bias, int32_t sigmoid, int32_t groups,
                                int32_t topk_groups, int32_t renormalize, double scale, float* weights, int64_t* sel,
                                int32_t* sorted_sel, int64_t* perm, int64_t* token_index, int64_t* offsets,
                                int32_t* route_pos, void* workspace, hipStream_t stream) {
   if (n_tokens <= 0) return hipSuccess;
-  const int64_t tpc = route_chunk_tokens(n_tokens, n_experts, top_k);
+  const int64_t tpc = scored_chunk_tokens(n_tokens, n_experts, top_k);
   const int64_t n_chunks = (n_tokens + tpc - 1) / tpc;
   if (n_chunks > 0x7fffffffll) return hipErrorInvalidValue;
   int32_t* counts = (int32_t*)workspace;
-  int32_t* n_invalid = (int32_t*)((char*)workspace + route_workspace_bytes(n_tokens, n_experts, top_k) - 256);
+  int32_t* n_invalid = (int32_t*)((char*)workspace + scored_workspace_bytes(n_tokens, n_experts, top_k) - 256);
   const ScoredParams p{logits_ld, n_tokens, n_experts, (int32_t)top_k, bias, sigmoid, groups, topk_groups,
                        renormalize, scale};
   const RouteSortOut so{sorted_sel, perm, token_index, offsets, route_pos};

@@ -323,7 +323,7 @@ std::vector<Tensor> route_scored(const Tensor& logits, int64_t top_k, const OptT
   Tensor i64 = T > 0 ? at::empty({2 * R + E}, opts(l, at::kLong)) : at::zeros({E}, opts(l, at::kLong));
   int32_t* a = tptr<int32_t>(i32);
   int64_t* b64 = tptr<int64_t>(i64);
-  const size_t ws_bytes = cvmm_route_topk_workspace_bytes(T, (int32_t)E, top_k);
+  const size_t ws_bytes = cvmm_route_scored_workspace_bytes(T, (int32_t)E, top_k);
   Tensor ws = sort_workspace(l, stream, ws_bytes);
   check(cvmm_route_scored(ptr(l), dtype_id(l.scalar_type()), T, std::max(l.stride(0), E), (int32_t)E, top_k,
                           tptr<float>(b), (int32_t)scores, (int32_t)groups, (int32_t)topk_groups, renormalize ? 1 : 0,

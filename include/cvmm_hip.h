@@ -280,10 +280,11 @@ int cvmm_route_topk_backward(const void* logits, int32_t logits_dtype, int64_t n
  * topk_groups with the greatest sum of their two best biased scores stay; the
  * top_k best remaining experts are chosen (ties to the lower id).  weights =
  * scale * s at the chosen experts, divided by their sum if renormalize.  Scores
- * and comparisons are 64-bit.  Outputs and workspace as cvmm_route_topk's
- * (cvmm_route_topk_workspace_bytes); at most 64 groups unless all stay. */
+ * and comparisons are 64-bit.  Outputs as cvmm_route_topk's; at most 64 groups
+ * unless all stay. */
 #define CVMM_SCORES_SOFTMAX 0
 #define CVMM_SCORES_SIGMOID 1
+size_t cvmm_route_scored_workspace_bytes(int64_t n_tokens, int32_t n_experts, int64_t top_k);
 int cvmm_route_scored(const void* logits, int32_t logits_dtype, int64_t n_tokens, int64_t logits_ld,
                       int32_t n_experts, int64_t top_k, const float* bias, int32_t scores, int32_t groups,
                       int32_t topk_groups, int32_t renormalize, double scale, float* weights, int64_t* sel,

@@ -22,6 +22,14 @@ CASES = [  # T, E, k, scores, groups, kept, bias, renormalize, scale, dtype
     (50, 500, 16, "softmax", 4, 2, True, True, 1.0, torch.float32),
     (70, 1000, 64, "sigmoid", 8, 3, True, True, 1.5, torch.bfloat16),
     (9, 1024, 8, "softmax", 32, 5, True, True, 1.0, torch.float32),
+    # either side of the chunk rule: 128 and 256 routes, chunks of 8, 32, 64 and more tokens
+    (16, 64, 8, "sigmoid", 1, 1, True, True, 1.0, torch.bfloat16),
+    (65, 64, 2, "softmax", 1, 1, True, True, 1.0, torch.float32),
+    (256, 40, 1, "sigmoid", 4, 3, True, True, 1.0, torch.float16),
+    (257, 200, 1, "softmax", 1, 1, False, True, 1.0, torch.float32),
+    (3000, 256, 4, "sigmoid", 8, 3, True, True, 2.5, torch.bfloat16),
+    (17000, 16, 2, "softmax", 1, 1, True, True, 1.0, torch.bfloat16),
+    (5000, 1000, 3, "sigmoid", 1, 1, True, False, 1.0, torch.float32),
 ]
 
 

@@ -54,6 +54,12 @@ def test_router_arguments(lib):
     assert lib.cvmm_route_scored_backward(FAKE, N.F32, 8, 16, 16, 2, 1, 1, 1.0, FAKE, FAKE, FAKE, 8, None) == 1
     assert lib.cvmm_route_scored_backward(FAKE, N.F32, 8, 16, 16, 2, 3, 1, 1.0, FAKE, FAKE, FAKE, 16, None) == 1
     assert lib.cvmm_route_scored_backward(None, N.F32, 8, 16, 16, 2, 1, 1, 1.0, FAKE, FAKE, FAKE, 16, None) == 1
+    # counts of every chunk (8 tokens of a short call, 64 of a long one) and the workspace's tail
+    need = lib.cvmm_route_scored_workspace_bytes
+    assert need(16, 64, 8) >= 65 * 4 and need(32, 256, 8) >= 4 * 257 * 4
+    assert need(16384, 128, 8) >= 256 * 129 * 4
+    assert need(1 << 20, 1024, 8) <= 3 * 65536 * 4
+    assert need(-1, 64, 8) == 0
     # no tokens: nothing to do
     assert lib.cvmm_route_scored_backward(None, N.F32, 0, 16, 16, 2, 1, 1, 1.0, None, None, None, 16, None) == 0
 
