@@ -339,6 +339,9 @@ hipError_t launch_gelu_rows(const void* h, int32_t h_dtype, int64_t h_ld, int64_
 hipError_t launch_gelu_backward(const void* dy, int32_t dy_dtype, int64_t dy_ld, const void* h, int32_t h_dtype,
                                 int64_t h_ld, int64_t rows, int64_t cols, void* dh, int32_t dh_dtype, int64_t dh_ld,
                                 hipStream_t stream);
+// Buffers from which products and row sums write and read past the caches: the
+// Infinity Cache's size.
+constexpr int64_t kStreamBytes = int64_t(256) << 20;
 // out[t][n] = rnd(rnd(sum_j rnd(w[t*k+j], w_round) * buf[row(t*k+j)][n], mid_dtype), out_dtype)
 // row(r) = inv[r] (checked against rp; rows at or past *rows_end, a device
 // pointer to the number of routes with a valid expert id -- the rows the

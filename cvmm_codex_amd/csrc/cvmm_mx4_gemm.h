@@ -31,6 +31,8 @@
 
 namespace cvmm {
 
+typedef unsigned int mx4_u32x4 __attribute__((ext_vector_type(4)));
+
 struct Mx4Params {
   GemmParams g;  // a: rows in the op type, or (4-bit rows) their codes; b unused
   const uint8_t* codes;
@@ -41,6 +43,7 @@ struct Mx4Params {
   int64_t a_groups;
   int32_t passes;           // 4-bit rows: column tiles per workgroup
   FastDiv a_div;            // input gradient: routes per row of A
+  int32_t stream;           // 16-bit output stored past the caches
   int32_t pieces;           // output rows not made of whole aligned 16-byte pieces
   int32_t dg_vec;           // x rows of the routing-weight gradient in 8-byte pieces
 };
@@ -145,7 +148,9 @@ __device__ __forceinline__ void mx4_store(const Mx4Params& p, const f32x4_t (&ac
         const int n = pr * 32 + 8 * fq;
         if (orow < 0 || n >= left) continue;
         if (!p.pieces) {  // N % 8 == 0
-          *reinterpret_cast<uint4*>(rowp + n * 2) = make_uint4(t0[0], t1[0], t0[1], t1[1]);
+          const mx4_u32x4 d = {t0[0], t1[0], t0[1], t1[1]};
+          if (p.stream) __builtin_nontemporal_store(d, reinterpret_cast<mx4_u32x4*>(rowp + n * 2));
+          else *reinterpret_cast<mx4_u32x4*>(rowp + n * 2) = d;
         } else {
           const uint32_t d[4] = {t0[0], t1[0], t0[1], t1[1]};
           store_piece16(rowp + n * 2, d, left - n);

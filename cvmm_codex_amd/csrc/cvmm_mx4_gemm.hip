@@ -100,6 +100,9 @@ static void finish(Mx4Params& p) {
   const GemmParams& g = p.g;
   const int64_t per = g.out_dtype == kF32 ? 4 : 8;
   p.pieces = g.out == nullptr || g.N % per != 0 || g.out_ld % per != 0 || (reinterpret_cast<uintptr_t>(g.out) & 15) != 0;
+  // (134 MB, which the Infinity Cache holds for its reader, 65 us stored and
+  // summed, 73 past it; 393 MB 276 and 226: launch_combine_rows)
+  p.stream = g.out != nullptr && g.n_routes * g.out_ld * 2 >= kStreamBytes;
   p.dg_vec = g.dg != nullptr && g.dg_x_dtype != kF32 && g.dg_x_ld % 4 == 0 && (reinterpret_cast<uintptr_t>(g.dg_x) & 7) == 0;
 }
 

@@ -358,6 +358,27 @@ def test_weights_past_32_bit_offsets():
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("quantize", [False, True])
+@pytest.mark.parametrize("d_out", [1000, 2056])
+def test_route_rows_past_the_caches(d_out, quantize, dtype):
+    """Weighted sums over more than 256 MB of route rows: a token's row does not
+    depend on where it lies."""
+    k, few, E, d_in = 4, 61, 3, 64
+    n = (256 << 20) // (few * k * d_out * 2) + 1
+    assert n * few * k * d_out * 2 >= 256 << 20
+    x, sel, keys, gates, _ = _case(few, d_in, d_out, E, min(k, E), dtype, "down", seed=2)
+    x = torch.cat([x, x[:, :1]], 1)
+    sel, gates = torch.cat([sel, sel[:, :1]], 1), torch.cat([gates, gates[:, 1:2]], 1)
+    packed = C.cvmm_mx4_quantize(keys.cuda(), dim=1)
+    s = C.cvmm_prepare_sel2(sel.repeat(n, 1).cuda(), gates.repeat(n, 1).cuda(), route_input=True)
+    with torch.no_grad():
+        y = C.cvmm_mx4(x.repeat(n, 1, 1).cuda(), s, packed, quantize_input=quantize)
+    o = O.product(O.quantize(x) if quantize else x, sel, keys, gates)
+    _within(y[:few], o["y"], _tol("y", o, dtype, d_in, d_out, k, False), "y")
+    assert torch.equal(y.view(n, few, d_out), y[:few].expand(n, few, d_out))
+
+
 def test_compiled():
     T, d_in, d_out, E, k = 24, 128, 64, 4, 2
     x, sel, keys, gates, grad = _case(T, d_in, d_out, E, k, BF, "down", seed=4)
