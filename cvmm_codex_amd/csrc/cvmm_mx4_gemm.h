@@ -671,6 +671,19 @@ __global__ __launch_bounds__(256, OCC) void mx4_gemm_t_kernel(const Mx4Params p)
     multiply(stage1);
   }
   const int64_t nwave = n0 + wn * 64;
+  // the x pieces of the routing-weight gradient, all in flight over the stores
+  uint2 xv[DG ? MB : 1][4];
+  const bool dg_whole = DG && p.dg_vec && nwave + 64 <= g.dg_n && g.dg_x_rows > 0;
+  if (dg_whole) {
+#pragma unroll
+    for (int j = 0; j < MB; ++j) {
+      const int64_t xr = meta.dgrow[wm * (BM / 2) + j * 16 + fr];
+      const uint16_t* x = static_cast<const uint16_t*>(g.dg_x) + (xr >= 0 ? xr : 0) * g.dg_x_ld + nwave + 4 * fq;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) xv[j][i] = *reinterpret_cast<const uint2*>(x + i * 16);
+    }
+    issue_fence();
+  }
   if (g.out != nullptr)
     mx4_store<OutT, MB, true>(p, acc, nwave, fr, fq, [&](int j, float& wt) {
       const int m = wm * (BM / 2) + j * 16 + fr;
@@ -689,9 +702,9 @@ __global__ __launch_bounds__(256, OCC) void mx4_gemm_t_kernel(const Mx4Params p)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int64_t n = nwave + i * 16 + 4 * fq;
-          if (p.dg_vec && n + 4 <= g.dg_n) {
+          if (dg_whole) {
             union { uint2 u; OpT e[4]; } c;
-            c.u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(g.dg_x) + xr * g.dg_x_ld + n);
+            c.u = xv[j][i];
 #pragma unroll
             for (int q = 0; q < 4; ++q) sum += acc[i][j][q] * to_f32(c.e[q]);
           } else {
