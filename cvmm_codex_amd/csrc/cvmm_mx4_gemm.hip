@@ -20,7 +20,7 @@ static hipError_t tile16(const Mx4Params& p, hipStream_t s) {
 //   routes per expert     2           8           16          32          125        1024
 //   16-row tiles      14.1 (14.6)  16.3        17.0 (18.7)  21.8 (24.3)   53         423
 //   32-row            15.5 (15.5)  16.5        19.6 (19.7)  21.3 (22.9)   46 (50)    323
-//   64-row            21.2 (20.3)  21.7        22.2 (23.9)  29.5 (25.9)   44 (48)    295
+//   64-row            21.2 (20.3)  21.7        22.2 (23.9)  29.5 (25.9)   44 (48)    276
 // 256-column tiles, 4 waves of 64 columns; 128-column ones where the columns
 // end there (64 experts of 1024 x 128, 250 routes: 18.1 -> 14.1 us) or
 // where they leave less than four fifths of the wide tiles filled.  A launch
@@ -45,9 +45,9 @@ static hipError_t fwd16(const Mx4Params& p, hipStream_t s) {
 }
 
 // 4-bit rows.  A tile of K <= 1024 keeps its rows for two column tiles: 16384
-// tokens, top-8 of 128 experts of 512 x 2048 take 240 / 218 / 228 us with 1 / 2
+// tokens, top-8 of 128 experts of 512 x 2048 take 239 / 212 / 219 us with 1 / 2
 // / 4 tiles per workgroup; past that the rows are read again either way, and
-// one tile each fills the GPU better (2048 x 512: 106 / 122 us with 1 / 2).
+// one tile each fills the GPU better (2048 x 512: 107 / 124 us with 1 / 2).
 template <typename OutT, int BM, int OCC>
 static hipError_t tile4(Mx4Params p, hipStream_t s) {
   const int64_t tiles = (p.g.N + 255) / 256;
@@ -55,11 +55,17 @@ static hipError_t tile4(Mx4Params p, hipStream_t s) {
   return launch(mx4_gemm4_kernel<OutT, BM, OCC>, p, mx4_grid<BM>(p.g, (tiles + p.passes - 1) / p.passes), 256, s);
 }
 
+// Times of bf16 outputs, 128 experts of 2048 x 512 (512 x 2048), us:
+//   routes per expert     4           32          64          128         187
+//   32-row tiles      13.7 (13.6)  16.2 (18.1)  19.1 (23.2)  26.3 (33.9)  33.7 (44.4)
+//   64-row            14.5 (14.9)  17.5 (20.6)  18.2 (21.6)  23.1 (32.4)  29.0 (39.0)
+//   128-row           16.2 (17.4)  17.7 (20.9)  21.9 (29.0)  24.2 (36.7)  25.5 (39.9)
 template <typename OutT>
 static hipError_t fwd4(const Mx4Params& p, hipStream_t s) {
   const GemmParams& g = p.g;
   const int64_t E = g.n_experts < g.n_routes ? g.n_experts : g.n_routes;
-  if (g.n_routes <= 64 * E) return tile4<OutT, 32, 4>(p, s);
+  if (g.n_routes <= 48 * E) return tile4<OutT, 32, 4>(p, s);
+  if (g.n_routes <= 160 * E) return tile4<OutT, 64, 3>(p, s);
   return tile4<OutT, 128, 2>(p, s);
 }
 
