@@ -59,6 +59,18 @@ def test_keys(E, K, N, dtype):
         _same(q.dequantize(BF), exp)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF, HF])
+def test_keys_past_the_caches(dtype):
+    """Over 256 MB of keys give what their experts give one by one."""
+    E, K = 2, 8200
+    N = 4100 if dtype == F32 else 8200
+    t = torch.randn(E, K, N, device="cuda").to(dtype)
+    assert t.numel() * t.element_size() >= 256 << 20
+    got = C.cvmm_mx4_quantize(t, dim=1).dequantize()
+    for e in range(E):
+        assert torch.equal(got[e:e + 1], C.cvmm_mx4_quantize(t[e:e + 1], dim=1).dequantize())
+
+
 def test_ties_extremes_and_non_finite_blocks():
     grid = torch.tensor([0, .25, .5, .75, 1, 1.25, 1.5, 1.75, 2, 2.5, 3, 3.5, 4, 5, 6, 7, 7.999])
     near = torch.cat([grid, grid * (1 + 2.0 ** -23), grid * (1 - 2.0 ** -23)])
