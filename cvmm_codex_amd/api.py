@@ -8,7 +8,9 @@ Function ``CVMM`` (:1521-1755), ``get_dtype`` / ``dtype_to_type_id`` (:30-44),
 attributes the reference tests patch (``cvmm_expert_offsets_call``,
 ``cvmm_lowmem_chunk_size``).  ``cvmm_route_topk`` and ``cvmm_gelu`` (no
 counterpart in cvmm.py) fuse the router lines its callers write before
-``cvmm`` and the GELU they apply to the up projection.
+``cvmm`` and the GELU they apply to the up projection.  ``cvmm_route_scored``,
+``cvmm_mx4_quantize`` and ``cvmm_mx4`` (none either) are the router of balanced
+MoE models and ``cvmm`` with expert weights in 4 bits.
 
 All arithmetic runs in the HIP kernels of ``libcvmm_hip.so`` (C ABI in
 ``include/cvmm_hip.h``), launched on torch's current stream; nothing here
@@ -663,7 +665,7 @@ def cvmm_route_scored(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor]
         sel = the k best c of the experts that stay (ties to the lower id, NaN lowest)
         weights = s[sel];  weights = scale * weights / weights.sum(-1)    # renormalize
 
-    Scores, sums and comparisons are 64-bit.  Returns ``(weights, sel,
+    The choice is that of 64-bit scores.  Returns ``(weights, sel,
     sel_up)`` as ``cvmm_route_topk``: fp32 weights ``[..., k]`` (gradient flows
     to ``logits``, not to ``bias``), int64 ids ``[..., k]`` by falling c and the
     sorted token-input selector.  At most 1024 experts, k <= 64 and, where some
