@@ -17,10 +17,10 @@ static hipError_t tile16(const Mx4Params& p, hipStream_t s) {
 }
 
 // 16-bit rows.  Times of bf16 launches, 128 experts of 2048 x 512 (512 x 2048):
-//   routes per expert     2           8           16          32          125        1024
-//   16-row tiles      14.1 (14.6)  16.3        17.0 (18.7)  21.8 (24.3)   53         423
-//   32-row            15.5 (15.5)  16.5        19.6 (19.7)  21.3 (22.9)   46 (50)    323
-//   64-row            21.2 (20.3)  21.7        22.2 (23.9)  29.5 (25.9)   44 (48)    276
+//   routes per expert     2           8     16          32          64          96          124         1024
+//   16-row tiles      14.1 (14.6)  16.3  17.0 (18.7)  21.8 (24.3)  32.5 (36.8)  43.7 (51.1)  53.9 (64.1)  423
+//   32-row            15.5 (15.5)  16.5  19.6 (19.7)  21.3 (22.9)  29.8 (31.9)  36.8 (41.4)  46.0 (51.1)  323
+//   64-row            21.2 (20.3)  21.7  22.2 (23.9)  29.5 (25.9)  33.2 (32.2)  35.3 (40.6)  44.6 (48.7)  276
 // 256-column tiles, 4 waves of 64 columns; 128-column ones where the columns
 // end there (64 experts of 1024 x 128, 250 routes: 18.1 -> 14.1 us) or
 // where they leave less than four fifths of the wide tiles filled.  A launch
@@ -40,7 +40,7 @@ static hipError_t fwd16(const Mx4Params& p, hipStream_t s) {
   const int64_t w128 = (g.N + 127) / 128 * 128, w256 = (g.N + 255) / 256 * 256;
   const bool narrow = 5 * w128 < 4 * w256;
   if (R <= 24 * E) return narrow ? tile16<OpT, 16, 128, 2, 4>(p, s) : tile16<OpT, 16, 256, 4, 4>(p, s);
-  if (R <= 128 * E) return narrow ? tile16<OpT, 32, 128, 2, 4>(p, s) : tile16<OpT, 32, 256, 4, 4>(p, s);
+  if (R <= 88 * E) return narrow ? tile16<OpT, 32, 128, 2, 4>(p, s) : tile16<OpT, 32, 256, 4, 4>(p, s);
   return narrow ? tile16<OpT, 64, 128, 4, 4>(p, s) : tile16<OpT, 64, 256, 4, 3>(p, s);
 }
 
