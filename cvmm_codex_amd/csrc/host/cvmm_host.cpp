@@ -1077,18 +1077,19 @@ std::vector<Tensor> route_scored_apply(const Tensor& logits, int64_t top_k, cons
 
 struct CvmmMx4Function : public torch::autograd::Function<CvmmMx4Function> {
   // x and reduction_weight (optional) are the differentiable inputs.  The
-  // selection: the sort's buffers i32 and i64, or (i32 undefined) sel_index in
-  // i64's place with out_index, offsets and route_pos.
-  static Mx4Routes routes(Tensor& i32, Tensor& i64, OptT& out_index, const OptT& offsets, const OptT& pos,
+  // selection: the sort's buffers i32 and i64, or (no i32: an optional, as
+  // apply() takes no undefined tensor) sel_index in i64's place with out_index,
+  // offsets and route_pos.
+  static Mx4Routes routes(const OptT& i32, Tensor& i64, OptT& out_index, const OptT& offsets, const OptT& pos,
                           bool route_input) {
-    if (i32.defined()) return routes_of_buffers(i32, i64, route_input);
+    if (i32.has_value()) return routes_of_buffers(*i32, i64, route_input);
     return routes_of_tensors(i64, out_index, *offsets, pos);
   }
 
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const OptT& rw, const Tensor& codes,
-                        const Tensor& scales, int64_t d_in, int64_t d_out, Tensor i32, Tensor i64, OptT out_index,
-                        const OptT& offsets, const OptT& route_pos, bool route_input, int64_t top_k, int64_t op_id,
-                        const std::vector<int64_t>& out_shape) {
+                        const Tensor& scales, int64_t d_in, int64_t d_out, const OptT& i32, Tensor i64,
+                        OptT out_index, const OptT& offsets, const OptT& route_pos, bool route_input, int64_t top_k,
+                        int64_t op_id, const std::vector<int64_t>& out_shape) {
     const bool need_x = x.requires_grad(), need_rw = rw.has_value() && rw->requires_grad();
     ctx->saved_data["d_in"] = d_in;
     ctx->saved_data["d_out"] = d_out;
@@ -1097,7 +1098,7 @@ struct CvmmMx4Function : public torch::autograd::Function<CvmmMx4Function> {
     ctx->saved_data["need"] = (int64_t)((need_x ? 1 : 0) | (need_rw ? 2 : 0) | (route_input ? 4 : 0));
     const Mx4Routes r = routes(i32, i64, out_index, offsets, route_pos, route_input);
     Tensor out = mx4_forward_impl(x, codes, scales, d_in, d_out, r, rw, op_id, false, current_stream(x), out_shape);
-    ctx->save_for_backward({x, opt_or_undef(rw), codes, scales, i32, i64, opt_or_undef(out_index),
+    ctx->save_for_backward({x, opt_or_undef(rw), codes, scales, opt_or_undef(i32), i64, opt_or_undef(out_index),
                             opt_or_undef(offsets), opt_or_undef(route_pos)});
     return out;
   }
@@ -1107,7 +1108,8 @@ struct CvmmMx4Function : public torch::autograd::Function<CvmmMx4Function> {
     auto v = ctx->get_saved_variables();
     const int64_t need = ctx->saved_data["need"].toInt();
     OptT out_index = undef_or_opt(v[6]);
-    const Mx4Routes r = routes(v[4], v[5], out_index, undef_or_opt(v[7]), undef_or_opt(v[8]), (need & 4) != 0);
+    const Mx4Routes r =
+        routes(undef_or_opt(v[4]), v[5], out_index, undef_or_opt(v[7]), undef_or_opt(v[8]), (need & 4) != 0);
     auto [gx, grw] = mx4_backward_impl(grads[0], v[0], v[2], v[3], ctx->saved_data["d_in"].toInt(),
                                        ctx->saved_data["d_out"].toInt(), r, undef_or_opt(v[1]),
                                        ctx->saved_data["top_k"].toInt(), ctx->saved_data["op_id"].toInt(),
@@ -1125,7 +1127,7 @@ Tensor mx4_apply(const Tensor& x, const OptT& rw, const Tensor& codes, const Ten
                  int64_t top_k, int64_t op_id, bool quantize_input, bool grad, const std::vector<int64_t>& out_shape) {
   require_device(x, "x");
   if (grad)
-    return CvmmMx4Function::apply(x, rw, codes, scales, d_in, d_out, Tensor(), sel_index, out_index, OptT(offsets),
+    return CvmmMx4Function::apply(x, rw, codes, scales, d_in, d_out, OptT(), sel_index, out_index, OptT(offsets),
                                   route_pos, !out_index.has_value(), top_k, op_id, out_shape);
   const Mx4Routes r = routes_of_tensors(sel_index, out_index, offsets, route_pos);
   return mx4_forward_impl(x, codes, scales, d_in, d_out, r, rw, op_id, quantize_input, current_stream(x), out_shape);
@@ -1150,8 +1152,8 @@ std::tuple<Tensor, Tensor, Tensor> mx4_apply_recorded(const Tensor& x, const Opt
   }
   Tensor y;
   if (grad)
-    y = CvmmMx4Function::apply(x, rw, codes, scales, d_in, d_out, i32, i64, OptT(), OptT(), OptT(), route_input, top_k,
-                               op_id, out_shape);
+    y = CvmmMx4Function::apply(x, rw, codes, scales, d_in, d_out, OptT(i32), i64, OptT(), OptT(), OptT(), route_input,
+                               top_k, op_id, out_shape);
   else
     y = mx4_forward_impl(x, codes, scales, d_in, d_out, routes_of_buffers(i32, i64, route_input), rw, op_id,
                          quantize_input, stream, out_shape);

@@ -425,3 +425,49 @@ def test_block_of_router_and_both_projections():
     # a step of h's rounding (2^-8, twice: product and GELU) reaches y as that part of its terms
     tol = _tol("y", o, BF, H, D, k, False) + 4 * 2.0 ** -8 * o["y_abs"]
     _within(y, o["y"], tol, "y")
+
+
+def _selector(kind, mode, sel, gates, keys):
+    """The same selection as a user may hold it: ids, a selector whose sort was
+    read, one that cvmm() sorted, one built by hand."""
+    if kind == "ids":
+        return sel
+    s = C.cvmm_prepare_sel2(sel, gates, route_input=mode == "down")
+    if kind == "resolved":
+        assert s.sel.numel() == sel.numel()
+    elif kind == "shared":
+        T, k = sel.shape
+        x = torch.randn(*((T, k) if mode == "down" else (T,)), keys.shape[1], device="cuda")
+        with torch.no_grad(), torch.autocast("cuda", dtype=BF):
+            C.cvmm(x, s, keys)
+    else:
+        ids, perm = torch.sort(sel.reshape(-1), stable=True)
+        up = mode != "down"
+        s = C.CVMMSel(sel.int(), ids.int().view(sel.shape), perm // sel.shape[1] if up else perm, perm if up else None,
+                      gates)
+    return s
+
+
+@pytest.mark.parametrize("kind,mode", [("ids", "down"), *((s, m) for s in ("resolved", "shared", "built")
+                                                          for m in MODES)])
+def test_gradients_of_every_kind_of_selection(kind, mode):
+    T, d_in, d_out, E, k = 50, 136, 72, 5, 3
+    x, sel, keys, gates, grad = _case(T, d_in, d_out, E, k, BF, mode, seed=21)
+    if kind == "ids":  # one row per route, no routing weights
+        gates, grad = None, torch.randn(T, k, d_out, generator=_gen(22)).to(BF)
+    packed = C.cvmm_mx4_quantize(keys.cuda(), dim=1)
+    xd = x.cuda().requires_grad_()
+    gd = None if gates is None else gates.cuda().requires_grad_()
+    y = C.cvmm_mx4(xd, _selector(kind, mode, sel.cuda(), gd, keys.cuda()), packed)
+    grads = torch.autograd.grad(y, [xd] + ([] if gd is None else [gd]), grad.cuda())
+    o = O.product(x, sel, keys, gates, grad)
+    _within(y, o["y"], _tol("y", o, BF, d_in, d_out, k, False), "y")
+    _within(grads[0], o["grad_x"], _tol("grad_x", o, BF, d_in, d_out, k, mode != "down"), "grad_x")
+    if gd is not None:
+        _within(grads[1], o["grad_gates"], _tol("grad_gates", o, BF, d_in, d_out, k, False), "grad_gates")
+    with torch.no_grad():
+        plain = C.cvmm_mx4(xd, _selector(kind, mode, sel.cuda(), gd, keys.cuda()), packed)
+        rows = C.cvmm_mx4(xd, _selector(kind, mode, sel.cuda(), gd, keys.cuda()), packed, quantize_input=True)
+    assert torch.equal(plain, y)
+    o = O.product(O.quantize(x), sel, keys, gates)
+    _within(rows, o["y"], _tol("y", o, BF, d_in, d_out, k, False), "4-bit rows")
