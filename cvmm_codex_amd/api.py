@@ -588,6 +588,20 @@ def _apply(fn, *args):
     return fn.forward(_NoGraph(), *args)
 
 
+def _differentiated(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a call on these tensors goes through its autograd function: one
+    asks for a gradient, or carries a tangent or is wrapped by a function
+    transform, which those functions refuse."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    if _compiling():
+        return False
+    if torch._C._are_functorch_transforms_active():
+        return True
+    return _forward_ad._current_level >= 0 and any(
+        t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 # ----------------------------------------------------------------------------
 # router
 # ----------------------------------------------------------------------------
@@ -690,7 +704,7 @@ def cvmm_route_scored(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor]
     if _compiling():
         w, sel, *sort = _ops.route_scored(*args)
     else:
-        w, sel, *sort = N.host().route_scored_apply(*args, torch.is_grad_enabled() and logits.requires_grad)
+        w, sel, *sort = N.host().route_scored_apply(*args, _differentiated(logits))
     if len(lead) != 1:
         w, sel = w.view(*lead, k), sel.view(*lead, k)
     routing = _Routing(sel.view(-1), k)
@@ -1150,7 +1164,7 @@ def cvmm_mx4(x: torch.Tensor, sel: Union[torch.Tensor, CVMMSel], keys: CVMMMx4,
     if not isinstance(sel, CVMMSel):
         sel = cvmm_prepare_sel(sel, E)
     rw = sel.reduction_weight
-    grad = torch.is_grad_enabled() and (x.requires_grad or (rw is not None and rw.requires_grad))
+    grad = _differentiated(x, rw)
     if grad and quantize_input:
         raise RuntimeError("cvmm_mx4: quantize_input is for inference (rounding to 4 bits has no gradient)")
     raw = sel._raw_shape_tensor()

@@ -471,3 +471,29 @@ def test_gradients_of_every_kind_of_selection(kind, mode):
     assert torch.equal(plain, y)
     o = O.product(O.quantize(x), sel, keys, gates)
     _within(rows, o["y"], _tol("y", o, BF, d_in, d_out, k, False), "4-bit rows")
+
+
+def test_forward_mode_is_refused():
+    """A tangent has no rule here: an error, not an output without one.  Plain
+    tensors inside a forward-mode level are multiplied as ever."""
+    T, d_in, d_out, E, k = 6, 64, 64, 3, 2
+    x, sel, keys, gates, _ = _case(T, d_in, d_out, E, k, BF, "down", seed=23)
+    packed = C.cvmm_mx4_quantize(keys.cuda(), dim=1)
+    xd, gd = x.cuda(), gates.cuda()
+
+    def call(xx, gg, quantize=False, pending=True):
+        s = C.cvmm_prepare_sel2(sel.cuda(), gg, route_input=True)
+        if not pending:
+            assert s.sel.numel()
+        return C.cvmm_mx4(xx, s, packed, quantize)
+
+    y, yq = call(xd, gd), call(xd, gd, True)
+    for mode in (torch.no_grad, torch.enable_grad):
+        with mode(), torch.autograd.forward_ad.dual_level():
+            for pending in (True, False):
+                for quantize in (False, True):
+                    with pytest.raises(Exception):
+                        call(torch.autograd.forward_ad.make_dual(xd, torch.ones_like(xd)), gd, quantize, pending)
+                    with pytest.raises(Exception):
+                        call(xd, torch.autograd.forward_ad.make_dual(gd, torch.ones_like(gd)), quantize, pending)
+                assert torch.equal(call(xd, gd, False, pending), y) and torch.equal(call(xd, gd, True, pending), yq)

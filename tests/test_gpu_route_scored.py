@@ -183,3 +183,17 @@ def test_compiled():
     w, sel = torch.compile(f, backend="eager", fullgraph=True)(logits.cuda())
     we, se = f(logits.cuda())
     assert torch.equal(w, we) and torch.equal(sel, se)
+
+
+def test_forward_mode_is_refused():
+    """A tangent has no rule here: an error, not weights without one.  Plain
+    tensors inside a forward-mode level are routed as ever."""
+    logits, b, _ = _logits(9, 16, torch.float32)
+    l, bd = logits.cuda(), b.cuda()
+    w, sel, _ = C.cvmm_route_scored(l, 3, bias=bd)
+    for mode in (torch.no_grad, torch.enable_grad):
+        with mode(), torch.autograd.forward_ad.dual_level():
+            with pytest.raises(Exception):
+                C.cvmm_route_scored(torch.autograd.forward_ad.make_dual(l, torch.ones_like(l)), 3, bias=bd)
+            w2, sel2, _ = C.cvmm_route_scored(l, 3, bias=bd)
+            assert torch.equal(w, w2) and torch.equal(sel, sel2)
