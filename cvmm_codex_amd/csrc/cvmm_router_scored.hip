@@ -213,7 +213,8 @@ __global__ __launch_bounds__(THREADS) void route_scored_kernel(
       unsure |= !(gap > 2.f * err + 0x1p-21f * top);
     }
     // candidates by falling score: the k best, and those after them that the
-    // error does not part from the one before
+    // error does not part from the one before; past the 64 that the lanes hold
+    // the token is unsure
     int32_t res_e[SLOTS];
 #pragma unroll
     for (int q = 0; q < SLOTS; ++q) res_e[q] = 0;
@@ -221,7 +222,7 @@ __global__ __launch_bounds__(THREADS) void route_scored_kernel(
     int n = 0;
     bool near = false;
 #pragma unroll 1
-    for (; n < 64; ++n) {
+    for (;; ++n) {
       if (n == k && by_logit) break;
       int32_t bv = key[0];
 #pragma unroll
@@ -235,6 +236,10 @@ __global__ __launch_bounds__(THREADS) void route_scored_kernel(
       const float now = __int_as_float(mv ^ ((mv >> 31) & 0x7fffffff));
       const bool apart = by_logit || n == 0 || before - now > err + 0x1p-23f * (fabsf(before) + fabsf(now));
       if (n >= k && apart) break;
+      if (n == 64) {
+        unsure = true;
+        break;
+      }
       near |= !apart;
       before = now;
 #pragma unroll
@@ -243,7 +248,7 @@ __global__ __launch_bounds__(THREADS) void route_scored_kernel(
       for (int q = 0; q < SLOTS; ++q)
         if (n == q * LPT + li) res_e[q] = win;
     }
-    unsure |= n > k + 8 || n < k || (near && n == 64);
+    unsure |= n > k + 8 || n < k;
     // ---- all scores in 64 bits, for a wave with an unsure token: NaN, groups within
     // the error, or a crowd of candidates
     const bool again = active && (__ballot(unsure) & seg_mask) != 0;

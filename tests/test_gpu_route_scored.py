@@ -197,3 +197,21 @@ def test_forward_mode_is_refused():
                 C.cvmm_route_scored(torch.autograd.forward_ad.make_dual(l, torch.ones_like(l)), 3, bias=bd)
             w2, sel2, _ = C.cvmm_route_scored(l, 3, bias=bd)
             assert torch.equal(w, w2) and torch.equal(sel, sel2)
+
+
+@pytest.mark.parametrize("k", [63, 64])
+@pytest.mark.parametrize("groups,kept", [(1, 1), (2, 1)])
+def test_last_of_64_choices_goes_by_64_bit_scores(k, groups, kept):
+    """The last chosen and the first left out differ by 2e-9 and are equal in 32
+    bits: a sigmoid of 20 and of 21, moved by the bias."""
+    n = k + 1
+    logits = torch.zeros(3, n * groups)
+    bias = torch.zeros(n * groups)
+    bias[:k - 1] = 0.5 + 0.01 * torch.arange(k - 1)
+    logits[:, k - 1], logits[:, k] = 20.0, 21.0
+    bias[k - 1:n] = -0.75
+    logits[:, n:] = -10.0
+    kw = dict(scores="sigmoid", groups=groups, topk_groups=kept, bias=bias)
+    w, sel, routed = C.cvmm_route_scored(logits.cuda(), k, **{**kw, "bias": bias.cuda()})
+    assert not bool((sel == k - 1).any())
+    _check(w, sel, routed, logits, k, kw)
