@@ -149,9 +149,16 @@ __global__ __launch_bounds__(THREADS) void route_scored_kernel(
     const int64_t t = t0 + seg;
     const bool active = t < t_hi;
     const LT* row = logits + (active ? t : t_lo) * p.ld;
-    // ---- 32 bits.  exp: |x| 2^-24 by its argument and an ulp, so a sigmoid is off
-    // by at most 0.6 * 2^-24 + two roundings < 2^-22, a softmax score by that
-    // part of the largest; the sum with the bias by half an ulp of itself.
+    // ---- 32 bits, and how far two of these scores can be off against each other,
+    // in units of 2^-24.  exp(x): 2 + 1.22 |x| of itself (two roundings of its
+    // argument and an ulp; 1 + 0.95 |x| measured).  Sigmoid: s (1 - s) of that,
+    // below 0.8, and at most 1 each for the sum and the reciprocal: 2^-21 for both
+    // sides.  Softmax: exp (l - m rounds too) and the product with 1 / sum, 3 of the
+    // largest score on either side.  The sum scales all scores alike; where a bias
+    // cancels the distance of two, its error counts once, of the largest score: 1
+    // per addition, of a lane's experts and over the lanes, 1 for the reciprocal,
+    // and the exps' 2 + 2.22 times their weighted mean |x|, at most 4.5 for 1024
+    // experts.  The sum with the bias rounds by half an ulp of itself.
     // (Loads at clamped places: a guard around each made them
     // wait for one another.)
     float l[MAXV], c[MAXV];
@@ -165,8 +172,8 @@ __global__ __launch_bounds__(THREADS) void route_scored_kernel(
 #pragma unroll
       for (int v = 0; v < MAXV; ++v) c[v] = p.bias[li + LPT * v < E ? li + LPT * v : E - 1];
     }
-    float m = -INFINITY, sum = 1.f, err = 0x1p-21f;  // of a score, both sides (below)
-    bool unsure = false;                             // NaN, or groups within the error
+    float m = -INFINITY, sum = 1.f, err = 0x1p-21f;
+    bool unsure = false;  // NaN, or groups within the error
     if (p.sigmoid) {
 #pragma unroll
       for (int v = 0; v < MAXV; ++v) c[v] += __frcp_rn(1.f + __expf(-l[v]));
@@ -183,7 +190,7 @@ __global__ __launch_bounds__(THREADS) void route_scored_kernel(
       sum = seg_sum<LPT>(s);
       unsure = isnan(sum);
       const float inv = 1.f / sum;
-      err *= inv;  // of the largest score, 1 / sum
+      err = (MAXV + __builtin_ctz(LPT) + 20) * 0x1p-24f * inv;  // of the largest score, 1 / sum
 #pragma unroll
       for (int v = 0; v < MAXV; ++v) c[v] += x[v] * inv;
     }

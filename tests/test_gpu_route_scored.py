@@ -215,3 +215,25 @@ def test_last_of_64_choices_goes_by_64_bit_scores(k, groups, kept):
     w, sel, routed = C.cvmm_route_scored(logits.cuda(), k, **{**kw, "bias": bias.cuda()})
     assert not bool((sel == k - 1).any())
     _check(w, sel, routed, logits, k, kw)
+
+
+@pytest.mark.parametrize("E,low", [(1024, -15.046297), (1024, -7.0), (1024, -5.0), (512, -15.046297), (512, -5.0),
+                                   (256, -14.0), (100, -4.0)])
+@pytest.mark.parametrize("groups,kept", [(1, 1), (2, 1)])
+def test_sum_of_many_equal_scores(E, low, groups, kept):
+    """One expert above E - 1 equal ones, whose 32-bit sum rounds the same way at
+    every addition; a bias that nearly cancels the distance to one of them, on
+    either side of the tie in steps of 2^-24."""
+    logits = torch.full((1, E), low)
+    logits[0, 0] = 0.0
+    other = 1 if groups == 1 else E // 2
+    s = O.scores_of(logits, "softmax")[0]
+    tie = (s[0] - s[other]).float()
+    for j in range(-24, 25):
+        bias = torch.zeros(E)
+        bias[other] = tie + j * 2.0 ** -24
+        if groups > 1:  # the same second best in both groups: they compare as the two do
+            bias[2], bias[other + 1] = 0.125, 0.125
+        kw = dict(bias=bias, groups=groups, topk_groups=kept)
+        w, sel, routed = C.cvmm_route_scored(logits.cuda(), 1, **{**kw, "bias": bias.cuda()})
+        _check(w, sel, routed, logits, 1, kw)
