@@ -17,8 +17,8 @@
 // is made in 32 bits, with the candidates that are within the error of the ones
 // before them ranked by their 64-bit scores, and in 64 bits throughout for the
 // few tokens where that is not enough; without a bias and groups the logits
-// themselves are compared.  (64-bit exps for all: 32 tokens of 256 experts, on
-// one CU, 33 us.)
+// themselves are compared, where different ones have different scores.  (64-bit
+// exps for all: 32 tokens of 256 experts, on one CU, 33 us.)
 #include <cmath>
 
 #include "cvmm_common.h"
@@ -225,12 +225,19 @@ __global__ __launch_bounds__(THREADS) void route_scored_kernel(
     int32_t res_e[SLOTS];
 #pragma unroll
     for (int q = 0; q < SLOTS; ++q) res_e[q] = 0;
+    // does every smaller logit have a smaller 64-bit score?  From 2^-15 on fp32
+    // numbers lie 2^-40 apart, which exp and the sums keep (2^-43 at most is lost)
+    // unless the score leaves the normal numbers (below e^-708), or a sigmoid nears
+    // 1: up to 16 its steps are 2^-43 still, from 24 on it repeats values.
+    auto sure = [&](float v) {
+      return fabsf(v) >= 0x1p-15f && (p.sigmoid ? v < 16.f && v > -700.f : v - m > -700.f);
+    };
     float before = INFINITY;
     int n = 0;
     bool near = false;
 #pragma unroll 1
     for (;; ++n) {
-      if (n == k && by_logit) break;
+      if (n == k && by_logit && sure(before)) break;
       int32_t bv = key[0];
 #pragma unroll
       for (int v = 1; v < MAXV; ++v) bv = max(bv, key[v]);
@@ -241,7 +248,8 @@ __global__ __launch_bounds__(THREADS) void route_scored_kernel(
       for (int v = MAXV - 1; v >= 0; --v) bi = key[v] == mv ? li + LPT * v : bi;
       const int32_t win = seg_min_i<LPT>(bi);
       const float now = __int_as_float(mv ^ ((mv >> 31) & 0x7fffffff));
-      const bool apart = by_logit || n == 0 || before - now > err + 0x1p-23f * (fabsf(before) + fabsf(now));
+      const bool apart = n == 0 || (by_logit ? sure(before)
+                                             : before - now > err + 0x1p-23f * (fabsf(before) + fabsf(now)));
       if (n >= k && apart) break;
       if (n == 64) {
         unsure = true;

@@ -237,3 +237,35 @@ def test_sum_of_many_equal_scores(E, low, groups, kept):
         kw = dict(bias=bias, groups=groups, topk_groups=kept)
         w, sel, routed = C.cvmm_route_scored(logits.cuda(), 1, **{**kw, "bias": bias.cuda()})
         _check(w, sel, routed, logits, 1, kw)
+
+
+@pytest.mark.parametrize("E,k", [(32, 5), (64, 64), (100, 63), (200, 8), (600, 3)])
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups", [1, 4])
+def test_equal_scores_of_different_logits(scores, groups, E, k):
+    """Logits whose 64-bit scores are the same number, with no bias or one of
+    zeros: the lower id first, also next to a NaN."""
+    T = 12
+    g = torch.Generator().manual_seed(E + k)
+    logits = torch.randn(T, E, generator=g)
+    up = torch.randperm(E, generator=g).float()
+    logits[0] = 40 + up                      # sigmoid 1
+    logits[1, ::2] = 40 + up[::2]
+    logits[2] = -800 - up                    # sigmoid 0
+    logits[3] = -800 - up                    # softmax 0 but for one
+    logits[3, E // 2] = 0
+    logits[4] = up * 1e-20                   # the logits' difference vanishes in either
+    logits[5, 1::3] = up[1::3] * 1e-22
+    logits[6] = logits[0]
+    logits[6, E - 1] = float("nan")
+    logits[7] = -800 - up
+    logits[7, :3] = torch.tensor([0.0, 1.0, -1.0])
+    logits[8, ::3] = -INF
+    logits[9, E // 3:] = torch.finfo(torch.float32).min
+    logits[10] = 28 + up / 64                # sigmoid: 1 - s from 2^-40 down to where 1 takes it
+    bias = torch.zeros(E)
+    kw = dict(scores=scores, groups=groups, topk_groups=groups)
+    w, sel, routed = C.cvmm_route_scored(logits.cuda(), k, **kw)
+    _check(w, sel, routed, logits, k, kw)
+    wb, selb, _ = C.cvmm_route_scored(logits.cuda(), k, bias=bias.cuda(), **kw)
+    assert torch.equal(selb, sel)
