@@ -677,9 +677,12 @@ def cvmm_route_scored(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor]
         # the experts stand in `groups` runs; the topk_groups with the greatest
         # sum of their two best c stay
         sel = the k best c of the experts that stay (ties to the lower id, NaN lowest)
-        weights = s[sel];  weights = scale * weights / weights.sum(-1)    # renormalize
+        weights = s[sel]
+        weights = scale * weights / weights.sum(-1).clamp_min(1e-20)   # renormalize
 
-    The choice is that of 64-bit scores.  Returns ``(weights, sel,
+    The choice is that of 64-bit scores.  A bias of -inf leaves an expert out (with
+    ``topk_groups < groups`` at some cost: such tokens are chosen in 64 bits
+    throughout).  Returns ``(weights, sel,
     sel_up)`` as ``cvmm_route_topk``: fp32 weights ``[..., k]`` (gradient flows
     to ``logits``, not to ``bias``), int64 ids ``[..., k]`` by falling c and the
     sorted token-input selector.  At most 1024 experts, k <= 64 and, where some

@@ -5,7 +5,7 @@
 //   experts stand in G groups of E / G; a group's score is the sum of its two
 //   best c (of its one); the Gk groups of the highest scores stay
 //   chosen: the k best c among the experts of those groups
-//   w_j = scale * s_j / sum_i s_i          (or scale * s_j)
+//   w_j = scale * s_j / max(sum_i s_i, 1e-20)   (or scale * s_j)
 // Ties go to the lower id, NaN ranks lowest.  The selection leaves sorted by
 // expert, as the softmax router's does: each workgroup owns the tokens of one
 // sort chunk and leaves its histogram to the scatter launch, or sorts all

@@ -279,9 +279,10 @@ int cvmm_route_topk_backward(const void* logits, int32_t logits_dtype, int64_t n
  * [E], or NULL); the experts stand in `groups` runs of E / groups, of which the
  * topk_groups with the greatest sum of their two best biased scores stay; the
  * top_k best remaining experts are chosen (ties to the lower id).  weights =
- * scale * s at the chosen experts, divided by their sum if renormalize.  Scores
- * and comparisons are 64-bit.  Outputs as cvmm_route_topk's; at most 64 groups
- * unless all stay. */
+ * scale * s at the chosen experts, divided by their sum (at least 1e-20) if
+ * renormalize.  The choice is that of 64-bit scores, made in 32 bits where those
+ * decide it; the weights are computed in 64 bits.  Outputs as
+ * cvmm_route_topk's; at most 64 groups unless all stay. */
 #define CVMM_SCORES_SOFTMAX 0
 #define CVMM_SCORES_SIGMOID 1
 size_t cvmm_route_scored_workspace_bytes(int64_t n_tokens, int32_t n_experts, int64_t top_k);

@@ -269,3 +269,29 @@ def test_equal_scores_of_different_logits(scores, groups, E, k):
     _check(w, sel, routed, logits, k, kw)
     wb, selb, _ = C.cvmm_route_scored(logits.cuda(), k, bias=bias.cuda(), **kw)
     assert torch.equal(selb, sel)
+
+
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_sum_below_the_clamp(scores):
+    """Chosen scores that sum to less than 1e-20 are divided by that: weights and
+    gradients of scale * s / 1e-20."""
+    T, E, k, scale = 6, 24, 4, 1.5
+    g = torch.Generator().manual_seed(8)
+    logits = -52 - 3 * torch.rand(T, E, generator=g)
+    logits[:, 5] = 0.0
+    b = torch.zeros(E)
+    b[5] = -2.0           # the one large score is not chosen
+    l = logits.cuda().requires_grad_()
+    w, sel, routed = C.cvmm_route_scored(l, k, bias=b.cuda(), scores=scores, scale=scale)
+    kw = dict(bias=b, scores=scores, scale=scale)
+    _check(w.detach(), sel, routed, logits, k, kw)
+    l64 = logits.double().requires_grad_()
+    s = O.scores_of(l64, scores).gather(1, sel.cpu())
+    assert float(s.sum(-1).max()) < 1e-20 and float(w.sum(-1).max()) < scale
+    gw = torch.randn(T, k, generator=g)
+    got, = torch.autograd.grad(w, [l], gw.cuda())
+    exp, = torch.autograd.grad(scale * s / 1e-20, [l64], gw.double())
+    # one rounding to fp32; the softmax row in 32 bits: |x| < 56 roundings of the
+    # exp's argument, a few more of exp, sum, quotient, difference and product
+    tol = exp.abs() * 2.0 ** -24 * (1.01 if scores == "sigmoid" else 70)
+    assert bool(((got.cpu().double() - exp).abs() <= tol + 1e-45).all())
