@@ -889,10 +889,32 @@ std::tuple<Tensor, Tensor> mx4_quantize_keys(const Tensor& t, int64_t stream) {
   return {codes, scales};
 }
 
+// A 4-bit tensor's buffers have the sizes and the alignment that the library lays
+// out for its shape: the kernels read and write by the shape alone.
+void mx4_check(const Tensor& codes, const Tensor& scales, const std::vector<int64_t>& shape, bool keys,
+               const char* what) {
+  bool ok = keys ? shape.size() == 3 : !shape.empty();
+  if (ok) {
+    const int64_t d = shape.back();
+    int64_t rows = 1;
+    for (size_t i = 0; i + 1 < shape.size(); ++i) rows *= shape[i];
+    const auto bytes = [&](int32_t part) {
+      return keys ? cvmm_mx4_keys_bytes(shape[0], shape[1], d, part) : cvmm_mx4_rows_bytes(rows, d, part);
+    };
+    ok = d > 0 && rows >= 0 && codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte &&
+         codes.is_contiguous() && scales.is_contiguous() && codes.device() == scales.device() &&
+         (size_t)codes.numel() == bytes(0) && (size_t)scales.numel() == bytes(1) &&
+         (reinterpret_cast<uintptr_t>(codes.data_ptr()) & (keys ? 15 : 3)) == 0 &&
+         (reinterpret_cast<uintptr_t>(scales.data_ptr()) & (keys ? 3 : 0)) == 0;
+  }
+  if (!ok) throw py::value_error(std::string(what) + ": codes and scales are not those of the shape");
+}
+
 Tensor mx4_dequantize(const Tensor& codes, const Tensor& scales, const std::vector<int64_t>& shape, bool keys,
                       int64_t dtype, int64_t stream) {
   require_device(codes, "codes");
   require_device(scales, "scales");
+  mx4_check(codes, scales, shape, keys, "cvmm_mx4_dequantize");
   Tensor out = at::empty(shape, opts(codes, dtype_of(dtype)));
   if (out.numel() == 0) return out;
   if (keys)
@@ -908,17 +930,6 @@ Tensor mx4_dequantize(const Tensor& codes, const Tensor& scales, const std::vect
 
 bool mx4_copied(const Tensor& rows, int64_t width) {
   return width % 8 != 0 || rows.stride(0) % 8 != 0 || (reinterpret_cast<uintptr_t>(rows.data_ptr()) & 15) != 0;
-}
-
-// The 4-bit weights of a call: buffers of the sizes the library lays out.
-void mx4_check_keys(const Tensor& codes, const Tensor& scales, int64_t E, int64_t d_in, int64_t d_out) {
-  require_device(codes, "keys");
-  require_device(scales, "keys");
-  if (codes.scalar_type() != at::kByte || scales.scalar_type() != at::kByte || !codes.is_contiguous() ||
-      !scales.is_contiguous() || (size_t)codes.numel() != cvmm_mx4_keys_bytes(E, d_in, d_out, 0) ||
-      (size_t)scales.numel() != cvmm_mx4_keys_bytes(E, d_in, d_out, 1) ||
-      (reinterpret_cast<uintptr_t>(codes.data_ptr()) & 15) != 0 || (reinterpret_cast<uintptr_t>(scales.data_ptr()) & 3) != 0)
-    throw py::value_error("cvmm_mx4: codes and scales are not those of the weights' shape");
 }
 
 // A sorted selection: pointers into the sort's buffers, or into a selector's own
@@ -942,7 +953,9 @@ Tensor mx4_forward_impl(const Tensor& x, const Tensor& codes, const Tensor& scal
                         at::IntArrayRef shape) {
   require_device(x, "x");
   const auto op = dtype_of(op_id);
-  mx4_check_keys(codes, scales, r.E, d_in, d_out);
+  require_device(codes, "keys");
+  require_device(scales, "keys");
+  mx4_check(codes, scales, {r.E, d_in, d_out}, true, "cvmm_mx4");
   if (x.dim() < 1 || x.size(-1) != d_in) throw py::value_error("cvmm_mx4: x.shape[-1] must equal the weights' d_in");
   Tensor xf = rows_of(x.scalar_type() == op ? x : x.to(op), d_in);
   OptT rwf;
@@ -1223,4 +1236,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   // operand rules, exposed for tests
   m.def("storage_for", [](const Tensor& t, int64_t op_id) { return storage_for(t, dtype_of(op_id)); });
   m.def("keys_view", &keys_view);
+  m.def("mx4_check", &mx4_check);
 }

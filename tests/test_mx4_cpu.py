@@ -135,3 +135,36 @@ def test_oracle_routes_within_the_best_groups():
     w, sel = O.route(logits, 2, scores="sigmoid", groups=4, topk_groups=1)
     assert sel.tolist() == [[3, 2]]            # the pair (1, 1.5) beats (3, -5)
     assert abs(float(w.sum()) - 1) < 1e-12
+
+
+def test_buffers_have_to_fit_the_shape(lib):
+    """What a caller puts together from stored codes and scales is checked before
+    any kernel reads them by the shape."""
+    def buf(n, at=0):
+        return torch.zeros(n + 64, dtype=torch.uint8)[at:at + n]
+
+    check = N.host().mx4_check
+    for shape, keys, codes, scales in (([2, 128, 64], True, 2 * 4096, 2 * 256), ([1, 129, 65], True, 4 * 4096, 4 * 256),
+                                       ([3, 200], False, 3 * 128, 3 * 16), ([2, 3, 513], False, 6 * 320, 6 * 32),
+                                       ([0, 64], False, 0, 0)):
+        assert check(buf(codes), buf(scales), shape, keys, "t") is None
+        bad = [(buf(codes + 16), buf(scales)), (buf(codes), buf(scales + 4)), (buf(codes).char(), buf(scales)),
+               (buf(codes), buf(scales).char())]
+        if codes:
+            bad += [(buf(codes - 16), buf(scales)), (buf(codes), buf(scales - 4)), (buf(codes, 2), buf(scales)),
+                    (torch.zeros(2 * codes, dtype=torch.uint8)[::2], buf(scales)),
+                    (buf(codes), torch.zeros(2 * scales, dtype=torch.uint8)[::2])]
+        if keys:
+            bad += [(buf(codes, 4), buf(scales)), (buf(codes), buf(scales, 1))]
+        for c, s in bad:
+            with pytest.raises(ValueError, match="shape"):
+                check(c, s, shape, keys, "t")
+        if codes:  # a larger or an impossible shape
+            for other in ([*shape[:-1], shape[-1] + 512], [*shape[:-1], 0], [-1, *shape[1:]], [shape[0] + 1, *shape[1:]]):
+                with pytest.raises(ValueError, match="shape"):
+                    check(buf(codes), buf(scales), other, keys, "t")
+    for shape in ([64], [2, 64], [2, 2, 64, 64]):
+        with pytest.raises(ValueError, match="shape"):
+            check(buf(8192), buf(512), shape, True, "t")
+    with pytest.raises(ValueError, match="shape"):
+        check(buf(0), buf(0), [], False, "t")
