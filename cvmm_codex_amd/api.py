@@ -1088,6 +1088,12 @@ class CVMMMx4:
     shape: torch.Size
     dim: int
 
+    def __post_init__(self):
+        n = len(self.shape)
+        if not (-n <= self.dim < n) or (self.dim % n != n - 1 and not (n == 3 and self.dim % n == 1)):
+            raise ValueError(f"CVMMMx4: dim {self.dim} of {tuple(self.shape)} is not the last, or 1 of [E, d_in, d_out]")
+        self.dim %= n
+
     @property
     def device(self) -> torch.device:
         return self.codes.device

@@ -168,3 +168,14 @@ def test_buffers_have_to_fit_the_shape(lib):
             check(buf(8192), buf(512), shape, True, "t")
     with pytest.raises(ValueError, match="shape"):
         check(buf(0), buf(0), [], False, "t")
+
+
+def test_dims_of_a_4_bit_tensor():
+    def make(shape, dim):
+        return C.CVMMMx4(torch.zeros(1, dtype=torch.uint8), torch.zeros(1, dtype=torch.uint8), torch.Size(shape), dim)
+    assert make([2, 128, 128], -1).dim == 2 and not make([2, 128, 128], -1)._keys
+    assert make([2, 128, 128], -2).dim == 1 and make([2, 128, 128], 1)._keys
+    assert not make([4, 64], 1)._keys and not make([64], 0)._keys
+    for shape, dim in (([2, 64, 64], 0), ([2, 64], 0), ([2, 64], 2), ([2, 64], -3), ([2, 3, 64, 64], 1), ([], 0)):
+        with pytest.raises(ValueError, match="dim"):
+            make(shape, dim)
