@@ -1768,7 +1768,7 @@ int cvmm_mx4_fwd(const void* x, int32_t x_dtype, int64_t x_rows, int64_t x_ld, c
     return fail(CVMM_ERR_INVALID, "cvmm_mx4_fwd: rows must be 16-bit");
   const bool weighted = reduction_weight != nullptr;
   if (!mx4_sizes_ok(n_experts, d_in, d_out) || n_routes < 0 || n_routes > 0x7fffffff || x_rows < 0 ||
-      (x_rows > 1 && x_ld < d_in) || (out_rows > 1 && out_ld < d_out) || out_ld >= int64_t(1) << 30 ||
+      x_rows > 0x7fffffff || (x_rows > 1 && x_ld < d_in) || (out_rows > 1 && out_ld < d_out) || out_ld >= int64_t(1) << 30 ||
       (weighted && reduce_k <= 0) ||
       out_rows * (weighted ? reduce_k : 1) != n_routes)
     return fail(CVMM_ERR_INVALID, "cvmm_mx4_fwd: bad sizes (E=%d, d_in=%lld, d_out=%lld, R=%lld, rows %lld -> %lld)",

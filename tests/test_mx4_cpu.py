@@ -179,3 +179,12 @@ def test_dims_of_a_4_bit_tensor():
     for shape, dim in (([2, 64, 64], 0), ([2, 64], 0), ([2, 64], 2), ([2, 64], -3), ([2, 3, 64, 64], 1), ([], 0)):
         with pytest.raises(ValueError, match="dim"):
             make(shape, dim)
+
+
+def test_row_indices_fit_32_bits(lib):
+    """The products hold row indices in 32 bits: more rows are refused, not read as
+    none."""
+    def fwd(rows):
+        return lib.cvmm_mx4_fwd(FAKE, N.BF16, rows, 64, FAKE, FAKE, 4, 64, 32, FAKE, FAKE, 16, FAKE, FAKE, None, 1, 0,
+                                FAKE, 16, 32, None, 0, None)
+    assert fwd(2 ** 31) == 1 and b"sizes" in lib.cvmm_last_error()
