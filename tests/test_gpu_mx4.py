@@ -497,3 +497,51 @@ def test_forward_mode_is_refused():
                     with pytest.raises(Exception):
                         call(xd, torch.autograd.forward_ad.make_dual(gd, torch.ones_like(gd)), quantize, pending)
                 assert torch.equal(call(xd, gd, False, pending), y) and torch.equal(call(xd, gd, True, pending), yq)
+
+
+@pytest.mark.parametrize("mode", MODES)
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_gradients_equal_exact_differences(mode, dtype):
+    """Rows of -1, 0 and 1, weights of the grid, powers of two as routing weights:
+    no output rounds, so the linear product's differences are its gradients,
+    to the last bit.  Every gradient of a routing weight and a spread of those
+    of the rows."""
+    T, d_in, d_out, E, k = 5, 40, 24, 3, 2
+    g = _gen(31)
+    levels = torch.tensor([-1.0, -0.5, 0.0, 0.5, 1.0])
+    keys = levels[torch.randint(0, 5, (E, d_in, d_out), generator=g)]
+    x = torch.randint(-1, 2, (T, k, d_in) if mode == "down" else (T, d_in), generator=g).to(dtype)
+    sel = torch.stack([torch.randperm(E, generator=g)[:k] for _ in range(T)])
+    gates = None if mode == "up" else 2.0 ** torch.randint(-1, 2, (T, k), generator=g)
+    grad = torch.randint(-1, 2, (T, k, d_out) if mode == "up" else (T, d_out), generator=g).to(dtype)
+    packed = C.cvmm_mx4_quantize(keys.cuda(), dim=1)
+    assert torch.equal(packed.dequantize().cpu(), keys)
+    xd = x.cuda().requires_grad_()
+    gd = None if gates is None else gates.cuda().requires_grad_()
+
+    def f(xx, gg):
+        return C.cvmm_mx4(xx, C.cvmm_prepare_sel2(sel.cuda(), gg, route_input=mode == "down"), packed)
+
+    y = f(xd, gd)
+    assert torch.equal(y.detach().cpu().double(), O.product(x, sel, keys, gates)["y"])   # nothing rounded
+    got = torch.autograd.grad(y, [xd] + ([] if gd is None else [gd]), grad.cuda())
+    weighed = lambda v: float((v.double() * grad.cuda().double()).sum())
+    with torch.no_grad():
+        base = weighed(y)
+
+        def differences(t, at, call):
+            out = []
+            for i in at:
+                moved = t.detach().clone()
+                moved.view(-1)[i] += 1
+                out.append(weighed(call(moved)) - base)
+            return torch.tensor(out, dtype=torch.float64)
+
+        at = list(range(0, x.numel(), 7))
+        num = differences(xd, at, lambda t: f(t, gd))
+        assert int((num != 0).sum()) > len(at) // 2
+        assert torch.equal(got[0].reshape(-1)[at].cpu().double(), num)
+        if gd is not None:
+            num = differences(gd, range(T * k), lambda t: f(xd, t))
+            assert int((num != 0).sum()) > T * k // 2
+            assert torch.equal(got[1].reshape(-1).cpu().double(), num)
