@@ -545,3 +545,32 @@ def test_gradients_equal_exact_differences(mode, dtype):
             num = differences(gd, range(T * k), lambda t: f(xd, t))
             assert int((num != 0).sum()) > T * k // 2
             assert torch.equal(got[1].reshape(-1).cpu().double(), num)
+
+
+def test_compiled_quantisation_and_block():
+    """Quantised rows and keys, and a router with both products traced as one graph,
+    against the same lines in eager mode."""
+    T, D, H, E, k = 24, 128, 96, 8, 2
+    g = _gen(41)
+    x, logits = torch.randn(T, D, generator=g).to(BF).cuda(), torch.randn(T, E, generator=g).cuda()
+    w_up, w_down = torch.randn(E, D, H, generator=g).cuda(), torch.randn(E, H, D, generator=g).cuda()
+
+    def values(t, w):
+        return C.cvmm_mx4_quantize(t).dequantize(BF), C.cvmm_mx4_quantize(w, dim=1).dequantize()
+
+    up, down = C.cvmm_mx4_quantize(w_up, dim=1), C.cvmm_mx4_quantize(w_down, dim=1)
+
+    def block(xx, ll):
+        gates, _, sel = C.cvmm_route_scored(ll, k, scores="sigmoid")
+        h = torch.relu(C.cvmm_mx4(xx, sel, up))
+        return C.cvmm_mx4(h, C.cvmm_prepare_sel2(sel, gates, route_input=True), down)
+
+    for a, c in zip(values(x, w_up), torch.compile(values, backend="aot_eager", fullgraph=True)(x, w_up)):
+        assert torch.equal(a, c)
+    res = []
+    for fn in (block, torch.compile(block, backend="aot_eager")):
+        xx, ll = x.clone().requires_grad_(), logits.clone().requires_grad_()
+        y = fn(xx, ll)
+        res.append((y, *torch.autograd.grad(y, [xx, ll], torch.ones_like(y))))
+    for a, c in zip(*res):
+        assert torch.equal(a, c)

@@ -295,3 +295,26 @@ def test_sum_below_the_clamp(scores):
     # exp's argument, a few more of exp, sum, quotient, difference and product
     tol = exp.abs() * 2.0 ** -24 * (1.01 if scores == "sigmoid" else 70)
     assert bool(((got.cpu().double() - exp).abs() <= tol + 1e-45).all())
+
+
+@pytest.mark.parametrize("scores,groups,kept,renorm,bias", [("sigmoid", 4, 2, True, True), ("softmax", 1, 1, False, False),
+                                                            ("softmax", 8, 3, True, True)])
+def test_compiled_with_gradients(scores, groups, kept, renorm, bias):
+    """Traced through the registered shapes and the registered backward: the eager
+    call's weights, choice, sorted selection and gradients, bit for bit."""
+    logits, b, g = _logits(21, 64, torch.bfloat16, 9)
+    bd = b.cuda() if bias else None
+    gw = torch.randn(21, 5, generator=g).cuda()
+
+    def f(l):
+        w, sel, routed = C.cvmm_route_scored(l, 5, bias=bd, scores=scores, groups=groups, topk_groups=kept,
+                                             renormalize=renorm, scale=2.0)
+        return w, sel, routed.sel, routed.sel_index, routed.out_index
+
+    res = []
+    for fn in (f, torch.compile(f, backend="aot_eager", fullgraph=True)):
+        l = logits.cuda().requires_grad_()
+        out = fn(l)
+        res.append((*out, *torch.autograd.grad(out[0], [l], gw)))
+    for a, c in zip(*res):
+        assert a.dtype == c.dtype and torch.equal(a, c)
