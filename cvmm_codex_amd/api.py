@@ -1157,8 +1157,9 @@ def cvmm_mx4(x: torch.Tensor, sel: Union[torch.Tensor, CVMMSel], keys: CVMMMx4,
     over a token's routes are fp32, routes' rows of a weighted sum rounded once to
     the op type.
 
-    ``quantize_input``: the rows are quantised to 4-bit values as well and
-    multiplied as such (four times the matrix rate); for inference, without
+    ``quantize_input``: the rows, in the op type (under autocast fp32 rows are
+    rounded to it first, as for any product), are quantised to 4-bit values as well
+    and multiplied as such (four times the matrix rate); for inference, without
     gradients."""
     if not isinstance(keys, CVMMMx4) or not keys._keys:
         raise TypeError("cvmm_mx4: keys must be cvmm_mx4_quantize(weights, dim=1)")
