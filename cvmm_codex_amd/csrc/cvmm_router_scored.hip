@@ -154,11 +154,14 @@ __global__ __launch_bounds__(THREADS) void route_scored_kernel(
     // argument and an ulp; 1 + 0.95 |x| measured).  Sigmoid: s (1 - s) of that,
     // below 0.8, and at most 1 each for the sum and the reciprocal: 2^-21 for both
     // sides.  Softmax: exp (l - m rounds too) and the product with 1 / sum, 3 of the
-    // largest score on either side.  The sum scales all scores alike; where a bias
-    // cancels the distance of two, its error counts once, of the largest score: 1
-    // per addition, of a lane's experts and over the lanes, 1 for the reciprocal,
-    // and the exps' 2 + 2.22 times their weighted mean |x|, at most 4.5 for 1024
-    // experts.  The sum with the bias rounds by half an ulp of itself.
+    // largest score on either side (8 for both, with the remainders).  The sum
+    // scales all scores alike: its error counts once, of the distance of the two
+    // scores, which is that of their biases where they nearly tie: 1 per addition,
+    // of a lane's experts and over the lanes, 1 for the reciprocal, and the exps'
+    // 2 + 2.22 times their weighted mean |x|, at most 4.5 for 1024 experts.
+    // (Taken of the largest score instead, 17 of 16384 tokens of 128 experts would
+    // be ranked in 64 bits, not 4.)  The sum with the bias rounds by half an ulp of
+    // itself.
     // (Loads at clamped places: a guard around each made them
     // wait for one another.)
     float l[MAXV], c[MAXV];
@@ -190,7 +193,14 @@ __global__ __launch_bounds__(THREADS) void route_scored_kernel(
       sum = seg_sum<LPT>(s);
       unsure = isnan(sum);
       const float inv = 1.f / sum;
-      err = (MAXV + __builtin_ctz(LPT) + 20) * 0x1p-24f * inv;  // of the largest score, 1 / sum
+      float b = 0.f;
+      if (p.bias != nullptr) {
+#pragma unroll
+        for (int v = 0; v < MAXV; ++v) b = fmaxf(b, fabsf(c[v]));
+        b = __int_as_float(seg_max_i<LPT>(__float_as_int(b)));  // (not negative: in the integers' order)
+      }
+      // (the largest score: 1 / sum)
+      err = 0x1p-24f * (8.f * inv + (MAXV + __builtin_ctz(LPT) + 12) * fminf(2.f * b, inv));
 #pragma unroll
       for (int v = 0; v < MAXV; ++v) c[v] += x[v] * inv;
     }
@@ -225,19 +235,12 @@ __global__ __launch_bounds__(THREADS) void route_scored_kernel(
     int32_t res_e[SLOTS];
 #pragma unroll
     for (int q = 0; q < SLOTS; ++q) res_e[q] = 0;
-    // does every smaller logit have a smaller 64-bit score?  From 2^-15 on fp32
-    // numbers lie 2^-40 apart, which exp and the sums keep (2^-43 at most is lost)
-    // unless the score leaves the normal numbers (below e^-708), or a sigmoid nears
-    // 1: up to 16 its steps are 2^-43 still, from 24 on it repeats values.
-    auto sure = [&](float v) {
-      return fabsf(v) >= 0x1p-15f && (p.sigmoid ? v < 16.f && v > -700.f : v - m > -700.f);
-    };
     float before = INFINITY;
     int n = 0;
-    bool near = false;
+    bool near = false, apart = true;
 #pragma unroll 1
     for (;; ++n) {
-      if (n == k && by_logit && sure(before)) break;
+      if (n == k && by_logit) break;
       int32_t bv = key[0];
 #pragma unroll
       for (int v = 1; v < MAXV; ++v) bv = max(bv, key[v]);
@@ -248,13 +251,8 @@ __global__ __launch_bounds__(THREADS) void route_scored_kernel(
       for (int v = MAXV - 1; v >= 0; --v) bi = key[v] == mv ? li + LPT * v : bi;
       const int32_t win = seg_min_i<LPT>(bi);
       const float now = __int_as_float(mv ^ ((mv >> 31) & 0x7fffffff));
-      const bool apart = n == 0 || (by_logit ? sure(before)
-                                             : before - now > err + 0x1p-23f * (fabsf(before) + fabsf(now)));
-      if (n >= k && apart) break;
-      if (n == 64) {
-        unsure = true;
-        break;
-      }
+      apart = by_logit || n == 0 || before - now > err + 0x1p-23f * (fabsf(before) + fabsf(now));
+      if (n >= k && (apart || n == 64)) break;
       near |= !apart;
       before = now;
 #pragma unroll
@@ -263,7 +261,24 @@ __global__ __launch_bounds__(THREADS) void route_scored_kernel(
       for (int q = 0; q < SLOTS; ++q)
         if (n == q * LPT + li) res_e[q] = win;
     }
-    unsure |= n > k + 8 || n < k;
+    unsure |= n > k + 8 || n < k || (n == 64 && !apart);
+    if (by_logit) {
+      // Does every logit below a chosen one have a smaller 64-bit score?  From 2^-15 on
+      // fp32 numbers lie 2^-40 apart, which exp and the sums keep (2^-43 at most is
+      // lost) unless the score leaves the normal numbers (below e^-708), or a sigmoid
+      // nears 1: up to 16 its steps are 2^-43 still, from 24 on it repeats values.
+      unsure |= !(before - (p.sigmoid ? 0.f : m) > -700.f);
+      if (before < 0x1p-15f) {
+#pragma unroll
+        for (int v = 0; v < MAXV; ++v) unsure |= l[v] >= before && fabsf(l[v]) < 0x1p-15f;
+      }
+      if (p.sigmoid) {
+        float high = l[0];
+#pragma unroll
+        for (int v = 1; v < MAXV; ++v) high = fmaxf(high, l[v]);
+        unsure |= high >= 16.f;
+      }
+    }
     // ---- all scores in 64 bits, for a wave with an unsure token: NaN, groups within
     // the error, or a crowd of candidates
     const bool again = active && (__ballot(unsure) & seg_mask) != 0;
