@@ -535,7 +535,7 @@ int cvmm_mx4_dequantize_keys(const void* codes, const void* scales, int32_t n_ex
  * values first (rows layout, in the workspace) and multiplied as such.
  * reduction_weight (fp32, or NULL): the weighted sum over each token's
  * reduce_k routes, summed in fp32.  Rows of routes with an expert id outside
- * [0, E) are zero.  x_copied of the workspace query: the rows are not made of
+ * [0, E) are zero; at most 2^31 - 1 rows and routes.  x_copied of the workspace query: the rows are not made of
  * aligned 16-byte pieces (d_in or x_ld no multiple of 8, or x not aligned). */
 size_t cvmm_mx4_fwd_workspace_bytes(int64_t n_routes, int64_t d_in, int64_t d_out, int64_t x_rows, int32_t weighted,
                                     int32_t have_route_pos, int32_t x_copied, int32_t quantize_input);
