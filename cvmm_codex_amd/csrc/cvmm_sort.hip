@@ -529,15 +529,20 @@ __global__ __launch_bounds__(kSortThreads) void sort_scatter_cast_kernel(const S
 }
 
 // Upper-bound binary search per expert over an already sorted int32 array
-// (the reference's cvmm_expert_offsets_kernel, cvmm.py:315-335).
+// (the reference's cvmm_expert_offsets_kernel, cvmm.py:315-335).  The sorts here
+// leave every id outside the experts last, negative ones too: compared as
+// unsigned numbers they stand above all experts.  Negative ids in front, as an
+// ascending sort leaves them, count as in the reference.
 __global__ void expert_offsets_kernel(const int32_t* __restrict__ sorted_sel, int64_t n_routes,
                                       int32_t n_experts, int64_t* __restrict__ offsets) {
   const int64_t e = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (e >= n_experts) return;
+  const bool in_front = n_routes > 0 && sorted_sel[0] < 0 && sorted_sel[n_routes - 1] >= 0;
   int64_t lo = 0, hi = n_routes;
   while (lo < hi) {
     const int64_t mid = (lo + hi) >> 1;
-    if ((int64_t)sorted_sel[mid] <= e) lo = mid + 1;
+    const int32_t id = sorted_sel[mid];
+    if ((in_front ? (int64_t)id : (int64_t)(uint32_t)id) <= e) lo = mid + 1;
     else hi = mid;
   }
   offsets[e] = lo;

@@ -281,8 +281,7 @@ int cvmm_route_topk_backward(const void* logits, int32_t logits_dtype, int64_t n
  * top_k best remaining experts are chosen (ties to the lower id).  weights =
  * scale * s at the chosen experts, divided by their sum (at least 1e-20) if
  * renormalize.  The choice is that of 64-bit scores, made in 32 bits where those
- * decide it; the weights are computed in 64 bits.  Outputs as
- * cvmm_route_topk's; at most 64 groups unless all stay. */
+ * decide it.  Outputs as cvmm_route_topk's; at most 64 groups unless all stay. */
 #define CVMM_SCORES_SOFTMAX 0
 #define CVMM_SCORES_SIGMOID 1
 size_t cvmm_route_scored_workspace_bytes(int64_t n_tokens, int32_t n_experts, int64_t top_k);
@@ -315,7 +314,8 @@ int cvmm_copy_ids_count(const void* sel, int32_t sel_is_int64, int64_t n, int32_
                         void* workspace, size_t workspace_bytes, void* stream);
 
 /* offsets[e] = #{i : sorted_sel[i] <= e}; replaces cvmm_expert_offsets
- * (cvmm.py:1108-1120, kernel cvmm.py:315-335). */
+ * (cvmm.py:1108-1120, kernel cvmm.py:315-335).  Negative ids that stand last, as
+ * the sorts here leave them, are counted for no expert. */
 int cvmm_expert_offsets(const int32_t* sorted_sel, int64_t n_routes, int32_t n_experts, int64_t* offsets,
                         void* stream);
 
@@ -535,8 +535,9 @@ int cvmm_mx4_dequantize_keys(const void* codes, const void* scales, int32_t n_ex
  * values first (rows layout, in the workspace) and multiplied as such.
  * reduction_weight (fp32, or NULL): the weighted sum over each token's
  * reduce_k routes, summed in fp32.  Rows of routes with an expert id outside
- * [0, E) are zero; at most 2^31 - 1 rows and routes.  x_copied of the workspace query: the rows are not made of
- * aligned 16-byte pieces (d_in or x_ld no multiple of 8, or x not aligned). */
+ * [0, E) are zero; at most 2^31 - 1 rows and routes.  x_copied of the workspace
+ * query: the rows are not made of aligned 16-byte pieces (d_in or x_ld no
+ * multiple of 8, or x not aligned). */
 size_t cvmm_mx4_fwd_workspace_bytes(int64_t n_routes, int64_t d_in, int64_t d_out, int64_t x_rows, int32_t weighted,
                                     int32_t have_route_pos, int32_t x_copied, int32_t quantize_input);
 int cvmm_mx4_fwd(const void* x, int32_t x_dtype, int64_t x_rows, int64_t x_ld, const void* codes, const void* scales,

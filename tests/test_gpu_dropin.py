@@ -227,3 +227,36 @@ def test_copy_ids_is_the_int32_conversion(dtype, n, offset):
     N.check(N.lib().cvmm_copy_ids(N.ptr(sel), 1 if dtype == torch.int64 else 0, n, N.ptr(out),
                                   N.stream_of(sel.device)), "cvmm_copy_ids")
     assert torch.equal(out.cpu(), sel.cpu().to(torch.int32))
+
+
+@pytest.mark.parametrize("ids", ["some", "all"])
+@pytest.mark.parametrize("compiled", [False, True])
+def test_negative_ids_of_a_selector_that_was_read(compiled, ids):
+    """Routes without an expert (-1) give zero rows also where the selection was
+    sorted before its product knew the expert count, and in a compiled call."""
+    E, T, k, D, H = 12, 40, 3, 64, 48
+    g = torch.Generator().manual_seed(24)
+    sel = torch.randint(0, 5, (T, k), generator=g)      # experts 5.. idle: a sort for 5 of them
+    sel[torch.rand(T, k, generator=g) < 0.2] = -1
+    if ids == "all":
+        sel[:] = -1
+    x = torch.randn(T, D, generator=g).to(torch.bfloat16).cuda()
+    keys = torch.randn(E, D, H, generator=g).to(torch.bfloat16).cuda()
+    sd = sel.cuda()
+
+    def f(xx):
+        s = C.cvmm_prepare_sel2(sd)
+        if not compiled:
+            assert s.sel.numel() == T * k
+        return C.cvmm(xx, s, keys)
+
+    with torch.no_grad(), torch.autocast("cuda", dtype=torch.bfloat16):
+        exp = C.cvmm(x, C.cvmm_prepare_sel2(sd), keys)
+        y = (torch.compile(f, backend="eager") if compiled else f)(x)
+        if not compiled:
+            p = C.cvmm_mx4_quantize(keys, dim=1)
+            s = C.cvmm_prepare_sel2(sd)
+            assert s.sel.numel() == T * k
+            assert torch.equal(C.cvmm_mx4(x, s, p), C.cvmm_mx4(x, C.cvmm_prepare_sel2(sd), p))
+    assert not bool(exp[sel.cuda() < 0].any())
+    assert torch.equal(y, exp)
