@@ -330,7 +330,8 @@ __global__ __launch_bounds__(THREADS) void route_scored_kernel(
       }
     }
     // the candidates' scores in 64 bits, by the lanes that hold them; a softmax's
-    // sum is 64-bit where it does not cancel
+    // sum is 64-bit where it does not cancel (but for chosen scores under the clamp:
+    // such weights are off by up to 2 ulp)
     double total = (double)sum;
     const bool rank = __any(active && near);
     if (!p.sigmoid && (rank || !p.renorm)) {
