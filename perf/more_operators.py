@@ -1,0 +1,352 @@
+"""The operators of fine-tuning and serving a mixture-of-experts block whose speed is measured.
+
+Two kinds of case:
+
+- ``lora``: low-rank adapters of many requests beside a projection that they
+  share.  Row t of x has the adapter i = ids[t] (-1: none):
+  y[t] = base[t] + x[t] W + s (x[t] A_i) B_i.  ``rows`` says how the ids stand:
+  "own": each row is another request's (decode); "runs": the rows of a request
+  stand together (prompts, training sequences); "routes": each row is a token's
+  route and its adapter that of the expert (the projection's output is the
+  frozen experts', given as ``base``, and there is no W).  ``train`` adds the
+  gradients of the rows and of the adapters; W and base are frozen.
+- ``balance``: the balance of a router.  With p the softmax of a token's logits
+  (or its sigmoids over their sum), P_e the mean of p_e over the tokens of a
+  group (a sequence, or all tokens) and c_e the routes to expert e:
+  "load": sum_e E c_e / (k n) P_e; "entropy": sum_e P_e log P_e; each averaged
+  over the groups.  Beside it z = the mean of logsumexp(l)^2, and the counts of
+  all routes per expert.  Padded tokens (mask) count nowhere.  Always with the
+  logits' gradient of loss + 0.01 z.
+"""
+import math
+
+import torch
+
+own = False
+
+_TYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
+_SCALE = 2.0
+_Z = 0.01
+
+
+def _lora(name, tokens, d_in, d_out, rank, adapters, rows, dtype, train=False):
+    case = {"kind": "lora", "tokens": tokens, "d_in": d_in, "d_out": d_out, "rank": rank, "adapters": adapters,
+            "rows": rows, "dtype": dtype, "train": train}
+    return {"name": name, **case} if name else case
+
+
+def _balance(name, sequences, tokens, experts, k, what, scores, per_sequence, masked, dtype):
+    case = {"kind": "balance", "sequences": sequences, "tokens": tokens, "experts": experts, "k": k, "what": what,
+            "scores": scores, "per_sequence": per_sequence, "masked": masked, "dtype": dtype}
+    return {"name": name, **case} if name else case
+
+
+def listed():
+    return [
+        # one sequence decoding with its adapter: the call's latency
+        _lora("lora_decode_1", 1, 1024, 1024, 16, 8, "own", "bfloat16"),
+        # a decode step of a served batch, a pool of adapters, some requests without one
+        _lora("lora_decode_32", 32, 2048, 2048, 16, 64, "own", "bfloat16"),
+        # a larger served batch on a wide projection
+        _lora("lora_decode_128", 128, 1024, 2048, 32, 100, "own", "float16"),
+        # prefill of a few prompts together, odd lengths
+        _lora("lora_prefill_1999", 1999, 2048, 1024, 32, 8, "runs", "float16"),
+        # widths and a rank that no tile divides
+        _lora("lora_odd", 777, 1000, 518, 12, 5, "runs", "bfloat16"),
+        # the largest prefill
+        _lora("lora_prefill_16384", 16384, 2048, 2048, 64, 16, "runs", "bfloat16"),
+        # a training step over the sequences of several adapters
+        _lora("lora_train_8192", 8192, 1024, 1024, 16, 8, "runs", "bfloat16", True),
+        # fine-tuning adapters of the experts beside their frozen down projection: 8 routes a token
+        _lora("lora_experts_16384", 16384, 128, 1024, 16, 64, "routes", "bfloat16", True),
+        # a small router's regulariser
+        _balance("balance_512", 1, 512, 16, 2, "entropy", "softmax", False, False, "float32"),
+        # padded sequences of a training step, balanced one by one
+        _balance("balance_padded_4x2048", 4, 2048, 64, 8, "load", "sigmoid", True, True, "float32"),
+        # the feed-forward stack's router over a whole step
+        _balance("balance_16384", 1, 16384, 128, 8, "load", "softmax", False, False, "bfloat16"),
+        # many experts, long sequences
+        _balance("balance_8x4096_256", 8, 4096, 256, 8, "entropy", "softmax", True, True, "bfloat16"),
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    """One more case of the listed ones' ranges."""
+    family = rng.choice(["balance", "balance", "decode", "decode", "prefill", "prefill", "train", "routes"])
+    if family == "balance":
+        experts = _log_int(rng, 8, 256)
+        sequences = rng.choice([1, 1, 2, 4, 8])
+        return _balance("", sequences, _log_int(rng, 64, 32768 // sequences), experts, rng.randint(1, min(8, experts)),
+                        rng.choice(["load", "load", "entropy"]), rng.choice(["softmax", "sigmoid"]),
+                        rng.choice([False, True]), rng.choice([False, True]),
+                        rng.choice(["float32", "bfloat16", "float16"]))
+    step = rng.choice([1, 8, 64, 64])
+    d_in, d_out = (step * _log_int(rng, max(1, 128 // step), 2048 // step) for _ in range(2))
+    rank = rng.choice([4, 8, 16, 16, 32, 64, rng.randint(3, 64)])
+    dtype = rng.choice(["bfloat16", "bfloat16", "float16"])
+    lo, hi = {"decode": (1, 256), "prefill": (200, 16384), "train": (200, 8192), "routes": (500, 16384)}[family]
+    tokens = _log_int(rng, lo, hi)
+    if family == "routes":
+        return _lora("", tokens, min(d_in, d_out), max(d_in, d_out), rank, _log_int(rng, 8, 128), "routes", dtype,
+                     rng.choice([False, True]))
+    adapters = _log_int(rng, 1, 128 if family == "decode" else 32)
+    return _lora("", tokens, d_in, d_out, rank, adapters, "own" if family == "decode" else "runs", dtype,
+                 family == "train")
+
+
+def _randn(g, *shape):
+    return torch.randn(*shape, generator=g, device="cuda")
+
+
+def _rand(g, *shape):
+    return torch.rand(*shape, generator=g, device="cuda")
+
+
+def _lora_ids(case, g):
+    T, n = case["tokens"], case["adapters"]
+    if case["rows"] == "routes":  # experts by a router's mildly uneven choice
+        p = torch.softmax(_randn(g, -(-T // 8), n) + 0.3 * _randn(g, n), dim=-1)
+        return p.topk(min(8, n), dim=-1).indices.repeat(1, -(-8 // min(8, n)))[:, :8].reshape(-1)[:T].contiguous()
+    if case["rows"] == "own":
+        ids = (_rand(g, T) * n).long().clamp_(max=n - 1)
+        return torch.where(_rand(g, T) < 0.1, -1, ids)
+    # runs of ragged lengths, one a request, each of some adapter; one of them without
+    m = min(T, max(2, n))
+    ends = (_rand(g, m) + 0.5).cumsum(0)
+    ends = (ends / ends[-1] * T).long()
+    run = torch.bucketize(torch.arange(T, device="cuda"), ends[:-1], right=True)
+    of = torch.randperm(m, generator=g, device="cuda") % n
+    if m > 2:
+        of[1] = -1
+    return of[run]
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    dtype = _TYPES[case["dtype"]]
+    state = {"case": case}
+    if case["kind"] == "lora":
+        T, d_in, d_out, r, n = (case[f] for f in ("tokens", "d_in", "d_out", "rank", "adapters"))
+        state["ids"] = _lora_ids(case, g)
+        state["x"] = _randn(g, T, d_in).to(dtype)
+        state["a"] = (_randn(g, n, d_in, r) / math.sqrt(d_in)).to(dtype)
+        state["b"] = (0.3 * _randn(g, n, r, d_out) / math.sqrt(r)).to(dtype)
+        state["weight"] = state["base"] = None
+        if case["rows"] == "routes":
+            state["base"] = _randn(g, T, d_out).to(dtype)
+        else:
+            state["weight"] = (_randn(g, d_in, d_out) / math.sqrt(d_in)).to(dtype)
+        if case["train"]:
+            state["grad"] = _randn(g, T, d_out).to(dtype)
+            for f in ("x", "a", "b"):
+                state[f].requires_grad_()
+        return state
+    S, T, E, k = (case[f] for f in ("sequences", "tokens", "experts", "k"))
+    # experts that the gate likes more or less, and a choice that a balance bias has moved a little
+    logits = 1.5 * _randn(g, S, T, E) + 0.5 * _randn(g, E)
+    state["sel"] = (logits + 0.2 * _randn(g, E)).topk(k, dim=-1).indices.contiguous()
+    state["logits"] = logits.to(dtype).requires_grad_()
+    state["mask"] = None
+    if case["masked"]:  # sequences padded to the longest
+        lengths = (T * (0.5 + 0.5 * _rand(g, S, 1))).long().clamp_(min=1)
+        state["mask"] = torch.arange(T, device="cuda") < lengths
+    return state
+
+
+def _by_adapter(rows, ids, mats):
+    """rows[t] @ mats[ids[t]], zero where there is none: the rows of each adapter
+    side by side, one product of all."""
+    n = mats.shape[0]
+    key, order = torch.sort(torch.where((ids >= 0) & (ids < n), ids, n), stable=True)
+    load = torch.bincount(key, minlength=n + 1)
+    at = torch.arange(key.numel(), device=key.device) - (load.cumsum(0) - load)[key]
+    padded = rows.new_zeros(n + 1, int(load.max()), rows.shape[1])
+    padded[key, at] = rows[order]
+    none = mats.new_zeros(1, *mats.shape[1:])
+    out = torch.bmm(padded, torch.cat([mats, none]))[key, at]
+    return torch.empty_like(out).index_copy_(0, order, out)
+
+
+def _outer_by_adapter(left, right, ids, n):
+    """sum over the rows t of each adapter of left[t]^T right[t]."""
+    key, order = torch.sort(torch.where((ids >= 0) & (ids < n), ids, n), stable=True)
+    load = torch.bincount(key, minlength=n + 1)
+    at = torch.arange(key.numel(), device=key.device) - (load.cumsum(0) - load)[key]
+    most = int(load.max())
+    pl, pr = (v.new_zeros(n + 1, most, v.shape[1]) for v in (left, right))
+    pl[key, at], pr[key, at] = left[order], right[order]
+    return torch.bmm(pl.transpose(1, 2), pr)[:n]
+
+
+def _plain_lora(state):
+    case, ids = state["case"], state["ids"]
+    dtype = _TYPES[case["dtype"]]
+    x, a, b = (state[f].detach().float() for f in ("x", "a", "b"))
+    h = _SCALE * _by_adapter(x, ids, a)
+    y = _by_adapter(h, ids, b)
+    if state["weight"] is not None:
+        y = y + x @ state["weight"].float()
+    if state["base"] is not None:
+        y = y + state["base"].float()
+    res = {"y": y.to(dtype)}
+    if case["train"]:
+        g = state["grad"].float()
+        u = _SCALE * _by_adapter(g, ids, b.transpose(1, 2).contiguous())
+        dx = _by_adapter(u, ids, a.transpose(1, 2).contiguous())
+        if state["weight"] is not None:
+            dx = dx + g @ state["weight"].float().t()
+        n = case["adapters"]
+        res.update({"grad_x": dx.to(dtype), "grad_a": _outer_by_adapter(x, u, ids, n).to(dtype),
+                    "grad_b": _outer_by_adapter(h, g, ids, n).to(dtype)})
+    return res
+
+
+def _plain_balance(state):
+    case = state["case"]
+    S, T, E, k = (case[f] for f in ("sequences", "tokens", "experts", "k"))
+    groups = S if case["per_sequence"] else 1
+    l = state["logits"].detach().float()
+    live = torch.ones(S, T, 1, device=l.device) if state["mask"] is None else state["mask"].unsqueeze(-1).float()
+    e = torch.exp(l - l.amax(-1, keepdim=True))
+    soft = e / e.sum(-1, keepdim=True)
+    lse = l.amax(-1, keepdim=True) + torch.log(e.sum(-1, keepdim=True))
+    if case["scores"] == "softmax":
+        p = soft
+    else:
+        s = torch.sigmoid(l)
+        total = s.sum(-1, keepdim=True)
+        p = s / total
+    routes = torch.zeros(S, T, E, device=l.device).scatter_(-1, state["sel"], 1.0) * live
+    counts = routes.view(S * T, E).sum(0).long()
+    n = live.reshape(groups, -1).sum(1).view(groups, 1)
+    c = routes.view(groups, -1, E).sum(1)
+    P = (p * live).view(groups, -1, E).sum(1) / n
+    if case["what"] == "load":
+        f = E * c / (k * n)
+        loss = (f * P).sum(-1).mean()
+    else:
+        f = torch.log(P) + 1
+        loss = (P * torch.log(P)).sum(-1).mean()
+    all_n = n.sum()
+    z = (lse * lse * live).sum() / all_n
+    coef = (f / (n * groups)).view(groups, 1, E).expand(groups, S // groups, E).reshape(S, 1, E)
+    inner = (coef * p).sum(-1, keepdim=True)
+    if case["scores"] == "softmax":
+        d = p * (coef - inner)
+    else:
+        d = s * torch.sigmoid(-l) * (coef - inner) / total
+    d = (d + _Z * 2 * lse * soft / all_n) * live
+    return {"loss": loss, "z": z, "counts": counts, "grad_logits": d.to(_TYPES[case["dtype"]])}
+
+
+def _own(state):
+    import cvmm_codex_amd as cvmm
+    case = state["case"]
+    if case["kind"] == "balance":
+        loss, z, counts = cvmm.cvmm_balance_loss(state["logits"], state["sel"], kind=case["what"],
+                                                 scores=case["scores"], mask=state["mask"],
+                                                 per_sequence=case["per_sequence"])
+        grad, = torch.autograd.grad(loss + _Z * z, [state["logits"]])
+        return {"loss": loss.detach(), "z": z.detach(), "counts": counts, "grad_logits": grad}
+    adapters = state["ids"]
+    if case["rows"] == "routes":  # the selection of the projection beside them
+        adapters = cvmm.cvmm_prepare_sel2(adapters, route_input=True)
+    with torch.set_grad_enabled(case["train"]):
+        y = cvmm.cvmm_lora(state["x"], adapters, state["a"], state["b"], weight=state["weight"], base=state["base"],
+                           scale=_SCALE)
+    res = {"y": y.detach()}
+    if case["train"]:
+        names = ["x", "a", "b"]
+        grads = torch.autograd.grad(y, [state[f] for f in names], state["grad"])
+        res.update({"grad_" + f: v for f, v in zip(names, grads)})
+    return res
+
+
+def run(state):
+    if own:
+        return _own(state)
+    return _plain_lora(state) if state["case"]["kind"] == "lora" else _plain_balance(state)
+
+
+def work(case):
+    """Inputs once, outputs once, and the multiply-adds.  (Of the adapters, those
+    that the rows can name at most.  A router's few operations per logit do not
+    count.)"""
+    size = 4 if case["dtype"] == "float32" else 2
+    if case["kind"] == "balance":
+        tokens = case["sequences"] * case["tokens"]
+        logits = size * tokens * case["experts"]
+        return {"bytes": 2 * logits + 8 * tokens * case["k"] + (tokens if case["masked"] else 0)
+                + 8 * case["experts"] + 8, "flops": 0}
+    T, d_in, d_out, r, n = (case[f] for f in ("tokens", "d_in", "d_out", "rank", "adapters"))
+    pairs = r * (d_in + d_out)
+    routes = case["rows"] == "routes"
+    shared = 0 if routes else d_in * d_out
+    nbytes = size * (T * (d_in + d_out) + min(n, T) * pairs + (T * d_out if routes else shared)) + 8 * T
+    flops = 2 * T * (shared + pairs)
+    if case["train"]:  # the output's gradient in, the rows' and the adapters' out
+        nbytes += size * (T * (d_in + d_out) + n * pairs)
+        flops += 2 * T * (shared + 2 * pairs)
+    return {"bytes": nbytes, "flops": flops}
+
+
+def exact(case, seed):
+    state = prepare(case, seed)
+    return _exact_lora(state) if case["kind"] == "lora" else _exact_balance(state)
+
+
+def _exact_lora(state):
+    case, ids = state["case"], state["ids"]
+    x, a, b = (state[f].detach().double() for f in ("x", "a", "b"))
+    y = torch.zeros(case["tokens"], case["d_out"], dtype=torch.float64, device=x.device)
+    for f, term in (("weight", lambda w: x @ w), ("base", lambda v: v)):
+        if state[f] is not None:
+            y += term(state[f].double())
+    train = case["train"]
+    if train:
+        g = state["grad"].double()
+        dx = torch.zeros_like(x) if state["weight"] is None else g @ state["weight"].double().t()
+        da, db = torch.zeros_like(a), torch.zeros_like(b)
+    for i in torch.unique(ids).tolist():
+        if not 0 <= i < case["adapters"]:
+            continue
+        at = torch.nonzero(ids == i).view(-1)
+        inner = x[at] @ a[i]
+        y[at] += _SCALE * (inner @ b[i])
+        if train:
+            back = g[at] @ b[i].t()
+            dx[at] += _SCALE * (back @ a[i].t())
+            da[i] = _SCALE * (x[at].t() @ back)
+            db[i] = _SCALE * (inner.t() @ g[at])
+    return {"y": y, "grad_x": dx, "grad_a": da, "grad_b": db} if train else {"y": y}
+
+
+def _exact_balance(state):
+    case = state["case"]
+    S, E = case["sequences"], case["experts"]
+    l = state["logits"].detach().double().requires_grad_()
+    live = [torch.arange(case["tokens"], device=l.device) if state["mask"] is None
+            else torch.nonzero(state["mask"][i]).view(-1) for i in range(S)]
+    lse = torch.logsumexp(l, dim=-1)
+    if case["scores"] == "softmax":
+        p = torch.exp(l - lse.unsqueeze(-1))
+    else:
+        s = 1 / (1 + torch.exp(-l))
+        p = s / s.sum(-1, keepdim=True)
+    groups = [[i] for i in range(S)] if case["per_sequence"] else [list(range(S))]
+    counts, loss = torch.zeros(E, dtype=torch.int64, device=l.device), 0.0
+    for group in groups:
+        P = torch.cat([p[i, live[i]] for i in group]).mean(0)
+        chosen = torch.cat([state["sel"][i, live[i]].reshape(-1) for i in group])
+        c = torch.bincount(chosen, minlength=E)
+        counts += c
+        loss = loss + ((E * c.double() / chosen.numel() * P).sum() if case["what"] == "load"
+                       else (P * torch.log(P)).sum()) / len(groups)
+    z = torch.cat([lse[i, live[i]] for i in range(S)]).square().mean()
+    grad, = torch.autograd.grad(loss + _Z * z, [l])
+    return {"loss": loss.detach(), "z": z.detach(), "counts": counts, "grad_logits": grad}
