@@ -14,9 +14,10 @@ Two kinds of case:
   (or its sigmoids over their sum), P_e the mean of p_e over the tokens of a
   group (a sequence, or all tokens) and c_e the routes to expert e:
   "load": sum_e E c_e / (k n) P_e; "entropy": sum_e P_e log P_e; each averaged
-  over the groups.  Beside it z = the mean of logsumexp(l)^2, and the counts of
-  all routes per expert.  Padded tokens (mask) count nowhere.  Always with the
-  logits' gradient of loss + 0.01 z.
+  over the groups.  The loss adds a little of z = the mean of logsumexp(l)^2 to
+  that; both terms and the counts of all routes per expert are returned beside
+  it.  Padded tokens (mask) count nowhere.  Always with the logits' gradient (in
+  float16 of the loss scaled up, as training in that type scales it).
 """
 import math
 
@@ -26,7 +27,7 @@ own = False
 
 _TYPES = {"float32": torch.float32, "bfloat16": torch.bfloat16, "float16": torch.float16}
 _SCALE = 2.0
-_Z = 0.01
+_WEIGHT, _Z = 0.5, 0.01
 
 
 def _lora(name, tokens, d_in, d_out, rank, adapters, rows, dtype, train=False):
@@ -151,6 +152,7 @@ def prepare(case, seed):
     logits = 1.5 * _randn(g, S, T, E) + 0.5 * _randn(g, E)
     state["sel"] = (logits + 0.2 * _randn(g, E)).topk(k, dim=-1).indices.contiguous()
     state["logits"] = logits.to(dtype).requires_grad_()
+    state["grad"] = torch.tensor(32768.0 if dtype == torch.float16 else 1.0, device="cuda")
     state["mask"] = None
     if case["masked"]:  # sequences padded to the longest
         lengths = (T * (0.5 + 0.5 * _rand(g, S, 1))).long().clamp_(min=1)
@@ -240,19 +242,20 @@ def _plain_balance(state):
         d = p * (coef - inner)
     else:
         d = s * torch.sigmoid(-l) * (coef - inner) / total
-    d = (d + _Z * 2 * lse * soft / all_n) * live
-    return {"loss": loss, "z": z, "counts": counts, "grad_logits": d.to(_TYPES[case["dtype"]])}
+    d = (_WEIGHT * d + _Z * 2 * lse * soft / all_n) * live * state["grad"]
+    return {"loss": _WEIGHT * loss + _Z * z, "terms": torch.stack([loss, z]), "counts": counts,
+            "grad_logits": d.to(_TYPES[case["dtype"]])}
 
 
 def _own(state):
     import cvmm_codex_amd as cvmm
     case = state["case"]
     if case["kind"] == "balance":
-        loss, z, counts = cvmm.cvmm_balance_loss(state["logits"], state["sel"], kind=case["what"],
-                                                 scores=case["scores"], mask=state["mask"],
-                                                 per_sequence=case["per_sequence"])
-        grad, = torch.autograd.grad(loss + _Z * z, [state["logits"]])
-        return {"loss": loss.detach(), "z": z.detach(), "counts": counts, "grad_logits": grad}
+        loss, terms, counts = cvmm.cvmm_balance_loss(
+            state["logits"], state["sel"], kind=case["what"], scores=case["scores"], mask=state["mask"],
+            per_sequence=case["per_sequence"], weight=_WEIGHT, z_weight=_Z)
+        grad, = torch.autograd.grad(loss, [state["logits"]], state["grad"])
+        return {"loss": loss.detach(), "terms": terms, "counts": counts, "grad_logits": grad}
     adapters = state["ids"]
     if case["rows"] == "routes":  # the selection of the projection beside them
         adapters = cvmm.cvmm_prepare_sel2(adapters, route_input=True)
@@ -348,5 +351,6 @@ def _exact_balance(state):
         loss = loss + ((E * c.double() / chosen.numel() * P).sum() if case["what"] == "load"
                        else (P * torch.log(P)).sum()) / len(groups)
     z = torch.cat([lse[i, live[i]] for i in range(S)]).square().mean()
-    grad, = torch.autograd.grad(loss + _Z * z, [l])
-    return {"loss": loss.detach(), "z": z.detach(), "counts": counts, "grad_logits": grad}
+    total = _WEIGHT * loss + _Z * z
+    grad, = torch.autograd.grad(total, [l], state["grad"].double())
+    return {"loss": total.detach(), "terms": torch.stack([loss, z]).detach(), "counts": counts, "grad_logits": grad}
