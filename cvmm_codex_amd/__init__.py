@@ -9,9 +9,11 @@ from .api import (  # noqa: F401
     CVMMSel,
     create_kernels,
     cvmm,
+    cvmm_balance_loss,
     cvmm_expert_offsets,
     cvmm_gate_logits,
     cvmm_gelu,
+    cvmm_lora,
     cvmm_mx4,
     cvmm_mx4_quantize,
     cvmm_prepare_sel,

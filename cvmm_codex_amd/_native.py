@@ -25,6 +25,7 @@ FLAG_ROWS_SCALED = 64
 # the weight gradient on a second stream, concurrent with the grad-input
 HOST_OVERLAP_BACKWARD = 1 << 48
 SCORES = {"softmax": 0, "sigmoid": 1}
+BALANCE_KINDS = {"load": 0, "entropy": 1}
 CAST_T_INTERLEAVED = 1
 CAST_N_INTERLEAVED = 2
 TUNE_PANEL_TILES_PER_WG = 1
@@ -137,6 +138,29 @@ _SIGS = {
         _P, _I32, _I64, _I32,                 # rw, rw dtype, top_k, op
         _P, _I32, _I64, _I64, _I64,           # grad_keys, dtype, strides
         _I32, _P, _SZ, _P, _SZ, _P]),         # flags, rows, workspace, stream
+    "cvmm_balance_loss_workspace_bytes": (_SZ, [_I64, _I64, _I32]),
+    "cvmm_balance_loss": (ctypes.c_int, [
+        _P, _I32, _I64, _I64, _I32,           # logits, dtype, tokens, ld, experts
+        _P, _I32, _I64, _P, _I64,             # sel, int64, top_k, mask, group tokens
+        _I32, _I32, ctypes.c_double, ctypes.c_double,  # kind, scores, weight, z_weight
+        _P, _P, _P, _P, _P, _SZ, _P]),        # loss, terms, counts, coef, ws, ws bytes, stream
+    "cvmm_balance_loss_backward": (ctypes.c_int, [_P, _I32, _I64, _I64, _I32, _P, _I64, _I32, _P, _P, _P, _I64, _P]),
+    "cvmm_lora_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I32]),
+    "cvmm_lora": (ctypes.c_int, [
+        _P, _I32, _I64, _I64,                 # x, op dtype, rows, ld
+        _P, _I64, _I64,                       # weight, strides
+        _P, _I64, _I64, _I64,                 # a, strides
+        _P, _I64, _I64, _I64,                 # b, strides
+        _I32, _I64, _I64, _I64,               # adapters, d_in, d_out, rank
+        _P, _I32, _P, _P, ctypes.c_float,     # ids, int64, order, scales, scale
+        _P, _I32, _I64, _P, _I64,             # base, dtype, ld, out, ld
+        _P, _I64, _P, _SZ, _P]),              # inner_t, ld, ws, ws bytes, stream
+    "cvmm_lora_bwd_adapters_workspace_bytes": (_SZ, [_I64, _I32, _I64, _I64, _I64]),
+    "cvmm_lora_bwd_adapters": (ctypes.c_int, [
+        _P, _I32, _I64, _I64, _P, _I64,       # x, op dtype, rows, ld, grad, ld
+        _P, _P, _I64,                         # inner_t, inner_grad_t, ld
+        _I32, _I64, _I64, _I64, _P, _P,       # adapters, d_in, d_out, rank, order, offsets
+        _P, _P, _I32, _P, _SZ, _P]),          # grad_a, grad_b, dtype, ws, ws bytes, stream
     "cvmm_mx4_rows_bytes": (_SZ, [_I64, _I64, _I32]),
     "cvmm_mx4_keys_bytes": (_SZ, [_I64, _I64, _I64, _I32]),
     "cvmm_mx4_quantize_rows": (ctypes.c_int, [_P, _I32, _I64, _I64, _I64, _P, _P, _P]),

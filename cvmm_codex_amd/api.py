@@ -719,6 +719,63 @@ def cvmm_route_scored(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor]
     return w, sel, CVMMSel._deferred(sel, routing, False, None)
 
 
+def cvmm_balance_loss(logits: torch.Tensor, sel: Union[torch.Tensor, CVMMSel], kind: str = "load",
+                      scores: str = "softmax", mask: Optional[torch.Tensor] = None, per_sequence: bool = False,
+                      weight: float = 1.0, z_weight: float = 0.0):
+    """What keeps a router's experts evenly loaded, with the experts' counts, in
+    one native call beside ``cvmm_route_topk`` / ``cvmm_route_scored``:
+
+        p = softmax(logits, -1)   or   sigmoid(logits) / sigmoid(logits).sum(-1).clamp_min(1e-20)
+        P = p.mean(tokens);  c = the routes to each expert;  n tokens, k routes each
+        balance = (E * c / (k * n) * P).sum()      # "load": 1 where the loads are even
+        balance = (P * log P).sum()                # "entropy"
+        z = (logsumexp(logits, -1) ** 2).mean(tokens)
+        loss = weight * balance + z_weight * z
+
+    ``logits`` ``[..., tokens, E]``, ``sel`` the chosen ids ``[..., tokens, k]`` (or
+    the router's selection of that shape); ids outside ``[0, E)`` are not counted.
+    ``mask`` ``[..., tokens]``, bool: tokens where it is False (padding) count
+    nowhere, whatever their logits hold.  ``per_sequence``: balance is taken over the
+    tokens of each sequence by itself and averaged over the sequences that have any
+    (at most 1024 sequences); z and the counts are over all tokens.
+
+    Returns ``(loss, terms, counts)``: the fp32 loss (gradient flows to ``logits``
+    through P and z, the counts are constants), fp32 ``[balance, z]`` for logging and
+    the int64 routes per expert, from which a trainer moves a balance bias.  No live
+    token: zeros.  The gradient is 0 at masked tokens and at experts of probability
+    0; a row of logits that are all -inf must be masked (its softmax is NaN).  At most
+    1024 experts; sums in fp32, over the tokens' chunks in fp64, in a fixed order."""
+    _require_device(logits, "logits")
+    if kind not in N.BALANCE_KINDS:
+        raise ValueError(f"cvmm_balance_loss: kind must be 'load' or 'entropy', not {kind!r}")
+    if scores not in N.SCORES:
+        raise ValueError(f"cvmm_balance_loss: scores must be 'softmax' or 'sigmoid', not {scores!r}")
+    if isinstance(sel, CVMMSel):
+        sel = sel._raw_shape_tensor()
+    _require_device(sel, "sel")
+    if sel.is_floating_point() or sel.is_complex() or sel.dtype == torch.bool:
+        raise TypeError(f"cvmm_balance_loss: sel must hold ids, not {sel.dtype}")
+    if not logits.is_floating_point():
+        raise TypeError(f"cvmm_balance_loss: logits must be of a floating type, not {logits.dtype}")
+    if logits.dim() < 2 or logits.shape[-1] == 0:
+        raise ValueError(f"cvmm_balance_loss: logits {tuple(logits.shape)} are not [..., tokens, experts]")
+    if sel.dim() != logits.dim() or sel.shape[:-1] != logits.shape[:-1] or sel.shape[-1] == 0:
+        raise ValueError(f"cvmm_balance_loss: sel {tuple(sel.shape)} does not hold k ids per token of logits "
+                         f"{tuple(logits.shape)}")
+    if mask is not None:
+        _require_device(mask, "mask")
+        if mask.dtype != torch.bool or mask.shape != logits.shape[:-1]:
+            raise ValueError(f"cvmm_balance_loss: mask must be bool of shape {tuple(logits.shape[:-1])}")
+    if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        logits = logits.float()
+    T = logits.numel() // logits.shape[-1]
+    group = max(logits.shape[-2] if per_sequence else T, 1)
+    args = (logits, sel, mask, group, N.BALANCE_KINDS[kind], N.SCORES[scores], float(weight), float(z_weight))
+    if _compiling():
+        return _ops.balance_loss(*args)[:3]
+    return tuple(N.host().balance_loss_apply(*args, _differentiated(logits)))
+
+
 def _gate_grad_chunks(n_tokens: int, d_in: int, n_experts: int) -> int:
     """Token chunks of the gate gradient's product: enough [E x D] output
     tiles to fill the GPU (a single [D x T] @ [T x E] product has D*E/8192
@@ -1202,3 +1259,94 @@ def cvmm_mx4(x: torch.Tensor, sel: Union[torch.Tensor, CVMMSel], keys: CVMMMx4,
     pos = _route_pos(out_index if out_index is not None else sel_index, s.numel())
     return N.host().mx4_apply(x, rw, keys.codes, keys.scales, d_in, d_out, sel_index, out_index, offsets, pos, top_k,
                               _DTYPE_IDS[op], quantize_input, grad, shape)
+
+
+# ----------------------------------------------------------------------------
+# low-rank adapters
+# ----------------------------------------------------------------------------
+
+def cvmm_lora(x: torch.Tensor, adapters: Union[torch.Tensor, CVMMSel], a: torch.Tensor, b: torch.Tensor,
+              weight: Optional[torch.Tensor] = None, base: Optional[torch.Tensor] = None,
+              scale: Union[float, torch.Tensor] = 1.0) -> torch.Tensor:
+    """Low-rank adapters of many requests beside a projection that they share:
+
+        y[t] = base[t] + x[t] @ weight + scale * (x[t] @ a[i]) @ b[i],   i = adapters[t]
+
+    ``x`` ``[..., d_in]``; ``adapters`` one id per row (``x.shape[:-1]``, any integer
+    type), a row with an id outside ``[0, n)`` has no adapter; ``a`` ``[n, d_in,
+    rank]``, ``b`` ``[n, rank, d_out]``, rank at most 256; ``weight`` ``[d_in,
+    d_out]`` (a ``torch.nn.Linear``'s as ``.weight.t()``), frozen; ``base`` of the
+    output's shape, such as what ``cvmm_mx4`` gave for the same rows (adapters beside
+    frozen 4-bit experts); ``scale`` a number or one value per adapter (a constant:
+    no gradient).  Without ``weight`` and ``base`` the adapters' product alone.
+
+    ``adapters`` may be a selection with one route per row of x
+    (``cvmm_prepare_sel2(ids, route_input=True)``): the sort is then shared with the
+    projections that use it; plain ids are sorted where the adapters' gradients are
+    asked for.  Rows of one adapter that stand together are fastest.
+
+    The op type is the autocast dtype, or ``x``'s where autocast is off; operands are
+    rounded to it (base: taken in it or in fp32), ``scale * x @ a[i]`` is rounded
+    to it once, all sums are fp32 and the output is rounded once.  In fp16 those
+    inner values must stay below 65520.  An adapter's infinities and NaN reach its
+    own rows only.  Gradients flow to x, a, b and base; the adapters' are summed in a
+    fixed order."""
+    _require_device(x, "x")
+    op = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
+    if op not in _DTYPE_IDS:
+        raise TypeError(f"cvmm_lora: the op type must be float32, bfloat16 or float16, not {op} (autocast, or x's type)")
+    for t, what in ((x, "x"), (a, "a"), (b, "b"), (weight, "weight"), (base, "base")):
+        if t is not None and not t.is_floating_point():
+            raise TypeError(f"cvmm_lora: {what} must be of a floating type, not {t.dtype}")
+    if x.dim() < 1 or a.dim() != 3 or b.dim() != 3 or a.shape[1] != x.shape[-1] or a.shape[0] != b.shape[0] \
+            or a.shape[2] != b.shape[1] or a.numel() == 0 or b.numel() == 0:
+        raise ValueError(f"cvmm_lora: x {tuple(x.shape)}, a {tuple(a.shape)} and b {tuple(b.shape)} are not "
+                         "[..., d_in], [n, d_in, rank] and [n, rank, d_out]")
+    n, d_in, rank = a.shape
+    d_out = b.shape[2]
+    if rank > 256:
+        raise ValueError(f"cvmm_lora: rank {rank} above 256")
+    if weight is not None:
+        if weight.shape != (d_in, d_out):
+            raise ValueError(f"cvmm_lora: weight {tuple(weight.shape)} is not [{d_in}, {d_out}]")
+        if weight.requires_grad and torch.is_grad_enabled():
+            raise ValueError("cvmm_lora: the shared weight is frozen (pass weight.detach())")
+    if base is not None and base.shape != (*x.shape[:-1], d_out):
+        raise ValueError(f"cvmm_lora: base {tuple(base.shape)} has not the output's shape {(*x.shape[:-1], d_out)}")
+    scales, factor = None, 1.0
+    if isinstance(scale, torch.Tensor):
+        if scale.requires_grad and torch.is_grad_enabled():
+            raise ValueError("cvmm_lora: scale has no gradient (pass scale.detach())")
+        if scale.shape != (n,):
+            raise ValueError(f"cvmm_lora: scale {tuple(scale.shape)} is not one value per adapter ({n})")
+        _require_device(scale, "scale")
+        scales = scale
+    else:
+        factor = float(scale)
+    grad = _differentiated(x, a, b, base)
+    order = offsets = None
+    if isinstance(adapters, CVMMSel):
+        if adapters.reduction_weight is not None:
+            raise ValueError("cvmm_lora: a selection with routing weights has no sum here")
+        ids = adapters._raw_shape_tensor()
+        _require_device(ids, "adapters")
+        if ids.numel() != x.numel() // d_in:
+            raise ValueError(f"cvmm_lora: the selection's {ids.numel()} routes are not the {x.numel() // d_in} rows of x")
+        if ids.numel() > 0:
+            adapters._resolve(n)
+            order = adapters._out_index if adapters._out_index is not None else adapters._sel_index
+            offsets = _offsets_for(adapters._sel, n)
+    else:
+        ids = adapters
+        _require_device(ids, "adapters")
+        if ids.shape != x.shape[:-1]:
+            raise ValueError(f"cvmm_lora: adapters {tuple(ids.shape)} are not one id per row of x {tuple(x.shape)}")
+    if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
+        raise TypeError(f"cvmm_lora: adapters must hold ids, not {ids.dtype}")
+    if (a.requires_grad or b.requires_grad) and grad and n > 32767:
+        raise ValueError(f"cvmm_lora: gradients of at most 32767 adapters, not {n}")
+    if _compiling():
+        if grad and order is None and ids.numel() > 0:
+            _, order, _, offsets, _ = _ops.sort_routes(ids, n, 1)
+        return _ops.lora(x, a, b, base, ids, weight, scales, factor, order, offsets, op)[0]
+    return N.host().lora_apply(x, ids, a, b, weight, base, scales, factor, order, offsets, _DTYPE_IDS[op], grad)

@@ -345,3 +345,107 @@ def _mx4_backward(ctx, grad):
 
 
 mx4_product.register_autograd(_mx4_backward, setup_context=_mx4_setup)
+
+
+# ---------------------------------------------------------------------------
+# balance loss (api.cvmm_balance_loss): loss, terms, counts, and the
+# coefficients its backward reads
+# ---------------------------------------------------------------------------
+@torch.library.custom_op(f"{NS}::balance_loss", mutates_args=())
+def balance_loss(logits: torch.Tensor, sel: torch.Tensor, mask: Optional[torch.Tensor], group_tokens: int, kind: int,
+                 scores: int, weight: float, z_weight: float) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor,
+                                                                       torch.Tensor]:
+    return tuple(N.host().balance_loss(logits, sel, mask, group_tokens, kind, scores, weight, z_weight))
+
+
+@balance_loss.register_fake
+def _(logits, sel, mask, group_tokens, kind, scores, weight, z_weight):
+    E = logits.shape[-1]
+    pairs = logits.numel() // E // group_tokens * E
+    f = lambda *shape: logits.new_empty(shape, dtype=torch.float32)
+    return f(), f(2), logits.new_empty((E,), dtype=torch.int64), f(pairs + 4)
+
+
+@torch.library.custom_op(f"{NS}::balance_loss_backward", mutates_args=())
+def balance_loss_backward(logits: torch.Tensor, mask: Optional[torch.Tensor], coef: torch.Tensor, grad: torch.Tensor,
+                          group_tokens: int, scores: int) -> torch.Tensor:
+    return N.host().balance_loss_backward(logits, mask, coef, grad, group_tokens, scores)
+
+
+@balance_loss_backward.register_fake
+def _(logits, mask, coef, grad, group_tokens, scores):
+    return torch.empty_like(logits, memory_format=torch.contiguous_format)
+
+
+def _balance_setup(ctx, inputs, output):
+    logits, _, mask, group_tokens, _, scores, _, _ = inputs
+    ctx.save_for_backward(logits, mask, output[3])
+    ctx.args = (group_tokens, scores)
+
+
+def _balance_backward(ctx, grad, *_):
+    if grad is None:
+        return (None,) * 8
+    return (balance_loss_backward(*ctx.saved_tensors, grad, *ctx.args),) + (None,) * 7
+
+
+balance_loss.register_autograd(_balance_backward, setup_context=_balance_setup)
+
+
+# ---------------------------------------------------------------------------
+# low-rank adapters (api.cvmm_lora): the output, and the inner rows that the
+# adapters' gradients read (made where a sorted order is given)
+# ---------------------------------------------------------------------------
+@torch.library.custom_op(f"{NS}::lora", mutates_args=())
+def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, base: Optional[torch.Tensor], ids: torch.Tensor,
+         weight: Optional[torch.Tensor], scales: Optional[torch.Tensor], scale: float,
+         order: Optional[torch.Tensor], offsets: Optional[torch.Tensor],
+         op_dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
+    out, inner = N.host().lora_forward(x, ids, a, b, weight, base, scales, scale, order, order is not None,
+                                       N.dtype_id(op_dtype))
+    return out.view(*x.shape[:-1], b.shape[2]), inner if inner is not None else _empty(x)
+
+
+@lora.register_fake
+def _(x, a, b, base, ids, weight, scales, scale, order, offsets, op_dtype):
+    rows = ids.numel()
+    inner = (x.new_empty((a.shape[2], (rows + 7) // 8 * 8), dtype=op_dtype) if order is not None else _empty(x))
+    return x.new_empty((*x.shape[:-1], b.shape[2]), dtype=op_dtype), inner
+
+
+@torch.library.custom_op(f"{NS}::lora_backward", mutates_args=())
+def lora_backward(grad: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor,
+                  weight: Optional[torch.Tensor], scales: Optional[torch.Tensor], scale: float,
+                  order: Optional[torch.Tensor], offsets: Optional[torch.Tensor], inner: torch.Tensor,
+                  op_dtype: torch.dtype, need_x: bool, need_a: bool,
+                  need_b: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    g = N.host().lora_backward(grad, x, ids, a, b, weight, scales, scale, order, offsets, inner, N.dtype_id(op_dtype),
+                               need_x, need_a, need_b)
+    return tuple(t if t is not None else _empty(like) for t, like in zip(g, (x, a, b)))
+
+
+@lora_backward.register_fake
+def _(grad, x, a, b, ids, weight, scales, scale, order, offsets, inner, op_dtype, need_x, need_a, need_b):
+    return tuple(torch.empty_like(t, memory_format=torch.contiguous_format) if need else _empty(t)
+                 for t, need in zip((x, a, b), (need_x, need_a, need_b)))
+
+
+def _lora_setup(ctx, inputs, output):
+    x, a, b, base, ids, weight, scales, scale, order, offsets, op_dtype = inputs
+    ctx.save_for_backward(x, a, b, ids, weight, scales, order, offsets, output[1])
+    ctx.args = (scale, op_dtype, base.dtype if base is not None else None)
+
+
+def _lora_backward(ctx, grad, _):
+    x, a, b, ids, weight, scales, order, offsets, inner = ctx.saved_tensors
+    scale, op_dtype, base_dtype = ctx.args
+    need = [bool(n) for n in ctx.needs_input_grad[:3]]
+    g = [None] * 3
+    if any(need):
+        g = [t if n else None for t, n in zip(lora_backward(grad, x, a, b, ids, weight, scales, scale, order, offsets,
+                                                            inner, op_dtype, *need), need)]
+    gb = grad.to(base_dtype) if base_dtype is not None and ctx.needs_input_grad[3] else None
+    return (*g, gb) + (None,) * 7
+
+
+lora.register_autograd(_lora_backward, setup_context=_lora_setup)

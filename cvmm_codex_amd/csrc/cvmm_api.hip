@@ -10,6 +10,7 @@
 
 #include "cvmm_common.h"
 #include "cvmm_internal.h"
+#include "cvmm_lora.h"
 #include "cvmm_mx4.h"
 #include "../../include/cvmm_hip.h"
 
@@ -770,6 +771,140 @@ int cvmm_route_scored_backward(const void* logits, int32_t logits_dtype, int64_t
                                                                           top_k, scores, renormalize, scale, sel,
                                                                           grad_weights, grad_logits, grad_ld, s); }),
                       "cvmm_route_scored_backward");
+}
+
+// ---------------------------------------------------------------------------
+static int balance_args_ok(const char* what, int32_t logits_dtype, int64_t n_tokens, int64_t logits_ld,
+                           int32_t n_experts, int64_t group_tokens, int32_t scores) {
+  if (!valid_dtype(logits_dtype)) return fail(CVMM_ERR_INVALID, "%s: invalid logits dtype", what);
+  if (n_tokens < 0 || n_experts <= 0 || logits_ld < n_experts || group_tokens <= 0 || n_tokens % group_tokens != 0)
+    return fail(CVMM_ERR_INVALID, "%s: bad sizes (T=%lld in groups of %lld, E=%d, ld=%lld)", what,
+                (long long)n_tokens, (long long)group_tokens, n_experts, (long long)logits_ld);
+  if (scores != CVMM_SCORES_SOFTMAX && scores != CVMM_SCORES_SIGMOID)
+    return fail(CVMM_ERR_INVALID, "%s: unknown scores %d", what, scores);
+  if (n_experts > kRouteMaxExperts) return fail(CVMM_ERR_UNSUPPORTED, "%s: at most %d experts", what, kRouteMaxExperts);
+  if (n_tokens / group_tokens > kBalanceMaxGroups)
+    return fail(CVMM_ERR_UNSUPPORTED, "%s: at most %d groups of tokens", what, kBalanceMaxGroups);
+  return CVMM_OK;
+}
+
+size_t cvmm_balance_loss_workspace_bytes(int64_t n_tokens, int64_t group_tokens, int32_t n_experts) {
+  if (n_tokens < 0 || group_tokens <= 0 || n_experts <= 0 || n_experts > kRouteMaxExperts) return 0;
+  return balance_workspace_bytes(n_tokens, group_tokens, n_experts);
+}
+
+int cvmm_balance_loss(const void* logits, int32_t logits_dtype, int64_t n_tokens, int64_t logits_ld,
+                      int32_t n_experts, const void* sel, int32_t sel_is_int64, int64_t top_k, const uint8_t* mask,
+                      int64_t group_tokens, int32_t kind, int32_t scores, double weight, double z_weight,
+                      float* loss, float* terms, int64_t* counts, float* coef, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+  const char* what = "cvmm_balance_loss";
+  int r = balance_args_ok(what, logits_dtype, n_tokens, logits_ld, n_experts, group_tokens, scores);
+  if (r) return r;
+  if (kind != CVMM_BALANCE_LOAD && kind != CVMM_BALANCE_ENTROPY)
+    return fail(CVMM_ERR_INVALID, "%s: unknown kind %d", what, kind);
+  if (top_k <= 0) return fail(CVMM_ERR_INVALID, "%s: top_k <= 0", what);
+  if (n_tokens > (int64_t)0x7fffffff / top_k) return fail(CVMM_ERR_UNSUPPORTED, "%s: too many routes", what);
+  const size_t need = balance_workspace_bytes(n_tokens, group_tokens, n_experts);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(CVMM_ERR_WORKSPACE, "%s: workspace too small (%zu < %zu)", what, workspace_bytes, need);
+  if (!loss || !terms || !counts || !coef || (n_tokens > 0 && (!logits || !sel)))
+    return fail(CVMM_ERR_INVALID, "%s: NULL pointer", what);
+  hipStream_t s = (hipStream_t)stream;
+  return check_launch(timed(CVMM_KC_ROUTE, s, [&] {
+    return launch_balance_loss(logits, logits_dtype, n_tokens, logits_ld, n_experts, sel, sel_is_int64, top_k, mask,
+                               group_tokens, kind == CVMM_BALANCE_ENTROPY, scores == CVMM_SCORES_SIGMOID, weight,
+                               z_weight, loss, terms, counts, coef, workspace, s);
+  }), what);
+}
+
+int cvmm_balance_loss_backward(const void* logits, int32_t logits_dtype, int64_t n_tokens, int64_t logits_ld,
+                               int32_t n_experts, const uint8_t* mask, int64_t group_tokens, int32_t scores,
+                               const float* coef, const float* grad_loss, void* grad_logits, int64_t grad_ld,
+                               void* stream) {
+  const char* what = "cvmm_balance_loss_backward";
+  int r = balance_args_ok(what, logits_dtype, n_tokens, logits_ld, n_experts, group_tokens, scores);
+  if (r) return r;
+  if (grad_ld < n_experts) return fail(CVMM_ERR_INVALID, "%s: grad row stride too small", what);
+  if (n_tokens == 0) return CVMM_OK;
+  if (n_tokens > 0x7fffffffll) return fail(CVMM_ERR_UNSUPPORTED, "%s: too many tokens", what);
+  if (!logits || !coef || !grad_loss || !grad_logits) return fail(CVMM_ERR_INVALID, "%s: NULL pointer", what);
+  hipStream_t s = (hipStream_t)stream;
+  return check_launch(timed(CVMM_KC_ROUTE, s, [&] {
+    return launch_balance_loss_backward(logits, logits_dtype, n_tokens, logits_ld, n_experts, mask, group_tokens,
+                                        scores == CVMM_SCORES_SIGMOID, coef, grad_loss, grad_logits, grad_ld, s);
+  }), what);
+}
+
+// ---------------------------------------------------------------------------
+static int lora_args_ok(const char* what, int32_t op_dtype, int64_t rows, int64_t x_ld, int32_t n_adapters,
+                        int64_t K, int64_t N, int64_t rank) {
+  if (!valid_dtype(op_dtype)) return fail(CVMM_ERR_INVALID, "%s: invalid op dtype", what);
+  if (rows < 0 || n_adapters <= 0 || K <= 0 || N <= 0 || rank <= 0 || x_ld < K)
+    return fail(CVMM_ERR_INVALID, "%s: bad sizes (rows=%lld, adapters=%d, %lld -> %lld, rank %lld, ld=%lld)", what,
+                (long long)rows, n_adapters, (long long)K, (long long)N, (long long)rank, (long long)x_ld);
+  if (rank > kLoraMaxRank) return fail(CVMM_ERR_UNSUPPORTED, "%s: rank above %lld", what, (long long)kLoraMaxRank);
+  if (rows > 0x7fffffffll || K > 0x7fffffffll || N > 0x7fffffffll)
+    return fail(CVMM_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 rows or columns", what);
+  return CVMM_OK;
+}
+
+size_t cvmm_lora_workspace_bytes(int64_t rows, int64_t d_in, int64_t d_out, int64_t rank, int32_t op_dtype) {
+  if (rows <= 0 || d_in <= 0 || d_out <= 0 || rank <= 0 || rank > kLoraMaxRank || !valid_dtype(op_dtype)) return 0;
+  return align_up((size_t)rows * (size_t)((rank + 31) / 32 * 32) * dtype_size(op_dtype), 256);
+}
+
+int cvmm_lora(const void* x, int32_t op_dtype, int64_t rows, int64_t x_ld, const void* weight, int64_t w_si,
+              int64_t w_so, const void* a, int64_t a_se, int64_t a_si, int64_t a_sr, const void* b, int64_t b_se,
+              int64_t b_sr, int64_t b_so, int32_t n_adapters, int64_t d_in, int64_t d_out, int64_t rank,
+              const void* ids, int32_t ids_is_int64, const int64_t* order, const float* scales, float scale,
+              const void* base, int32_t base_dtype, int64_t base_ld, void* out, int64_t out_ld, void* inner_t,
+              int64_t inner_ld, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "cvmm_lora";
+  int r = lora_args_ok(what, op_dtype, rows, x_ld, n_adapters, d_in, d_out, rank);
+  if (r) return r;
+  if (out && out_ld < d_out) return fail(CVMM_ERR_INVALID, "%s: output row stride too small", what);
+  if (base && (base_ld < d_out || (base_dtype != op_dtype && base_dtype != kF32)))
+    return fail(CVMM_ERR_INVALID, "%s: base must be rows of the op type or fp32", what);
+  if (inner_t && inner_ld < rows) return fail(CVMM_ERR_INVALID, "%s: inner row stride too small", what);
+  const size_t need = cvmm_lora_workspace_bytes(rows, d_in, d_out, rank, op_dtype);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(CVMM_ERR_WORKSPACE, "%s: workspace too small (%zu < %zu)", what, workspace_bytes, need);
+  if (rows == 0) return CVMM_OK;
+  if (!x || !a || !b || !ids || (!out && !inner_t)) return fail(CVMM_ERR_INVALID, "%s: NULL pointer", what);
+  const LoraParams p{x, rows, x_ld, weight, w_si, w_so, a, a_se, a_si, a_sr, b, b_se, b_sr, b_so, n_adapters,
+                     d_in, d_out, rank, ids, ids_is_int64, order, scales, scale, base, base_dtype, base_ld,
+                     out, out_ld, workspace, (rank + 31) / 32 * 32, inner_t, inner_ld};
+  hipStream_t s = (hipStream_t)stream;
+  return check_launch(timed(CVMM_KC_LORA, s, [&] { return launch_lora(p, op_dtype, s); }), what);
+}
+
+size_t cvmm_lora_bwd_adapters_workspace_bytes(int64_t rows, int32_t n_adapters, int64_t d_in, int64_t d_out,
+                                              int64_t rank) {
+  if (rows < 0 || n_adapters <= 0 || d_in <= 0 || d_out <= 0 || rank <= 0 || rank > kLoraMaxRank) return 0;
+  return lora_wgrad_workspace_bytes(rows, n_adapters, d_in, d_out, rank);
+}
+
+int cvmm_lora_bwd_adapters(const void* x, int32_t op_dtype, int64_t rows, int64_t x_ld, const void* grad,
+                           int64_t grad_ld, const void* inner_t, const void* inner_grad_t, int64_t inner_ld,
+                           int32_t n_adapters, int64_t d_in, int64_t d_out, int64_t rank, const int64_t* order,
+                           const int64_t* offsets, void* grad_a, void* grad_b, int32_t grad_dtype, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  const char* what = "cvmm_lora_bwd_adapters";
+  int r = lora_args_ok(what, op_dtype, rows, x_ld, n_adapters, d_in, d_out, rank);
+  if (r) return r;
+  if (grad_ld < d_out || inner_ld < rows) return fail(CVMM_ERR_INVALID, "%s: row stride too small", what);
+  if (!valid_dtype(grad_dtype)) return fail(CVMM_ERR_INVALID, "%s: invalid gradient dtype", what);
+  const size_t need = lora_wgrad_workspace_bytes(rows, n_adapters, d_in, d_out, rank);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(CVMM_ERR_WORKSPACE, "%s: workspace too small (%zu < %zu)", what, workspace_bytes, need);
+  if (!grad_a && !grad_b) return CVMM_OK;
+  if (!offsets || (rows > 0 && (!order || (grad_a && (!x || !inner_grad_t)) || (grad_b && (!grad || !inner_t)))))
+    return fail(CVMM_ERR_INVALID, "%s: NULL pointer", what);
+  LoraWgradParams p{x, x_ld, grad, grad_ld, inner_t, inner_grad_t, inner_ld, rows, n_adapters, d_in, d_out, rank,
+                    order, offsets, grad_a, grad_b, grad_dtype, (float*)workspace, 1};
+  hipStream_t s = (hipStream_t)stream;
+  return check_launch(timed(CVMM_KC_LORA, s, [&] { return launch_lora_wgrad(p, op_dtype, s); }), what);
 }
 
 // ---------------------------------------------------------------------------

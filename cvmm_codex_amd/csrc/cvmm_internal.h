@@ -299,6 +299,31 @@ hipError_t launch_route_scored_backward(const void* logits, int32_t logits_dtype
                                         hipStream_t stream);
 
 // ---------------------------------------------------------------------------
+// balance loss of a router (cvmm_balance.hip): coef holds groups * n_experts + 1
+// values for the backward pass
+// ---------------------------------------------------------------------------
+constexpr int32_t kBalanceMaxGroups = 1024;
+size_t balance_workspace_bytes(int64_t n_tokens, int64_t group_tokens, int32_t n_experts);
+hipError_t launch_balance_loss(const void* logits, int32_t dtype, int64_t n_tokens, int64_t ld, int32_t n_experts,
+                               const void* sel, int32_t sel_is_int64, int64_t top_k, const uint8_t* mask,
+                               int64_t group_tokens, int32_t entropy, int32_t sigmoid, double weight,
+                               double z_weight, float* loss, float* terms, int64_t* counts, float* coef,
+                               void* workspace, hipStream_t stream);
+hipError_t launch_balance_loss_backward(const void* logits, int32_t dtype, int64_t n_tokens, int64_t ld,
+                                        int32_t n_experts, const uint8_t* mask, int64_t group_tokens,
+                                        int32_t sigmoid, const float* coef, const float* grad_loss,
+                                        void* grad_logits, int64_t grad_ld, hipStream_t stream);
+
+// ---------------------------------------------------------------------------
+// low-rank adapters beside a shared projection (cvmm_lora.h)
+// ---------------------------------------------------------------------------
+struct LoraParams;
+struct LoraWgradParams;
+hipError_t launch_lora(const LoraParams& p, int32_t op_dtype, hipStream_t stream);
+size_t lora_wgrad_workspace_bytes(int64_t rows, int32_t n, int64_t d_in, int64_t d_out, int64_t rank);
+hipError_t launch_lora_wgrad(const LoraWgradParams& p, int32_t op_dtype, hipStream_t stream);
+
+// ---------------------------------------------------------------------------
 // microscaled 4-bit values (cvmm_mx4.h: format and layouts)
 // ---------------------------------------------------------------------------
 hipError_t launch_mx4_quantize_rows(const void* src, int32_t dtype, int64_t ld, int64_t rows, int64_t K, void* codes,

@@ -1,0 +1,335 @@
+// Low-rank adapters of many requests beside a shared projection, no counterpart
+// in cvmm.py.  Rows of any order; any types, strides and widths.
+//
+// Two launches: the inner rows h = s x A_i, then the projection with h B_i added
+// in its accumulators.  A tile holds rows of several adapters: it walks the
+// adapters that occur in it, by rising id, forms each one's product for the whole
+// tile and keeps it in that adapter's rows alone (selected, not multiplied by
+// zero: an infinity or a NaN of one request's adapter stays with its rows).
+// h is rounded to the op type, whose matrix instructions form h B_i: an error of
+// at most half a step of each of its values, beside the one of the output's own
+// rounding.  All sums are 32-bit.
+#include "cvmm_common.h"
+#include "cvmm_internal.h"
+#include "cvmm_lora.h"
+#include "cvmm_mfma.h"
+
+namespace cvmm {
+
+constexpr int kLoraTile = 64;
+
+// LDS slice of 64 rows by BK values of k, 16 bytes of padding a row.
+template <typename OpT>
+struct LoraSlice {
+  static constexpr int BK = 128 / sizeof(OpT);
+  static constexpr int LD = BK + 16 / sizeof(OpT);
+  static constexpr int PER = kLoraTile * BK / 256;  // values per thread
+};
+
+// A 64 x BK block src[r * sr + k * sk], zero from n_r and n_k on: consecutive
+// threads along the unit stride.
+template <typename OpT>
+__device__ __forceinline__ void lora_load(const OpT* __restrict__ src, int64_t sr, int64_t sk, int64_t n_r,
+                                          int64_t n_k, OpT (&v)[LoraSlice<OpT>::PER]) {
+  using S = LoraSlice<OpT>;
+  const bool along_k = sk == 1;
+#pragma unroll
+  for (int j = 0; j < S::PER; ++j) {
+    const int i = j * 256 + (int)threadIdx.x;
+    const int r = along_k ? i / S::BK : i % kLoraTile, k = along_k ? i % S::BK : i / kLoraTile;
+    v[j] = r < n_r && k < n_k ? src[r * sr + k * sk] : from_f32<OpT>(0.f);
+  }
+}
+template <typename OpT>
+__device__ __forceinline__ void lora_store(OpT* __restrict__ dst, bool along_k, const OpT (&v)[LoraSlice<OpT>::PER]) {
+  using S = LoraSlice<OpT>;
+#pragma unroll
+  for (int j = 0; j < S::PER; ++j) {
+    const int i = j * 256 + (int)threadIdx.x;
+    const int r = along_k ? i / S::BK : i % kLoraTile, k = along_k ? i % S::BK : i / kLoraTile;
+    dst[r * S::LD + k] = v[j];
+  }
+}
+// Rows gathered by an LDS table of row indices (or -1: zeros).
+template <typename OpT>
+__device__ __forceinline__ void lora_load_rows(const OpT* __restrict__ src, int64_t ld, const int64_t* rows,
+                                               int64_t n_k, OpT (&v)[LoraSlice<OpT>::PER]) {
+  using S = LoraSlice<OpT>;
+#pragma unroll
+  for (int j = 0; j < S::PER; ++j) {
+    const int i = j * 256 + (int)threadIdx.x, r = i / S::BK, k = i % S::BK;
+    const int64_t row = rows[r];
+    v[j] = row >= 0 && k < n_k ? src[row * ld + k] : from_f32<OpT>(0.f);
+  }
+}
+
+// acc[j] += 16 rows of this wave x 64 columns over one slice.
+template <typename OpT>
+__device__ __forceinline__ void lora_mfma(f32x4_t (&acc)[4], const OpT* as, const OpT* bs, int wave, int lane) {
+  using S = LoraSlice<OpT>;
+  constexpr int EPC = MfmaOp<OpT>::EPC;
+  const int r = lane & 15, q = lane >> 4;
+#pragma unroll
+  for (int st = 0; st < S::BK / MfmaOp<OpT>::KSTEP; ++st) {
+    const int k = st * MfmaOp<OpT>::KSTEP + q * EPC;
+    const uint4 a = *reinterpret_cast<const uint4*>(as + (wave * 16 + r) * S::LD + k);
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      MfmaOp<OpT>::step(acc[j], a, *reinterpret_cast<const uint4*>(bs + (j * 16 + r) * S::LD + k));
+  }
+}
+
+// The product of 64 rows (gathered by `rows`) with src[k * sk + c * sc], c < n_c,
+// over all K, into acc; every thread of the workgroup enters.
+template <typename OpT>
+__device__ __forceinline__ void lora_product(f32x4_t (&acc)[4], OpT* as, OpT* bs, const OpT* __restrict__ x,
+                                             int64_t x_ld, const int64_t* rows, const OpT* __restrict__ src,
+                                             int64_t sk, int64_t sc, int64_t n_c, int64_t K, int wave, int lane) {
+  using S = LoraSlice<OpT>;
+  OpT va[S::PER], vb[S::PER];
+  lora_load_rows(x, x_ld, rows, K, va);
+  lora_load(src, sc, sk, n_c, K, vb);
+  for (int64_t k0 = 0; k0 < K; k0 += S::BK) {
+    __syncthreads();  // the last slice's reads
+    lora_store(as, true, va);
+    lora_store(bs, sk == 1, vb);
+    __syncthreads();
+    if (k0 + S::BK < K) {
+      lora_load_rows(x + k0 + S::BK, x_ld, rows, K - k0 - S::BK, va);
+      lora_load(src + (k0 + S::BK) * sk, sc, sk, n_c, K - k0 - S::BK, vb);
+    }
+    lora_mfma(acc, as, bs, wave, lane);
+  }
+}
+
+// The ids of the tile's rows and the rows' indices; rows past the last: -1.
+__device__ __forceinline__ void lora_tile_rows(const LoraParams& p, int64_t m0, bool ordered, int32_t* ids,
+                                               int64_t* rows) {
+  if (threadIdx.x < kLoraTile) {
+    const int64_t m = m0 + threadIdx.x;
+    int64_t row = m < p.rows ? (ordered && p.order != nullptr ? p.order[m] : m) : -1;
+    if (row < 0 || row >= p.rows) row = -1;  // (an order that is no permutation)
+    ids[threadIdx.x] = row >= 0 ? lora_id(p, row) : -1;
+    rows[threadIdx.x] = row;
+  }
+  __syncthreads();
+}
+
+// h of 64 rows and 64 columns of the rank.
+template <typename OpT>
+__global__ __launch_bounds__(256) void lora_inner_kernel(const LoraParams p) {
+  using S = LoraSlice<OpT>;
+  __shared__ __attribute__((aligned(16))) OpT as[kLoraTile * S::LD], bs[kLoraTile * S::LD];
+  __shared__ int64_t rows[kLoraTile];
+  __shared__ int32_t ids[kLoraTile];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t m0 = (int64_t)blockIdx.x * kLoraTile, c0 = (int64_t)blockIdx.y * kLoraTile;
+  lora_tile_rows(p, m0, true, ids, rows);
+  f32x4_t res[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) res[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  const int col = lane & 15, r0 = wave * 16 + (lane >> 4) * 4;
+  const int32_t mine = ids[lane];
+  for (int32_t cur = -1;;) {
+    const int32_t a = wave_min_i32(mine > cur ? mine : INT32_MAX);  // the same in every wave
+    if (a == INT32_MAX) break;
+    cur = a;
+    f32x4_t acc[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    lora_product<OpT>(acc, as, bs, (const OpT*)p.x, p.x_ld, rows,
+                      (const OpT*)p.a + a * p.a_se + c0 * p.a_sr, p.a_sk, p.a_sr, p.rank - c0, p.K, wave, lane);
+    const float s = lora_scale(p, a);
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+      if (ids[r0 + v] == a) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) res[j][v] = s * acc[j][v];
+      }
+  }
+  OpT* h = (OpT*)p.h;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int64_t c = c0 + j * 16 + col;
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const int64_t row = rows[r0 + v];
+      const OpT o = from_f32<OpT>(c < p.rank ? res[j][v] : 0.f);
+      if (row >= 0 && c < p.h_ld) h[row * p.h_ld + c] = o;
+      if (p.ht != nullptr && m0 + r0 + v < p.rows && c < p.rank) ((OpT*)p.ht)[c * p.ht_ld + m0 + r0 + v] = o;
+    }
+  }
+}
+
+// 64 x 64 of the output.
+template <typename OpT>
+__global__ __launch_bounds__(256) void lora_out_kernel(const LoraParams p) {
+  using S = LoraSlice<OpT>;
+  __shared__ __attribute__((aligned(16))) OpT as[kLoraTile * S::LD], bs[kLoraTile * S::LD];
+  __shared__ int64_t rows[kLoraTile];
+  __shared__ int32_t ids[kLoraTile];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t tiles_n = (p.N + kLoraTile - 1) / kLoraTile;
+  const int64_t id = xcd_remap((int64_t)blockIdx.x, (int64_t)gridDim.x);
+  const int64_t m0 = (id / tiles_n) * kLoraTile, n0 = (id % tiles_n) * kLoraTile;
+  lora_tile_rows(p, m0, false, ids, rows);
+  f32x4_t res[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) res[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  if (p.w != nullptr)
+    lora_product<OpT>(res, as, bs, (const OpT*)p.x, p.x_ld, rows, (const OpT*)p.w + n0 * p.w_sn, p.w_sk, p.w_sn,
+                      p.N - n0, p.K, wave, lane);
+  const int col = lane & 15, r0 = wave * 16 + (lane >> 4) * 4;
+  const int32_t mine = ids[lane];
+  for (int32_t cur = -1;;) {
+    const int32_t a = wave_min_i32(mine > cur ? mine : INT32_MAX);
+    if (a == INT32_MAX) break;
+    cur = a;
+    f32x4_t acc[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    lora_product<OpT>(acc, as, bs, (const OpT*)p.h, p.h_ld, rows,
+                      (const OpT*)p.b + a * p.b_se + n0 * p.b_sn, p.b_sr, p.b_sn, p.N - n0, p.rank, wave, lane);
+#pragma unroll
+    for (int v = 0; v < 4; ++v)
+      if (ids[r0 + v] == a) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) res[j][v] += acc[j][v];
+      }
+  }
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    const int64_t row = rows[r0 + v];
+    if (row < 0) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t c = n0 + j * 16 + col;
+      if (c >= p.N) continue;
+      float o = res[j][v];
+      if (p.base != nullptr) o += load_as_f32(p.base, p.base_dtype, row * p.base_ld + c);
+      ((OpT*)p.out)[row * p.out_ld + c] = from_f32<OpT>(o);
+    }
+  }
+}
+
+template <typename OpT>
+static hipError_t launch_general(const LoraParams& p, hipStream_t s) {
+  const int64_t tm = (p.rows + kLoraTile - 1) / kLoraTile, tn = (p.N + kLoraTile - 1) / kLoraTile;
+  if (tm * tn > 0x7fffffffll) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((lora_inner_kernel<OpT>), dim3((unsigned)tm, (unsigned)((p.rank + kLoraTile - 1) / kLoraTile)),
+                     dim3(256), 0, s, p);
+  if (p.out == nullptr) return hipGetLastError();
+  hipLaunchKernelGGL((lora_out_kernel<OpT>), dim3((unsigned)(tm * tn)), dim3(256), 0, s, p);
+  return hipGetLastError();
+}
+
+hipError_t launch_lora(const LoraParams& p, int32_t op, hipStream_t s) {
+  if (op == kBF16) return launch_general<bf16_t>(p, s);
+  if (op == kF16) return launch_general<f16_t>(p, s);
+  return launch_general<float>(p, s);
+}
+
+// ---------------------------------------------------------------------------
+// The adapters' gradients: dA_i = sum_p x[p]^T u[p], dB_i = sum_p h[p]^T g[p]
+// over the rows p of adapter i, in the sorted order in which u and h stand
+// transposed.  One block of 64 x 64 values per workgroup and share of the
+// adapter's rows; the shares are added in order by a second launch.
+// ---------------------------------------------------------------------------
+template <typename OpT>
+__global__ __launch_bounds__(256) void lora_wgrad_kernel(const LoraWgradParams p) {
+  using S = LoraSlice<OpT>;
+  __shared__ __attribute__((aligned(16))) OpT as[kLoraTile * S::LD], bs[kLoraTile * S::LD];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // dA's blocks, then dB's: wide dimension (columns of x or g) by rank
+  const int64_t bi = (p.d_in + 63) / 64;
+  const bool in = (int64_t)blockIdx.x < bi;
+  const int64_t w0 = (in ? blockIdx.x : blockIdx.x - bi) * 64, r0 = (int64_t)blockIdx.y * 64;
+  if ((in ? p.ga : p.gb) == nullptr) return;
+  const int32_t e = blockIdx.z / p.shares, share = blockIdx.z % p.shares;
+  const int64_t lo = e > 0 && p.offsets[e - 1] > 0 ? p.offsets[e - 1] : 0;
+  const int64_t hi = p.offsets[e] < p.rows ? p.offsets[e] : p.rows;
+  const int64_t len = hi > lo ? hi - lo : 0;
+  const int64_t from = lo + len * share / p.shares, to = lo + len * (share + 1) / p.shares;
+  const OpT* rows = (const OpT*)(in ? p.x : p.g);
+  const int64_t ld = in ? p.x_ld : p.g_ld, width = in ? p.d_in : p.d_out;
+  const OpT* t = (const OpT*)(in ? p.ut : p.ht) + r0 * p.t_ld;
+  f32x4_t acc[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  for (int64_t p0 = from; p0 < to; p0 += S::BK) {
+    __syncthreads();
+    // wide operand: as[c][k], k = sorted position; thin operand: bs[r][k]
+#pragma unroll
+    for (int j = 0; j < S::PER; ++j) {
+      const int i = j * 256 + (int)threadIdx.x, c = i % 64, k = i / 64;
+      OpT v = from_f32<OpT>(0.f);
+      if (p0 + k < to && w0 + c < width) {
+        const int64_t row = p.order[p0 + k];
+        if (row >= 0 && row < p.rows) v = rows[row * ld + w0 + c];
+      }
+      as[c * S::LD + k] = v;
+    }
+    OpT vb[S::PER];
+    lora_load(t + p0, p.t_ld, 1, p.rank - r0, to - p0, vb);
+    lora_store(bs, true, vb);
+    __syncthreads();
+    lora_mfma(acc, as, bs, wave, lane);
+  }
+  const int64_t total = p.d_in * p.rank * p.n;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const int64_t c = w0 + wave * 16 + (lane >> 4) * 4 + v, r = r0 + j * 16 + (lane & 15);
+      if (c >= width || r >= p.rank) continue;
+      const int64_t at = in ? (e * p.d_in + c) * p.rank + r : (e * p.rank + r) * p.d_out + c;
+      if (p.shares > 1)
+        p.part[(int64_t)share * (total + p.d_out * p.rank * p.n) + (in ? at : total + at)] = acc[j][v];
+      else
+        store_from_f32(in ? p.ga : p.gb, p.g_dtype, at, acc[j][v]);
+    }
+  }
+}
+
+__global__ __launch_bounds__(256) void lora_wgrad_sum_kernel(const LoraWgradParams p) {
+  const int64_t na = p.d_in * p.rank * p.n, total = na + p.d_out * p.rank * p.n;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    if ((i < na ? p.ga : p.gb) == nullptr) continue;
+    float s = 0.f;
+#pragma unroll 4
+    for (int32_t q = 0; q < p.shares; ++q) s += p.part[q * total + i];
+    if (i < na) store_from_f32(p.ga, p.g_dtype, i, s);
+    else store_from_f32(p.gb, p.g_dtype, i - na, s);
+  }
+}
+
+int32_t lora_wgrad_shares(int64_t rows, int32_t n, int64_t d_in, int64_t d_out, int64_t rank) {
+  const int64_t blocks = ((d_in + 63) / 64 + (d_out + 63) / 64) * ((rank + 63) / 64) * n;
+  int64_t s = 1;
+  while (s < 64 && blocks * s < 512 && rows / (n * s) > 128) s *= 2;
+  return (int32_t)s;
+}
+
+size_t lora_wgrad_workspace_bytes(int64_t rows, int32_t n, int64_t d_in, int64_t d_out, int64_t rank) {
+  const int32_t s = lora_wgrad_shares(rows, n, d_in, d_out, rank);
+  return s > 1 ? (size_t)s * (size_t)n * (size_t)rank * (size_t)(d_in + d_out) * 4 : 0;
+}
+
+hipError_t launch_lora_wgrad(const LoraWgradParams& q, int32_t op, hipStream_t s) {
+  LoraWgradParams p = q;
+  p.shares = lora_wgrad_shares(p.rows, p.n, p.d_in, p.d_out, p.rank);
+  const int64_t bx = (p.d_in + 63) / 64 + (p.d_out + 63) / 64, by = (p.rank + 63) / 64, bz = (int64_t)p.n * p.shares;
+  if (bx > 0x7fffffffll || bz > 65535) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)bx, (unsigned)by, (unsigned)bz);
+  if (op == kBF16) hipLaunchKernelGGL((lora_wgrad_kernel<bf16_t>), grid, dim3(256), 0, s, p);
+  else if (op == kF16) hipLaunchKernelGGL((lora_wgrad_kernel<f16_t>), grid, dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((lora_wgrad_kernel<float>), grid, dim3(256), 0, s, p);
+  if (p.shares > 1) {
+    const int64_t total = (p.d_in + p.d_out) * p.rank * p.n;
+    const int64_t wg = (total + 1023) / 1024;
+    hipLaunchKernelGGL(lora_wgrad_sum_kernel, dim3((unsigned)(wg < 4096 ? wg : 4096)), dim3(256), 0, s, p);
+  }
+  return hipGetLastError();
+}
+
+}  // namespace cvmm

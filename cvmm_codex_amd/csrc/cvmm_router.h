@@ -2,6 +2,8 @@
 // routes within one workgroup.
 #pragma once
 
+#include <type_traits>
+
 #include "cvmm_common.h"
 
 namespace cvmm {
@@ -118,6 +120,24 @@ __device__ __forceinline__ uint32_t seg_or(uint32_t v) {
     v = a | b;
   }
   return v;
+}
+
+// Segment width: 8 experts per lane up to 512 experts, then 16.
+template <typename F>
+inline void by_experts(int32_t E, F&& f) {
+  if (E <= 32) f(std::integral_constant<int, 4>(), std::integral_constant<int, 8>());
+  else if (E <= 64) f(std::integral_constant<int, 8>(), std::integral_constant<int, 8>());
+  else if (E <= 128) f(std::integral_constant<int, 16>(), std::integral_constant<int, 8>());
+  else if (E <= 256) f(std::integral_constant<int, 32>(), std::integral_constant<int, 8>());
+  else if (E <= 512) f(std::integral_constant<int, 64>(), std::integral_constant<int, 8>());
+  else f(std::integral_constant<int, 64>(), std::integral_constant<int, 16>());
+}
+
+template <typename F>
+inline void by_dtype(int32_t dt, F&& f) {
+  if (dt == kF32) f(float());
+  else if (dt == kBF16) f(bf16_t());
+  else f(f16_t());
 }
 
 // The sort's outputs, written by the router's own launch where one workgroup

@@ -500,24 +500,6 @@ static void launch_scored(const LT* logits, const ScoredParams& p, int64_t tpc, 
                        dim3(scored_threads<LPT>(false)), 0, s, logits, p, tpc, w, sel, counts, so);
 }
 
-// Segment width: 8 experts per lane up to 512 experts, then 16.
-template <typename F>
-static void by_experts(int32_t E, F&& f) {
-  if (E <= 32) f(std::integral_constant<int, 4>(), std::integral_constant<int, 8>());
-  else if (E <= 64) f(std::integral_constant<int, 8>(), std::integral_constant<int, 8>());
-  else if (E <= 128) f(std::integral_constant<int, 16>(), std::integral_constant<int, 8>());
-  else if (E <= 256) f(std::integral_constant<int, 32>(), std::integral_constant<int, 8>());
-  else if (E <= 512) f(std::integral_constant<int, 64>(), std::integral_constant<int, 8>());
-  else f(std::integral_constant<int, 64>(), std::integral_constant<int, 16>());
-}
-
-template <typename F>
-static void by_dtype(int32_t dt, F&& f) {
-  if (dt == kF32) f(float());
-  else if (dt == kBF16) f(bf16_t());
-  else f(f16_t());
-}
-
 // Tokens per workgroup (= per sort chunk).  Up to 128 routes one workgroup chooses
 // and sorts them; past that its CU's instruction rate is the bound and a second
 // launch to sort costs less (32 tokens, top-8 of 256 experts in 8 groups 22.1 ->

@@ -1173,6 +1173,315 @@ std::tuple<Tensor, Tensor, Tensor> mx4_apply_recorded(const Tensor& x, const Opt
   return {y, i32, i64};
 }
 
+// ---------------------------------------------------------------------------
+// balance loss of a router (no counterpart in cvmm.py)
+// ---------------------------------------------------------------------------
+Tensor logits_rows(const Tensor& logits) {
+  Tensor l = logits.reshape({-1, logits.size(-1)});
+  if (l.stride(-1) != 1 || (l.size(0) > 1 && l.stride(0) < l.size(1))) l = l.contiguous();
+  return l;
+}
+
+// (loss, terms, counts, coef); group_tokens: tokens per group.
+std::vector<Tensor> balance_loss(const Tensor& logits, const Tensor& sel, const OptT& mask, int64_t group_tokens,
+                                 int64_t kind, int64_t scores, double weight, double z_weight) {
+  require_device(logits, "logits");
+  require_device(sel, "sel");
+  c10::DeviceGuard guard(logits.device());
+  const int64_t stream = current_stream(logits);
+  Tensor l = logits_rows(logits);
+  const int64_t T = l.size(0), E = l.size(1), k = sel.size(-1);
+  if (sel.device() != l.device() || sel.numel() != T * k || group_tokens <= 0 || T % group_tokens != 0)
+    throw py::value_error("cvmm_balance_loss: sel must hold k ids per token of the logits");
+  Tensor s = sel.scalar_type() == at::kInt || sel.scalar_type() == at::kLong ? sel : sel.to(at::kLong);
+  s = s.contiguous();
+  OptT m;
+  if (mask.has_value()) {
+    require_device(*mask, "mask");
+    if (mask->scalar_type() != at::kBool || mask->numel() != T || mask->device() != l.device())
+      throw py::value_error("cvmm_balance_loss: mask must hold one truth value per token");
+    m = mask->contiguous();
+  }
+  const int64_t pairs = T / group_tokens * E;
+  Tensor f = at::empty({pairs + 4}, opts(l, at::kFloat));
+  Tensor loss = at::empty({}, opts(l, at::kFloat)), terms = at::empty({2}, opts(l, at::kFloat));
+  Tensor counts = at::empty({E}, opts(l, at::kLong));
+  const size_t ws_bytes = cvmm_balance_loss_workspace_bytes(T, group_tokens, (int32_t)E);
+  OptT ws;
+  if (ws_bytes) ws = at::empty({(int64_t)ws_bytes}, opts(l, at::kByte));
+  check(cvmm_balance_loss(ptr(l), dtype_id(l.scalar_type()), T, std::max(l.stride(0), E), (int32_t)E, ptr(s),
+                          s.scalar_type() == at::kLong ? 1 : 0, k, tptr<uint8_t>(m), group_tokens, (int32_t)kind,
+                          (int32_t)scores, weight, z_weight, tptr<float>(loss), tptr<float>(terms),
+                          tptr<int64_t>(counts), tptr<float>(f), ptr(ws), ws_bytes, (void*)stream),
+        "cvmm_balance_loss");
+  return {loss, terms, counts, f};
+}
+
+Tensor balance_loss_backward(const Tensor& logits, const OptT& mask, const Tensor& coef, const Tensor& grad,
+                             int64_t group_tokens, int64_t scores) {
+  c10::DeviceGuard guard(logits.device());
+  Tensor l = logits_rows(logits);
+  const int64_t T = l.size(0), E = l.size(1);
+  Tensor out = at::empty({T, E}, opts(l, l.scalar_type()));
+  OptT m;
+  if (mask.has_value()) m = mask->contiguous();
+  Tensor g = grad.to(at::kFloat);
+  check(cvmm_balance_loss_backward(ptr(l), dtype_id(l.scalar_type()), T, std::max(l.stride(0), E), (int32_t)E,
+                                   tptr<uint8_t>(m), group_tokens, (int32_t)scores, tptr<float>(coef),
+                                   tptr<float>(g), ptr(out), E, (void*)current_stream(l)),
+        "cvmm_balance_loss backward");
+  return out.view(logits.sizes());
+}
+
+struct BalanceLossFunction : public torch::autograd::Function<BalanceLossFunction> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits,
+                                                const Tensor& sel, const OptT& mask, int64_t group_tokens,
+                                                int64_t kind, int64_t scores, double weight, double z_weight) {
+    auto out = balance_loss(logits, sel, mask, group_tokens, kind, scores, weight, z_weight);
+    ctx->saved_data["group_tokens"] = group_tokens;
+    ctx->saved_data["scores"] = scores;
+    ctx->save_for_backward({logits, opt_or_undef(mask), out[3]});
+    out.pop_back();
+    ctx->mark_non_differentiable({out[1], out[2]});
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    torch::autograd::variable_list res(8);
+    if (!grads[0].defined()) return res;
+    const auto v = ctx->get_saved_variables();
+    res[0] = balance_loss_backward(v[0], undef_or_opt(v[1]), v[2], grads[0], ctx->saved_data["group_tokens"].toInt(),
+                                   ctx->saved_data["scores"].toInt());
+    return res;
+  }
+};
+
+std::vector<Tensor> balance_loss_apply(const Tensor& logits, const Tensor& sel, const OptT& mask,
+                                       int64_t group_tokens, int64_t kind, int64_t scores, double weight,
+                                       double z_weight, bool grad) {
+  if (grad) return BalanceLossFunction::apply(logits, sel, mask, group_tokens, kind, scores, weight, z_weight);
+  auto out = balance_loss(logits, sel, mask, group_tokens, kind, scores, weight, z_weight);
+  out.pop_back();
+  return out;
+}
+
+// ---------------------------------------------------------------------------
+// low-rank adapters beside a shared projection (no counterpart in cvmm.py)
+// ---------------------------------------------------------------------------
+Tensor to_op(const Tensor& t, at::ScalarType op) { return t.scalar_type() == op ? t : t.to(op); }
+
+struct LoraShape {
+  int64_t rows, n, d_in, d_out, rank;
+};
+
+// Sizes and devices of a call; the operands may have any strides.
+LoraShape lora_check(const Tensor& x, const Tensor& ids, const Tensor& a, const Tensor& b, const OptT& weight,
+                     const OptT& base, const OptT& scales) {
+  require_device(x, "x");
+  const auto same = [&](const Tensor& t, const char* what) {
+    require_device(t, what);
+    if (t.device() != x.device())
+      throw py::value_error(std::string("cvmm_lora: ") + what + " is on another device than x");
+  };
+  same(ids, "adapters");
+  same(a, "a");
+  same(b, "b");
+  if (x.dim() < 1 || a.dim() != 3 || b.dim() != 3 || a.size(0) != b.size(0) || a.size(2) != b.size(1) ||
+      a.size(1) != x.size(-1) || a.numel() == 0 || b.numel() == 0)
+    throw py::value_error("cvmm_lora: x [..., d_in], a [n, d_in, rank] and b [n, rank, d_out] do not multiply");
+  const LoraShape s{x.numel() / x.size(-1), a.size(0), a.size(1), b.size(2), a.size(2)};
+  if (ids.numel() != s.rows) throw py::value_error("cvmm_lora: adapters must hold one id per row of x");
+  if (weight.has_value()) {
+    same(*weight, "weight");
+    if (weight->dim() != 2 || weight->size(0) != s.d_in || weight->size(1) != s.d_out)
+      throw py::value_error("cvmm_lora: weight must be [d_in, d_out]");
+  }
+  if (base.has_value()) {
+    same(*base, "base");
+    if (base->dim() != x.dim() || base->size(-1) != s.d_out || base->numel() != s.rows * s.d_out ||
+        !x.sizes().slice(0, x.dim() - 1).equals(base->sizes().slice(0, x.dim() - 1)))
+      throw py::value_error("cvmm_lora: base must have the output's shape");
+  }
+  if (scales.has_value()) {
+    same(*scales, "scale");
+    if (scales->dim() != 1 || scales->numel() != s.n)
+      throw py::value_error("cvmm_lora: scale must be a number or hold one value per adapter");
+  }
+  return s;
+}
+
+// One product: (out or none, inner rows transposed or none).  x [rows, K], ids
+// int32 or int64 and a, b, w in the op type with the strides given.
+std::tuple<OptT, OptT> lora_product(const Tensor& xf, const Tensor& ids, const Tensor& a, const Tensor& b,
+                                    const OptT& w, const OptT& base, const OptT& scales, double scale,
+                                    const OptT& order, bool want_out, bool want_inner, at::ScalarType op,
+                                    int64_t stream) {
+  const int64_t rows = xf.size(0), K = a.size(1), N = b.size(2), rank = a.size(2);
+  const int32_t od = dtype_id(op);
+  OptT out, inner, ws, bf;
+  if (want_out) out = at::empty({rows, N}, opts(xf, op));
+  // (columns of whole 16-byte pieces)
+  const int64_t ld = (rows + 7) / 8 * 8;
+  if (want_inner) inner = at::empty({rank, ld}, opts(xf, op));
+  if (rows == 0) return {out, inner};
+  if (base.has_value())
+    bf = rows_of(base->scalar_type() == op || base->scalar_type() == at::kFloat ? *base : base->to(op), N);
+  const size_t ws_bytes = cvmm_lora_workspace_bytes(rows, K, N, rank, od);
+  if (ws_bytes) ws = at::empty({(int64_t)ws_bytes}, opts(xf, at::kByte));
+  check(cvmm_lora(ptr(xf), od, rows, xf.stride(0) < K ? K : xf.stride(0), ptr(w), w.has_value() ? w->stride(0) : 0,
+                  w.has_value() ? w->stride(1) : 0, ptr(a), a.stride(0), a.stride(1), a.stride(2), ptr(b), b.stride(0),
+                  b.stride(1), b.stride(2), (int32_t)a.size(0), K, N, rank, ptr(ids),
+                  ids.scalar_type() == at::kLong ? 1 : 0, tptr<int64_t>(order), tptr<float>(scales), (float)scale,
+                  ptr(bf), bf.has_value() ? dtype_id(bf->scalar_type()) : 0,
+                  bf.has_value() ? std::max(bf->stride(0), N) : 0, ptr(out), N, ptr(inner), ld, ptr(ws), ws_bytes,
+                  (void*)stream),
+        "cvmm_lora");
+  return {out, inner};
+}
+
+// A sorted selection's order and offsets have an entry per row and per adapter.
+void lora_check_order(const LoraShape& s, const OptT& order, const OptT& offsets, const Tensor& x) {
+  if (order.has_value() && (order->numel() != s.rows || order->device() != x.device()))
+    throw py::value_error("cvmm_lora: the selection's order must hold one entry per row of x");
+  if (offsets.has_value() && (offsets->numel() != s.n || offsets->device() != x.device()))
+    throw py::value_error("cvmm_lora: the selection's offsets must hold one entry per adapter");
+}
+
+Tensor lora_ids(const Tensor& ids) {
+  Tensor f = ids.scalar_type() == at::kInt || ids.scalar_type() == at::kLong ? ids : ids.to(at::kLong);
+  return f.reshape({-1}).contiguous();
+}
+
+OptT lora_scales(const OptT& scales) {
+  if (!scales.has_value()) return std::nullopt;
+  return scales->to(at::kFloat).contiguous();
+}
+
+// The forward: (out [rows, d_out], inner rows transposed in sorted order or none).
+std::tuple<Tensor, OptT> lora_forward(const Tensor& x, const Tensor& ids, const Tensor& a, const Tensor& b,
+                                      const OptT& weight, const OptT& base, const OptT& scales, double scale,
+                                      const OptT& order, bool want_inner, int64_t op_id) {
+  const LoraShape s = lora_check(x, ids, a, b, weight, base, scales);
+  lora_check_order(s, order, std::nullopt, x);
+  c10::DeviceGuard guard(x.device());
+  const auto op = dtype_of(op_id);
+  OptT w;
+  if (weight.has_value()) w = to_op(*weight, op);
+  auto [out, inner] = lora_product(rows_of(to_op(x, op), s.d_in), lora_ids(ids), to_op(a, op), to_op(b, op), w, base,
+                                   lora_scales(scales), scale, as_i64(order), true, want_inner, op,
+                                   current_stream(x));
+  return {*out, inner};
+}
+
+// (grad x, grad a, grad b); order and offsets as the sort leaves them (for the
+// adapters' gradients), inner: the forward's.
+std::tuple<OptT, OptT, OptT> lora_backward(const Tensor& grad_output, const Tensor& x, const Tensor& ids,
+                                           const Tensor& a, const Tensor& b, const OptT& weight, const OptT& scales,
+                                           double scale, const OptT& order, const OptT& offsets, const OptT& inner,
+                                           int64_t op_id, bool need_x, bool need_a, bool need_b) {
+  const LoraShape s = lora_check(x, ids, a, b, weight, std::nullopt, scales);
+  lora_check_order(s, order, offsets, x);
+  if ((need_a || need_b) && s.rows > 0 && (!order.has_value() || !offsets.has_value()))
+    throw py::value_error("cvmm_lora: the adapters' gradients need a sorted selection");
+  c10::DeviceGuard guard(x.device());
+  const int64_t stream = current_stream(x);
+  const auto op = dtype_of(op_id);
+  Tensor g = rows_of(to_op(grad_output, op), s.d_out);
+  if (g.size(0) != s.rows) throw py::value_error("cvmm_lora: the gradient must have the output's shape");
+  OptT gx, ga, gb, u, ord = as_i64(order);
+  if (need_x || need_a) {
+    OptT w;
+    if (weight.has_value()) w = to_op(*weight, op).t();
+    std::tie(gx, u) = lora_product(g, lora_ids(ids), to_op(b, op).transpose(1, 2), to_op(a, op).transpose(1, 2), w,
+                                   std::nullopt, lora_scales(scales), scale, ord, need_x, need_a, op, stream);
+    if (gx.has_value()) gx = to_op(*gx, x.scalar_type()).view(x.sizes());
+  }
+  if (need_a || need_b) {
+    const auto gt = a.scalar_type() == b.scalar_type() && (a.scalar_type() == at::kHalf || a.scalar_type() == at::kBFloat16)
+                        ? a.scalar_type() : at::kFloat;
+    if (need_a) ga = at::empty({s.n, s.d_in, s.rank}, opts(x, gt));
+    if (need_b) gb = at::empty({s.n, s.rank, s.d_out}, opts(x, gt));
+    if (s.rows == 0) {
+      if (need_a) ga->zero_();
+      if (need_b) gb->zero_();
+    } else {
+      Tensor xr = rows_of(to_op(x, op), s.d_in), off = as_i64(*offsets);
+      const size_t ws_bytes = cvmm_lora_bwd_adapters_workspace_bytes(s.rows, (int32_t)s.n, s.d_in, s.d_out, s.rank);
+      OptT ws;
+      if (ws_bytes) ws = at::empty({(int64_t)ws_bytes}, opts(x, at::kByte));
+      check(cvmm_lora_bwd_adapters(ptr(xr), dtype_id(op), s.rows, std::max(xr.stride(0), s.d_in), ptr(g),
+                                   std::max(g.stride(0), s.d_out), ptr(inner), ptr(u), (s.rows + 7) / 8 * 8,
+                                   (int32_t)s.n, s.d_in, s.d_out, s.rank, tptr<int64_t>(ord), tptr<int64_t>(off),
+                                   ptr(ga), ptr(gb), dtype_id(gt), ptr(ws), ws_bytes, (void*)stream),
+            "cvmm_lora backward");
+    }
+    if (need_a) ga = to_op(*ga, a.scalar_type());
+    if (need_b) gb = to_op(*gb, b.scalar_type());
+  }
+  return {gx, ga, gb};
+}
+
+struct LoraFunction : public torch::autograd::Function<LoraFunction> {
+  // x, a, b and base (optional) are the differentiable inputs.  order, offsets: a
+  // sorted selection's, or none: sorted here where an adapter's gradient is asked for.
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& a, const Tensor& b,
+                        const OptT& base, const Tensor& ids, const OptT& weight, const OptT& scales, double scale,
+                        const OptT& order_in, const OptT& offsets_in, int64_t op_id) {
+    const bool adapters = a.requires_grad() || b.requires_grad();
+    OptT order = order_in, offsets = offsets_in;
+    if (adapters && !order.has_value()) {
+      lora_check(x, ids, a, b, weight, base, scales);
+      c10::DeviceGuard guard(x.device());
+      const Tensor flat = lora_ids(ids);
+      auto [i32, i64] = sort_routes_buffers(flat, a.size(0), 1, current_stream(x), std::nullopt);
+      const int64_t R = flat.numel();
+      order = i64.narrow(0, 0, R);
+      offsets = i64.narrow(0, 2 * R, a.size(0));
+    }
+    auto [out, inner] = lora_forward(x, ids, a, b, weight, base, scales, scale, order, b.requires_grad(), op_id);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["op_id"] = op_id;
+    ctx->saved_data["need"] = (int64_t)((x.requires_grad() ? 1 : 0) | (a.requires_grad() ? 2 : 0) |
+                                        (b.requires_grad() ? 4 : 0));
+    ctx->saved_data["base"] = base.has_value() && base->requires_grad() ? (int64_t)base->scalar_type() : (int64_t)-1;
+    ctx->save_for_backward({x, a, b, ids, opt_or_undef(weight), opt_or_undef(scales), opt_or_undef(order),
+                            opt_or_undef(offsets), opt_or_undef(inner)});
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = b.size(2);
+    return at::_unsafe_view(out, shape);
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto v = ctx->get_saved_variables();
+    const int64_t need = ctx->saved_data["need"].toInt(), base = ctx->saved_data["base"].toInt();
+    torch::autograd::variable_list res(11);
+    if (need != 0) {
+      auto [gx, ga, gb] = lora_backward(grads[0], v[0], v[3], v[1], v[2], undef_or_opt(v[4]), undef_or_opt(v[5]),
+                                        ctx->saved_data["scale"].toDouble(), undef_or_opt(v[6]), undef_or_opt(v[7]),
+                                        undef_or_opt(v[8]), ctx->saved_data["op_id"].toInt(), (need & 1) != 0,
+                                        (need & 2) != 0, (need & 4) != 0);
+      res[0] = opt_or_undef(gx);
+      res[1] = opt_or_undef(ga);
+      res[2] = opt_or_undef(gb);
+    }
+    if (base >= 0) res[3] = grads[0].to((at::ScalarType)base);
+    return res;
+  }
+};
+
+Tensor lora_apply(const Tensor& x, const Tensor& ids, const Tensor& a, const Tensor& b, const OptT& weight,
+                  const OptT& base, const OptT& scales, double scale, const OptT& order, const OptT& offsets,
+                  int64_t op_id, bool grad) {
+  if (grad) return LoraFunction::apply(x, a, b, base, ids, weight, scales, scale, order, offsets, op_id);
+  Tensor out = std::get<0>(lora_forward(x, ids, a, b, weight, base, scales, scale, order, false, op_id));
+  std::vector<int64_t> shape = x.sizes().vec();
+  shape.back() = b.size(2);
+  return out.view(shape);
+}
+
 // The Python-facing forward and backward (torch.compile's ops): no kept rows.
 Tensor forward_py(const Tensor& x, const Tensor& keys, const OptT& keys_op, bool keys_op_is_t, const Tensor& sel,
                   const Tensor& sel_index, const OptT& out_index, const Tensor& offsets, const OptT& route_pos,
@@ -1233,6 +1542,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mx4_apply", &mx4_apply);
   m.def("mx4_apply_recorded", &mx4_apply_recorded);
   m.def("routing_views", &routing_views);
+  m.def("balance_loss", &balance_loss);
+  m.def("balance_loss_backward", &balance_loss_backward);
+  m.def("balance_loss_apply", &balance_loss_apply);
+  m.def("lora_forward", &lora_forward);
+  m.def("lora_backward", &lora_backward);
+  m.def("lora_apply", &lora_apply);
   // operand rules, exposed for tests
   m.def("storage_for", [](const Tensor& t, int64_t op_id) { return storage_for(t, dtype_of(op_id)); });
   m.def("keys_view", &keys_view);

@@ -73,7 +73,9 @@ extern "C" {
                                  top-k slot table and row scaling / weighted rows of the weight
                                  gradient */
 #define CVMM_KC_FILL 128      /* zero fills */
-#define CVMM_KC_ROUTE 512     /* router (softmax, top-k, histogram) + its scatter; router backward */
+#define CVMM_KC_ROUTE 512     /* router (softmax, top-k, histogram) + its scatter; router backward;
+                                 balance loss */
+#define CVMM_KC_LORA 1024     /* adapters: cvmm_lora and the adapters' gradients */
 
 /* Thread-local description of the last error. */
 const char* cvmm_last_error(void);
@@ -509,6 +511,73 @@ int cvmm_bwd_w_rows(const void* x, int32_t x_dtype, int64_t x_rows, int64_t x_ld
                     int32_t op_dtype, void* grad_keys, int32_t grad_keys_dtype, int64_t gk_se, int64_t gk_si,
                     int64_t gk_sj, int32_t flags, void* rows, size_t rows_bytes, void* workspace,
                     size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Balance loss of a router with per-expert counts (no counterpart in cvmm.py,
+ * whose callers add such a term to their loss).  n_tokens tokens in groups of
+ * group_tokens (a sequence each, or all of them); mask: one byte per token, 0
+ * for tokens that count nowhere, or NULL.  With p the softmax of a token's
+ * logits (or its sigmoids over their sum, at least 1e-20), n live tokens of a
+ * group, P_e the mean of p_e over them and c_e their routes to e (sel: n_tokens
+ * x top_k ids; those outside [0, n_experts) are not counted):
+ *   CVMM_BALANCE_LOAD:    sum_e (n_experts c_e / (top_k n)) P_e
+ *   CVMM_BALANCE_ENTROPY: sum_e P_e log P_e
+ * terms[0]: that, averaged over the groups that have a live token (0 if none);
+ * terms[1]: the mean of logsumexp(l)^2 over the live tokens; loss: weight *
+ * terms[0] + z_weight * terms[1]; counts: int64 per expert, over all groups;
+ * coef: groups * n_experts + 1 values for the backward, which writes
+ * grad_logits in the logits' dtype (0 at masked tokens) from grad_loss, one
+ * fp32 value on the device.  At most 1024 experts and 1024 groups. */
+#define CVMM_BALANCE_LOAD 0
+#define CVMM_BALANCE_ENTROPY 1
+size_t cvmm_balance_loss_workspace_bytes(int64_t n_tokens, int64_t group_tokens, int32_t n_experts);
+int cvmm_balance_loss(const void* logits, int32_t logits_dtype, int64_t n_tokens, int64_t logits_ld,
+                      int32_t n_experts, const void* sel, int32_t sel_is_int64, int64_t top_k, const uint8_t* mask,
+                      int64_t group_tokens, int32_t kind, int32_t scores, double weight, double z_weight,
+                      float* loss, float* terms, int64_t* counts, float* coef, void* workspace,
+                      size_t workspace_bytes, void* stream);
+int cvmm_balance_loss_backward(const void* logits, int32_t logits_dtype, int64_t n_tokens, int64_t logits_ld,
+                               int32_t n_experts, const uint8_t* mask, int64_t group_tokens, int32_t scores,
+                               const float* coef, const float* grad_loss, void* grad_logits, int64_t grad_ld,
+                               void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Low-rank adapters of many requests beside a shared projection (no counterpart
+ * in cvmm.py):
+ *   out[t] = base[t] + x[t] W + h[t] B_i,  h[t] = rnd_op(s_i x[t] A_i),  i = ids[t]
+ * x, W [d_in][d_out] (or NULL), A [n_adapters][d_in][rank], B [n_adapters]
+ * [rank][d_out] in the op dtype with any element strides (rows of x, base and out
+ * with unit column stride); base (or NULL) in the op dtype or fp32; s_i = scale,
+ * times scales[i] where that is given.  Rows whose id is outside [0, n_adapters)
+ * take base and projection alone.  An adapter's infinities and NaN reach its own
+ * rows only.  order (or NULL): a permutation of the rows with equal ids side by
+ * side (cvmm_sort_routes' perm), the order in which the inner rows are formed;
+ * inner_t (or NULL): h transposed, [rank][inner_ld], column p the row order[p].
+ * out may be NULL where inner_t is given.
+ *
+ * The backward for a frozen W: grad_x is cvmm_lora of grad with W, A and B
+ * transposed (B's transpose in A's place and the other way round; no base), whose
+ * inner_t are the inner gradients; cvmm_lora_bwd_adapters then sums over the rows
+ * of each adapter, in a fixed order,
+ *   grad_a[i] = x^T inner_grad, grad_b[i] = inner^T grad
+ * ([n_adapters][d_in][rank] and [n_adapters][rank][d_out], contiguous, grad_dtype,
+ * NULL: not wanted; zero for adapters without rows).  order and offsets: as
+ * cvmm_sort_routes leaves them.  At most rank 256 and 2^31 - 1 rows; adapter
+ * gradients: at most 32767 adapters (the sort's limit). */
+size_t cvmm_lora_workspace_bytes(int64_t rows, int64_t d_in, int64_t d_out, int64_t rank, int32_t op_dtype);
+int cvmm_lora(const void* x, int32_t op_dtype, int64_t rows, int64_t x_ld, const void* weight, int64_t w_si,
+              int64_t w_so, const void* a, int64_t a_se, int64_t a_si, int64_t a_sr, const void* b, int64_t b_se,
+              int64_t b_sr, int64_t b_so, int32_t n_adapters, int64_t d_in, int64_t d_out, int64_t rank,
+              const void* ids, int32_t ids_is_int64, const int64_t* order, const float* scales, float scale,
+              const void* base, int32_t base_dtype, int64_t base_ld, void* out, int64_t out_ld, void* inner_t,
+              int64_t inner_ld, void* workspace, size_t workspace_bytes, void* stream);
+size_t cvmm_lora_bwd_adapters_workspace_bytes(int64_t rows, int32_t n_adapters, int64_t d_in, int64_t d_out,
+                                              int64_t rank);
+int cvmm_lora_bwd_adapters(const void* x, int32_t op_dtype, int64_t rows, int64_t x_ld, const void* grad,
+                           int64_t grad_ld, const void* inner_t, const void* inner_grad_t, int64_t inner_ld,
+                           int32_t n_adapters, int64_t d_in, int64_t d_out, int64_t rank, const int64_t* order,
+                           const int64_t* offsets, void* grad_a, void* grad_b, int32_t grad_dtype, void* workspace,
+                           size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Microscaled 4-bit values: blocks of 32 share a scale 2^s, s = floor(log2
