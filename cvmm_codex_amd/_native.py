@@ -145,7 +145,7 @@ _SIGS = {
         _I32, _I32, ctypes.c_double, ctypes.c_double,  # kind, scores, weight, z_weight
         _P, _P, _P, _P, _P, _SZ, _P]),        # loss, terms, counts, coef, ws, ws bytes, stream
     "cvmm_balance_loss_backward": (ctypes.c_int, [_P, _I32, _I64, _I64, _I32, _P, _I64, _I32, _P, _P, _P, _I64, _P]),
-    "cvmm_lora_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I64, _I32]),
+    "cvmm_lora_workspace_bytes": (_SZ, [_I64, _I32, _I64, _I64, _I64, _I32, _I32, _I32]),
     "cvmm_lora": (ctypes.c_int, [
         _P, _I32, _I64, _I64,                 # x, op dtype, rows, ld
         _P, _I64, _I64,                       # weight, strides
@@ -155,7 +155,7 @@ _SIGS = {
         _P, _I32, _P, _P, ctypes.c_float,     # ids, int64, order, scales, scale
         _P, _I32, _I64, _P, _I64,             # base, dtype, ld, out, ld
         _P, _I64, _P, _SZ, _P]),              # inner_t, ld, ws, ws bytes, stream
-    "cvmm_lora_bwd_adapters_workspace_bytes": (_SZ, [_I64, _I32, _I64, _I64, _I64]),
+    "cvmm_lora_bwd_adapters_workspace_bytes": (_SZ, [_I64, _I32, _I64, _I64, _I64, _I32]),
     "cvmm_lora_bwd_adapters": (ctypes.c_int, [
         _P, _I32, _I64, _I64, _P, _I64,       # x, op dtype, rows, ld, grad, ld
         _P, _P, _I64,                         # inner_t, inner_grad_t, ld

@@ -849,9 +849,12 @@ static int lora_args_ok(const char* what, int32_t op_dtype, int64_t rows, int64_
   return CVMM_OK;
 }
 
-size_t cvmm_lora_workspace_bytes(int64_t rows, int64_t d_in, int64_t d_out, int64_t rank, int32_t op_dtype) {
-  if (rows <= 0 || d_in <= 0 || d_out <= 0 || rank <= 0 || rank > kLoraMaxRank || !valid_dtype(op_dtype)) return 0;
-  return align_up((size_t)rows * (size_t)((rank + 31) / 32 * 32) * dtype_size(op_dtype), 256);
+size_t cvmm_lora_workspace_bytes(int64_t rows, int32_t n_adapters, int64_t d_in, int64_t d_out, int64_t rank,
+                                 int32_t op_dtype, int32_t has_weight, int32_t copied) {
+  if (rows <= 0 || n_adapters <= 0 || d_in <= 0 || d_out <= 0 || rank <= 0 || rank > kLoraMaxRank ||
+      !valid_dtype(op_dtype))
+    return 0;
+  return lora_workspace_bytes(rows, n_adapters, d_in, d_out, rank, op_dtype, has_weight != 0, copied != 0);
 }
 
 int cvmm_lora(const void* x, int32_t op_dtype, int64_t rows, int64_t x_ld, const void* weight, int64_t w_si,
@@ -867,22 +870,22 @@ int cvmm_lora(const void* x, int32_t op_dtype, int64_t rows, int64_t x_ld, const
   if (base && (base_ld < d_out || (base_dtype != op_dtype && base_dtype != kF32)))
     return fail(CVMM_ERR_INVALID, "%s: base must be rows of the op type or fp32", what);
   if (inner_t && inner_ld < rows) return fail(CVMM_ERR_INVALID, "%s: inner row stride too small", what);
-  const size_t need = cvmm_lora_workspace_bytes(rows, d_in, d_out, rank, op_dtype);
+  const size_t need = cvmm_lora_workspace_bytes(rows, n_adapters, d_in, d_out, rank, op_dtype, weight != nullptr, 0);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(CVMM_ERR_WORKSPACE, "%s: workspace too small (%zu < %zu)", what, workspace_bytes, need);
   if (rows == 0) return CVMM_OK;
   if (!x || !a || !b || !ids || (!out && !inner_t)) return fail(CVMM_ERR_INVALID, "%s: NULL pointer", what);
   const LoraParams p{x, rows, x_ld, weight, w_si, w_so, a, a_se, a_si, a_sr, b, b_se, b_sr, b_so, n_adapters,
                      d_in, d_out, rank, ids, ids_is_int64, order, scales, scale, base, base_dtype, base_ld,
-                     out, out_ld, workspace, (rank + 31) / 32 * 32, inner_t, inner_ld};
+                     out, out_ld, nullptr, (rank + 31) / 32 * 32, inner_t, inner_ld, d_out, rank, 0, 0};
   hipStream_t s = (hipStream_t)stream;
-  return check_launch(timed(CVMM_KC_LORA, s, [&] { return launch_lora(p, op_dtype, s); }), what);
+  return check_launch(timed(CVMM_KC_LORA, s, [&] { return launch_lora(p, op_dtype, workspace, workspace_bytes, s); }), what);
 }
 
 size_t cvmm_lora_bwd_adapters_workspace_bytes(int64_t rows, int32_t n_adapters, int64_t d_in, int64_t d_out,
-                                              int64_t rank) {
+                                              int64_t rank, int32_t copied) {
   if (rows < 0 || n_adapters <= 0 || d_in <= 0 || d_out <= 0 || rank <= 0 || rank > kLoraMaxRank) return 0;
-  return lora_wgrad_workspace_bytes(rows, n_adapters, d_in, d_out, rank);
+  return lora_wgrad_workspace_bytes(rows, n_adapters, d_in, d_out, rank, copied != 0);
 }
 
 int cvmm_lora_bwd_adapters(const void* x, int32_t op_dtype, int64_t rows, int64_t x_ld, const void* grad,
@@ -895,7 +898,7 @@ int cvmm_lora_bwd_adapters(const void* x, int32_t op_dtype, int64_t rows, int64_
   if (r) return r;
   if (grad_ld < d_out || inner_ld < rows) return fail(CVMM_ERR_INVALID, "%s: row stride too small", what);
   if (!valid_dtype(grad_dtype)) return fail(CVMM_ERR_INVALID, "%s: invalid gradient dtype", what);
-  const size_t need = lora_wgrad_workspace_bytes(rows, n_adapters, d_in, d_out, rank);
+  const size_t need = lora_wgrad_workspace_bytes(rows, n_adapters, d_in, d_out, rank, false);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(CVMM_ERR_WORKSPACE, "%s: workspace too small (%zu < %zu)", what, workspace_bytes, need);
   if (!grad_a && !grad_b) return CVMM_OK;
@@ -904,7 +907,7 @@ int cvmm_lora_bwd_adapters(const void* x, int32_t op_dtype, int64_t rows, int64_
   LoraWgradParams p{x, x_ld, grad, grad_ld, inner_t, inner_grad_t, inner_ld, rows, n_adapters, d_in, d_out, rank,
                     order, offsets, grad_a, grad_b, grad_dtype, (float*)workspace, 1};
   hipStream_t s = (hipStream_t)stream;
-  return check_launch(timed(CVMM_KC_LORA, s, [&] { return launch_lora_wgrad(p, op_dtype, s); }), what);
+  return check_launch(timed(CVMM_KC_LORA, s, [&] { return launch_lora_wgrad(p, op_dtype, workspace_bytes, s); }), what);
 }
 
 // ---------------------------------------------------------------------------

@@ -47,6 +47,23 @@ __device__ __forceinline__ void wg_barrier() {
 
 __device__ __forceinline__ void issue_fence() { asm volatile("" ::: "memory"); }
 
+// Word 3 of a raw buffer descriptor on gfx9 (no format conversion).
+constexpr int kBufferRsrcWord3 = 0x00020000;
+
+// BYTES (4 or 16) per lane from the descriptor's memory at voff + soff + IMM
+// into LDS at lds + IMM + BYTES x the lane index (the immediate moves both
+// addresses; lds goes to M0): one instruction per wave, counted by vmcnt.
+template <int BYTES, int IMM>
+__device__ __forceinline__ void buf_dma(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff, void* lds) {
+  static_assert(BYTES == 4 || BYTES == 16, "dword or dwordx4");
+  static_assert(IMM >= 0 && IMM < 4096, "12-bit immediate");
+  auto* l = (__attribute__((address_space(3))) void*)lds;
+  if constexpr (BYTES == 16)
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, l, 16, voff, soff, IMM, 0);
+  else
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, l, 4, voff, soff, IMM, 0);
+}
+
 // 16-byte LDS read issued as inline asm.  The compiler does not see it as an
 // LDS access, so its wait-count pass inserts no vmcnt wait for in-flight DMA
 // into other LDS buffers (it cannot always tell those apart and then waits

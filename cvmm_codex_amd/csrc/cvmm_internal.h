@@ -319,9 +319,13 @@ hipError_t launch_balance_loss_backward(const void* logits, int32_t dtype, int64
 // ---------------------------------------------------------------------------
 struct LoraParams;
 struct LoraWgradParams;
-hipError_t launch_lora(const LoraParams& p, int32_t op_dtype, hipStream_t stream);
-size_t lora_wgrad_workspace_bytes(int64_t rows, int32_t n, int64_t d_in, int64_t d_out, int64_t rank);
-hipError_t launch_lora_wgrad(const LoraWgradParams& p, int32_t op_dtype, hipStream_t stream);
+// `copied`: with room for copies of operands that are not made of aligned 16-byte
+// pieces; without it such calls run the general kernels.
+size_t lora_workspace_bytes(int64_t rows, int32_t n, int64_t K, int64_t N, int64_t rank, int32_t op_dtype,
+                            bool weight, bool copied);
+hipError_t launch_lora(const LoraParams& p, int32_t op_dtype, void* ws, size_t ws_bytes, hipStream_t stream);
+size_t lora_wgrad_workspace_bytes(int64_t rows, int32_t n, int64_t d_in, int64_t d_out, int64_t rank, bool copied);
+hipError_t launch_lora_wgrad(const LoraWgradParams& p, int32_t op_dtype, size_t ws_bytes, hipStream_t stream);
 
 // ---------------------------------------------------------------------------
 // microscaled 4-bit values (cvmm_mx4.h: format and layouts)

@@ -38,6 +38,23 @@ struct LoraParams {
   // or NULL: h transposed, [rank][ht_ld], column p the row order[p]
   void* ht;
   int64_t ht_ld;
+  // 16-byte kernels: the output's own width and the rank that ht has (N and rank
+  // count zero padding up to multiples of 8), and whether the rows of out and of
+  // base are made of aligned pieces
+  int64_t n_out, rank_out;
+  int32_t out_vec, base_vec;
+};
+
+// K split over workgroups: fp32 partial products [splits][rows][part_ld], each
+// of `slices` slices of 32 k; inner rows alike, [h_splits][rows][rank].
+struct LoraSplit {
+  float* part;
+  int64_t part_ld;
+  int32_t splits, slices;
+  uint32_t gemm_blocks;  // the workgroups after them form inner rows
+  float* h_part;
+  int32_t h_splits;
+  int32_t h_k;           // k per share of the inner rows
 };
 
 struct LoraWgradParams {

@@ -223,7 +223,158 @@ static hipError_t launch_general(const LoraParams& p, hipStream_t s) {
   return hipGetLastError();
 }
 
-hipError_t launch_lora(const LoraParams& p, int32_t op, hipStream_t s) {
+template <typename OpT> hipError_t launch_lora_gemm_op(const LoraParams& p, hipStream_t s);
+template <typename OpT> hipError_t launch_lora_inner_op(const LoraParams& p, hipStream_t s);
+template <typename OpT> hipError_t launch_lora_few_op(const LoraParams& p, const LoraSplit& sp, hipStream_t s);
+template <typename OpT> hipError_t launch_lora_wgrad_op(const LoraWgradParams& p, hipStream_t s);
+
+namespace {
+bool al16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; }
+
+// A matrix [rows][cols] of aligned 16-byte pieces along the dimension of stride 1.
+bool pieces(const void* q, int64_t se, int64_t sr, int64_t sc) {
+  return al16(q) && se % 8 == 0 && ((sc == 1 && sr % 8 == 0) || (sr == 1 && sc % 8 == 0));
+}
+
+// What the 16-byte kernels take: whole pieces, and distances that their 32-bit
+// offsets hold (a tile's rows and columns, a matrix along k).
+bool fast_ok(const LoraParams& p, int32_t op) {
+  constexpr int64_t kReach = (int64_t)1 << 30;  // elements below 2^31 bytes, the slack off
+  auto reach = [&](int64_t k, int64_t sk, int64_t sn) { return k * sk + 256 * sn < kReach - 8192; };
+  return op != kF32 && p.K % 8 == 0 && p.N % 8 == 0 && p.rank % 8 == 0 && al16(p.x) && p.x_ld % 8 == 0 &&
+         p.x_ld < kReach / 512 && pieces(p.a, p.a_se, p.a_sk, p.a_sr) && pieces(p.b, p.b_se, p.b_sr, p.b_sn) &&
+         reach(p.rank, p.b_sr, p.b_sn) &&
+         (p.w == nullptr || (pieces(p.w, 0, p.w_sk, p.w_sn) && reach(p.K, p.w_sk, p.w_sn)));
+}
+
+// Rows up to which a call is two launches of plain multiply-adds beside a GEMM
+// split along k.
+constexpr int64_t kLoraFewRows = 256;
+bool few_rows(int64_t rows) { return rows <= kLoraFewRows; }
+
+// Workgroups of the split GEMM (64 x 128 tiles) and shares of the inner rows:
+// enough for every CU, at least 64 k each.
+LoraSplit few_split(int64_t rows, int64_t K, int64_t N, int64_t rank) {
+  LoraSplit sp{};
+  const int64_t tiles = ((rows + 63) / 64) * ((N + 127) / 128), all = (K + 31) / 32;
+  int64_t splits = (256 + tiles - 1) / tiles;
+  if (splits > (all + 1) / 2) splits = (all + 1) / 2;
+  if (splits < 1) splits = 1;
+  sp.slices = (int32_t)((all + splits - 1) / splits);
+  sp.splits = (int32_t)((all + sp.slices - 1) / sp.slices);
+  sp.gemm_blocks = (uint32_t)(tiles * sp.splits);
+  sp.part_ld = (N + 7) / 8 * 8;
+  const int64_t per = 4 * (256 / (rank / 8 > 0 ? rank / 8 : 1));  // k that a workgroup takes in four loads a thread
+  int64_t shares = (K + per - 1) / per;
+  if (shares > 16) shares = 16;
+  sp.h_k = (int32_t)(((K + shares - 1) / shares + 7) / 8 * 8);
+  sp.h_splits = (int32_t)((K + sp.h_k - 1) / sp.h_k);
+  return sp;
+}
+
+size_t h_bytes(int64_t rows, int64_t rank, int32_t op) {
+  return align_up((size_t)rows * (size_t)((rank + 31) / 32 * 32) * dtype_size(op), 256);
+}
+
+struct LoraCopies {
+  size_t x, w, a, b;
+  size_t total() const { return x + w + a + b; }
+};
+LoraCopies copies_bytes(int64_t rows, int64_t n, int64_t K, int64_t N, int64_t rank, bool weight) {
+  const size_t k8 = (size_t)pad8(K), n8 = (size_t)pad8(N), r8 = (size_t)pad8(rank);
+  return {align_up((size_t)rows * k8 * 2, 256), weight ? align_up(k8 * n8 * 2, 256) : 0,
+          align_up((size_t)n * k8 * r8 * 2, 256), align_up((size_t)n * r8 * n8 * 2, 256)};
+}
+
+// [n][d_i][d_j] of any strides -> whole pieces, the unit stride's dimension kept.
+hipError_t copy_matrix(const void*& q, int64_t& se, int64_t& si, int64_t& sj, int64_t n, int64_t d_i, int64_t d_j,
+                       int32_t op, char*& at, size_t bytes, hipStream_t s) {
+  const bool t = si == 1 && sj != 1;
+  const hipError_t e = launch_pad_keys(q, op, se, si, sj, (int32_t)n, d_i, d_j, op, at, t, s);
+  q = at;
+  at += bytes;
+  se = pad8(d_i) * pad8(d_j);
+  si = t ? 1 : pad8(d_j);
+  sj = t ? pad8(d_i) : 1;
+  return e;
+}
+
+template <typename OpT>
+hipError_t launch_fast(const LoraParams& q, void* ws, hipStream_t s) {
+  LoraParams p = q;
+  p.out_vec = al16(p.out) && p.out_ld % 8 == 0 && p.n_out % 8 == 0;
+  p.base_vec = p.base != nullptr && al16(p.base) && p.base_ld % 4 == 0;
+  if (few_rows(p.rows) && p.ht == nullptr) {
+    LoraSplit sp = few_split(p.rows, p.K, p.N, p.rank);
+    sp.h_part = (float*)ws;
+    if (p.w != nullptr)
+      sp.part = (float*)((char*)ws + align_up((size_t)sp.h_splits * (size_t)(p.rows * p.rank) * 4, 256));
+    return launch_lora_few_op<OpT>(p, sp, s);
+  }
+  p.h = ws;
+  const hipError_t e = launch_lora_inner_op<OpT>(p, s);
+  if (e != hipSuccess || p.out == nullptr) return e;
+  // the projection takes the rows by their order where 32-bit offsets reach them all
+  const int64_t wide = p.x_ld > p.h_ld ? p.x_ld : p.h_ld;
+  if (p.order != nullptr && p.rows * wide >= ((int64_t)1 << 30) - 8192) p.order = nullptr;
+  return launch_lora_gemm_op<OpT>(p, s);
+}
+}  // namespace
+
+size_t lora_workspace_bytes(int64_t rows, int32_t n, int64_t K, int64_t N, int64_t rank, int32_t op, bool weight,
+                            bool copied) {
+  size_t own = h_bytes(rows, rank, op);
+  if (op == kF32) return own;
+  if (few_rows(rows)) {
+    const LoraSplit sp = few_split(rows, pad8(K), pad8(N), pad8(rank));
+    const size_t few = align_up((size_t)sp.h_splits * (size_t)(rows * pad8(rank)) * 4, 256) +
+                       (weight ? (size_t)sp.splits * (size_t)rows * (size_t)sp.part_ld * 4 : 0);
+    own = own > few ? own : few;
+  }
+  own = align_up(own, 256);
+  return own + (copied ? copies_bytes(rows, n, K, N, rank, weight).total() : 0);
+}
+
+hipError_t launch_lora(const LoraParams& q, int32_t op, void* ws, size_t ws_bytes, hipStream_t s) {
+  LoraParams p = q;
+  p.n_out = p.N;
+  p.rank_out = p.rank;
+  if (op != kF32 && !fast_ok(p, op)) {
+    // copies of whole pieces, where there is room for them
+    const bool weight = p.w != nullptr;
+    const size_t own = lora_workspace_bytes(p.rows, p.n, p.K, p.N, p.rank, op, weight, false);
+    const LoraCopies c = copies_bytes(p.rows, p.n, p.K, p.N, p.rank, weight);
+    // (what the copies' own grids and indices hold)
+    const bool small = p.n <= 65535 && c.x < ((size_t)1 << 34) && c.a < ((size_t)1 << 34) && c.b < ((size_t)1 << 34);
+    if (small && ws_bytes >= own + c.total()) {
+      char* at = (char*)ws + own;
+      hipError_t e = hipSuccess;
+      if (p.K % 8 != 0 || p.x_ld % 8 != 0 || !al16(p.x)) {
+        e = launch_pad_rows(p.x, op, p.x_ld, p.rows, p.K, nullptr, 0, op, at, s);
+        p.x = at;
+        p.x_ld = pad8(p.K);
+      }
+      at += c.x;
+      int64_t se = 0;
+      if (e == hipSuccess && weight && (p.K % 8 != 0 || p.N % 8 != 0 || !pieces(p.w, 0, p.w_sk, p.w_sn)))
+        e = copy_matrix(p.w, se, p.w_sk, p.w_sn, 1, p.K, p.N, op, at, c.w, s);
+      else
+        at += c.w;
+      if (e == hipSuccess && (p.K % 8 != 0 || p.rank % 8 != 0 || !pieces(p.a, p.a_se, p.a_sk, p.a_sr)))
+        e = copy_matrix(p.a, p.a_se, p.a_sk, p.a_sr, p.n, p.K, p.rank, op, at, c.a, s);
+      else
+        at += c.a;
+      if (e == hipSuccess && (p.N % 8 != 0 || p.rank % 8 != 0 || !pieces(p.b, p.b_se, p.b_sr, p.b_sn)))
+        e = copy_matrix(p.b, p.b_se, p.b_sr, p.b_sn, p.n, p.rank, p.N, op, at, c.b, s);
+      if (e != hipSuccess) return e;
+      p.K = pad8(p.K);
+      p.N = pad8(p.N);
+      p.rank = pad8(p.rank);
+      p.h_ld = (p.rank + 31) / 32 * 32;
+    }
+  }
+  if (fast_ok(p, op)) return op == kBF16 ? launch_fast<bf16_t>(p, ws, s) : launch_fast<f16_t>(p, ws, s);
+  p.h = ws;
   if (op == kBF16) return launch_general<bf16_t>(p, s);
   if (op == kF16) return launch_general<f16_t>(p, s);
   return launch_general<float>(p, s);
@@ -303,25 +454,57 @@ __global__ __launch_bounds__(256) void lora_wgrad_sum_kernel(const LoraWgradPara
   }
 }
 
-int32_t lora_wgrad_shares(int64_t rows, int32_t n, int64_t d_in, int64_t d_out, int64_t rank) {
-  const int64_t blocks = ((d_in + 63) / 64 + (d_out + 63) / 64) * ((rank + 63) / 64) * n;
+static int32_t lora_wgrad_shares(int64_t rows, int32_t n, int64_t d_in, int64_t d_out, int64_t rank) {
+  const int64_t blocks = ((d_in + 127) / 128 + (d_out + 127) / 128) * ((rank + 63) / 64) * n;
   int64_t s = 1;
   while (s < 64 && blocks * s < 512 && rows / (n * s) > 128) s *= 2;
   return (int32_t)s;
 }
 
-size_t lora_wgrad_workspace_bytes(int64_t rows, int32_t n, int64_t d_in, int64_t d_out, int64_t rank) {
+static size_t wgrad_part_bytes(int64_t rows, int32_t n, int64_t d_in, int64_t d_out, int64_t rank) {
   const int32_t s = lora_wgrad_shares(rows, n, d_in, d_out, rank);
-  return s > 1 ? (size_t)s * (size_t)n * (size_t)rank * (size_t)(d_in + d_out) * 4 : 0;
+  return s > 1 ? align_up((size_t)s * (size_t)n * (size_t)rank * (size_t)(d_in + d_out) * 4, 256) : 0;
 }
 
-hipError_t launch_lora_wgrad(const LoraWgradParams& q, int32_t op, hipStream_t s) {
+size_t lora_wgrad_workspace_bytes(int64_t rows, int32_t n, int64_t d_in, int64_t d_out, int64_t rank, bool copied) {
+  return wgrad_part_bytes(rows, n, d_in, d_out, rank) +
+         (copied ? align_up((size_t)rows * (size_t)pad8(d_in) * 2, 256) + (size_t)rows * (size_t)pad8(d_out) * 2 : 0);
+}
+
+hipError_t launch_lora_wgrad(const LoraWgradParams& q, int32_t op, size_t ws_bytes, hipStream_t s) {
   LoraWgradParams p = q;
   p.shares = lora_wgrad_shares(p.rows, p.n, p.d_in, p.d_out, p.rank);
+  auto rows_ok = [&] {
+    return (p.ga == nullptr || (al16(p.x) && p.x_ld % 8 == 0 && p.d_in % 8 == 0)) &&
+           (p.gb == nullptr || (al16(p.g) && p.g_ld % 8 == 0 && p.d_out % 8 == 0));
+  };
+  bool fast = op != kF32 && p.t_ld % 8 == 0 && al16(p.ht) && al16(p.ut);
+  if (fast && !rows_ok()) {
+    // rows of whole pieces, where there is room for the copies
+    fast = ws_bytes >= lora_wgrad_workspace_bytes(p.rows, p.n, p.d_in, p.d_out, p.rank, true) &&
+           p.rows * ((p.d_in > p.d_out ? p.d_in : p.d_out) + 8) < ((int64_t)1 << 33);
+    char* at = (char*)p.part + wgrad_part_bytes(p.rows, p.n, p.d_in, p.d_out, p.rank);
+    if (fast && p.ga != nullptr) {
+      const hipError_t e = launch_pad_rows(p.x, op, p.x_ld, p.rows, p.d_in, nullptr, 0, op, at, s);
+      if (e != hipSuccess) return e;
+      p.x = at;
+      p.x_ld = pad8(p.d_in);
+    }
+    at += align_up((size_t)p.rows * (size_t)pad8(p.d_in) * 2, 256);
+    if (fast && p.gb != nullptr) {
+      const hipError_t e = launch_pad_rows(p.g, op, p.g_ld, p.rows, p.d_out, nullptr, 0, op, at, s);
+      if (e != hipSuccess) return e;
+      p.g = at;
+      p.g_ld = pad8(p.d_out);
+    }
+  }
   const int64_t bx = (p.d_in + 63) / 64 + (p.d_out + 63) / 64, by = (p.rank + 63) / 64, bz = (int64_t)p.n * p.shares;
   if (bx > 0x7fffffffll || bz > 65535) return hipErrorInvalidValue;
   const dim3 grid((unsigned)bx, (unsigned)by, (unsigned)bz);
-  if (op == kBF16) hipLaunchKernelGGL((lora_wgrad_kernel<bf16_t>), grid, dim3(256), 0, s, p);
+  if (fast) {
+    const hipError_t e = op == kBF16 ? launch_lora_wgrad_op<bf16_t>(p, s) : launch_lora_wgrad_op<f16_t>(p, s);
+    if (e != hipSuccess) return e;
+  } else if (op == kBF16) hipLaunchKernelGGL((lora_wgrad_kernel<bf16_t>), grid, dim3(256), 0, s, p);
   else if (op == kF16) hipLaunchKernelGGL((lora_wgrad_kernel<f16_t>), grid, dim3(256), 0, s, p);
   else hipLaunchKernelGGL((lora_wgrad_kernel<float>), grid, dim3(256), 0, s, p);
   if (p.shares > 1) {

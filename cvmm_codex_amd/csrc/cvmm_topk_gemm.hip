@@ -221,11 +221,9 @@ __global__ __launch_bounds__(256) void copy_rows_op_kernel(const void* __restric
 // the GEMM
 // ---------------------------------------------------------------------------
 
-// Word 3 of a raw buffer descriptor on gfx9 (no format conversion), and the
-// descriptors' byte range: every offset the kernel issues is either below
+// The descriptors' byte range: every offset the kernel issues is either below
 // kTopkOob (the launcher checks it, soffset included) or at or past it, which
 // reads zeros whether or not the hardware adds soffset before the range check.
-constexpr int kBufferRsrcWord3 = 0x00020000;
 constexpr uint32_t kTkRange = kTopkOob;
 // the descriptors' bases sit this far before the data, so that the lane
 // offsets stay positive when instruction j's immediate 1024 j is taken off them
@@ -233,20 +231,6 @@ constexpr uint32_t kTkBaseBack = 4096;
 
 template <int J>
 using TkRow = std::integral_constant<int, J>;
-
-// BYTES (4 or 16) per lane from the descriptor's memory at voff + soff + IMM
-// into LDS at lds + IMM + BYTES x the lane index (the immediate moves both
-// addresses; lds goes to M0): one instruction per wave, counted by vmcnt.
-template <int BYTES, int IMM>
-__device__ __forceinline__ void buf_dma(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff, void* lds) {
-  static_assert(BYTES == 4 || BYTES == 16, "dword or dwordx4");
-  static_assert(IMM >= 0 && IMM < 4096, "12-bit immediate");
-  auto* l = (__attribute__((address_space(3))) void*)lds;
-  if constexpr (BYTES == 16)
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, l, 16, voff, soff, IMM, 0);
-  else
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, l, 4, voff, soff, IMM, 0);
-}
 
 // lgkmcnt(0) / lgkmcnt(8) tied to the table entries (read before the 8 LDS
 // reads still allowed to be pending)

@@ -1312,6 +1312,13 @@ LoraShape lora_check(const Tensor& x, const Tensor& ids, const Tensor& a, const 
   return s;
 }
 
+// Whether t is made of aligned 16-byte pieces along one of its last two dimensions.
+bool whole_pieces(const Tensor& t) {
+  const int64_t d = t.dim(), r = t.stride(d - 2), c = t.stride(d - 1);
+  return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0 && (d < 3 || t.stride(0) % 8 == 0) &&
+         ((c == 1 && r % 8 == 0) || (r == 1 && c % 8 == 0));
+}
+
 // One product: (out or none, inner rows transposed or none).  x [rows, K], ids
 // int32 or int64 and a, b, w in the op type with the strides given.
 std::tuple<OptT, OptT> lora_product(const Tensor& xf, const Tensor& ids, const Tensor& a, const Tensor& b,
@@ -1328,7 +1335,10 @@ std::tuple<OptT, OptT> lora_product(const Tensor& xf, const Tensor& ids, const T
   if (rows == 0) return {out, inner};
   if (base.has_value())
     bf = rows_of(base->scalar_type() == op || base->scalar_type() == at::kFloat ? *base : base->to(op), N);
-  const size_t ws_bytes = cvmm_lora_workspace_bytes(rows, K, N, rank, od);
+  const bool copied = !whole_pieces(xf) || !whole_pieces(a) || !whole_pieces(b) || (w.has_value() && !whole_pieces(*w)) ||
+                      K % 8 != 0 || N % 8 != 0 || rank % 8 != 0;
+  const size_t ws_bytes = cvmm_lora_workspace_bytes(rows, (int32_t)a.size(0), K, N, rank, od, w.has_value() ? 1 : 0,
+                                                    copied ? 1 : 0);
   if (ws_bytes) ws = at::empty({(int64_t)ws_bytes}, opts(xf, at::kByte));
   check(cvmm_lora(ptr(xf), od, rows, xf.stride(0) < K ? K : xf.stride(0), ptr(w), w.has_value() ? w->stride(0) : 0,
                   w.has_value() ? w->stride(1) : 0, ptr(a), a.stride(0), a.stride(1), a.stride(2), ptr(b), b.stride(0),
@@ -1408,7 +1418,9 @@ std::tuple<OptT, OptT, OptT> lora_backward(const Tensor& grad_output, const Tens
       if (need_b) gb->zero_();
     } else {
       Tensor xr = rows_of(to_op(x, op), s.d_in), off = as_i64(*offsets);
-      const size_t ws_bytes = cvmm_lora_bwd_adapters_workspace_bytes(s.rows, (int32_t)s.n, s.d_in, s.d_out, s.rank);
+      const bool copied = s.d_in % 8 != 0 || s.d_out % 8 != 0 || !whole_pieces(xr) || !whole_pieces(g);
+      const size_t ws_bytes =
+          cvmm_lora_bwd_adapters_workspace_bytes(s.rows, (int32_t)s.n, s.d_in, s.d_out, s.rank, copied ? 1 : 0);
       OptT ws;
       if (ws_bytes) ws = at::empty({(int64_t)ws_bytes}, opts(x, at::kByte));
       check(cvmm_lora_bwd_adapters(ptr(xr), dtype_id(op), s.rows, std::max(xr.stride(0), s.d_in), ptr(g),

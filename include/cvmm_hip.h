@@ -563,8 +563,13 @@ int cvmm_balance_loss_backward(const void* logits, int32_t logits_dtype, int64_t
  * ([n_adapters][d_in][rank] and [n_adapters][rank][d_out], contiguous, grad_dtype,
  * NULL: not wanted; zero for adapters without rows).  order and offsets: as
  * cvmm_sort_routes leaves them.  At most rank 256 and 2^31 - 1 rows; adapter
- * gradients: at most 32767 adapters (the sort's limit). */
-size_t cvmm_lora_workspace_bytes(int64_t rows, int64_t d_in, int64_t d_out, int64_t rank, int32_t op_dtype);
+ * gradients: at most 32767 adapters (the sort's limit).
+ *
+ * copied of the workspace queries: room for copies of 16-bit operands that are not
+ * made of aligned 16-byte pieces (widths, rank or strides no multiple of 8, or an
+ * unaligned base address); without it such calls run slower, general kernels. */
+size_t cvmm_lora_workspace_bytes(int64_t rows, int32_t n_adapters, int64_t d_in, int64_t d_out, int64_t rank,
+                                 int32_t op_dtype, int32_t has_weight, int32_t copied);
 int cvmm_lora(const void* x, int32_t op_dtype, int64_t rows, int64_t x_ld, const void* weight, int64_t w_si,
               int64_t w_so, const void* a, int64_t a_se, int64_t a_si, int64_t a_sr, const void* b, int64_t b_se,
               int64_t b_sr, int64_t b_so, int32_t n_adapters, int64_t d_in, int64_t d_out, int64_t rank,
@@ -572,7 +577,7 @@ int cvmm_lora(const void* x, int32_t op_dtype, int64_t rows, int64_t x_ld, const
               const void* base, int32_t base_dtype, int64_t base_ld, void* out, int64_t out_ld, void* inner_t,
               int64_t inner_ld, void* workspace, size_t workspace_bytes, void* stream);
 size_t cvmm_lora_bwd_adapters_workspace_bytes(int64_t rows, int32_t n_adapters, int64_t d_in, int64_t d_out,
-                                              int64_t rank);
+                                              int64_t rank, int32_t copied);
 int cvmm_lora_bwd_adapters(const void* x, int32_t op_dtype, int64_t rows, int64_t x_ld, const void* grad,
                            int64_t grad_ld, const void* inner_t, const void* inner_grad_t, int64_t inner_ld,
                            int32_t n_adapters, int64_t d_in, int64_t d_out, int64_t rank, const int64_t* order,

@@ -68,6 +68,13 @@ CASES = [
     (1999, 512, 768, 32, 8, "runs", F16, True, False),
     (2500, 264, 520, 8, 3, "none", BF, True, True),
     (4099, 256, 320, 64, 16, "runs", BF, True, False),
+    # the largest tiles: 192 and more of 256 x 256
+    (12345, 96, 1032, 16, 40, "runs", BF, True, True),
+    (12345, 40, 1280, 72, 3, "alternate", F16, True, False),
+    (16000, 64, 1000, 8, 5, "own", BF, False, True),
+    # and of 128 x 128
+    (3001, 160, 1032, 40, 6, "runs", F16, True, True),
+    (3100, 33, 1000, 6, 11, "alternate", BF, True, False),
 ]
 
 

@@ -113,8 +113,10 @@ def test_lora_arguments_fail_before_launch(lib):
                              None, None, 1.0, base, base_dtype, base_ld, out, out_ld, inner, inner_ld, ws, ws_bytes,
                              None)
 
-    assert lib.cvmm_lora_workspace_bytes(100, 64, 64, 5, N.BF16) >= 100 * 32 * 2
-    assert lib.cvmm_lora_workspace_bytes(100, 64, 64, 300, N.BF16) == 0
+    assert lib.cvmm_lora_workspace_bytes(1000, 4, 64, 64, 5, N.BF16, 1, 0) >= 1000 * 32 * 2
+    assert lib.cvmm_lora_workspace_bytes(1000, 4, 64, 64, 5, N.BF16, 1, 1) >= 1000 * (32 + 64) * 2 + 2 * 4 * 64 * 8 * 2
+    assert lib.cvmm_lora_workspace_bytes(100, 4, 64, 64, 300, N.BF16, 1, 0) == 0
+    assert lib.cvmm_lora_workspace_bytes(0, 4, 64, 64, 8, N.BF16, 1, 1) == 0
     assert call(op=9) == 1 and call(rows=-1) == 1 and call(ld=8) == 1 and call(n=0) == 1 and call(rank=0) == 1
     assert call(rank=257) == 2 and call(rows=1 << 31) == 2
     assert call(out_ld=4) == 1 and call(base=FAKE, base_ld=4) == 1 and call(base=FAKE, base_dtype=N.F16) == 1
