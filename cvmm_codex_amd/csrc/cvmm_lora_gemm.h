@@ -13,13 +13,14 @@
 // swapped (C^T = W^T x^T): a lane ends with 4 consecutive columns of one row, 8
 // after two lane swaps, stored as one 16-byte write.
 //
-// Adapters: the tile walks the adapters of its rows by rising id.  A block of 16
-// rows that all have the adapter takes its product in its accumulators; one that
-// has it in some rows forms it apart and adds it where it belongs (no product
-// with zero: infinities of one request's adapter stay with its rows); others skip
-// it.  Rows of a request stand together, so nearly all blocks are of the first or
-// the last kind, and the adapters' slices cost what they add: rank / 32 slices
-// beside K / 32.
+// Adapters: the tile walks the adapters of its rows by rising id, each a product
+// of the rows' inner values, zero in the rows of others, with B_i's columns.  Rows
+// of a request stand together, so most tiles have one, and the adapters cost rank /
+// 32 slices beside K / 32.  Zero times an infinity or a NaN would carry one
+// request's to another's rows: where a tile has several adapters such values of
+// B_i are left out, and added to their own rows after the stores.  (Chosen per
+// element of the accumulators instead, 256 of them through branches, the compiler
+// spilled: 800 us against 130 for 16384 rows of 2048 -> 2048.)
 #pragma once
 
 #include <type_traits>
@@ -65,6 +66,82 @@ __device__ __forceinline__ uint4 lora_frag(const lds_u32x2 (&v)[2]) {
   return make_uint4(v[0].x, v[0].y, v[1].x, v[1].y);
 }
 
+// Infinities and NaN of a fragment's 16-bit values -> 0; dropped: there were some.
+template <typename OpT>
+__device__ __forceinline__ uint32_t lora_finite_pair(uint32_t v, bool& dropped) {
+  constexpr uint32_t kExp = DTypeOf<OpT>::value == kBF16 ? 0x7f80u : 0x7c00u;
+  const bool lo = (v & kExp) == kExp, hi = (v & (kExp << 16)) == (kExp << 16);
+  dropped |= lo | hi;
+  return (lo ? 0u : v & 0xffffu) | (hi ? 0u : v & 0xffff0000u);
+}
+template <typename OpT, int N>
+__device__ __forceinline__ void lora_finite(lds_u32x4 (&f)[N], bool& dropped) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) f[i][q] = lora_finite_pair<OpT>(f[i][q], dropped);
+}
+template <typename OpT, int N>
+__device__ __forceinline__ void lora_finite(lds_u32x2 (&f)[N][2], bool& dropped) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) f[i][q / 2][q % 2] = lora_finite_pair<OpT>(f[i][q / 2][q % 2], dropped);
+}
+
+// c[i] += w x_i^T: the row blocks of one column block.  AGPR (eight of them): in
+// accumulation registers by name, as one block of instructions.  Of 256 accumulators
+// the compiler moved 200 to other registers and back in every slice, as many
+// instructions as the matrix unit leaves room for.  The compiler does not see matrix
+// instructions here: the block starts with the two wait states that they need after
+// a vector instruction wrote their operands, and lora_mfma_done comes before c is read.
+template <typename OpT, bool AGPR, int MI>
+__device__ __forceinline__ void lora_mfma_col(f32x4_t (&c)[MI], const uint4& w, const lds_u32x4 (&x)[MI]) {
+  if constexpr (!AGPR) {
+#pragma unroll
+    for (int i = 0; i < MI; ++i) MfmaOp<OpT>::step(c[i], w, make_uint4(x[i].x, x[i].y, x[i].z, x[i].w));
+  } else {
+    static_assert(MI == 8, "eight row blocks");
+    const lds_u32x4 a{w.x, w.y, w.z, w.w};
+    if constexpr (DTypeOf<OpT>::value == kBF16) {
+      asm("s_nop 1\n\t"
+                   "v_mfma_f32_16x16x32_bf16 %0, %8, %9, %0\n\t"
+                   "v_mfma_f32_16x16x32_bf16 %1, %8, %10, %1\n\t"
+                   "v_mfma_f32_16x16x32_bf16 %2, %8, %11, %2\n\t"
+                   "v_mfma_f32_16x16x32_bf16 %3, %8, %12, %3\n\t"
+                   "v_mfma_f32_16x16x32_bf16 %4, %8, %13, %4\n\t"
+                   "v_mfma_f32_16x16x32_bf16 %5, %8, %14, %5\n\t"
+                   "v_mfma_f32_16x16x32_bf16 %6, %8, %15, %6\n\t"
+                   "v_mfma_f32_16x16x32_bf16 %7, %8, %16, %7"
+                   : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]), "+a"(c[4]), "+a"(c[5]), "+a"(c[6]), "+a"(c[7])
+                   : "v"(a), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]), "v"(x[5]), "v"(x[6]), "v"(x[7]));
+    } else {
+      asm("s_nop 1\n\t"
+                   "v_mfma_f32_16x16x32_f16 %0, %8, %9, %0\n\t"
+                   "v_mfma_f32_16x16x32_f16 %1, %8, %10, %1\n\t"
+                   "v_mfma_f32_16x16x32_f16 %2, %8, %11, %2\n\t"
+                   "v_mfma_f32_16x16x32_f16 %3, %8, %12, %3\n\t"
+                   "v_mfma_f32_16x16x32_f16 %4, %8, %13, %4\n\t"
+                   "v_mfma_f32_16x16x32_f16 %5, %8, %14, %5\n\t"
+                   "v_mfma_f32_16x16x32_f16 %6, %8, %15, %6\n\t"
+                   "v_mfma_f32_16x16x32_f16 %7, %8, %16, %7"
+                   : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]), "+a"(c[4]), "+a"(c[5]), "+a"(c[6]), "+a"(c[7])
+                   : "v"(a), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]), "v"(x[5]), "v"(x[6]), "v"(x[7]));
+    }
+  }
+}
+// After the last of them: more wait states than the last result needs before a
+// vector instruction reads it, and every accumulator handed on, so that no read of
+// one comes earlier.
+template <int NJ, int MI>
+__device__ __forceinline__ void lora_mfma_done(f32x4_t (&c)[NJ][MI]) {
+  asm volatile("s_nop 15\n\ts_nop 15" : "+a"(c[0][0]));
+#pragma unroll
+  for (int j = 0; j < NJ; ++j)
+#pragma unroll
+    for (int i = 0; i < MI; ++i) asm volatile("" : "+a"(c[j][i]));
+}
+
 template <int MI, int NJ, int WMW, int WNW>
 struct LoraTile {
   static_assert(WMW * WNW == 4, "four waves");
@@ -74,23 +151,28 @@ struct LoraTile {
   static constexpr int D = (A_INSTS + B_INSTS) / 4;
   static constexpr int A_BYTES = BM * 64, SLICE = (BM + BN) * 64, STAGES = 4;
   static constexpr int OCC = MI * NJ > 16 ? 1 : 2;
+  static constexpr bool AGPR = MI * NJ == 64;
 };
 
-// Lane offsets of a slice's B half.  KC: [n][k] pieces, as the A half; else [k][n]
-// rows of BN columns, read back transposed.
+// Lane offset of load `inst` of a slice's B half, and the k that its piece starts
+// at.  KC: [n][k] pieces, as the A half; else [k][n] rows of BN columns, read back
+// transposed.
 template <bool KC, int BN>
-__device__ __forceinline__ void lora_b_lane(int inst, int lane, int64_t sk, int64_t sn, int64_t cols, uint32_t& off,
-                                            int& k) {
+__device__ __forceinline__ uint32_t lora_b_off(int inst, int lane, int64_t sk, int64_t sn, int64_t cols) {
   if constexpr (KC) {
-    const int n = inst * 16 + (lane >> 2), c = (lane & 3) ^ ((n >> 1) & 3);
-    k = c * 8;
-    off = n < cols ? (uint32_t)(n * sn * 2) + (uint32_t)c * 16 + kLoraBack : kLoraOob;
+    const int n = inst * 16 + (lane >> 2), c = (lane & 3) ^ ((lane >> 3) & 3);
+    return n < cols ? (uint32_t)(n * sn * 2) + (uint32_t)c * 16 + kLoraBack : kLoraOob;
   } else {
     constexpr int CPR = BN / 8;
-    const int q = inst * 64 + lane, row = q / CPR, c = (q % CPR) ^ tr_row_swz<CPR>(row);
-    k = row;
-    off = c * 8 < cols ? (uint32_t)(row * sk * 2) + (uint32_t)c * 16 + kLoraBack : kLoraOob;
+    const int row = inst * (64 / CPR) + lane / CPR, c = (lane % CPR) ^ tr_row_swz<CPR>(row);
+    return c * 8 < cols ? (uint32_t)(row * sk * 2) + (uint32_t)c * 16 + kLoraBack : kLoraOob;
   }
+}
+template <bool KC, int BN>
+__device__ __forceinline__ int lora_b_k(int inst, int lane) {
+  constexpr int CPR = BN / 8;
+  if constexpr (KC) return ((lane & 3) ^ ((lane >> 3) & 3)) * 8;
+  else return inst * (64 / CPR) + lane / CPR;
 }
 
 template <typename OpT, int MI, int NJ, int WMW, int WNW, bool WKC, bool BKC, bool SPLIT>
@@ -138,18 +220,17 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
   const int64_t first = p.order != nullptr ? 0 : m0;
   const __amdgpu_buffer_rsrc_t ra = lora_rsrc(reinterpret_cast<const OpT*>(p.x) + first * p.x_ld + k_lo);
   const __amdgpu_buffer_rsrc_t rw = lora_rsrc(reinterpret_cast<const OpT*>(p.w) + n0 * p.w_sn + k_lo * p.w_sk);
+  const int a_k = ((lane & 3) ^ ((lane >> 3) & 3)) * 8;  // the k that a lane's pieces of x start at
   uint32_t off[D];
-  int kc[D];
 #pragma unroll
   for (int j = 0; j < D; ++j) {
     const int g = wave * D + j;
     if (g < T::A_INSTS) {
-      const int r = g * 16 + (lane >> 2), c = (lane & 3) ^ ((r >> 1) & 3);
+      const int r = g * 16 + (lane >> 2), c = (lane & 3) ^ ((lane >> 3) & 3);
       const int32_t row = s_row[r];
-      kc[j] = c * 8;
       off[j] = row >= 0 ? (uint32_t)(((int64_t)row - first) * p.x_ld * 2) + (uint32_t)c * 16 + kLoraBack : kLoraOob;
     } else {
-      lora_b_lane<WKC, BN>(g - T::A_INSTS, lane, p.w_sk, p.w_sn, p.N - n0, off[j], kc[j]);
+      off[j] = lora_b_off<WKC, BN>(g - T::A_INSTS, lane, p.w_sk, p.w_sn, p.N - n0);
     }
     if (off[j] != kLoraOob) off[j] -= 1024u * (uint32_t)(j & 3);
   }
@@ -165,7 +246,9 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
   uint32_t i_a = 0, i_b = 0;
   auto issue_part = [&](auto jc, char* dst) {
     constexpr int J = decltype(jc)::value;
-    issue_one(jc, ra, rw, i_k + kc[J] < kw ? off[J] : kLoraOob, i_a, i_b, dst);
+    const int g = wave * D + J;
+    const int k = i_k + (g < T::A_INSTS ? a_k : lora_b_k<WKC, BN>(g - T::A_INSTS, lane));
+    issue_one(jc, ra, rw, k < kw ? off[J] : kLoraOob, i_a, i_b, dst);
   };
   auto issue_next = [&]() {
     i_k += 32;
@@ -202,41 +285,13 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
     }
   };
 
-  // ---- accumulators, from base: acc[j][i] holds columns 16 j + 4 fq + {0..3} of row 16 i + fr
+  // ---- accumulators: acc[j][i] holds columns 16 j + 4 fq + {0..3} of row 16 i + fr
   f32x4_t acc[NJ][MI];
   const int64_t nw = n0 + wn * NJ * 16;
 #pragma unroll
   for (int j = 0; j < NJ; ++j)
 #pragma unroll
     for (int i = 0; i < MI; ++i) acc[j][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  if constexpr (!SPLIT) {
-    if (p.base != nullptr) {
-#pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        const int64_t row = s_row[(wm * MI + i) * 16 + fr];
-        if (row < 0) continue;
-        const int64_t at = row * p.base_ld;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const int64_t n = nw + j * 16 + 4 * fq;
-          if (n + 4 <= p.n_out && p.base_vec) {
-            if (p.base_dtype == kF32) {
-              const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.base) + at + n);
-              acc[j][i] = f32x4_t{v.x, v.y, v.z, v.w};
-            } else {
-              const uint2 raw = *reinterpret_cast<const uint2*>(reinterpret_cast<const OpT*>(p.base) + at + n);
-              const OpT* v = reinterpret_cast<const OpT*>(&raw);
-              acc[j][i] = f32x4_t{to_f32(v[0]), to_f32(v[1]), to_f32(v[2]), to_f32(v[3])};
-            }
-          } else {
-#pragma unroll
-            for (int v = 0; v < 4; ++v)
-              if (n + v < p.n_out) acc[j][i][v] = load_as_f32(p.base, p.base_dtype, at + n + v);
-          }
-        }
-      }
-    }
-  }
 
   // ---- the shared weights
   using WFrag = std::conditional_t<WKC, lds_u32x4[NJ], lds_u32x2[NJ][2]>;
@@ -269,9 +324,7 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
       read_b((uint32_t)nbuf * SLICE, nb);
       static_for<NJ>([&](auto jb) {
         constexpr int JB = decltype(jb)::value;
-        const uint4 w = lora_frag(cb[JB]);
-#pragma unroll
-        for (int i = 0; i < MI; ++i) MfmaOp<OpT>::step(acc[JB][i], w, lora_frag(ca[i]));
+        lora_mfma_col<OpT, T::AGPR>(acc[JB], lora_frag(cb[JB]), ca);
         static_for<D>([&](auto j) {
           if constexpr (decltype(j)::value * NJ / D == JB) issue_part(j, dst);
         });
@@ -289,6 +342,7 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
       step(a1, b1, a0, b0);
     }
     vm_wait<0>();
+    if constexpr (T::AGPR) lora_mfma_done(acc);
   }
 
   if constexpr (SPLIT) {
@@ -314,21 +368,25 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
   for (int i = 0; i < MI; ++i) ids[i] = s_id[(wm * MI + i) * 16 + fr];
   const __amdgpu_buffer_rsrc_t rh = lora_rsrc(reinterpret_cast<const OpT*>(p.h) + first * p.h_ld);
   uint32_t hoff[D];
-  int hk[D];
 #pragma unroll
   for (int j = 0; j < D; ++j) {
     const int g = wave * D + j;
     if (g < T::A_INSTS) {
-      const int r = g * 16 + (lane >> 2), c = (lane & 3) ^ ((r >> 1) & 3);
+      const int r = g * 16 + (lane >> 2), c = (lane & 3) ^ ((lane >> 3) & 3);
       const int32_t row = s_row[r];
-      hk[j] = 0;  // (zeros up to h_ld)
       hoff[j] = row >= 0 ? (uint32_t)(((int64_t)row - first) * p.h_ld * 2) + (uint32_t)c * 16 + kLoraBack : kLoraOob;
     } else {
-      lora_b_lane<BKC, BN>(g - T::A_INSTS, lane, p.b_sr, p.b_sn, p.N - n0, hoff[j], hk[j]);
+      hoff[j] = lora_b_off<BKC, BN>(g - T::A_INSTS, lane, p.b_sr, p.b_sn, p.N - n0);
     }
     if (hoff[j] != kLoraOob) hoff[j] -= 1024u * (uint32_t)(j & 3);
   }
   const int32_t rank = (int32_t)p.rank;
+  // one adapter, or none, for the whole tile?
+  bool uniform = true;
+#pragma unroll
+  for (int i = 0; i < BM / 64; ++i) uniform &= s_id[i * 64 + lane] == s_id[0];
+  uniform = __all(uniform);
+  bool dropped = false;  // this lane left infinities or NaN out of an adapter's values
   const uint32_t hb_step = (uint32_t)((BKC ? 1 : p.b_sr) * 64);
   for (int32_t cur = -1;;) {
     int32_t a = INT32_MAX;
@@ -349,7 +407,9 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
         if (k < rank)
           static_for<D>([&](auto j) {
             constexpr int J = decltype(j)::value;
-            issue_one(j, rh, rb, k + hk[J] < rank ? hoff[J] : kLoraOob, (uint32_t)k * 2,
+            const int g = wave * D + J;  // (h holds zeros up to h_ld)
+            const bool in = g < T::A_INSTS || k + lora_b_k<BKC, BN>(g - T::A_INSTS, lane) < rank;
+            issue_one(j, rh, rb, in ? hoff[J] : kLoraOob, (uint32_t)k * 2,
                       (uint32_t)(k / 32) * hb_step, ring + s * SLICE);
           });
       }
@@ -363,43 +423,62 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         lora_wait(af);
         lora_wait(bf);
+        if (!uniform) {
 #pragma unroll
-        for (int i = 0; i < MI; ++i) {
-          const bool mine = ids[i] == a;
-          const uint64_t in = __ballot(mine);
-          if (in == 0) continue;
-          if (in == ~0ull) {
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) MfmaOp<OpT>::step(acc[j][i], lora_frag(bf[j]), lora_frag(af[i]));
-          } else {
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-              f32x4_t t{0.f, 0.f, 0.f, 0.f};
-              MfmaOp<OpT>::step(t, lora_frag(bf[j]), lora_frag(af[i]));
-#pragma unroll
-              for (int v = 0; v < 4; ++v) acc[j][i][v] = mine ? acc[j][i][v] + t[v] : acc[j][i][v];
-            }
-          }
+          for (int i = 0; i < MI; ++i)
+            if (ids[i] != a) af[i] = lds_u32x4{0u, 0u, 0u, 0u};
+          lora_finite<OpT>(bf, dropped);
         }
+        static_for<NJ>([&](auto jc) {
+          constexpr int j = decltype(jc)::value;
+          lora_mfma_col<OpT, T::AGPR>(acc[j], lora_frag(bf[j]), af);
+        });
+        if constexpr (T::AGPR) lora_mfma_done(acc);
       }
     }
   }
 
-  // ---- stores
-#pragma unroll
-  for (int i = 0; i < MI; ++i) {
+  // ---- base, and the stores
+  // (a row block at a time: with the loads of several in flight the compiler ran
+  // out of registers)
+  static_for<MI>([&](auto ic) {
+    constexpr int i = decltype(ic)::value;
     const int64_t row = s_row[(wm * MI + i) * 16 + fr];
     OpT* dst = reinterpret_cast<OpT*>(p.out) + row * p.out_ld;
+    f32x4_t add[NJ];
 #pragma unroll
-    for (int pr = 0; pr < NJ / 2; ++pr) {
+    for (int j = 0; j < NJ; ++j) add[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    if (p.base != nullptr && row >= 0) {
+      const int64_t at = row * p.base_ld;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int64_t n = nw + j * 16 + 4 * fq;
+        if (n + 4 <= p.n_out && p.base_vec) {
+          if (p.base_dtype == kF32) {
+            const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.base) + at + n);
+            add[j] = f32x4_t{v.x, v.y, v.z, v.w};
+          } else {
+            const uint2 raw = *reinterpret_cast<const uint2*>(reinterpret_cast<const OpT*>(p.base) + at + n);
+            const OpT* v = reinterpret_cast<const OpT*>(&raw);
+            add[j] = f32x4_t{to_f32(v[0]), to_f32(v[1]), to_f32(v[2]), to_f32(v[3])};
+          }
+        } else {
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            if (n + v < p.n_out) add[j][v] = load_as_f32(p.base, p.base_dtype, at + n + v);
+        }
+      }
+    }
+    static_for<NJ / 2>([&](auto pc) {
+      constexpr int pr = decltype(pc)::value;
       uint32_t a[2], b[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         union { uint32_t u; OpT e[2]; } pa, pb;
-        pa.e[0] = from_f32<OpT>(acc[2 * pr][i][2 * h]);
-        pa.e[1] = from_f32<OpT>(acc[2 * pr][i][2 * h + 1]);
-        pb.e[0] = from_f32<OpT>(acc[2 * pr + 1][i][2 * h]);
-        pb.e[1] = from_f32<OpT>(acc[2 * pr + 1][i][2 * h + 1]);
+        pa.e[0] = from_f32<OpT>(acc[2 * pr][i][2 * h] + add[2 * pr][2 * h]);
+        pa.e[1] = from_f32<OpT>(acc[2 * pr][i][2 * h + 1] + add[2 * pr][2 * h + 1]);
+        pb.e[0] = from_f32<OpT>(acc[2 * pr + 1][i][2 * h] + add[2 * pr + 1][2 * h]);
+        pb.e[1] = from_f32<OpT>(acc[2 * pr + 1][i][2 * h + 1] + add[2 * pr + 1][2 * h + 1]);
         a[h] = pa.u;
         b[h] = pb.u;
       }
@@ -408,15 +487,38 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
       const auto u0 = __builtin_amdgcn_permlane16_swap(s0[0], s0[1], false, false);
       const auto u1 = __builtin_amdgcn_permlane16_swap(s1[0], s1[1], false, false);
       const int64_t n = nw + pr * 32 + 8 * fq;
-      if (row < 0 || n >= p.n_out) continue;
-      const uint4 v = make_uint4(u0[0], u1[0], u0[1], u1[1]);
-      if (p.out_vec) {
-        *reinterpret_cast<uint4*>(dst + n) = v;
-      } else {
-        const OpT* e = reinterpret_cast<const OpT*>(&v);
+      if (row >= 0 && n < p.n_out) {
+        const uint4 v = make_uint4(u0[0], u1[0], u0[1], u1[1]);
+        if (p.out_vec) {
+          *reinterpret_cast<uint4*>(dst + n) = v;
+        } else {
+          const OpT* e = reinterpret_cast<const OpT*>(&v);
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
-          if (n + q < p.n_out) dst[n + q] = e[q];
+          for (int q = 0; q < 8; ++q)
+            if (n + q < p.n_out) dst[n + q] = e[q];
+        }
+      }
+    });
+    __builtin_amdgcn_sched_barrier(0);
+  });
+
+  // ---- what was left out: added to the rows it belongs to, a row at a time (its
+  // products are infinities or NaN, beside which the stored value does not count)
+  if (__any(dropped)) {
+    vm_wait<0>();  // the stores above
+    for (int i = 0; i < MI * 16; ++i) {
+      const int64_t row = s_row[wm * MI * 16 + i];
+      const int32_t a = s_id[wm * MI * 16 + i];
+      if (a < 0) continue;
+      const OpT* h = reinterpret_cast<const OpT*>(p.h) + row * p.h_ld;
+      const OpT* b = reinterpret_cast<const OpT*>(p.b) + a * p.b_se;
+      for (int64_t n = nw + lane; n < nw + NJ * 16 && n < p.n_out; n += 64) {
+        float sum = 0.f;
+        for (int32_t r = 0; r < rank; ++r) {
+          const float v = to_f32(b[r * p.b_sr + n * p.b_sn]);
+          if (!isfinite(v)) sum += to_f32(h[r]) * v;
+        }
+        if (!isfinite(sum)) reinterpret_cast<OpT*>(p.out)[row * p.out_ld + n] = from_f32<OpT>(sum);
       }
     }
   }
