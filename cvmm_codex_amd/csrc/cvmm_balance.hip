@@ -14,8 +14,8 @@
 //
 // Bound by launches and by the latency of one pass: 16384 tokens of 128 experts
 // in bf16 are 4 MB, under a microsecond of the card's bandwidth.  So two
-// launches forward (chunks of tokens, then one workgroup that adds them in a
-// fixed order) and one backward.  Terms of a token are 32-bit; a chunk's sums
+// launches forward (chunks of tokens, then their sums in a fixed order) and one
+// backward.  Terms of a token are 32-bit; a chunk's sums
 // too (at most some hundred addends per lane); sums over chunks are 64-bit.
 #include <cmath>
 
@@ -26,7 +26,18 @@
 namespace cvmm {
 
 constexpr int kBalanceThreads = 256;
-constexpr int kBalanceSumThreads = 1024;
+
+// e^x to 2 ulp: x log2 e in two parts, the second (its rounding error, and log2 e's)
+// to first order.  Below -150 it is 0 in 32 bits either way, and the parts of an
+// infinity are none; NaN stays.
+__device__ __forceinline__ float balance_exp(float x) {
+  x = x < -150.f ? -150.f : x;
+  const float t = x * 1.44269504f;
+  const float r = fmaf(x, 1.92596299e-8f, fmaf(x, 1.44269504f, -t));
+  const float e = __builtin_amdgcn_exp2f(t);
+  return fmaf(e, r * 0.693147181f, e);
+}
+constexpr int kBalanceSumThreads = 512;
 
 // The expert of a lane's slot v: runs of 8, so that a lane's slots are whole
 // 16-byte pieces of the row.
@@ -76,7 +87,7 @@ struct BalanceTerms {
       m = seg_max<LPT>(m);
 #pragma unroll
       for (int v = 0; v < MAXV; ++v) {
-        soft[v] = expf(l[v] - m);
+        soft[v] = balance_exp(l[v] - m);
         s += soft[v];
       }
       s = seg_sum<LPT>(s);
@@ -114,12 +125,25 @@ struct BalanceParams {
   double weight, z_weight;
 };
 
+// The chunks' sums, rows of ld values (experts rounded up to 4), and what the sums'
+// workgroups leave each other.
+struct BalanceParts {
+  int64_t ld;
+  int32_t eb;           // workgroups per group of tokens: 64 experts each
+  float* p;             // [chunks][ld]
+  int32_t* c;           // [chunks][ld]
+  float* z;             // [chunks]
+  int32_t* n;           // [chunks]
+  double* block_term;   // [groups * eb]
+  int32_t* group_c;     // [groups][E]
+  int32_t* arrived;
+};
+
 // One chunk: sums of p per expert, counts per expert, sum of lse^2, live tokens.
 template <typename LT, int LPT, int MAXV, bool VEC>
 __global__ __launch_bounds__(kBalanceThreads) void balance_chunk_kernel(
     const LT* __restrict__ logits, const void* __restrict__ sel, int32_t sel_is_int64, const BalanceParams p,
-    float* __restrict__ part_p, int32_t* __restrict__ part_c, float* __restrict__ part_z,
-    int32_t* __restrict__ part_n) {
+    const BalanceParts w) {
   constexpr int SEGS = kBalanceThreads / LPT, PER = LPT * MAXV;
   __shared__ float sums[SEGS * PER];
   __shared__ int32_t hist[PER];
@@ -167,12 +191,12 @@ __global__ __launch_bounds__(kBalanceThreads) void balance_chunk_kernel(
     ns[seg] = n;
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < E; e += kBalanceThreads) {
+  for (int e = threadIdx.x; e < w.ld; e += kBalanceThreads) {  // (ld <= PER)
     float s = 0.f;
 #pragma unroll 8
     for (int q = 0; q < SEGS; ++q) s += sums[q * PER + e];
-    part_p[b * E + e] = s;
-    part_c[b * E + e] = hist[e];
+    w.p[b * w.ld + e] = s;
+    w.c[b * w.ld + e] = hist[e];
   }
   if (threadIdx.x == 0) {
     float zt = 0.f;
@@ -181,120 +205,143 @@ __global__ __launch_bounds__(kBalanceThreads) void balance_chunk_kernel(
       zt += zs[q];
       nt += ns[q];
     }
-    part_z[b] = zt;
-    part_n[b] = nt;
+    w.z[b] = zt;
+    w.n[b] = nt;
+    if (b == 0) *w.arrived = 0;
   }
 }
 
-__device__ __forceinline__ double wave_sum_f64(double v) {
+// Sums of a workgroup, in a fixed tree; every thread gets them.
+template <typename T>
+__device__ __forceinline__ T block_sum(T v, T* red) {
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
-  return v;
+  __syncthreads();
+  if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = v;
+  __syncthreads();
+  T s = red[0];
+#pragma unroll
+  for (int w = 1; w < kBalanceSumThreads / 64; ++w) s += red[w];
+  return s;
 }
 
-// The chunks' sums added, in chunk order per thread and threads in a fixed tree:
-// the two terms, the counts and the coefficients of the backward pass.
+// The chunks' sums added, in a fixed order: a workgroup per group and 64 experts
+// makes the coefficients of the backward pass, its part of the balance term and its
+// counts; the last of them to end adds those, in their order.
 __global__ __launch_bounds__(kBalanceSumThreads) void balance_sum_kernel(
-    const BalanceParams p, int32_t groups, const float* __restrict__ part_p, const int32_t* __restrict__ part_c,
-    const float* __restrict__ part_z, const int32_t* __restrict__ part_n, float* __restrict__ loss,
-    float* __restrict__ terms, int64_t* __restrict__ counts, float* __restrict__ coef) {
-  __shared__ int32_t n_of[kBalanceMaxGroups];  // live tokens of each group
-  __shared__ int32_t c_of[kRouteMaxExperts];   // routes of each expert
-  __shared__ double red_p[kBalanceSumThreads];
-  __shared__ int32_t red_c[kBalanceSumThreads];
-  __shared__ double wave_b[kBalanceSumThreads / 64], wave_z[kBalanceSumThreads / 64];
-  __shared__ int32_t n_total, n_groups;
+    const BalanceParams p, int32_t groups, const BalanceParts w, float* __restrict__ loss, float* __restrict__ terms,
+    int64_t* __restrict__ counts, float* __restrict__ coef) {
+  constexpr int SLOTS = kBalanceSumThreads / 16;  // chunks at a time, four experts a thread
+  __shared__ int32_t n_of[kBalanceMaxGroups];     // live tokens of each group
+  __shared__ double s_p[SLOTS][64];
+  __shared__ int32_t s_c[SLOTS][64];
+  __shared__ double red_d[kBalanceSumThreads / 64];
+  __shared__ int32_t red_i[kBalanceSumThreads / 64];
+  __shared__ bool last;
   const int tid = threadIdx.x;
-  const int32_t E = p.E;
+  const int32_t E = p.E, blocks = (int32_t)gridDim.x;
+  const int32_t g = (int32_t)(blockIdx.x / (uint32_t)w.eb), e0 = (int32_t)(blockIdx.x % (uint32_t)w.eb) * 64;
+  // this group's chunks
+  {
+    const int q = tid % 16, slot = tid / 16;
+    double P[4] = {0.0, 0.0, 0.0, 0.0};
+    int32_t c[4] = {0, 0, 0, 0};
+    if (e0 + 4 * q < w.ld) {
+      const int64_t at = (int64_t)g * p.per_group;
+#pragma unroll 4
+      for (int64_t i = slot; i < p.per_group; i += SLOTS) {
+        const float4 v = *reinterpret_cast<const float4*>(w.p + (at + i) * w.ld + e0 + 4 * q);
+        const int4 u = *reinterpret_cast<const int4*>(w.c + (at + i) * w.ld + e0 + 4 * q);
+        P[0] += (double)v.x, P[1] += (double)v.y, P[2] += (double)v.z, P[3] += (double)v.w;
+        c[0] += u.x, c[1] += u.y, c[2] += u.z, c[3] += u.w;
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      s_p[slot][4 * q + v] = P[v];
+      s_c[slot][4 * q + v] = c[v];
+    }
+  }
+  // live tokens, of all groups
   for (int i = tid; i < groups; i += kBalanceSumThreads) n_of[i] = 0;
-  for (int i = tid; i < E; i += kBalanceSumThreads) c_of[i] = 0;
-  if (tid == 0) n_total = n_groups = 0;
   __syncthreads();
   const int64_t chunks = (int64_t)groups * p.per_group;
   double z = 0.0;
-  for (int64_t c = tid; c < chunks; c += kBalanceSumThreads) {
-    z += (double)part_z[c];
-    atomicAdd(&n_of[c / p.per_group], part_n[c]);
+  for (int64_t i = tid; i < chunks; i += kBalanceSumThreads) {
+    atomicAdd(&n_of[i / p.per_group], w.n[i]);
+    z += (double)w.z[i];
   }
   __syncthreads();
-  for (int i = tid; i < groups; i += kBalanceSumThreads)
-    if (n_of[i] > 0) {
-      atomicAdd(&n_total, n_of[i]);
-      atomicAdd(&n_groups, 1);
-    }
-  __syncthreads();
-  // pairs (group, expert), each by `splits` threads
-  const int64_t pairs = (int64_t)groups * E;
-  int splits = 1;
-  while (splits < kBalanceSumThreads && pairs * splits * 2 <= kBalanceSumThreads) splits *= 2;
-  const int per_pass = kBalanceSumThreads / splits, s = tid / per_pass;
-  double total = 0.0;
-  for (int64_t base = 0; base < pairs; base += per_pass) {
-    const int64_t pair = base + tid % per_pass;
-    const bool in = pair < pairs;
-    const int32_t g = in ? (int32_t)(pair / E) : 0, e = in ? (int32_t)(pair - (int64_t)g * E) : 0;
-    double P = 0.0;
+  int32_t n_all = 0, n_live = 0;
+  for (int i = tid; i < groups; i += kBalanceSumThreads) {
+    n_all += n_of[i];
+    n_live += n_of[i] > 0 ? 1 : 0;
+  }
+  n_all = block_sum(n_all, red_i);
+  n_live = block_sum(n_live, red_i);
+  double term = 0.0;
+  if (tid < 64 && e0 + tid < E) {
+    double P = 0.0, a = 0.0;
     int32_t c = 0;
-    if (in) {
-      const int64_t at = (int64_t)g * p.per_group;
 #pragma unroll 8
-      for (int64_t i = s; i < p.per_group; i += splits) {
-        P += (double)part_p[(at + i) * E + e];
-        c += part_c[(at + i) * E + e];
-      }
+    for (int i = 0; i < SLOTS; ++i) {
+      P += s_p[i][tid];
+      c += s_c[i][tid];
     }
-    if (splits > 1) {
-      __syncthreads();
-      red_p[tid] = P;
-      red_c[tid] = c;
-      __syncthreads();
-      if (s == 0)
-        for (int q = 1; q < splits; ++q) {
-          P += red_p[q * per_pass + tid];
-          c += red_c[q * per_pass + tid];
-        }
-    }
-    if (s != 0 || !in) continue;
-    atomicAdd(&c_of[e], c);
-    double a = 0.0;
     if (n_of[g] > 0) {
-      const double n = (double)n_of[g], each = 1.0 / (double)n_groups;
+      const double n = (double)n_of[g], each = 1.0 / (double)n_live;
       P /= n;
       if (p.entropy) {
         // P = 0: every p is 0 there, and so is its part of the gradient
         const double lg = P == 0.0 ? 0.0 : log(P);
-        total += P * lg * each;
+        term = P * lg * each;
         a = P == 0.0 ? 0.0 : (lg + 1.0) * each / n;
       } else {
         const double f = (double)E * (double)c / ((double)p.k * n);
-        total += f * P * each;
+        term = f * P * each;
         a = f * each / n;
       }
     }
-    coef[pair] = (float)(p.weight * a);
+    coef[(int64_t)g * E + e0 + tid] = (float)(p.weight * a);
+    __hip_atomic_store(&w.group_c[(int64_t)g * E + e0 + tid], c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  total = wave_sum_f64(total);
-  z = wave_sum_f64(z);
-  if (tid % 64 == 0) {
-    wave_b[tid / 64] = total;
-    wave_z[tid / 64] = z;
-  }
+  term = block_sum(term, red_d);
+  if (tid == 0) __hip_atomic_store(&w.block_term[blockIdx.x], term, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  splitk_published();
   __syncthreads();
-  for (int e = tid; e < E; e += kBalanceSumThreads) counts[e] = c_of[e];
-  if (tid == 0) {
-    double bt = 0.0, zt = 0.0;
-    for (int w = 0; w < kBalanceSumThreads / 64; ++w) {
-      bt += wave_b[w];
-      zt += wave_z[w];
-    }
-    const double inv = n_total > 0 ? 1.0 / (double)n_total : 0.0;
-    zt *= inv;
-    terms[0] = (float)bt;
-    terms[1] = (float)zt;
-    // (a term of weight 0 does not pass its NaN or infinity on)
-    loss[0] = (float)((p.weight != 0.0 ? p.weight * bt : 0.0) + (p.z_weight != 0.0 ? p.z_weight * zt : 0.0));
-    coef[pairs] = (float)(2.0 * p.z_weight * inv);
+  if (tid == 0) last = splitk_arrive(w.arrived, blocks);
+  __syncthreads();
+  if (!last) return;
+  splitk_acquired();
+  double total = 0.0;
+  for (int i = tid; i < blocks; i += kBalanceSumThreads)
+    total += __hip_atomic_load(&w.block_term[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  total = block_sum(total, red_d);
+  z = block_sum(z, red_d);
+  for (int e = tid; e < E; e += kBalanceSumThreads) {
+    int64_t c = 0;
+#pragma unroll 4
+    for (int i = 0; i < groups; ++i)
+      c += __hip_atomic_load(&w.group_c[(int64_t)i * E + e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    counts[e] = c;
   }
+  if (tid == 0) {
+    const double inv = n_all > 0 ? 1.0 / (double)n_all : 0.0;
+    z *= inv;
+    terms[0] = (float)total;
+    terms[1] = (float)z;
+    // (a term of weight 0 does not pass its NaN or infinity on)
+    loss[0] = (float)((p.weight != 0.0 ? p.weight * total : 0.0) + (p.z_weight != 0.0 ? p.z_weight * z : 0.0));
+    coef[(int64_t)groups * E] = (float)(2.0 * p.z_weight * inv);
+  }
+}
+
+// No tokens: zeros.
+__global__ __launch_bounds__(256) void balance_none_kernel(int32_t E, float* __restrict__ loss,
+                                                           float* __restrict__ terms, int64_t* __restrict__ counts,
+                                                           float* __restrict__ coef) {
+  for (int e = threadIdx.x; e < E; e += 256) counts[e] = 0;
+  if (threadIdx.x == 0) loss[0] = terms[0] = terms[1] = coef[0] = 0.f;
 }
 
 template <typename LT, int LPT, int MAXV, bool VEC>
@@ -372,10 +419,34 @@ static int64_t balance_chunks(int64_t n_tokens, int64_t group_tokens, int32_t n_
   return (group_tokens + *tpc - 1) / *tpc;
 }
 
+static BalanceParts balance_parts(void* ws, int64_t chunks, int64_t groups, int32_t n_experts, size_t* bytes) {
+  BalanceParts w{};
+  w.ld = (n_experts + 3) / 4 * 4;
+  w.eb = (n_experts + 63) / 64;
+  size_t used = 0;
+  auto take = [&](size_t n) {
+    void* q = ws != nullptr ? (char*)ws + used : nullptr;
+    used = align_up(used + n, 16);
+    return q;
+  };
+  w.block_term = (double*)take((size_t)groups * (size_t)w.eb * 8);
+  w.p = (float*)take((size_t)chunks * (size_t)w.ld * 4);
+  w.c = (int32_t*)take((size_t)chunks * (size_t)w.ld * 4);
+  w.z = (float*)take((size_t)chunks * 4);
+  w.n = (int32_t*)take((size_t)chunks * 4);
+  w.group_c = (int32_t*)take((size_t)groups * (size_t)n_experts * 4);
+  w.arrived = (int32_t*)take(4);
+  *bytes = used;
+  return w;
+}
+
 size_t balance_workspace_bytes(int64_t n_tokens, int64_t group_tokens, int32_t n_experts) {
+  if (n_tokens == 0) return 0;
   int64_t tpc;
-  const int64_t chunks = balance_chunks(n_tokens, group_tokens, n_experts, &tpc) * (n_tokens / group_tokens);
-  return (size_t)chunks * ((size_t)n_experts + 1) * 8;
+  const int64_t groups = n_tokens / group_tokens;
+  size_t bytes;
+  balance_parts(nullptr, balance_chunks(n_tokens, group_tokens, n_experts, &tpc) * groups, groups, n_experts, &bytes);
+  return bytes;
 }
 
 static bool balance_vec(const void* logits, int64_t ld, int32_t E) {
@@ -392,18 +463,20 @@ hipError_t launch_balance_loss(const void* logits, int32_t dtype, int64_t n_toke
   const int32_t groups = (int32_t)(n_tokens / group_tokens);
   const int64_t chunks = p.per_group * groups;
   if (chunks > 0x7fffffffll) return hipErrorInvalidValue;
-  float* part_p = (float*)workspace;
-  int32_t* part_c = (int32_t*)(part_p + chunks * n_experts);
-  float* part_z = (float*)(part_c + chunks * n_experts);
-  int32_t* part_n = (int32_t*)(part_z + chunks);
+  if (chunks == 0) {
+    hipLaunchKernelGGL(balance_none_kernel, dim3(1), dim3(256), 0, stream, n_experts, loss, terms, counts, coef);
+    return hipGetLastError();
+  }
+  size_t bytes;
+  const BalanceParts w = balance_parts(workspace, chunks, groups, n_experts, &bytes);
   const bool vec = balance_vec(logits, ld, n_experts);
-  if (chunks > 0) by_dtype(dtype, [&](auto lt) {
+  by_dtype(dtype, [&](auto lt) {
     using LT = decltype(lt);
     by_experts(n_experts, [&](auto lpt, auto maxv) {
       constexpr int LPT = decltype(lpt)::value, MAXV = decltype(maxv)::value;
       auto go = [&](auto kern) {
         hipLaunchKernelGGL(kern, dim3((unsigned)chunks), dim3(kBalanceThreads), 0, stream, (const LT*)logits, sel,
-                           sel_is_int64, p, part_p, part_c, part_z, part_n);
+                           sel_is_int64, p, w);
       };
       if (vec) go(balance_chunk_kernel<LT, LPT, MAXV, true>);
       else go(balance_chunk_kernel<LT, LPT, MAXV, false>);
@@ -411,8 +484,8 @@ hipError_t launch_balance_loss(const void* logits, int32_t dtype, int64_t n_toke
   });
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(balance_sum_kernel, dim3(1), dim3(kBalanceSumThreads), 0, stream, p, groups, part_p, part_c,
-                     part_z, part_n, loss, terms, counts, coef);
+  hipLaunchKernelGGL(balance_sum_kernel, dim3((unsigned)(groups * w.eb)), dim3(kBalanceSumThreads), 0, stream, p,
+                     groups, w, loss, terms, counts, coef);
   return hipGetLastError();
 }
 

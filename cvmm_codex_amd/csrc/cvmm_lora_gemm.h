@@ -152,6 +152,8 @@ struct LoraTile {
   static constexpr int A_BYTES = BM * 64, SLICE = (BM + BN) * 64, STAGES = 4;
   static constexpr int OCC = MI * NJ > 16 ? 1 : 2;
   static constexpr bool AGPR = MI * NJ == 64;
+  static constexpr bool MIXED = A_INSTS % D != 0;  // a wave loads pieces of x and of W
+  static_assert(2 * SLICE <= 65536, "offsets of an LDS instruction");
 };
 
 // Lane offset of load `inst` of a slice's B half, and the k that its piece starts
@@ -239,29 +241,37 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
   auto issue_one = [&](auto jc, __amdgpu_buffer_rsrc_t rsa, __amdgpu_buffer_rsrc_t rsb, uint32_t o, uint32_t sa,
                        uint32_t sb, char* dst) {
     constexpr int J = decltype(jc)::value;
-    const bool is_a = wave * D + J < T::A_INSTS;
+    const bool is_a = wave * D + (T::MIXED ? J : 0) < T::A_INSTS;
     buf_dma<16, (J & 3) * 1024>(is_a ? rsa : rsb, o, is_a ? sa : sb, dst + (wave * D + (J & ~3)) * 1024);
   };
-  int32_t i_k = 0;       // k of the slice to be issued, and its offsets
+  int32_t i_k = 0;  // k of the slice to be issued, and its offsets
   uint32_t i_a = 0, i_b = 0;
-  auto issue_part = [&](auto jc, char* dst) {
-    constexpr int J = decltype(jc)::value;
-    const int g = wave * D + J;
-    const int k = i_k + (g < T::A_INSTS ? a_k : lora_b_k<WKC, BN>(g - T::A_INSTS, lane));
-    issue_one(jc, ra, rw, k < kw ? off[J] : kLoraOob, i_a, i_b, dst);
+  auto issue_part = [&](auto jc, char* dst) { issue_one(jc, ra, rw, off[decltype(jc)::value], i_a, i_b, dst); };
+  // before a slice is issued that k ends in, or past: its pieces from there on read zeros
+  auto issue_mask = [&]() {
+    if (i_k + 32 <= kw) return;
+    static_for<D>([&](auto jc) {
+      constexpr int J = decltype(jc)::value;
+      const int g = wave * D + J;
+      if (i_k + (g < T::A_INSTS ? a_k : lora_b_k<WKC, BN>(g - T::A_INSTS, lane)) >= kw) off[J] = kLoraOob;
+    });
   };
   auto issue_next = [&]() {
     i_k += 32;
     i_a += 64;
     i_b += b_step;
     if (i_k >= kw) i_a = i_b = 0;  // (only offsets past the range from here on)
+    issue_mask();
   };
+  issue_mask();
 
-  // ---- fragments
+  // ---- fragments: buffers 2 and 3 from a base of their own, the rest of the
+  // address in the instruction
+  constexpr int kHalf = 2 * SLICE;
   const uint32_t st0 = lds_addr(ring);
   const uint32_t a_f = st0 + (uint32_t)((wm * MI * 16 + fr) * 64 + ((fq ^ ((fr >> 1) & 3)) << 4));
-  uint32_t kc_f, tr_f[NJ];
-  kc_f = st0 + T::A_BYTES + (uint32_t)((wn * NJ * 16 + fr) * 64 + ((fq ^ ((fr >> 1) & 3)) << 4));
+  const uint32_t kc_f = st0 + T::A_BYTES + (uint32_t)((wn * NJ * 16 + fr) * 64 + ((fq ^ ((fr >> 1) & 3)) << 4));
+  uint32_t tr_f[NJ];
   {
     constexpr int CPR = BN / 8;
     const int r = fq * 8 + (fr >> 2);
@@ -270,18 +280,23 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
     for (int i = 0; i < NJ; ++i)
       tr_f[i] = st0 + T::A_BYTES + (uint32_t)(r * BN * 2 + lo + (((wn * NJ * 2 + 2 * i) ^ tr_row_swz<CPR>(r)) << 4));
   }
-  auto read_a = [&](uint32_t at, lds_u32x4 (&f)[MI]) {
-    static_for<MI>([&](auto i) { f[i] = lds_read128_at<decltype(i)::value * 1024>(a_f + at); });
+  auto read_a = [&](auto buf, lds_u32x4 (&f)[MI]) {
+    constexpr int B = decltype(buf)::value;
+    const uint32_t at = a_f + (B >= 2 ? kHalf : 0);
+    static_for<MI>([&](auto i) { f[i] = lds_read128_at<(B & 1) * SLICE + decltype(i)::value * 1024>(at); });
   };
-  auto read_b = [&](uint32_t at, auto& f) {
+  auto read_b = [&](auto buf, auto& f) {
+    constexpr int B = decltype(buf)::value;
     if constexpr (std::is_same_v<std::remove_reference_t<decltype(f)>, lds_u32x4[NJ]>) {
-      static_for<NJ>([&](auto i) { f[i] = lds_read128_at<decltype(i)::value * 1024>(kc_f + at); });
+      const uint32_t at = kc_f + (B >= 2 ? kHalf : 0);
+      static_for<NJ>([&](auto i) { f[i] = lds_read128_at<(B & 1) * SLICE + decltype(i)::value * 1024>(at); });
     } else {
-#pragma unroll
-      for (int i = 0; i < NJ; ++i) {
-        f[i][0] = lds_read_tr<0>(tr_f[i] + at);
-        f[i][1] = lds_read_tr<4 * BN * 2>(tr_f[i] + at);
-      }
+      static_for<NJ>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        const uint32_t at = tr_f[i] + (B >= 2 ? kHalf : 0);
+        f[i][0] = lds_read_tr<(B & 1) * SLICE>(at);
+        f[i][1] = lds_read_tr<(B & 1) * SLICE + 4 * BN * 2>(at);
+      });
     }
   };
 
@@ -307,21 +322,20 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
     WFrag b0, b1;
     vm_wait<3 * D>();
     lds_barrier();
-    read_a(0, a0);
-    read_b(0, b0);
+    read_a(std::integral_constant<int, 0>(), a0);
+    read_b(std::integral_constant<int, 0>(), b0);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     lora_wait(a0);
     lora_wait(b0);
-    int buf = 0;
-    // slice s is in (ca, cb): slice s + 1 is read into (na, nb), slice s + 4
-    // issued into the buffer of s, which every wave has read
-    auto step = [&](lds_u32x4 (&ca)[MI], WFrag& cb, lds_u32x4 (&na)[MI], WFrag& nb) {
-      const int nbuf = (buf + 1) & 3;
+    // slice s, in buffer B, is in (ca, cb): slice s + 1 is read into (na, nb), slice
+    // s + 4 issued into the buffer of s, which every wave has read
+    auto step = [&](auto bc, lds_u32x4 (&ca)[MI], WFrag& cb, lds_u32x4 (&na)[MI], WFrag& nb) {
+      constexpr int B = decltype(bc)::value;
       vm_wait<2 * D>();
       lds_barrier();
-      char* dst = ring + buf * SLICE;
-      read_a((uint32_t)nbuf * SLICE, na);
-      read_b((uint32_t)nbuf * SLICE, nb);
+      char* dst = ring + B * SLICE;
+      read_a(std::integral_constant<int, (B + 1) & 3>(), na);
+      read_b(std::integral_constant<int, (B + 1) & 3>(), nb);
       static_for<NJ>([&](auto jb) {
         constexpr int JB = decltype(jb)::value;
         lora_mfma_col<OpT, T::AGPR>(acc[JB], lora_frag(cb[JB]), ca);
@@ -334,12 +348,13 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       lora_wait(na);
       lora_wait(nb);
-      buf = nbuf;
     };
-    // in pairs; an odd count gets a slice of zeros
-    for (int32_t s = 0; s < S; s += 2) {
-      step(a0, b0, a1, b1);
-      step(a1, b1, a0, b0);
+    // (four at a time, zeros past the last: leaving within them made the compiler spill)
+    for (int32_t s = 0; s < S; s += 4) {
+      step(std::integral_constant<int, 0>(), a0, b0, a1, b1);
+      step(std::integral_constant<int, 1>(), a1, b1, a0, b0);
+      step(std::integral_constant<int, 2>(), a0, b0, a1, b1);
+      step(std::integral_constant<int, 3>(), a1, b1, a0, b0);
     }
     vm_wait<0>();
     if constexpr (T::AGPR) lora_mfma_done(acc);
@@ -415,11 +430,12 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
       }
       vm_wait<0>();
       lds_barrier();
-      for (int s = 0; s < 4 && r0 + s * 32 < rank; ++s) {
+      static_for<4>([&](auto sc) {
+        if (r0 + decltype(sc)::value * 32 >= rank) return;
         lds_u32x4 af[MI];
         BFrag bf;
-        read_a((uint32_t)s * SLICE, af);
-        read_b((uint32_t)s * SLICE, bf);
+        read_a(sc, af);
+        read_b(sc, bf);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         lora_wait(af);
         lora_wait(bf);
@@ -434,7 +450,7 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
           lora_mfma_col<OpT, T::AGPR>(acc[j], lora_frag(bf[j]), af);
         });
         if constexpr (T::AGPR) lora_mfma_done(acc);
-      }
+      });
     }
   }
 
@@ -560,11 +576,11 @@ hipError_t launch_lora_inner_op(const LoraParams& p, hipStream_t s) {
   const bool akc = p.a_sr != 1;
   auto go = [&](auto rb, auto kw) {
     constexpr int RB = decltype(rb)::value, KW = decltype(kw)::value;
-    const int64_t wg = (p.rows + (KW == 1 ? 63 : 15)) / (KW == 1 ? 64 : 16);
+    const dim3 grid((unsigned)((p.rows + (KW == 1 ? 63 : 15)) / (KW == 1 ? 64 : 16)), kLoraInnerTurns);
     if (akc)
-      hipLaunchKernelGGL((lora_inner_tile_kernel<OpT, RB, KW, true>), dim3((unsigned)wg), dim3(256), 0, s, p);
+      hipLaunchKernelGGL((lora_inner_tile_kernel<OpT, RB, KW, true>), grid, dim3(256), 0, s, p);
     else
-      hipLaunchKernelGGL((lora_inner_tile_kernel<OpT, RB, KW, false>), dim3((unsigned)wg), dim3(256), 0, s, p);
+      hipLaunchKernelGGL((lora_inner_tile_kernel<OpT, RB, KW, false>), grid, dim3(256), 0, s, p);
   };
   auto by_rank = [&](auto kw) {
     using std::integral_constant;

@@ -32,10 +32,15 @@ __device__ __forceinline__ void lora_transpose8(const uint4 (&r)[8], uint4 (&c)[
 // [k][rank].  Bound by reading x once; each workgroup reads its adapters whole,
 // from L2.
 // ---------------------------------------------------------------------------
+// Workgroups that share the adapters of a tile, in turns: nearly all tiles have one
+// or two (a request ends within), and a second one, taken after the first, doubled
+// the launch (16384 rows of 2048, rank 64: 43 us).
+constexpr int kLoraInnerTurns = 4;
+
 template <int RB, int KW>
 struct LoraInnerCfg {
   // k per LDS stage; 4 waves of 16 rows: each all of it, else a quarter each
-  static constexpr int KS = RB >= 8 ? 128 : 256;
+  static constexpr int KS = RB >= 16 ? 128 : KW > 1 && RB <= 4 ? 512 : 256;
   static constexpr int KWAVE = KS / KW;        // k per wave and stage
   static constexpr int LDB = KS * 2 + 16;      // bytes per LDS row
   static constexpr int CHUNKS = RB * 16 * (KS / 8);  // 16-byte pieces of a stage
@@ -72,16 +77,20 @@ __global__ __launch_bounds__(256) void lora_inner_tile_kernel(const LoraParams p
   f32x4_t res[RB];  // res[b]: rank 16 b + 4 fq + {0..3} of row `my`
 #pragma unroll
   for (int b = 0; b < RB; ++b) res[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  bool made = my_id < 0 && blockIdx.y == 0;  // the row is this workgroup's to write
+  int turn = 0;
   for (int32_t cur = -1;;) {
     int32_t a = lane < ROWS ? s_id[lane % ROWS] : -1;
     a = wave_min_i32(a > cur ? a : INT32_MAX);
     if (a == INT32_MAX) break;
     cur = a;
+    if (turn++ % kLoraInnerTurns != (int)blockIdx.y) continue;
     const bool mine = my_id == a;
+    made |= mine;
     const bool any = KW > 1 || __ballot(mine) != 0;  // a wave without rows of it still stages A
     const OpT* am = reinterpret_cast<const OpT*>(p.a) + a * p.a_se;
-    uint4 xv[XS], av[C::PER][8];
-    auto load_x = [&](int32_t k0) {
+    uint4 x0[XS], x1[XS], av[C::PER][8];
+    auto load_x = [&](int32_t k0, uint4 (&xv)[XS]) {
 #pragma unroll
       for (int s = 0; s < XS; ++s) {
         const int32_t k = k0 + k_wave + s * 32 + fq * 8;
@@ -124,19 +133,17 @@ __global__ __launch_bounds__(256) void lora_inner_tile_kernel(const LoraParams p
     f32x4_t acc[RB];
 #pragma unroll
     for (int b = 0; b < RB; ++b) acc[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    load_a(0);
-    load_x(0);
-    for (int32_t k0 = 0; k0 < K; k0 += C::KS) {
+    // a stage: A's values, loaded one stage ahead, go to LDS; x is two ahead
+    auto stage = [&](int32_t k0, uint4 (&xv)[XS]) {
+      if (k0 >= K) return;
       __syncthreads();  // the last stage's reads
       store_a();
       uint4 xc[XS];
 #pragma unroll
       for (int s = 0; s < XS; ++s) xc[s] = xv[s];
       __syncthreads();
-      if (k0 + C::KS < K) {
-        load_a(k0 + C::KS);
-        load_x(k0 + C::KS);
-      }
+      if (k0 + C::KS < K) load_a(k0 + C::KS);
+      if (k0 + 2 * C::KS < K) load_x(k0 + 2 * C::KS, xv);
       if (any) {
 #pragma unroll
         for (int s = 0; s < XS; ++s)
@@ -147,6 +154,13 @@ __global__ __launch_bounds__(256) void lora_inner_tile_kernel(const LoraParams p
             MfmaOp<OpT>::step(acc[b], w, xc[s]);
           }
       }
+    };
+    load_a(0);
+    load_x(0, x0);
+    load_x(C::KS, x1);
+    for (int32_t k0 = 0; k0 < K; k0 += 2 * C::KS) {
+      stage(k0, x0);
+      stage(k0 + C::KS, x1);
     }
     if constexpr (KW > 1) {
       // the waves' sums, added in wave order by the first
@@ -170,7 +184,7 @@ __global__ __launch_bounds__(256) void lora_inner_tile_kernel(const LoraParams p
       for (int b = 0; b < RB; ++b) res[b] = sc * acc[b];
     }
   }
-  if (KW > 1 && wave != 0) return;
+  if (!made || (KW > 1 && wave != 0)) return;
   OpT* h = reinterpret_cast<OpT*>(p.h);
   OpT* ht = reinterpret_cast<OpT*>(p.ht);
 #pragma unroll
