@@ -89,47 +89,37 @@ __device__ __forceinline__ void lora_finite(lds_u32x2 (&f)[N][2], bool& dropped)
     for (int q = 0; q < 4; ++q) f[i][q / 2][q % 2] = lora_finite_pair<OpT>(f[i][q / 2][q % 2], dropped);
 }
 
-// c[i] += w x_i^T: the row blocks of one column block.  AGPR (eight of them): in
-// accumulation registers by name, as one block of instructions.  Of 256 accumulators
-// the compiler moved 200 to other registers and back in every slice, as many
-// instructions as the matrix unit leaves room for.  The compiler does not see matrix
-// instructions here: the block starts with the two wait states that they need after
-// a vector instruction wrote their operands, and lora_mfma_done comes before c is read.
-template <typename OpT, bool AGPR, int MI>
-__device__ __forceinline__ void lora_mfma_col(f32x4_t (&c)[MI], const uint4& w, const lds_u32x4 (&x)[MI]) {
+// c += w x^T.  AGPR: in accumulation registers by name.  Of 256 accumulators the
+// compiler moved 200 to other registers and back in every slice, as many
+// instructions as the matrix unit leaves room for.  It does not see a matrix
+// instruction here: lora_mfma_ready comes before the first of a slice, whose operands
+// vector instructions may have written (two wait states), and lora_mfma_done before
+// an accumulator is read.
+template <typename OpT, bool AGPR>
+__device__ __forceinline__ void lora_mfma_one(f32x4_t& c, const uint4& w, const lds_u32x4& x) {
   if constexpr (!AGPR) {
-#pragma unroll
-    for (int i = 0; i < MI; ++i) MfmaOp<OpT>::step(c[i], w, make_uint4(x[i].x, x[i].y, x[i].z, x[i].w));
+    MfmaOp<OpT>::step(c, w, make_uint4(x.x, x.y, x.z, x.w));
   } else {
-    static_assert(MI == 8, "eight row blocks");
     const lds_u32x4 a{w.x, w.y, w.z, w.w};
-    if constexpr (DTypeOf<OpT>::value == kBF16) {
-      asm("s_nop 1\n\t"
-                   "v_mfma_f32_16x16x32_bf16 %0, %8, %9, %0\n\t"
-                   "v_mfma_f32_16x16x32_bf16 %1, %8, %10, %1\n\t"
-                   "v_mfma_f32_16x16x32_bf16 %2, %8, %11, %2\n\t"
-                   "v_mfma_f32_16x16x32_bf16 %3, %8, %12, %3\n\t"
-                   "v_mfma_f32_16x16x32_bf16 %4, %8, %13, %4\n\t"
-                   "v_mfma_f32_16x16x32_bf16 %5, %8, %14, %5\n\t"
-                   "v_mfma_f32_16x16x32_bf16 %6, %8, %15, %6\n\t"
-                   "v_mfma_f32_16x16x32_bf16 %7, %8, %16, %7"
-                   : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]), "+a"(c[4]), "+a"(c[5]), "+a"(c[6]), "+a"(c[7])
-                   : "v"(a), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]), "v"(x[5]), "v"(x[6]), "v"(x[7]));
-    } else {
-      asm("s_nop 1\n\t"
-                   "v_mfma_f32_16x16x32_f16 %0, %8, %9, %0\n\t"
-                   "v_mfma_f32_16x16x32_f16 %1, %8, %10, %1\n\t"
-                   "v_mfma_f32_16x16x32_f16 %2, %8, %11, %2\n\t"
-                   "v_mfma_f32_16x16x32_f16 %3, %8, %12, %3\n\t"
-                   "v_mfma_f32_16x16x32_f16 %4, %8, %13, %4\n\t"
-                   "v_mfma_f32_16x16x32_f16 %5, %8, %14, %5\n\t"
-                   "v_mfma_f32_16x16x32_f16 %6, %8, %15, %6\n\t"
-                   "v_mfma_f32_16x16x32_f16 %7, %8, %16, %7"
-                   : "+a"(c[0]), "+a"(c[1]), "+a"(c[2]), "+a"(c[3]), "+a"(c[4]), "+a"(c[5]), "+a"(c[6]), "+a"(c[7])
-                   : "v"(a), "v"(x[0]), "v"(x[1]), "v"(x[2]), "v"(x[3]), "v"(x[4]), "v"(x[5]), "v"(x[6]), "v"(x[7]));
-    }
+    if constexpr (DTypeOf<OpT>::value == kBF16)
+      asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(x));
+    else
+      asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(x));
   }
 }
+// Operands that vector instructions made, in their registers from here on.
+template <int N, int M>
+__device__ __forceinline__ void lora_operands(uint4 (&w)[N], lds_u32x4 (&x)[M]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    lds_u32x4 v{w[i].x, w[i].y, w[i].z, w[i].w};
+    asm volatile("" : "+v"(v));
+    w[i] = make_uint4(v.x, v.y, v.z, v.w);
+  }
+#pragma unroll
+  for (int i = 0; i < M; ++i) asm volatile("" : "+v"(x[i]));
+}
+__device__ __forceinline__ void lora_mfma_ready() { asm volatile("s_nop 1" ::: "memory"); }
 // After the last of them: more wait states than the last result needs before a
 // vector instruction reads it, and every accumulator handed on, so that no read of
 // one comes earlier.
@@ -244,6 +234,7 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
     const bool is_a = wave * D + (T::MIXED ? J : 0) < T::A_INSTS;
     buf_dma<16, (J & 3) * 1024>(is_a ? rsa : rsb, o, is_a ? sa : sb, dst + (wave * D + (J & ~3)) * 1024);
   };
+  const int32_t S = (kw + 31) / 32;
   int32_t i_k = 0;  // k of the slice to be issued, and its offsets
   uint32_t i_a = 0, i_b = 0;
   auto issue_part = [&](auto jc, char* dst) { issue_one(jc, ra, rw, off[decltype(jc)::value], i_a, i_b, dst); };
@@ -300,6 +291,20 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
     }
   };
 
+  // the R-th of a slice's reads: x's, then W's
+  auto read_one = [&](auto buf, auto rc, lds_u32x4 (&fa)[MI], auto& fb) {
+    constexpr int B = decltype(buf)::value, R = decltype(rc)::value, OFF = (B & 1) * SLICE;
+    constexpr uint32_t hi = B >= 2 ? kHalf : 0;
+    if constexpr (R < MI) {
+      fa[R] = lds_read128_at<OFF + R * 1024>(a_f + hi);
+    } else if constexpr (std::is_same_v<std::remove_reference_t<decltype(fb)>, lds_u32x4[NJ]>) {
+      fb[R - MI] = lds_read128_at<OFF + (R - MI) * 1024>(kc_f + hi);
+    } else {
+      constexpr int i = (R - MI) / 2, h = (R - MI) % 2;
+      fb[i][h] = lds_read_tr<OFF + h * 4 * BN * 2>(tr_f[i] + hi);
+    }
+  };
+
   // ---- accumulators: acc[j][i] holds columns 16 j + 4 fq + {0..3} of row 16 i + fr
   f32x4_t acc[NJ][MI];
   const int64_t nw = n0 + wn * NJ * 16;
@@ -310,7 +315,6 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
 
   // ---- the shared weights
   using WFrag = std::conditional_t<WKC, lds_u32x4[NJ], lds_u32x2[NJ][2]>;
-  const int32_t S = (kw + 31) / 32;
   if (S > 0) {
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
@@ -334,13 +338,18 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
       vm_wait<2 * D>();
       lds_barrier();
       char* dst = ring + B * SLICE;
-      read_a(std::integral_constant<int, (B + 1) & 3>(), na);
-      read_b(std::integral_constant<int, (B + 1) & 3>(), nb);
-      static_for<NJ>([&](auto jb) {
-        constexpr int JB = decltype(jb)::value;
-        lora_mfma_col<OpT, T::AGPR>(acc[JB], lora_frag(cb[JB]), ca);
+      // between the products, a read or a load each: the matrix unit is busy for 16
+      // cycles with each, in which up to three others issue
+      constexpr int P = MI * NJ, R = MI + (WKC ? NJ : 2 * NJ);
+      lora_mfma_ready();
+      static_for<P>([&](auto tc) {
+        constexpr int t = decltype(tc)::value, jb = t / MI, i = t % MI;
+        lora_mfma_one<OpT, T::AGPR>(acc[jb][i], lora_frag(cb[jb]), ca[i]);
+        static_for<R>([&](auto rc) {
+          if constexpr (decltype(rc)::value * (P - P / 4) / R == t) read_one(std::integral_constant<int, (B + 1) & 3>(), rc, na, nb);
+        });
         static_for<D>([&](auto j) {
-          if constexpr (decltype(j)::value * NJ / D == JB) issue_part(j, dst);
+          if constexpr (decltype(j)::value * P / D + 1 == t) issue_part(j, dst);
         });
         __builtin_amdgcn_sched_barrier(0);
       });
@@ -445,9 +454,14 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
             if (ids[i] != a) af[i] = lds_u32x4{0u, 0u, 0u, 0u};
           lora_finite<OpT>(bf, dropped);
         }
-        static_for<NJ>([&](auto jc) {
-          constexpr int j = decltype(jc)::value;
-          lora_mfma_col<OpT, T::AGPR>(acc[j], lora_frag(bf[j]), af);
+        uint4 w[NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) w[j] = lora_frag(bf[j]);
+        lora_operands(w, af);
+        lora_mfma_ready();
+        static_for<MI * NJ>([&](auto tc) {
+          constexpr int j = decltype(tc)::value / MI, i = decltype(tc)::value % MI;
+          lora_mfma_one<OpT, T::AGPR>(acc[j][i], w[j], af[i]);
         });
         if constexpr (T::AGPR) lora_mfma_done(acc);
       });

@@ -118,7 +118,7 @@ __global__ __launch_bounds__(256) void lora_inner_tile_kernel(const LoraParams p
         const int i = u * 256 + tid;
         if (i >= C::CHUNKS / 8) break;
         const int ro = AKC ? i / (C::KS / 8) : i % (RB * 2), ko = AKC ? i % (C::KS / 8) : i / (RB * 2);
-        char* at = lds + ro * 8 * C::LDB + ko * 16;
+        char* at = lds + ro * 8 * C::LDB + (ko ^ (ro & 7)) * 16;  // (8 threads' writes: 8 chunks)
         if constexpr (AKC) {
 #pragma unroll
           for (int v = 0; v < 8; ++v) *reinterpret_cast<uint4*>(at + v * C::LDB) = av[u][v];
@@ -133,34 +133,40 @@ __global__ __launch_bounds__(256) void lora_inner_tile_kernel(const LoraParams p
     f32x4_t acc[RB];
 #pragma unroll
     for (int b = 0; b < RB; ++b) acc[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    // a stage: A's values, loaded one stage ahead, go to LDS; x is two ahead
-    auto stage = [&](int32_t k0, uint4 (&xv)[XS]) {
-      if (k0 >= K) return;
+    // a stage: A's values, loaded one stage ahead, go to LDS; x is two ahead.  The
+    // stages in turn from one that depends on the tile: in step, all tiles read the
+    // same columns of rows that lie a power of two apart, which a few of the memory's
+    // channels hold
+    const int32_t stages = (K + C::KS - 1) / C::KS;
+    const int32_t first = (int32_t)(blockIdx.x % (uint32_t)stages);
+    auto at = [&](int32_t i) { return (i + first < stages ? i + first : i + first - stages) * C::KS; };
+    auto stage = [&](int32_t i, uint4 (&xv)[XS]) {
+      if (i >= stages) return;
       __syncthreads();  // the last stage's reads
       store_a();
       uint4 xc[XS];
 #pragma unroll
       for (int s = 0; s < XS; ++s) xc[s] = xv[s];
       __syncthreads();
-      if (k0 + C::KS < K) load_a(k0 + C::KS);
-      if (k0 + 2 * C::KS < K) load_x(k0 + 2 * C::KS, xv);
+      if (i + 1 < stages) load_a(at(i + 1));
+      if (i + 2 < stages) load_x(at(i + 2), xv);
       if (any) {
 #pragma unroll
         for (int s = 0; s < XS; ++s)
 #pragma unroll
           for (int b = 0; b < RB; ++b) {
-            const uint4 w = *reinterpret_cast<const uint4*>(lds + (b * 16 + fr) * C::LDB +
-                                                            (k_wave + s * 32 + fq * 8) * 2);
+            const uint4 w = *reinterpret_cast<const uint4*>(
+                lds + (b * 16 + fr) * C::LDB + ((k_wave / 8 + s * 4 + fq) ^ ((b * 2 + fr / 8) & 7)) * 16);
             MfmaOp<OpT>::step(acc[b], w, xc[s]);
           }
       }
     };
-    load_a(0);
-    load_x(0, x0);
-    load_x(C::KS, x1);
-    for (int32_t k0 = 0; k0 < K; k0 += 2 * C::KS) {
-      stage(k0, x0);
-      stage(k0 + C::KS, x1);
+    load_a(at(0));
+    load_x(at(0), x0);
+    if (stages > 1) load_x(at(1), x1);
+    for (int32_t i = 0; i < stages; i += 2) {
+      stage(i, x0);
+      stage(i + 1, x1);
     }
     if constexpr (KW > 1) {
       // the waves' sums, added in wave order by the first
