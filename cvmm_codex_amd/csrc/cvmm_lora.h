@@ -46,7 +46,7 @@ struct LoraParams {
 };
 
 // K split over workgroups: fp32 partial products [splits][rows][part_ld], each
-// of `slices` slices of 32 k; inner rows alike, [h_splits][rows][rank].
+// of `slices` slices of 64 k; inner rows alike, [h_splits][rows][rank].
 struct LoraSplit {
   float* part;
   int64_t part_ld;

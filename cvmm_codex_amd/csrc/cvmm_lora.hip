@@ -256,9 +256,9 @@ bool few_rows(int64_t rows) { return rows <= kLoraFewRows; }
 // enough for every CU, at least 64 k each.
 LoraSplit few_split(int64_t rows, int64_t K, int64_t N, int64_t rank) {
   LoraSplit sp{};
-  const int64_t tiles = ((rows + 63) / 64) * ((N + 127) / 128), all = (K + 31) / 32;
+  const int64_t tiles = ((rows + 63) / 64) * ((N + 127) / 128), all = (K + 63) / 64;
   int64_t splits = (256 + tiles - 1) / tiles;
-  if (splits > (all + 1) / 2) splits = (all + 1) / 2;
+  if (splits > all) splits = all;
   if (splits < 1) splits = 1;
   sp.slices = (int32_t)((all + splits - 1) / splits);
   sp.splits = (int32_t)((all + sp.slices - 1) / sp.slices);

@@ -4,12 +4,12 @@
 // that occurs in the tile.
 //
 // A workgroup of four waves owns BM rows x BN columns; a wave MI x NJ blocks of
-// 16 x 16.  Slices of 32 k (64-byte row pieces of x, 64-byte pieces or whole rows
-// of W, by which of its strides is 1) go by buffer loads straight into a ring of
-// four LDS buffers, three in flight while one is multiplied; the fragments of
-// slice s + 1 are read while the products of slice s run.  Every slice is the
-// same number of loads, those past the last k included (offsets past the
-// descriptor's range read zeros), so every wait is an exact vmcnt.  Operands are
+// 16 x 16.  Slices of 64 k (128-byte row pieces of x: whole lines; such pieces or
+// whole rows of W, by which of its strides is 1) go by buffer loads straight into a
+// ring of LDS buffers; the fragments of one half of a slice are read while the
+// products of the other run.  Every slice is the same number of loads, those past
+// the last k included (offsets past the descriptor's range read zeros), so every
+// wait is an exact vmcnt.  Operands are
 // swapped (C^T = W^T x^T): a lane ends with 4 consecutive columns of one row, 8
 // after two lane swaps, stored as one 16-byte write.
 //
@@ -132,28 +132,30 @@ __device__ __forceinline__ void lora_mfma_done(f32x4_t (&c)[NJ][MI]) {
     for (int i = 0; i < MI; ++i) asm volatile("" : "+a"(c[j][i]));
 }
 
-template <int MI, int NJ, int WMW, int WNW>
+template <int MI, int NJ, int WMW, int WNW, int STAGES_>
 struct LoraTile {
   static_assert(WMW * WNW == 4, "four waves");
-  static constexpr int BM = 16 * MI * WMW, BN = 16 * NJ * WNW;
-  static constexpr int A_INSTS = BM / 16, B_INSTS = BN / 16;  // 1 KB each
+  static constexpr int BM = 16 * MI * WMW, BN = 16 * NJ * WNW, STAGES = STAGES_;
+  static constexpr int A_INSTS = BM / 8, B_INSTS = BN / 8;  // 1 KB each
   static_assert((A_INSTS + B_INSTS) % 4 == 0, "whole instructions per wave");
   static constexpr int D = (A_INSTS + B_INSTS) / 4;
-  static constexpr int A_BYTES = BM * 64, SLICE = (BM + BN) * 64, STAGES = 4;
-  static constexpr int OCC = MI * NJ > 16 ? 1 : 2;
+  static constexpr int A_BYTES = BM * 128, SLICE = (BM + BN) * 128;
+  static constexpr int LDS = STAGES * SLICE + BM * 8;
+  static constexpr int OCC = MI * NJ > 16 || LDS > 80 * 1024 ? 1 : 2;
   static constexpr bool AGPR = MI * NJ == 64;
   static constexpr bool MIXED = A_INSTS % D != 0;  // a wave loads pieces of x and of W
-  static_assert(2 * SLICE <= 65536, "offsets of an LDS instruction");
+  static_assert((STAGES - 2) * D < 64, "vmcnt range");
 };
 
 // Lane offset of load `inst` of a slice's B half, and the k that its piece starts
 // at.  KC: [n][k] pieces, as the A half; else [k][n] rows of BN columns, read back
 // transposed.
+__device__ __forceinline__ int lora_chunk(int lane) { return (lane & 7) ^ ((lane >> 3) & 7); }
 template <bool KC, int BN>
 __device__ __forceinline__ uint32_t lora_b_off(int inst, int lane, int64_t sk, int64_t sn, int64_t cols) {
   if constexpr (KC) {
-    const int n = inst * 16 + (lane >> 2), c = (lane & 3) ^ ((lane >> 3) & 3);
-    return n < cols ? (uint32_t)(n * sn * 2) + (uint32_t)c * 16 + kLoraBack : kLoraOob;
+    const int n = inst * 8 + (lane >> 3);
+    return n < cols ? (uint32_t)(n * sn * 2) + (uint32_t)lora_chunk(lane) * 16 + kLoraBack : kLoraOob;
   } else {
     constexpr int CPR = BN / 8;
     const int row = inst * (64 / CPR) + lane / CPR, c = (lane % CPR) ^ tr_row_swz<CPR>(row);
@@ -163,16 +165,16 @@ __device__ __forceinline__ uint32_t lora_b_off(int inst, int lane, int64_t sk, i
 template <bool KC, int BN>
 __device__ __forceinline__ int lora_b_k(int inst, int lane) {
   constexpr int CPR = BN / 8;
-  if constexpr (KC) return ((lane & 3) ^ ((lane >> 3) & 3)) * 8;
+  if constexpr (KC) return lora_chunk(lane) * 8;
   else return inst * (64 / CPR) + lane / CPR;
 }
 
-template <typename OpT, int MI, int NJ, int WMW, int WNW, bool WKC, bool BKC, bool SPLIT>
-__global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_gemm_kernel(const LoraParams p,
-                                                                                           const LoraSplit sp) {
-  using T = LoraTile<MI, NJ, WMW, WNW>;
+template <typename OpT, int MI, int NJ, int WMW, int WNW, int STAGES, bool WKC, bool BKC, bool SPLIT>
+__global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW, STAGES>::OCC)) void lora_gemm_kernel(
+    const LoraParams p, const LoraSplit sp) {
+  using T = LoraTile<MI, NJ, WMW, WNW, STAGES>;
   constexpr int BM = T::BM, BN = T::BN, D = T::D, SLICE = T::SLICE;
-  __shared__ __attribute__((aligned(1024))) char ring[T::STAGES * SLICE];
+  __shared__ __attribute__((aligned(1024))) char ring[STAGES * SLICE];
   __shared__ int32_t s_row[BM], s_id[BM];
 
   if constexpr (SPLIT) {
@@ -192,8 +194,8 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
   if constexpr (SPLIT) {
     split = id % (uint32_t)sp.splits;
     id /= (uint32_t)sp.splits;
-    k_lo = (int64_t)split * sp.slices * 32;
-    k_hi = k_lo + (int64_t)sp.slices * 32 < p.K ? k_lo + (int64_t)sp.slices * 32 : p.K;
+    k_lo = (int64_t)split * sp.slices * 64;
+    k_hi = k_lo + (int64_t)sp.slices * 64 < p.K ? k_lo + (int64_t)sp.slices * 64 : p.K;
   }
   const int64_t m0 = (int64_t)(id / tiles_n) * BM, n0 = (int64_t)(id % tiles_n) * BN;
 
@@ -212,35 +214,34 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
   const int64_t first = p.order != nullptr ? 0 : m0;
   const __amdgpu_buffer_rsrc_t ra = lora_rsrc(reinterpret_cast<const OpT*>(p.x) + first * p.x_ld + k_lo);
   const __amdgpu_buffer_rsrc_t rw = lora_rsrc(reinterpret_cast<const OpT*>(p.w) + n0 * p.w_sn + k_lo * p.w_sk);
-  const int a_k = ((lane & 3) ^ ((lane >> 3) & 3)) * 8;  // the k that a lane's pieces of x start at
+  const int a_k = lora_chunk(lane) * 8;  // the k that a lane's pieces of x start at
   uint32_t off[D];
 #pragma unroll
   for (int j = 0; j < D; ++j) {
     const int g = wave * D + j;
     if (g < T::A_INSTS) {
-      const int r = g * 16 + (lane >> 2), c = (lane & 3) ^ ((lane >> 3) & 3);
-      const int32_t row = s_row[r];
-      off[j] = row >= 0 ? (uint32_t)(((int64_t)row - first) * p.x_ld * 2) + (uint32_t)c * 16 + kLoraBack : kLoraOob;
+      const int32_t row = s_row[g * 8 + (lane >> 3)];
+      off[j] = row >= 0 ? (uint32_t)(((int64_t)row - first) * p.x_ld * 2) + (uint32_t)a_k * 2 + kLoraBack : kLoraOob;
     } else {
       off[j] = lora_b_off<WKC, BN>(g - T::A_INSTS, lane, p.w_sk, p.w_sn, p.N - n0);
     }
     if (off[j] != kLoraOob) off[j] -= 1024u * (uint32_t)(j & 3);
   }
   const int32_t kw = (int32_t)(k_hi - k_lo);
-  const uint32_t b_step = (uint32_t)((WKC ? 1 : p.w_sk) * 64);  // bytes a slice moves W by
+  const uint32_t b_step = (uint32_t)((WKC ? 1 : p.w_sk) * 128);  // bytes a slice moves W by
   auto issue_one = [&](auto jc, __amdgpu_buffer_rsrc_t rsa, __amdgpu_buffer_rsrc_t rsb, uint32_t o, uint32_t sa,
                        uint32_t sb, char* dst) {
     constexpr int J = decltype(jc)::value;
     const bool is_a = wave * D + (T::MIXED ? J : 0) < T::A_INSTS;
     buf_dma<16, (J & 3) * 1024>(is_a ? rsa : rsb, o, is_a ? sa : sb, dst + (wave * D + (J & ~3)) * 1024);
   };
-  const int32_t S = (kw + 31) / 32;
+  const int32_t S = (kw + 63) / 64;
   int32_t i_k = 0;  // k of the slice to be issued, and its offsets
   uint32_t i_a = 0, i_b = 0;
   auto issue_part = [&](auto jc, char* dst) { issue_one(jc, ra, rw, off[decltype(jc)::value], i_a, i_b, dst); };
   // before a slice is issued that k ends in, or past: its pieces from there on read zeros
   auto issue_mask = [&]() {
-    if (i_k + 32 <= kw) return;
+    if (i_k + 64 <= kw) return;
     static_for<D>([&](auto jc) {
       constexpr int J = decltype(jc)::value;
       const int g = wave * D + J;
@@ -248,20 +249,20 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
     });
   };
   auto issue_next = [&]() {
-    i_k += 32;
-    i_a += 64;
+    i_k += 64;
+    i_a += 128;
     i_b += b_step;
     if (i_k >= kw) i_a = i_b = 0;  // (only offsets past the range from here on)
     issue_mask();
   };
   issue_mask();
 
-  // ---- fragments: buffers 2 and 3 from a base of their own, the rest of the
-  // address in the instruction
-  constexpr int kHalf = 2 * SLICE;
+  // ---- fragments of the two halves of a slice.  [row][k] rows of 128 bytes hold
+  // chunk c at c ^ (row & 7); the second half's chunks are 4 on, bit 6 of the address
   const uint32_t st0 = lds_addr(ring);
-  const uint32_t a_f = st0 + (uint32_t)((wm * MI * 16 + fr) * 64 + ((fq ^ ((fr >> 1) & 3)) << 4));
-  const uint32_t kc_f = st0 + T::A_BYTES + (uint32_t)((wn * NJ * 16 + fr) * 64 + ((fq ^ ((fr >> 1) & 3)) << 4));
+  const uint32_t kc_lane = (uint32_t)(fr * 128 + ((fq ^ (fr & 7)) << 4));
+  const uint32_t a_f = st0 + (uint32_t)(wm * MI * 2048) + kc_lane;
+  const uint32_t kc_f = st0 + T::A_BYTES + (uint32_t)(wn * NJ * 2048) + kc_lane;
   uint32_t tr_f[NJ];
   {
     constexpr int CPR = BN / 8;
@@ -271,38 +272,25 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
     for (int i = 0; i < NJ; ++i)
       tr_f[i] = st0 + T::A_BYTES + (uint32_t)(r * BN * 2 + lo + (((wn * NJ * 2 + 2 * i) ^ tr_row_swz<CPR>(r)) << 4));
   }
-  auto read_a = [&](auto buf, lds_u32x4 (&f)[MI]) {
-    constexpr int B = decltype(buf)::value;
-    const uint32_t at = a_f + (B >= 2 ? kHalf : 0);
-    static_for<MI>([&](auto i) { f[i] = lds_read128_at<(B & 1) * SLICE + decltype(i)::value * 1024>(at); });
-  };
-  auto read_b = [&](auto buf, auto& f) {
-    constexpr int B = decltype(buf)::value;
-    if constexpr (std::is_same_v<std::remove_reference_t<decltype(f)>, lds_u32x4[NJ]>) {
-      const uint32_t at = kc_f + (B >= 2 ? kHalf : 0);
-      static_for<NJ>([&](auto i) { f[i] = lds_read128_at<(B & 1) * SLICE + decltype(i)::value * 1024>(at); });
-    } else {
-      static_for<NJ>([&](auto ic) {
-        constexpr int i = decltype(ic)::value;
-        const uint32_t at = tr_f[i] + (B >= 2 ? kHalf : 0);
-        f[i][0] = lds_read_tr<(B & 1) * SLICE>(at);
-        f[i][1] = lds_read_tr<(B & 1) * SLICE + 4 * BN * 2>(at);
-      });
-    }
-  };
-
-  // the R-th of a slice's reads: x's, then W's
-  auto read_one = [&](auto buf, auto rc, lds_u32x4 (&fa)[MI], auto& fb) {
-    constexpr int B = decltype(buf)::value, R = decltype(rc)::value, OFF = (B & 1) * SLICE;
-    constexpr uint32_t hi = B >= 2 ? kHalf : 0;
+  // the R-th read of half H of the slice in buffer B: x's blocks, then W's
+  auto read_one = [&](auto buf, auto half, auto rc, lds_u32x4 (&fa)[MI], auto& fb) {
+    constexpr int B = decltype(buf)::value, H = decltype(half)::value, R = decltype(rc)::value;
+    constexpr uint32_t at = (uint32_t)B * SLICE;
     if constexpr (R < MI) {
-      fa[R] = lds_read128_at<OFF + R * 1024>(a_f + hi);
+      fa[R] = lds_read128_at<R * 2048>((a_f ^ (H * 64)) + at);
     } else if constexpr (std::is_same_v<std::remove_reference_t<decltype(fb)>, lds_u32x4[NJ]>) {
-      fb[R - MI] = lds_read128_at<OFF + (R - MI) * 1024>(kc_f + hi);
+      fb[R - MI] = lds_read128_at<(R - MI) * 2048>((kc_f ^ (H * 64)) + at);
     } else {
       constexpr int i = (R - MI) / 2, h = (R - MI) % 2;
-      fb[i][h] = lds_read_tr<OFF + h * 4 * BN * 2>(tr_f[i] + hi);
+      fb[i][h] = lds_read_tr<(H * 32 + h * 4) * BN * 2>(tr_f[i] + at);
     }
+  };
+  auto read_all = [&](auto buf, auto half, lds_u32x4 (&fa)[MI], auto& fb) {
+    constexpr int R = std::is_same_v<std::remove_reference_t<decltype(fb)>, lds_u32x4[NJ]> ? MI + NJ : MI + 2 * NJ;
+    static_for<R>([&](auto rc) { read_one(buf, half, rc, fa, fb); });
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    lora_wait(fa);
+    lora_wait(fb);
   };
 
   // ---- accumulators: acc[j][i] holds columns 16 j + 4 fq + {0..3} of row 16 i + fr
@@ -317,54 +305,57 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
   using WFrag = std::conditional_t<WKC, lds_u32x4[NJ], lds_u32x2[NJ][2]>;
   if (S > 0) {
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
+    for (int s = 0; s < STAGES; ++s) {
       static_for<D>([&](auto j) { issue_part(j, ring + s * SLICE); });
       issue_next();
       issue_fence();
     }
     lds_u32x4 a0[MI], a1[MI];
     WFrag b0, b1;
-    vm_wait<3 * D>();
+    vm_wait<(STAGES - 1) * D>();
     lds_barrier();
-    read_a(std::integral_constant<int, 0>(), a0);
-    read_b(std::integral_constant<int, 0>(), b0);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    lora_wait(a0);
-    lora_wait(b0);
-    // slice s, in buffer B, is in (ca, cb): slice s + 1 is read into (na, nb), slice
-    // s + 4 issued into the buffer of s, which every wave has read
-    auto step = [&](auto bc, lds_u32x4 (&ca)[MI], WFrag& cb, lds_u32x4 (&na)[MI], WFrag& nb) {
-      constexpr int B = decltype(bc)::value;
-      vm_wait<2 * D>();
-      lds_barrier();
-      char* dst = ring + B * SLICE;
-      // between the products, a read or a load each: the matrix unit is busy for 16
-      // cycles with each, in which up to three others issue
+    read_all(std::integral_constant<int, 0>(), std::integral_constant<int, 0>(), a0, b0);
+    // The products of a half of the slice in buffer B, with the next half's reads and
+    // (LOAD) the loads of slice s + STAGES between them: the matrix unit is busy for
+    // 16 cycles with each, in which up to three others issue.
+    auto half = [&](auto bc, auto hc, lds_u32x4 (&ca)[MI], WFrag& cb, lds_u32x4 (&na)[MI], WFrag& nb) {
+      constexpr int B = decltype(bc)::value, H = decltype(hc)::value;
       constexpr int P = MI * NJ, R = MI + (WKC ? NJ : 2 * NJ);
+      using NB = std::integral_constant<int, H == 0 ? B : (B + 1) % STAGES>;
+      using NH = std::integral_constant<int, 1 - H>;
+      char* dst = ring + B * SLICE;
       lora_mfma_ready();
       static_for<P>([&](auto tc) {
         constexpr int t = decltype(tc)::value, jb = t / MI, i = t % MI;
         lora_mfma_one<OpT, T::AGPR>(acc[jb][i], lora_frag(cb[jb]), ca[i]);
         static_for<R>([&](auto rc) {
-          if constexpr (decltype(rc)::value * (P - P / 4) / R == t) read_one(std::integral_constant<int, (B + 1) & 3>(), rc, na, nb);
+          if constexpr (decltype(rc)::value * (P - P / 4) / R == t) read_one(NB(), NH(), rc, na, nb);
         });
-        static_for<D>([&](auto j) {
-          if constexpr (decltype(j)::value * P / D + 1 == t) issue_part(j, dst);
-        });
+        if constexpr (H == 1)
+          static_for<D>([&](auto j) {
+            if constexpr (decltype(j)::value * P / D == t) issue_part(j, dst);
+          });
         __builtin_amdgcn_sched_barrier(0);
       });
-      issue_next();
+      if constexpr (H == 1) issue_next();
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       lora_wait(na);
       lora_wait(nb);
     };
-    // (four at a time, zeros past the last: leaving within them made the compiler spill)
-    for (int32_t s = 0; s < S; s += 4) {
-      step(std::integral_constant<int, 0>(), a0, b0, a1, b1);
-      step(std::integral_constant<int, 1>(), a1, b1, a0, b0);
-      step(std::integral_constant<int, 2>(), a0, b0, a1, b1);
-      step(std::integral_constant<int, 3>(), a1, b1, a0, b0);
-    }
+    // slice s: its first half is in (a0, b0).  After the first half's products every
+    // wave has the second in registers, so that the buffer takes slice s + STAGES.
+    auto slice = [&](auto bc) {
+      half(bc, std::integral_constant<int, 0>(), a0, b0, a1, b1);
+      vm_wait<(STAGES - 2) * D>();  // slice s + 1 has landed
+      lds_barrier();
+      half(bc, std::integral_constant<int, 1>(), a1, b1, a0, b0);
+    };
+    // (the ring's slices at a time, zeros past the last: leaving within them made the
+    // compiler spill the largest tile's registers)
+    for (int32_t s = 0; s < S; s += STAGES)
+      static_for<STAGES>([&](auto bc) {
+        if (T::AGPR || s + decltype(bc)::value < S) slice(bc);
+      });
     vm_wait<0>();
     if constexpr (T::AGPR) lora_mfma_done(acc);
   }
@@ -396,9 +387,8 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
   for (int j = 0; j < D; ++j) {
     const int g = wave * D + j;
     if (g < T::A_INSTS) {
-      const int r = g * 16 + (lane >> 2), c = (lane & 3) ^ ((lane >> 3) & 3);
-      const int32_t row = s_row[r];
-      hoff[j] = row >= 0 ? (uint32_t)(((int64_t)row - first) * p.h_ld * 2) + (uint32_t)c * 16 + kLoraBack : kLoraOob;
+      const int32_t row = s_row[g * 8 + (lane >> 3)];
+      hoff[j] = row >= 0 ? (uint32_t)(((int64_t)row - first) * p.h_ld * 2) + (uint32_t)a_k * 2 + kLoraBack : kLoraOob;
     } else {
       hoff[j] = lora_b_off<BKC, BN>(g - T::A_INSTS, lane, p.b_sr, p.b_sn, p.N - n0);
     }
@@ -411,7 +401,7 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
   for (int i = 0; i < BM / 64; ++i) uniform &= s_id[i * 64 + lane] == s_id[0];
   uniform = __all(uniform);
   bool dropped = false;  // this lane left infinities or NaN out of an adapter's values
-  const uint32_t hb_step = (uint32_t)((BKC ? 1 : p.b_sr) * 64);
+  const uint32_t hb_step = (uint32_t)((BKC ? 1 : p.b_sr) * 128);
   for (int32_t cur = -1;;) {
     int32_t a = INT32_MAX;
 #pragma unroll
@@ -423,31 +413,28 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
     if (a == INT32_MAX) break;
     cur = a;
     const __amdgpu_buffer_rsrc_t rb = lora_rsrc(reinterpret_cast<const OpT*>(p.b) + a * p.b_se + n0 * p.b_sn);
-    for (int32_t r0 = 0; r0 < rank; r0 += 128) {  // four slices at a time
-      lds_barrier();                              // the buffers' last reads
+    for (int32_t r0 = 0; r0 < rank; r0 += STAGES * 64) {  // the ring's slices at a time
+      lds_barrier();                                        // the buffers' last reads
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int32_t k = r0 + s * 32;
+      for (int s = 0; s < STAGES; ++s) {
+        const int32_t k = r0 + s * 64;
         if (k < rank)
           static_for<D>([&](auto j) {
             constexpr int J = decltype(j)::value;
-            const int g = wave * D + J;  // (h holds zeros up to h_ld)
-            const bool in = g < T::A_INSTS || k + lora_b_k<BKC, BN>(g - T::A_INSTS, lane) < rank;
+            const int g = wave * D + J;
+            const bool in = g < T::A_INSTS ? k + a_k < p.h_ld : k + lora_b_k<BKC, BN>(g - T::A_INSTS, lane) < rank;
             issue_one(j, rh, rb, in ? hoff[J] : kLoraOob, (uint32_t)k * 2,
-                      (uint32_t)(k / 32) * hb_step, ring + s * SLICE);
+                      (uint32_t)(k / 64) * hb_step, ring + s * SLICE);
           });
       }
       vm_wait<0>();
       lds_barrier();
-      static_for<4>([&](auto sc) {
-        if (r0 + decltype(sc)::value * 32 >= rank) return;
+      static_for<2 * STAGES>([&](auto sc) {
+        constexpr int s = decltype(sc)::value;
+        if (r0 + s * 32 >= rank) return;
         lds_u32x4 af[MI];
         BFrag bf;
-        read_a(sc, af);
-        read_b(sc, bf);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        lora_wait(af);
-        lora_wait(bf);
+        read_all(std::integral_constant<int, s / 2>(), std::integral_constant<int, s % 2>(), af, bf);
         if (!uniform) {
 #pragma unroll
           for (int i = 0; i < MI; ++i)
@@ -560,12 +547,13 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW>::OCC)) void lora_g
 template <typename OpT, bool WKC, bool BKC>
 hipError_t launch_lora_gemm_kc(const LoraParams& p, hipStream_t s) {
   auto tiles = [&](int64_t bm, int64_t bn) { return ((p.rows + bm - 1) / bm) * ((p.N + bn - 1) / bn); };
-  auto go = [&](auto mi, auto nj, auto wm, auto wn) {
+  auto go = [&](auto mi, auto nj, auto wm, auto wn, auto st) {
     constexpr int MI = decltype(mi)::value, NJ = decltype(nj)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
-    using T = LoraTile<MI, NJ, WM, WN>;
+    constexpr int ST = decltype(st)::value;
+    using T = LoraTile<MI, NJ, WM, WN, ST>;
     const int64_t n = tiles(T::BM, T::BN);
     if (n > 0x7fffffffll) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((lora_gemm_kernel<OpT, MI, NJ, WM, WN, WKC, BKC, false>), dim3((unsigned)n), dim3(256), 0, s, p,
+    hipLaunchKernelGGL((lora_gemm_kernel<OpT, MI, NJ, WM, WN, ST, WKC, BKC, false>), dim3((unsigned)n), dim3(256), 0, s, p,
                        LoraSplit{});
     return hipGetLastError();
   };
@@ -573,9 +561,10 @@ hipError_t launch_lora_gemm_kc(const LoraParams& p, hipStream_t s) {
   using i2 = integral_constant<int, 2>;
   using i4 = integral_constant<int, 4>;
   using i8 = integral_constant<int, 8>;
-  if (tiles(256, 256) >= 192) return go(i8(), i8(), i2(), i2());
-  if (tiles(128, 128) >= 192) return go(i4(), i4(), i2(), i2());
-  return go(i2(), i4(), i2(), i2());
+  if (tiles(256, 256) >= 192) return go(i8(), i8(), i2(), i2(), i2());
+  if (tiles(256, 128) >= 192) return go(i8(), i4(), i2(), i2(), integral_constant<int, 3>());
+  if (tiles(128, 128) >= 192) return go(i4(), i4(), i2(), i2(), i2());
+  return go(i2(), i4(), i2(), i2(), i4());
 }
 
 template <typename OpT>
@@ -617,9 +606,9 @@ hipError_t launch_lora_few_op(const LoraParams& p, const LoraSplit& sp, hipStrea
   } else {
     const dim3 grid(sp.gemm_blocks + row_blocks);
     if (p.w_sn == 1)
-      hipLaunchKernelGGL((lora_gemm_kernel<OpT, 2, 4, 2, 2, false, false, true>), grid, dim3(256), 0, s, p, sp);
+      hipLaunchKernelGGL((lora_gemm_kernel<OpT, 2, 4, 2, 2, 2, false, false, true>), grid, dim3(256), 0, s, p, sp);
     else
-      hipLaunchKernelGGL((lora_gemm_kernel<OpT, 2, 4, 2, 2, true, false, true>), grid, dim3(256), 0, s, p, sp);
+      hipLaunchKernelGGL((lora_gemm_kernel<OpT, 2, 4, 2, 2, 2, true, false, true>), grid, dim3(256), 0, s, p, sp);
   }
   hipLaunchKernelGGL((lora_join_kernel<OpT>),
                      dim3((unsigned)((p.n_out + kLoraJoinThreads * 4 - 1) / (kLoraJoinThreads * 4)), (unsigned)p.rows),
