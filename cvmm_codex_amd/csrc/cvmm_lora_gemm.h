@@ -176,6 +176,7 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW, STAGES>::OCC)) voi
   constexpr int BM = T::BM, BN = T::BN, D = T::D, SLICE = T::SLICE;
   __shared__ __attribute__((aligned(1024))) char ring[STAGES * SLICE];
   __shared__ int32_t s_row[BM], s_id[BM];
+  static_assert(BM <= 256, "a row per thread");
 
   if constexpr (SPLIT) {
     if (blockIdx.x >= sp.gemm_blocks) {
@@ -199,14 +200,17 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW, STAGES>::OCC)) voi
   }
   const int64_t m0 = (int64_t)(id / tiles_n) * BM, n0 = (int64_t)(id % tiles_n) * BN;
 
-  for (int i = tid; i < BM; i += 256) {
-    const int64_t m = m0 + i;
-    int64_t row = m < p.rows ? (p.order != nullptr ? p.order[m] : m) : -1;
-    if (row < 0 || row >= p.rows) row = -1;
-    s_row[i] = (int32_t)row;
-    if constexpr (!SPLIT) s_id[i] = row >= 0 ? lora_id(p, row) : -1;
+  // the tile's rows; their ids are in flight until the projection is done
+  int64_t my_row = -1, my_id = -1;
+  if (tid < BM) {
+    const int64_t m = m0 + tid;
+    my_row = m < p.rows ? (p.order != nullptr ? p.order[m] : m) : -1;
+    if (my_row < 0 || my_row >= p.rows) my_row = -1;
+    s_row[tid] = (int32_t)my_row;
+    if (!SPLIT && my_row >= 0)
+      my_id = p.ids_is_int64 ? ((const int64_t*)p.ids)[my_row] : (int64_t)((const int32_t*)p.ids)[my_row];
   }
-  __syncthreads();
+  lds_barrier();
 
   // ---- sources of this wave's loads: instruction g = wave * D + j fills 1 KB of
   // the slice, A rows first
@@ -293,13 +297,56 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW, STAGES>::OCC)) voi
     lora_wait(fb);
   };
 
-  // ---- accumulators: acc[j][i] holds columns 16 j + 4 fq + {0..3} of row 16 i + fr
-  f32x4_t acc[NJ][MI];
+  // ---- accumulators: acc[j][i] holds columns 16 j + 4 fq + {0..3} of row 16 i + fr.
+  // base's values of row block i:
   const int64_t nw = n0 + wn * NJ * 16;
+  auto base_of = [&](int i, f32x4_t (&v)[NJ]) {
+    const int64_t row = s_row[(wm * MI + i) * 16 + fr];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) v[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    if (p.base == nullptr || row < 0) return;
+    const int64_t at = row * p.base_ld;
+    if (p.base_vec && nw + NJ * 16 <= p.n_out) {
+      if (p.base_dtype == kF32) {
+        const float* q = reinterpret_cast<const float*>(p.base) + at + nw + 4 * fq;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) v[j] = *reinterpret_cast<const f32x4_t*>(q + j * 16);
+      } else {
+        const OpT* q = reinterpret_cast<const OpT*>(p.base) + at + nw + 4 * fq;
+        uint2 raw[NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) raw[j] = *reinterpret_cast<const uint2*>(q + j * 16);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          const OpT* e = reinterpret_cast<const OpT*>(&raw[j]);
+          v[j] = f32x4_t{to_f32(e[0]), to_f32(e[1]), to_f32(e[2]), to_f32(e[3])};
+        }
+      }
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t n = nw + j * 16 + 4 * fq + q;
+        if (n < p.n_out) v[j][q] = load_as_f32(p.base, p.base_dtype, at + n);
+      }
+  };
+  f32x4_t acc[NJ][MI];
 #pragma unroll
   for (int j = 0; j < NJ; ++j)
 #pragma unroll
     for (int i = 0; i < MI; ++i) acc[j][i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  if constexpr (!SPLIT && !T::AGPR) {
+    if (p.base != nullptr)
+      static_for<MI>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        f32x4_t v[NJ];
+        base_of(i, v);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) acc[j][i] = v[j];
+      });
+  }
 
   // ---- the shared weights
   using WFrag = std::conditional_t<WKC, lds_u32x4[NJ], lds_u32x2[NJ][2]>;
@@ -377,6 +424,8 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW, STAGES>::OCC)) voi
   }
 
   // ---- the adapters of the tile's rows
+  if (tid < BM) s_id[tid] = my_id >= 0 && my_id < p.n ? (int32_t)my_id : -1;
+  lds_barrier();
   using BFrag = std::conditional_t<BKC, lds_u32x4[NJ], lds_u32x2[NJ][2]>;
   int32_t ids[MI];
 #pragma unroll
@@ -455,47 +504,26 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW, STAGES>::OCC)) voi
     }
   }
 
-  // ---- base, and the stores
-  // (a row block at a time: with the loads of several in flight the compiler ran
-  // out of registers)
+  // ---- the stores (the largest tile adds base here, a row block at a time: with the
+  // loads of several in flight the compiler ran out of registers)
   static_for<MI>([&](auto ic) {
     constexpr int i = decltype(ic)::value;
     const int64_t row = s_row[(wm * MI + i) * 16 + fr];
     OpT* dst = reinterpret_cast<OpT*>(p.out) + row * p.out_ld;
     f32x4_t add[NJ];
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) add[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    if (p.base != nullptr && row >= 0) {
-      const int64_t at = row * p.base_ld;
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int64_t n = nw + j * 16 + 4 * fq;
-        if (n + 4 <= p.n_out && p.base_vec) {
-          if (p.base_dtype == kF32) {
-            const float4 v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.base) + at + n);
-            add[j] = f32x4_t{v.x, v.y, v.z, v.w};
-          } else {
-            const uint2 raw = *reinterpret_cast<const uint2*>(reinterpret_cast<const OpT*>(p.base) + at + n);
-            const OpT* v = reinterpret_cast<const OpT*>(&raw);
-            add[j] = f32x4_t{to_f32(v[0]), to_f32(v[1]), to_f32(v[2]), to_f32(v[3])};
-          }
-        } else {
-#pragma unroll
-          for (int v = 0; v < 4; ++v)
-            if (n + v < p.n_out) add[j][v] = load_as_f32(p.base, p.base_dtype, at + n + v);
-        }
-      }
-    }
+    if constexpr (T::AGPR) base_of(i, add);
     static_for<NJ / 2>([&](auto pc) {
       constexpr int pr = decltype(pc)::value;
       uint32_t a[2], b[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         union { uint32_t u; OpT e[2]; } pa, pb;
-        pa.e[0] = from_f32<OpT>(acc[2 * pr][i][2 * h] + add[2 * pr][2 * h]);
-        pa.e[1] = from_f32<OpT>(acc[2 * pr][i][2 * h + 1] + add[2 * pr][2 * h + 1]);
-        pb.e[0] = from_f32<OpT>(acc[2 * pr + 1][i][2 * h] + add[2 * pr + 1][2 * h]);
-        pb.e[1] = from_f32<OpT>(acc[2 * pr + 1][i][2 * h + 1] + add[2 * pr + 1][2 * h + 1]);
+        f32x4_t va = acc[2 * pr][i], vb = acc[2 * pr + 1][i];
+        if constexpr (T::AGPR) va += add[2 * pr], vb += add[2 * pr + 1];
+        pa.e[0] = from_f32<OpT>(va[2 * h]);
+        pa.e[1] = from_f32<OpT>(va[2 * h + 1]);
+        pb.e[0] = from_f32<OpT>(vb[2 * h]);
+        pb.e[1] = from_f32<OpT>(vb[2 * h + 1]);
         a[h] = pa.u;
         b[h] = pb.u;
       }
@@ -561,6 +589,7 @@ hipError_t launch_lora_gemm_kc(const LoraParams& p, hipStream_t s) {
   using i2 = integral_constant<int, 2>;
   using i4 = integral_constant<int, 4>;
   using i8 = integral_constant<int, 8>;
+  if (p.w == nullptr) return go(i2(), i4(), i2(), i2(), i2());
   if (tiles(256, 256) >= 192) return go(i8(), i8(), i2(), i2(), i2());
   if (tiles(256, 128) >= 192) return go(i8(), i4(), i2(), i2(), integral_constant<int, 3>());
   if (tiles(128, 128) >= 192) return go(i4(), i4(), i2(), i2(), i2());
@@ -579,7 +608,7 @@ hipError_t launch_lora_inner_op(const LoraParams& p, hipStream_t s) {
   const bool akc = p.a_sr != 1;
   auto go = [&](auto rb, auto kw) {
     constexpr int RB = decltype(rb)::value, KW = decltype(kw)::value;
-    const dim3 grid((unsigned)((p.rows + (KW == 1 ? 63 : 15)) / (KW == 1 ? 64 : 16)), kLoraInnerTurns);
+    const dim3 grid((unsigned)((p.rows + 64 / KW - 1) / (64 / KW) * kLoraInnerTurns));
     if (akc)
       hipLaunchKernelGGL((lora_inner_tile_kernel<OpT, RB, KW, true>), grid, dim3(256), 0, s, p);
     else
@@ -593,7 +622,7 @@ hipError_t launch_lora_inner_op(const LoraParams& p, hipStream_t s) {
     else if (p.rank <= 128) go(integral_constant<int, 8>(), kw);
     else go(integral_constant<int, 16>(), kw);
   };
-  if (p.rows >= 8192) by_rank(std::integral_constant<int, 1>());
+  if (p.rows >= 8192) by_rank(std::integral_constant<int, 2>());
   else by_rank(std::integral_constant<int, 4>());
   return hipGetLastError();
 }

@@ -25,8 +25,17 @@ __device__ __forceinline__ void lora_transpose8(const uint4 (&r)[8], uint4 (&c)[
   }
 }
 
+// v, or zeros: by bits, where a choice became a branch around a wait for v.
+__device__ __forceinline__ uint4 keep_if(const uint4& v, bool keep) {
+  const uint32_t m = keep ? ~0u : 0u;
+  return make_uint4(v.x & m, v.y & m, v.z & m, v.w & m);
+}
+
 // ---------------------------------------------------------------------------
-// h of 16 rows (KW = 4: the waves split k) or 64 (KW = 1: 16 per wave).  A lane
+// (Loads at clamped places, zeroed where they are used: a guard around each made
+// them wait for one another.)
+//
+// h of 64 / KW rows, 16 per wave, KW of the four waves sharing k.  A lane
 // loads the pieces of x that its matrix operand holds straight from memory; A
 // comes through LDS as [rank][k] rows, transposed on the way where it is stored
 // [k][rank].  Bound by reading x once; each workgroup reads its adapters whole,
@@ -39,8 +48,8 @@ constexpr int kLoraInnerTurns = 4;
 
 template <int RB, int KW>
 struct LoraInnerCfg {
-  // k per LDS stage; 4 waves of 16 rows: each all of it, else a quarter each
-  static constexpr int KS = RB >= 16 ? 128 : KW > 1 && RB <= 4 ? 512 : 256;
+  // k per LDS stage, a part of which each wave takes
+  static constexpr int KS = RB >= 16 ? 128 : KW == 4 && RB <= 4 ? 512 : 256;
   static constexpr int KWAVE = KS / KW;        // k per wave and stage
   static constexpr int LDB = KS * 2 + 16;      // bytes per LDS row
   static constexpr int CHUNKS = RB * 16 * (KS / 8);  // 16-byte pieces of a stage
@@ -48,17 +57,23 @@ struct LoraInnerCfg {
 };
 
 template <typename OpT, int RB, int KW, bool AKC>
-__global__ __launch_bounds__(256) void lora_inner_tile_kernel(const LoraParams p) {
+__global__ __launch_bounds__(256, RB <= 4 ? 3 : 1) void lora_inner_tile_kernel(const LoraParams p) {
   using C = LoraInnerCfg<RB, KW>;
-  constexpr int ROWS = KW == 1 ? 64 : 16;
+  constexpr int ROWS = 64 / KW;
   constexpr int XS = C::KWAVE / 32;  // 32-k steps of a wave per stage
-  constexpr int RED = KW > 1 ? (KW - 1) * RB * 64 * 16 : 0;
+  constexpr int RED = 4 * (KW - 1) / KW * RB * 64 * 16;
   constexpr int A_LDS = RB * 16 * C::LDB;
   __shared__ __attribute__((aligned(16))) char lds[A_LDS > RED ? A_LDS : RED];
   __shared__ int32_t s_row[ROWS], s_id[ROWS];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int fr = lane & 15, fq = lane >> 4;
-  const int64_t m0 = (int64_t)blockIdx.x * ROWS;
+  // Tiles that stand together on one XCD, whose L2 then holds their adapters; the
+  // first turns of all tiles before the second (mixed, the tiles with work came to
+  // every fourth CU).
+  const uint32_t tiles = gridDim.x / kLoraInnerTurns;
+  const uint32_t tile = xcd_remap((uint32_t)blockIdx.x % tiles, tiles);
+  const int my_turn = (int)(blockIdx.x / tiles);
+  const int64_t m0 = (int64_t)tile * ROWS;
   const int32_t rank = (int32_t)p.rank;  // at most 16 RB
   if (tid < ROWS) {
     const int64_t m = m0 + tid;
@@ -68,33 +83,33 @@ __global__ __launch_bounds__(256) void lora_inner_tile_kernel(const LoraParams p
     s_id[tid] = row >= 0 ? lora_id(p, row) : -1;
   }
   __syncthreads();
-  const int my = KW == 1 ? wave * 16 + fr : fr;  // the tile row of this lane's operand
+  const int my = wave / KW * 16 + fr;  // the tile row of this lane's operand
   const int32_t row = s_row[my], my_id = s_id[my];
   const OpT* xrow = reinterpret_cast<const OpT*>(p.x) + (int64_t)(row >= 0 ? row : 0) * p.x_ld;
-  const int k_wave = KW == 1 ? 0 : wave * C::KWAVE;
+  const int k_part = wave % KW, k_wave = k_part * C::KWAVE;
   const int32_t K = (int32_t)p.K;
 
   f32x4_t res[RB];  // res[b]: rank 16 b + 4 fq + {0..3} of row `my`
 #pragma unroll
   for (int b = 0; b < RB; ++b) res[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  bool made = my_id < 0 && blockIdx.y == 0;  // the row is this workgroup's to write
+  bool made = my_id < 0 && my_turn == 0;  // the row is this workgroup's to write
   int turn = 0;
   for (int32_t cur = -1;;) {
     int32_t a = lane < ROWS ? s_id[lane % ROWS] : -1;
     a = wave_min_i32(a > cur ? a : INT32_MAX);
     if (a == INT32_MAX) break;
     cur = a;
-    if (turn++ % kLoraInnerTurns != (int)blockIdx.y) continue;
+    if (turn++ % kLoraInnerTurns != my_turn) continue;
     const bool mine = my_id == a;
     made |= mine;
-    const bool any = KW > 1 || __ballot(mine) != 0;  // a wave without rows of it still stages A
+    const bool any = __ballot(mine) != 0;  // (a wave without rows of it still stages A)
     const OpT* am = reinterpret_cast<const OpT*>(p.a) + a * p.a_se;
-    uint4 x0[XS], x1[XS], av[C::PER][8];
-    auto load_x = [&](int32_t k0, uint4 (&xv)[XS]) {
+    uint4 xv[XS], av[C::PER][8];
+    auto load_x = [&](int32_t k0) {
 #pragma unroll
       for (int s = 0; s < XS; ++s) {
         const int32_t k = k0 + k_wave + s * 32 + fq * 8;
-        xv[s] = any && mine && k < K ? *reinterpret_cast<const uint4*>(xrow + k) : make_uint4(0, 0, 0, 0);
+        xv[s] = *reinterpret_cast<const uint4*>(xrow + (k < K ? k : K - 8));
       }
     };
     // blocks of 8 k x 8 of the rank
@@ -104,21 +119,23 @@ __global__ __launch_bounds__(256) void lora_inner_tile_kernel(const LoraParams p
         const int i = u * 256 + tid;
         const int ro = AKC ? i / (C::KS / 8) : i % (RB * 2), ko = AKC ? i % (C::KS / 8) : i / (RB * 2);
         const int32_t k = k0 + ko * 8, r = ro * 8;
-        const bool in = i < C::CHUNKS / 8 && k < K && r < rank;
+        if (C::CHUNKS / 8 % 256 != 0 && i >= C::CHUNKS / 8) break;  // (whole waves)
+        const OpT* at = am + (int64_t)(r < rank ? r : 0) * p.a_sr + (int64_t)(k < K ? k : 0) * p.a_sk;
 #pragma unroll
         for (int v = 0; v < 8; ++v) {
-          const OpT* at = AKC ? am + (int64_t)(r + v) * p.a_sr + k : am + (int64_t)(k + v) * p.a_sk + r;
-          av[u][v] = in ? *reinterpret_cast<const uint4*>(at) : make_uint4(0, 0, 0, 0);
+          av[u][v] = *reinterpret_cast<const uint4*>(at + v * (AKC ? p.a_sr : p.a_sk));
         }
       }
     };
-    auto store_a = [&]() {
+    auto store_a = [&](int32_t k0) {
 #pragma unroll
       for (int u = 0; u < C::PER; ++u) {
         const int i = u * 256 + tid;
         if (i >= C::CHUNKS / 8) break;
         const int ro = AKC ? i / (C::KS / 8) : i % (RB * 2), ko = AKC ? i % (C::KS / 8) : i / (RB * 2);
         char* at = lds + ro * 8 * C::LDB + (ko ^ (ro & 7)) * 16;  // (8 threads' writes: 8 chunks)
+#pragma unroll
+        for (int v = 0; v < 8; ++v) av[u][v] = keep_if(av[u][v], k0 + ko * 8 < K && ro * 8 < rank);
         if constexpr (AKC) {
 #pragma unroll
           for (int v = 0; v < 8; ++v) *reinterpret_cast<uint4*>(at + v * C::LDB) = av[u][v];
@@ -133,55 +150,61 @@ __global__ __launch_bounds__(256) void lora_inner_tile_kernel(const LoraParams p
     f32x4_t acc[RB];
 #pragma unroll
     for (int b = 0; b < RB; ++b) acc[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    // a stage: A's values, loaded one stage ahead, go to LDS; x is two ahead.  The
-    // stages in turn from one that depends on the tile: in step, all tiles read the
-    // same columns of rows that lie a power of two apart, which a few of the memory's
-    // channels hold
+    // The stages in turn from one that depends on the tile: in step, all tiles read
+    // the same columns of rows that lie a power of two apart, which a few of the
+    // memory's channels hold.
     const int32_t stages = (K + C::KS - 1) / C::KS;
-    const int32_t first = (int32_t)(blockIdx.x % (uint32_t)stages);
+    const int32_t first = (int32_t)(tile % (uint32_t)stages);
     auto at = [&](int32_t i) { return (i + first < stages ? i + first : i + first - stages) * C::KS; };
-    auto stage = [&](int32_t i, uint4 (&xv)[XS]) {
-      if (i >= stages) return;
+    load_a(at(0));
+    load_x(at(0));
+    for (int32_t i = 0; i < stages; ++i) {
       __syncthreads();  // the last stage's reads
-      store_a();
+      const int32_t k0 = at(i);
+      store_a(k0);
       uint4 xc[XS];
 #pragma unroll
-      for (int s = 0; s < XS; ++s) xc[s] = xv[s];
-      __syncthreads();
-      if (i + 1 < stages) load_a(at(i + 1));
-      if (i + 2 < stages) load_x(at(i + 2), xv);
-      if (any) {
-#pragma unroll
-        for (int s = 0; s < XS; ++s)
-#pragma unroll
-          for (int b = 0; b < RB; ++b) {
-            const uint4 w = *reinterpret_cast<const uint4*>(
-                lds + (b * 16 + fr) * C::LDB + ((k_wave / 8 + s * 4 + fq) ^ ((b * 2 + fr / 8) & 7)) * 16);
-            MfmaOp<OpT>::step(acc[b], w, xc[s]);
-          }
+      for (int s = 0; s < XS; ++s) xc[s] = keep_if(xv[s], k0 + k_wave + s * 32 + fq * 8 < K);
+      lds_barrier();
+      if (i + 1 < stages) {
+        load_a(at(i + 1));
+        load_x(at(i + 1));
       }
-    };
-    load_a(at(0));
-    load_x(at(0), x0);
-    if (stages > 1) load_x(at(1), x1);
-    for (int32_t i = 0; i < stages; i += 2) {
-      stage(i, x0);
-      stage(i + 1, x1);
+      if (any) {
+        // (one step's operands are read while the last's products run)
+        uint4 w[2][RB];
+        auto read_w = [&](int s) {
+#pragma unroll
+          for (int b = 0; b < RB; ++b)
+            w[s & 1][b] = *reinterpret_cast<const uint4*>(
+                lds + (b * 16 + fr) * C::LDB + ((k_wave / 8 + s * 4 + fq) ^ ((b * 2 + fr / 8) & 7)) * 16);
+        };
+        read_w(0);
+#pragma unroll
+        for (int s = 0; s < XS; ++s) {
+          if (s + 1 < XS) read_w(s + 1);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int b = 0; b < RB; ++b) MfmaOp<OpT>::step(acc[b], w[s & 1][b], xc[s]);
+        }
+      }
     }
     if constexpr (KW > 1) {
       // the waves' sums, added in wave order by the first
+      const int group = wave / KW * (KW - 1);
       __syncthreads();
-      if (wave > 0) {
+      if (k_part > 0) {
 #pragma unroll
         for (int b = 0; b < RB; ++b)
-          *reinterpret_cast<f32x4_t*>(lds + (((wave - 1) * RB + b) * 64 + lane) * 16) = acc[b];
+          *reinterpret_cast<f32x4_t*>(lds + (((group + k_part - 1) * RB + b) * 64 + lane) * 16) = acc[b];
       }
       __syncthreads();
-      if (wave == 0) {
+      if (k_part == 0) {
 #pragma unroll
         for (int w = 0; w < KW - 1; ++w)
 #pragma unroll
-          for (int b = 0; b < RB; ++b) acc[b] += *reinterpret_cast<const f32x4_t*>(lds + ((w * RB + b) * 64 + lane) * 16);
+          for (int b = 0; b < RB; ++b)
+            acc[b] += *reinterpret_cast<const f32x4_t*>(lds + (((group + w) * RB + b) * 64 + lane) * 16);
       }
     }
     const float sc = lora_scale(p, a);
@@ -190,7 +213,7 @@ __global__ __launch_bounds__(256) void lora_inner_tile_kernel(const LoraParams p
       for (int b = 0; b < RB; ++b) res[b] = sc * acc[b];
     }
   }
-  if (!made || (KW > 1 && wave != 0)) return;
+  if (!made || k_part != 0) return;
   OpT* h = reinterpret_cast<OpT*>(p.h);
   OpT* ht = reinterpret_cast<OpT*>(p.ht);
 #pragma unroll
@@ -375,40 +398,46 @@ __global__ __launch_bounds__(256) void lora_wgrad_fast_kernel(const LoraWgradPar
 #pragma unroll
     for (int b = 0; b < RB; ++b) acc[j][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   const bool col_in = c0 < width;
+  const OpT* col = rows + (col_in ? c0 : 0);
   uint4 xv[8], tv[RB];
+  uint32_t x_in = 0;  // which of them count, as bits
   auto load = [&](int64_t s) {
     const int64_t q0 = base + s * 32 + fq * 8;
+    int64_t at[8];
 #pragma unroll
     for (int v = 0; v < 8; ++v) {
       const int64_t q = q0 + v;
-      xv[v] = make_uint4(0, 0, 0, 0);
-      if (q >= lo && q < hi && col_in) {
-        const int64_t row = p.order[q];
-        if (row >= 0 && row < p.rows) xv[v] = *reinterpret_cast<const uint4*>(rows + row * ld + c0);
-      }
+      at[v] = p.order[q < lo ? lo : q < hi ? q : hi - 1];
+    }
+#pragma unroll
+    for (int v = 0; v < 8; ++v) {
+      const bool in = q0 + v >= lo && q0 + v < hi && at[v] >= 0 && at[v] < p.rows;
+      xv[v] = *reinterpret_cast<const uint4*>(col + (in ? at[v] : 0) * ld);
+      x_in = v == 0 ? (in ? 1u : 0u) : x_in | (in ? 1u << v : 0u);
     }
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
       const int64_t r = r0 + b * 16 + fr;
-      Chunk16 c;
-      c.u = r < p.rank && q0 < hi ? *reinterpret_cast<const uint4*>(t + r * p.t_ld + q0) : make_uint4(0, 0, 0, 0);
-      // the neighbours' rows: zeros, whatever they hold
-      if (q0 < lo || q0 + 8 > hi) {
-#pragma unroll
-        for (int v = 0; v < 8; ++v)
-          if (q0 + v < lo || q0 + v >= hi) c.s[v] = 0;
-      }
-      tv[b] = c.u;
+      tv[b] = *reinterpret_cast<const uint4*>(t + (r < p.rank && q0 < hi ? r * p.t_ld + q0 : 0));
     }
   };
   int64_t s = s_from + wave;
   if (s < s_to) load(s);
   for (; s < s_to; s += 4) {
     uint4 xc[8], xt[8], tc[RB];
+    // the neighbours' rows: zeros, whatever they hold
 #pragma unroll
-    for (int v = 0; v < 8; ++v) xc[v] = xv[v];
+    for (int v = 0; v < 8; ++v) xc[v] = keep_if(xv[v], (x_in >> v) & 1u);
 #pragma unroll
-    for (int b = 0; b < RB; ++b) tc[b] = tv[b];
+    for (int b = 0; b < RB; ++b) {
+      Chunk16 c;
+      c.u = tv[b];
+      const bool in = r0 + b * 16 + fr < p.rank;
+#pragma unroll
+      for (int v = 0; v < 8; ++v)
+        if (!in || !((x_in >> v) & 1u)) c.s[v] = 0;
+      tc[b] = c.u;
+    }
     if (s + 4 < s_to) load(s + 4);
     lora_transpose8(xc, xt);
 #pragma unroll
