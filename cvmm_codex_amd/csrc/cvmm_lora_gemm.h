@@ -144,7 +144,7 @@ struct LoraTile {
   static constexpr int OCC = MI * NJ > 16 || LDS > 80 * 1024 ? 1 : 2;
   static constexpr bool AGPR = MI * NJ == 64;
   static constexpr bool MIXED = A_INSTS % D != 0;  // a wave loads pieces of x and of W
-  static_assert((STAGES - 2) * D < 64, "vmcnt range");
+  static_assert(STAGES >= 1 && STAGES * D < 64, "vmcnt range");
 };
 
 // Lane offset of load `inst` of a slice's B half, and the k that its piece starts
@@ -350,7 +350,8 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW, STAGES>::OCC)) voi
 
   // ---- the shared weights
   using WFrag = std::conditional_t<WKC, lds_u32x4[NJ], lds_u32x2[NJ][2]>;
-  if (S > 0) {
+  if (STAGES > 1 && S > 0) {  // (one stage: calls without W)
+    constexpr int kAhead = STAGES > 1 ? STAGES - 2 : 0;
 #pragma unroll
     for (int s = 0; s < STAGES; ++s) {
       static_for<D>([&](auto j) { issue_part(j, ring + s * SLICE); });
@@ -359,7 +360,7 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW, STAGES>::OCC)) voi
     }
     lds_u32x4 a0[MI], a1[MI];
     WFrag b0, b1;
-    vm_wait<(STAGES - 1) * D>();
+    vm_wait<(kAhead + 1) * D>();
     lds_barrier();
     read_all(std::integral_constant<int, 0>(), std::integral_constant<int, 0>(), a0, b0);
     // The products of a half of the slice in buffer B, with the next half's reads and
@@ -393,7 +394,7 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW, STAGES>::OCC)) voi
     // wave has the second in registers, so that the buffer takes slice s + STAGES.
     auto slice = [&](auto bc) {
       half(bc, std::integral_constant<int, 0>(), a0, b0, a1, b1);
-      vm_wait<(STAGES - 2) * D>();  // slice s + 1 has landed
+      vm_wait<kAhead * D>();  // slice s + 1 has landed
       lds_barrier();
       half(bc, std::integral_constant<int, 1>(), a1, b1, a0, b0);
     };
@@ -589,7 +590,10 @@ hipError_t launch_lora_gemm_kc(const LoraParams& p, hipStream_t s) {
   using i2 = integral_constant<int, 2>;
   using i4 = integral_constant<int, 4>;
   using i8 = integral_constant<int, 8>;
-  if (p.w == nullptr) return go(i2(), i4(), i2(), i2(), i2());
+  // without W the reads of base and the stores are all there is: small tiles with one
+  // buffer, so that a CU holds more of them (16384 rows of 1024 of base and 8 adapters of
+  // rank 32: 24.7 us, 29 with a ring of two)
+  if (p.w == nullptr) return go(i2(), i4(), i2(), i2(), integral_constant<int, 1>());
   if (tiles(256, 256) >= 192) return go(i8(), i8(), i2(), i2(), i2());
   if (tiles(256, 128) >= 192) return go(i8(), i4(), i2(), i2(), integral_constant<int, 3>());
   if (tiles(128, 128) >= 192) return go(i4(), i4(), i2(), i2(), i2());

@@ -381,14 +381,16 @@ __global__ __launch_bounds__(256) void lora_wgrad_fast_kernel(const LoraWgradPar
   if ((in ? p.ga : p.gb) == nullptr) return;
   const int64_t c0 = (in ? blockIdx.x : blockIdx.x - bi) * 128 + fr * 8;
   const int64_t r0 = (int64_t)blockIdx.y * RB * 16;
-  const int32_t e = blockIdx.z / p.shares, share = blockIdx.z % p.shares;
-  const int64_t lo = e > 0 && p.offsets[e - 1] > 0 ? p.offsets[e - 1] : 0;
-  const int64_t hi = p.offsets[e] < p.rows ? p.offsets[e] : p.rows;
-  const int64_t len = hi > lo ? hi - lo : 0;
-  // shares of whole steps
-  const int64_t base = lo & ~(int64_t)31;
-  const int64_t steps = len > 0 ? (hi - base + 31) / 32 : 0;
-  const int64_t s_from = steps * share / p.shares, s_to = steps * (share + 1) / p.shares;
+  const int32_t e = (int32_t)(blockIdx.z / (uint32_t)p.shares), share = (int32_t)(blockIdx.z % (uint32_t)p.shares);
+  // (32 bits: at most 2^31 - 1 rows)
+  const int64_t lo64 = p.offsets[e > 0 ? e - 1 : 0], hi64 = p.offsets[e], rows64 = p.rows;
+  const int32_t lo = e > 0 && lo64 > 0 ? (int32_t)(lo64 < rows64 ? lo64 : rows64) : 0;
+  const int32_t hi = hi64 < 0 ? 0 : (int32_t)(hi64 < rows64 ? hi64 : rows64);
+  // shares of whole steps (a power of two of them)
+  const int32_t base = lo & ~31;
+  const int32_t steps = hi > lo ? (hi - base + 31) / 32 : 0;
+  const int sh = __builtin_ctz(p.shares);
+  const int32_t s_from = (int32_t)(((int64_t)steps * share) >> sh), s_to = (int32_t)(((int64_t)steps * (share + 1)) >> sh);
   const OpT* rows = reinterpret_cast<const OpT*>(in ? p.x : p.g);
   const int64_t ld = in ? p.x_ld : p.g_ld, width = in ? p.d_in : p.d_out;
   const OpT* t = reinterpret_cast<const OpT*>(in ? p.ut : p.ht);
@@ -401,12 +403,12 @@ __global__ __launch_bounds__(256) void lora_wgrad_fast_kernel(const LoraWgradPar
   const OpT* col = rows + (col_in ? c0 : 0);
   uint4 xv[8], tv[RB];
   uint32_t x_in = 0;  // which of them count, as bits
-  auto load = [&](int64_t s) {
-    const int64_t q0 = base + s * 32 + fq * 8;
+  auto load = [&](int32_t s) {
+    const int32_t q0 = base + s * 32 + fq * 8;
     int64_t at[8];
 #pragma unroll
     for (int v = 0; v < 8; ++v) {
-      const int64_t q = q0 + v;
+      const int32_t q = q0 + v;
       at[v] = p.order[q < lo ? lo : q < hi ? q : hi - 1];
     }
 #pragma unroll
@@ -421,7 +423,7 @@ __global__ __launch_bounds__(256) void lora_wgrad_fast_kernel(const LoraWgradPar
       tv[b] = *reinterpret_cast<const uint4*>(t + (r < p.rank && q0 < hi ? r * p.t_ld + q0 : 0));
     }
   };
-  int64_t s = s_from + wave;
+  int32_t s = s_from + wave;
   if (s < s_to) load(s);
   for (; s < s_to; s += 4) {
     uint4 xc[8], xt[8], tc[RB];
