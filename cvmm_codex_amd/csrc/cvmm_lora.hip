@@ -247,18 +247,27 @@ bool fast_ok(const LoraParams& p, int32_t op) {
          (p.w == nullptr || (pieces(p.w, 0, p.w_sk, p.w_sn) && reach(p.K, p.w_sk, p.w_sn)));
 }
 
-// Rows up to which a call is two launches of plain multiply-adds beside a GEMM
-// split along k.
-constexpr int64_t kLoraFewRows = 256;
-bool few_rows(int64_t rows) { return rows <= kLoraFewRows; }
+// Calls that are two launches of plain multiply-adds beside a GEMM split along k:
+// the tiles of the others take one adapter after the other, which rows of many
+// adapters pay for.  Whole calls of 2048 -> 2048 in us, this way / by tiles:
+//   rows of 32 adapters  rank 16: 256 20.1 / 88.9, 512 29.7 / 93.1, 768 38 / 93;
+//                        rank 64: 256 36.3 / 126, 512 60.3 / 127
+//   rows of one or two   rank 16: 256 20.0 / 25.4, 512 29.2 / 26.4, 768 37 / 27;
+//                        rank 64: 256 35.4 / 31.1, 512 58.0 / 31.9
+// The ids are not known here; the limits are where the second kind, a prompt's, loses
+// a few us at most.
+bool few_rows(int64_t rows, int64_t rank) { return rows <= (rank <= 16 ? 512 : 256); }
 
-// Workgroups of the split GEMM (64 x 128 tiles) and shares of the inner rows:
-// enough for every CU, at least 64 k each.
+// Workgroups of the split GEMM (64 x 128 tiles): one per CU, with 256 k each where
+// k allows (32 rows of 2048 -> 2048: 9.3 us, 11.2 with 128 each and 10.8 with 512; 8
+// rows of 4096 -> 4096: 13.2 with 512 k each in 256 workgroups, 16.8 with 1024 in
+// 128).  Shares of the inner rows: four loads a thread (32 rows: 11.2 us; one 12.1,
+// sixteen 13.5).
 LoraSplit few_split(int64_t rows, int64_t K, int64_t N, int64_t rank) {
   LoraSplit sp{};
   const int64_t tiles = ((rows + 63) / 64) * ((N + 127) / 128), all = (K + 63) / 64;
   int64_t splits = (256 + tiles - 1) / tiles;
-  if (splits > all) splits = all;
+  if (splits > all / 4) splits = all / 4;
   if (splits < 1) splits = 1;
   sp.slices = (int32_t)((all + splits - 1) / splits);
   sp.splits = (int32_t)((all + sp.slices - 1) / sp.slices);
@@ -304,7 +313,7 @@ hipError_t launch_fast(const LoraParams& q, void* ws, hipStream_t s) {
   LoraParams p = q;
   p.out_vec = al16(p.out) && p.out_ld % 8 == 0 && p.n_out % 8 == 0;
   p.base_vec = p.base != nullptr && al16(p.base) && p.base_ld % 4 == 0;
-  if (few_rows(p.rows) && p.ht == nullptr) {
+  if (few_rows(p.rows, p.rank) && p.ht == nullptr) {
     LoraSplit sp = few_split(p.rows, p.K, p.N, p.rank);
     sp.h_part = (float*)ws;
     if (p.w != nullptr)
@@ -325,7 +334,7 @@ size_t lora_workspace_bytes(int64_t rows, int32_t n, int64_t K, int64_t N, int64
                             bool copied) {
   size_t own = h_bytes(rows, rank, op);
   if (op == kF32) return own;
-  if (few_rows(rows)) {
+  if (few_rows(rows, pad8(rank))) {
     const LoraSplit sp = few_split(rows, pad8(K), pad8(N), pad8(rank));
     const size_t few = align_up((size_t)sp.h_splits * (size_t)(rows * pad8(rank)) * 4, 256) +
                        (weight ? (size_t)sp.splits * (size_t)rows * (size_t)sp.part_ld * 4 : 0);
@@ -456,8 +465,10 @@ __global__ __launch_bounds__(256) void lora_wgrad_sum_kernel(const LoraWgradPara
 
 static int32_t lora_wgrad_shares(int64_t rows, int32_t n, int64_t d_in, int64_t d_out, int64_t rank) {
   const int64_t blocks = ((d_in + 127) / 128 + (d_out + 127) / 128) * ((rank + 63) / 64) * n;
+  // (8192 rows, 4 adapters of rank 32, 1024 -> 1024, forward and backward: 107 us; for
+  // 128 workgroups 110, for 1024 119)
   int64_t s = 1;
-  while (s < 64 && blocks * s < 512 && rows / (n * s) > 128) s *= 2;
+  while (s < 64 && blocks * s < 256 && rows / (n * s) > 128) s *= 2;
   return (int32_t)s;
 }
 

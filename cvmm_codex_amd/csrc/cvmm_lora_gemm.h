@@ -594,9 +594,20 @@ hipError_t launch_lora_gemm_kc(const LoraParams& p, hipStream_t s) {
   // buffer, so that a CU holds more of them (16384 rows of 1024 of base and 8 adapters of
   // rank 32: 24.7 us, 29 with a ring of two)
   if (p.w == nullptr) return go(i2(), i4(), i2(), i2(), integral_constant<int, 1>());
-  if (tiles(256, 256) >= 192) return go(i8(), i8(), i2(), i2(), i2());
-  if (tiles(256, 128) >= 192) return go(i8(), i4(), i2(), i2(), integral_constant<int, 3>());
-  if (tiles(128, 128) >= 192) return go(i4(), i4(), i2(), i2(), i2());
+  // Otherwise the tile of least time, by rounds of tiles over the 256 CUs.  At 2048 k
+  // a round took 53 us of 256 x 256 (one on a CU), 33 of 128 x 128 (two on a CU; 29 when
+  // each has one) and 17 of 64 x 128 (one); at 1024 k in the same proportion.  Whole
+  // calls of rank 32 in us, with 256 x 256 / 128 x 128 / 64 x 128 tiles:
+  //   rows x k x columns  1024 x 2048 x 2048: 62 / 39 / 28.5;  4096 x 2048 x 2048: 61 / 47 / 76;
+  //   12288 x 2048 x 2048: 124 / 120 / 207;  16384 x 2048 x 2048: 136 / 152 / 270;
+  //   2560 x 1024 x 1024: 41 / 22 / 26;  12288 x 2048 x 1024: 71 / 76 / 109
+  // (256 x 128 tiles in a ring of three were behind one of these at every size).
+  auto rounds = [](int64_t t, int64_t per) { return (t + per - 1) / per; };
+  const int64_t t128 = tiles(128, 128);
+  const int64_t c256 = 53 * rounds(tiles(256, 256), 256), c64 = 17 * rounds(tiles(64, 128), 256);
+  const int64_t c128 = 33 * rounds(t128, 512) - (t128 % 512 > 0 && t128 % 512 <= 256 ? 4 : 0);
+  if (c256 <= c128 && c256 <= c64) return go(i8(), i8(), i2(), i2(), i2());
+  if (c128 <= c64) return go(i4(), i4(), i2(), i2(), i2());
   return go(i2(), i4(), i2(), i2(), i4());
 }
 
@@ -626,6 +637,9 @@ hipError_t launch_lora_inner_op(const LoraParams& p, hipStream_t s) {
     else if (p.rank <= 128) go(integral_constant<int, 8>(), kw);
     else go(integral_constant<int, 16>(), kw);
   };
+  // (whole calls of 2048 -> 1024 at rank 64 in us, k shared by 2 waves / 4: 4096 rows 45.7 /
+  // 41.7, 8192 57.1 / 60.5, 16384 85.4 / 103.2: few rows need more workgroups, many fewer
+  // readers of A)
   if (p.rows >= 8192) by_rank(std::integral_constant<int, 2>());
   else by_rank(std::integral_constant<int, 4>());
   return hipGetLastError();
