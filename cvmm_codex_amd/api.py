@@ -1290,7 +1290,7 @@ def cvmm_lora(x: torch.Tensor, adapters: Union[torch.Tensor, CVMMSel], a: torch.
     to it once, all sums are fp32 and the output is rounded once.  In fp16 those
     inner values must stay below 65520.  An adapter's infinities and NaN reach its
     own rows only.  Gradients flow to x, a, b and base; the adapters' are summed in a
-    fixed order."""
+    fixed order; no second derivatives."""
     _require_device(x, "x")
     op = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
     if op not in _DTYPE_IDS:
@@ -1334,8 +1334,11 @@ def cvmm_lora(x: torch.Tensor, adapters: Union[torch.Tensor, CVMMSel], a: torch.
             raise ValueError(f"cvmm_lora: the selection's {ids.numel()} routes are not the {x.numel() // d_in} rows of x")
         if ids.numel() > 0:
             adapters._resolve(n)
-            order = adapters._out_index if adapters._out_index is not None else adapters._sel_index
-            offsets = _offsets_for(adapters._sel, n)
+            # this library's own sorts put rows without an adapter last; a selection built
+            # by hand may have them first, as rows of adapter 0, and is sorted again
+            if _compiling() or hasattr(adapters._sel, "_cvmm_i32"):
+                order = adapters._out_index if adapters._out_index is not None else adapters._sel_index
+                offsets = _offsets_for(adapters._sel, n)
     else:
         ids = adapters
         _require_device(ids, "adapters")

@@ -332,6 +332,27 @@ def test_compiled_with_gradients(weight, base, presorted):
         assert e.dtype == c.dtype and torch.equal(e, c)
 
 
+@pytest.mark.parametrize("T", [20, 700])
+def test_selection_built_by_hand(T):
+    """Rows without an adapter sorted first (ids below 0), their infinities and NaN in
+    no adapter's gradient."""
+    t = _make(T, 128, 64, 16, 5, "own", BF, False, False, 8)
+    t["ids"][::7] = -1
+    none = t["ids"] < 0
+    t["x"][none], t["grad"][none] = NAN, INF
+    ids = t["ids"].cuda()
+    key, at = torch.sort(ids, stable=True)
+    outs = []
+    for sel in (ids, C.CVMMSel(ids, key, at), C.cvmm_prepare_sel(ids, 5), C.cvmm_prepare_sel2(ids.view(T, 1))):
+        x, a, b, g = _dev(t, "x", "a", "b", "grad")
+        x, a, b = (v.requires_grad_() for v in (x, a, b))
+        y = C.cvmm_lora(x, sel, a, b)
+        outs.append((y, *torch.autograd.grad(y, [x, a, b], g)))
+    assert all(bool(v.isfinite().all()) for v in outs[0])
+    for out in outs[1:]:
+        assert all(torch.equal(v, w) for v, w in zip(outs[0], out))
+
+
 def test_forward_mode_is_refused():
     t = _make(9, 16, 8, 4, 2, "own", F32)
     x, ids, a, b, w = _dev(t, "x", "ids", "a", "b", "weight")
