@@ -401,12 +401,15 @@ class CVMMSel:
         self.reduction_weight = reduction_weight
         self._routing = None
         self._route_mode = False
+        self._sorted_for: Optional[int] = None   # expert count of this library's sort
 
     def clone(self) -> "CVMMSel":
         if self._pending():
             return CVMMSel._deferred(self._raw_shape_tensor(), self._routing, self._route_mode,
                                      self.reduction_weight)
-        return CVMMSel(self.raw_sel, self.sel, self.sel_index, self.out_index, self.reduction_weight)
+        out = CVMMSel(self.raw_sel, self.sel, self.sel_index, self.out_index, self.reduction_weight)
+        out._sorted_for = self._sorted_for
+        return out
 
     @classmethod
     def _deferred(cls, raw_src: torch.Tensor, routing: "_Routing", route_mode: bool, w) -> "CVMMSel":
@@ -438,6 +441,7 @@ class CVMMSel:
             sel._cvmm_offsets = {e: v[3] for e, v in r.by_e.items()}
             sel._cvmm_i32 = ssel
         self._sel = sel
+        self._sorted_for = n_experts if n_experts is not None else r.first_e
         if self._route_mode:
             self._sel_index, self._out_index = perm, None
         else:
@@ -463,6 +467,7 @@ def _get_raw_sel(self):
 def _set_raw_sel(self, v):
     self._raw_sel = v
     self._raw_src = None
+    self._sorted_for = None
 
 
 def _resolved_field(name):
@@ -475,6 +480,7 @@ def _resolved_field(name):
     def set_(self, v):
         self._resolve()
         setattr(self, attr, v)
+        self._sorted_for = None
 
     return property(get, set_)
 
@@ -507,6 +513,7 @@ def cvmm_prepare_sel(sel: torch.Tensor, n_experts: int) -> CVMMSel:
     s._cvmm_i32 = ssel
     out = CVMMSel(None, s, perm, None)
     out._raw_src = sel
+    out._sorted_for = n_experts
     return out
 
 
@@ -526,7 +533,7 @@ def cvmm_prepare_sel2(sel: Union[torch.Tensor, CVMMSel], w: Optional[torch.Tenso
         else:
             out = CVMMSel(None, sel.sel, sel.sel_index, sel.out_index, w)
         # raw_sel as the parent holds it: its int32 copy is made if it is read
-        out._raw_sel, out._raw_src = sel._raw_sel, sel._raw_src
+        out._raw_sel, out._raw_src, out._sorted_for = sel._raw_sel, sel._raw_src, sel._sorted_for
         return out
 
     n_per_batch = sel.shape[-1]
@@ -1334,9 +1341,10 @@ def cvmm_lora(x: torch.Tensor, adapters: Union[torch.Tensor, CVMMSel], a: torch.
             raise ValueError(f"cvmm_lora: the selection's {ids.numel()} routes are not the {x.numel() // d_in} rows of x")
         if ids.numel() > 0:
             adapters._resolve(n)
-            # this library's own sorts put rows without an adapter last; a selection built
-            # by hand may have them first, as rows of adapter 0, and is sorted again
-            if _compiling() or hasattr(adapters._sel, "_cvmm_i32"):
+            # this library's own sorts put ids outside [0, n) last, in any order; one for another
+            # count, or built by hand (which may have them first, as rows of adapter 0), is
+            # not used and the ids are sorted again
+            if adapters._sorted_for == n:
                 order = adapters._out_index if adapters._out_index is not None else adapters._sel_index
                 offsets = _offsets_for(adapters._sel, n)
     else:

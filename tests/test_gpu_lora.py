@@ -353,6 +353,23 @@ def test_selection_built_by_hand(T):
         assert all(torch.equal(v, w) for v, w in zip(outs[0], out))
 
 
+@pytest.mark.parametrize("n", [3, 8, 12])
+def test_selection_sorted_for_another_count(n):
+    T = 500
+    t = _make(T, 128, 64, 16, n, "own", BF, False, False, 9)
+    ids = torch.randint(-2, 12, (T, 1), generator=torch.Generator().manual_seed(9)).cuda()
+    sel = C.cvmm_prepare_sel2(ids, route_input=True)
+    C.cvmm(torch.zeros(T, 1, 64, device="cuda", dtype=BF), sel, torch.zeros(8, 64, 64, device="cuda", dtype=BF))
+    outs = []
+    for s in (ids.view(T), sel, C.cvmm_prepare_sel2(sel, route_input=True)):
+        x, a, b, g = _dev(t, "x", "a", "b", "grad")
+        x, a, b = (v.requires_grad_() for v in (x, a, b))
+        y = C.cvmm_lora(x, s, a, b)
+        outs.append((y, *torch.autograd.grad(y, [x, a, b], g)))
+    for out in outs[1:]:
+        assert all(torch.equal(v, w) for v, w in zip(outs[0], out))
+
+
 def test_forward_mode_is_refused():
     t = _make(9, 16, 8, 4, 2, "own", F32)
     x, ids, a, b, w = _dev(t, "x", "ids", "a", "b", "weight")
