@@ -17,6 +17,9 @@
 // launches forward (chunks of tokens, then their sums in a fixed order) and one
 // backward.  Terms of a token are 32-bit; a chunk's sums
 // too (at most some hundred addends per lane); sums over chunks are 64-bit.
+// Measured (chunks, sums, backward), us: 512 tokens of 16 experts 4.4, 6.2, 3.4; 16384 of
+// 128 in bf16 5.4, 9.6, 7.3; 32768 of 256 in 8 sequences 12.8, 8.5, 20.9 (the last
+// 34 MB at 1.6 TB/s: exponentials, 8 a lane, and coefficients beside them).
 #include <cmath>
 
 #include "cvmm_common.h"
