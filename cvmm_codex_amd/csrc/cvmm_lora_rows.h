@@ -44,8 +44,10 @@ __device__ __forceinline__ uint4 keep_if(const uint4& v, bool keep) {
 // 16384 of 128: 11, the chain order, id, row, store.
 // ---------------------------------------------------------------------------
 // Workgroups that share the adapters of a tile, in turns: nearly all tiles have one
-// or two (a request ends within), and a second one, taken after the first, doubled
-// the launch (16384 rows of 2048, rank 64: 43 us).
+// or two (a request ends within), and a second one, taken after the first, made the
+// launch wait for the few tiles that have two (1999 rows of 2048 in runs of 8
+// adapters of rank 32, whole call without W: 23.9 us, with four turns 17.5; 16384
+// rows in runs that end with tiles: 30 either way).
 constexpr int kLoraInnerTurns = 4;
 
 template <int RB, int KW>
@@ -152,25 +154,18 @@ __global__ __launch_bounds__(256, RB <= 4 ? 3 : 1) void lora_inner_tile_kernel(c
     f32x4_t acc[RB];
 #pragma unroll
     for (int b = 0; b < RB; ++b) acc[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    // The stages in turn from one that depends on the tile: in step, all tiles read
-    // the same columns of rows that lie a power of two apart, which a few of the
-    // memory's channels hold.
-    const int32_t stages = (K + C::KS - 1) / C::KS;
-    const int32_t first = (int32_t)(tile % (uint32_t)stages);
-    auto at = [&](int32_t i) { return (i + first < stages ? i + first : i + first - stages) * C::KS; };
-    load_a(at(0));
-    load_x(at(0));
-    for (int32_t i = 0; i < stages; ++i) {
+    load_a(0);
+    load_x(0);
+    for (int32_t k0 = 0; k0 < K; k0 += C::KS) {
       __syncthreads();  // the last stage's reads
-      const int32_t k0 = at(i);
       store_a(k0);
       uint4 xc[XS];
 #pragma unroll
       for (int s = 0; s < XS; ++s) xc[s] = keep_if(xv[s], k0 + k_wave + s * 32 + fq * 8 < K);
       lds_barrier();
-      if (i + 1 < stages) {
-        load_a(at(i + 1));
-        load_x(at(i + 1));
+      if (k0 + C::KS < K) {
+        load_a(k0 + C::KS);
+        load_x(k0 + C::KS);
       }
       if (any) {
         // (one step's operands are read while the last's products run)
