@@ -312,7 +312,7 @@ template <typename OpT>
 hipError_t launch_fast(const LoraParams& q, void* ws, hipStream_t s) {
   LoraParams p = q;
   p.out_vec = al16(p.out) && p.out_ld % 8 == 0 && p.n_out % 8 == 0;
-  p.base_vec = p.base != nullptr && al16(p.base) && p.base_ld % 4 == 0;
+  p.base_vec = p.base != nullptr && al16(p.base) && p.base_ld % (p.base_dtype == kF32 ? 4 : 8) == 0;
   if (few_rows(p.rows, p.rank) && p.ht == nullptr) {
     LoraSplit sp = few_split(p.rows, p.K, p.N, p.rank);
     sp.h_part = (float*)ws;

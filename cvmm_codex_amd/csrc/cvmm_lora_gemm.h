@@ -312,22 +312,32 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW, STAGES>::OCC)) voi
     const int64_t row = s_row[(wm * MI + i) * 16 + fr];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) v[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    if (p.base == nullptr || row < 0) return;
-    const int64_t at = row * p.base_ld;
+    if (p.base == nullptr) return;
+    const int64_t at = (row >= 0 ? row : 0) * p.base_ld;  // (rows past the last are not stored)
     if (p.base_vec && nw + NJ * 16 <= p.n_out) {
       if (p.base_dtype == kF32) {
         const float* q = reinterpret_cast<const float*>(p.base) + at + nw + 4 * fq;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) v[j] = *reinterpret_cast<const f32x4_t*>(q + j * 16);
       } else {
-        const OpT* q = reinterpret_cast<const OpT*>(p.base) + at + nw + 4 * fq;
-        uint2 raw[NJ];
+        // as the stores below write it, and the lane swaps backwards
+        const OpT* q = reinterpret_cast<const OpT*>(p.base) + at + nw + 8 * fq;
+        uint4 raw[NJ / 2];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) raw[j] = *reinterpret_cast<const uint2*>(q + j * 16);
+        for (int j = 0; j < NJ / 2; ++j) raw[j] = *reinterpret_cast<const uint4*>(q + j * 32);
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const OpT* e = reinterpret_cast<const OpT*>(&raw[j]);
-          v[j] = f32x4_t{to_f32(e[0]), to_f32(e[1]), to_f32(e[2]), to_f32(e[3])};
+        for (int j = 0; j < NJ / 2; ++j) {
+          const auto s0 = __builtin_amdgcn_permlane16_swap(raw[j].x, raw[j].z, false, false);
+          const auto s1 = __builtin_amdgcn_permlane16_swap(raw[j].y, raw[j].w, false, false);
+          const auto u0 = __builtin_amdgcn_permlane32_swap(s0[0], s0[1], false, false);
+          const auto u1 = __builtin_amdgcn_permlane32_swap(s1[0], s1[1], false, false);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            union { uint32_t u[2]; OpT e[4]; } c;
+            c.u[0] = u0[h];
+            c.u[1] = u1[h];
+            v[2 * j + h] = f32x4_t{to_f32(c.e[0]), to_f32(c.e[1]), to_f32(c.e[2]), to_f32(c.e[3])};
+          }
         }
       }
       return;

@@ -406,14 +406,18 @@ __global__ __launch_bounds__(256) void lora_wgrad_fast_kernel(const LoraWgradPar
   const OpT* col = rows + (col_in ? c0 : 0);
   uint4 xv[8], tv[RB];
   uint32_t x_in = 0;  // which of them count, as bits
-  auto load = [&](int32_t s) {
-    const int32_t q0 = base + s * 32 + fq * 8;
-    int64_t at[8];
+  // the rows of the step after the one that is loaded: the order's loads do not stand
+  // before the rows' own
+  int64_t at[8];
+  auto load_order = [&](int32_t s) {
 #pragma unroll
     for (int v = 0; v < 8; ++v) {
-      const int32_t q = q0 + v;
+      const int32_t q = base + s * 32 + fq * 8 + v;
       at[v] = p.order[q < lo ? lo : q < hi ? q : hi - 1];
     }
+  };
+  auto load = [&](int32_t s) {
+    const int32_t q0 = base + s * 32 + fq * 8;
 #pragma unroll
     for (int v = 0; v < 8; ++v) {
       const bool in = q0 + v >= lo && q0 + v < hi && at[v] >= 0 && at[v] < p.rows;
@@ -425,9 +429,13 @@ __global__ __launch_bounds__(256) void lora_wgrad_fast_kernel(const LoraWgradPar
       const int64_t r = r0 + b * 16 + fr;
       tv[b] = *reinterpret_cast<const uint4*>(t + (r < p.rank && q0 < hi ? r * p.t_ld + q0 : 0));
     }
+    if (s + 4 < s_to) load_order(s + 4);
   };
   int32_t s = s_from + wave;
-  if (s < s_to) load(s);
+  if (s < s_to) {
+    load_order(s);
+    load(s);
+  }
   for (; s < s_to; s += 4) {
     uint4 xc[8], xt[8], tc[RB];
     // the neighbours' rows: zeros, whatever they hold
