@@ -1341,6 +1341,17 @@ def cvmm_lora(x: torch.Tensor, adapters: Union[torch.Tensor, CVMMSel], a: torch.
         if ids.numel() != x.numel() // d_in:
             raise ValueError(f"cvmm_lora: the selection's {ids.numel()} routes are not the {x.numel() // d_in} rows of x")
         if ids.numel() > 0:
+            r = adapters._routing
+            if not _compiling() and adapters._pending() and n not in r.by_e and n <= 32767:
+                # a recorded selection: its sort (if still to be made) and the product in
+                # one host call
+                bufs = r.buffers.get(n)
+                y, i32, i64 = N.host().lora_apply_recorded(
+                    x, r.raw, a, b, weight, base, scales, factor, r.k, r.counts(n) if bufs is None else None,
+                    *(bufs or (None, None)), _DTYPE_IDS[op], grad)
+                if bufs is None:
+                    r.keep(n, i32, i64)
+                return y
             adapters._resolve(n)
             # this library's own sorts put ids outside [0, n) last, in any order; one for another
             # count, or built by hand (which may have them first, as rows of adapter 0), is

@@ -1494,6 +1494,27 @@ Tensor lora_apply(const Tensor& x, const Tensor& ids, const Tensor& a, const Ten
   return out.view(shape);
 }
 
+// With a recorded selection in one call: sorted here unless its buffers are given.
+// Returns (y, i32, i64).
+std::tuple<Tensor, Tensor, Tensor> lora_apply_recorded(const Tensor& x, const Tensor& raw, const Tensor& a,
+                                                       const Tensor& b, const OptT& weight, const OptT& base,
+                                                       const OptT& scales, double scale, int64_t top_k,
+                                                       const OptT& counted_ws, const OptT& i32_in, const OptT& i64_in,
+                                                       int64_t op_id, bool grad) {
+  const LoraShape s = lora_check(x, raw, a, b, weight, base, scales);
+  c10::DeviceGuard guard(x.device());
+  Tensor i32, i64;
+  if (i32_in.has_value()) {
+    i32 = *i32_in;
+    i64 = *i64_in;
+  } else {
+    std::tie(i32, i64) = sort_routes_buffers(raw, s.n, top_k, current_stream(x), counted_ws);
+  }
+  return {lora_apply(x, raw, a, b, weight, base, scales, scale, i64.narrow(0, 0, s.rows),
+                     i64.narrow(0, 2 * s.rows, s.n), op_id, grad),
+          i32, i64};
+}
+
 // The Python-facing forward and backward (torch.compile's ops): no kept rows.
 Tensor forward_py(const Tensor& x, const Tensor& keys, const OptT& keys_op, bool keys_op_is_t, const Tensor& sel,
                   const Tensor& sel_index, const OptT& out_index, const Tensor& offsets, const OptT& route_pos,
@@ -1560,6 +1581,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("lora_forward", &lora_forward);
   m.def("lora_backward", &lora_backward);
   m.def("lora_apply", &lora_apply);
+  m.def("lora_apply_recorded", &lora_apply_recorded);
   // operand rules, exposed for tests
   m.def("storage_for", [](const Tensor& t, int64_t op_id) { return storage_for(t, dtype_of(op_id)); });
   m.def("keys_view", &keys_view);
