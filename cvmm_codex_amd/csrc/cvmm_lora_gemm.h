@@ -26,8 +26,8 @@
 // PFLOP/s; the library's product without adapters 113).  Bound by the matrix pipe,
 // busy for 60 % of the cycles: a further 2048 k cost 1.4 PFLOP/s, but each round of
 // tiles starts with an empty ring and ends with its CU's stores, 11 us together.
-// 8192 rows, 1024 -> 1024, rank 16: 25 (library 23.2), each way.
-// Without W, 16384 rows of 1024 with base, rank 16: 24.2, 67 MB at 2.8 TB/s: a tile
+// 8192 rows, 1024 -> 1024, rank 16: 24.6 (library 23.2), each way.
+// Without W, 16384 rows of 1024 with base, rank 16: 22.9, 67 MB at 2.9 TB/s: a tile
 // is a chain of loads (order, id, inner row) before its stores.
 #pragma once
 

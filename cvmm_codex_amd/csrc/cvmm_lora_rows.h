@@ -41,7 +41,7 @@ __device__ __forceinline__ uint4 keep_if(const uint4& v, bool keep) {
 // [k][rank].  Bound by reading x once; each workgroup reads its adapters whole,
 // from L2.  Measured: 16384 rows of 2048, rank 64: 29-32 us (67 MB at 2.2 TB/s: a
 // stage's A waits for its LDS turn); 8192 of 1024, rank 16: 11 (1.5 TB/s);
-// 16384 of 128: 11, the chain order, id, row, store.
+// 16384 of 128: 10, the chain order, id, row, store.
 // ---------------------------------------------------------------------------
 // Workgroups that share the adapters of a tile, in turns: nearly all tiles have one
 // or two (a request ends within), and a second one, taken after the first, made the
@@ -370,8 +370,8 @@ __global__ __launch_bounds__(kLoraJoinThreads) void lora_join_kernel(const LoraP
 // operands as they are.  No LDS in the loop; bound by reading x and g once.  The
 // waves of a workgroup share its rows; an adapter's rows are dealt out to `shares`
 // workgroups, whose partial sums the second launch adds in order.  Measured: 8192
-// rows, 8 adapters of rank 16, 1024 -> 1024: 14.9 us (34 MB at 2.3 TB/s) and 4.5 for the
-// sums; 16384 rows, 64 adapters, 128 -> 1024: 18.6 (38 MB at 2.0 TB/s): eight gathered
+// rows, 8 adapters of rank 16, 1024 -> 1024: 14.3 us (34 MB at 2.4 TB/s) and 4.5 for the
+// sums; 16384 rows, 64 adapters, 128 -> 1024: 18.2 (38 MB at 2.1 TB/s): eight gathered
 // rows in flight per lane.
 // ---------------------------------------------------------------------------
 template <typename OpT, int RB>
