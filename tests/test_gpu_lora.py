@@ -75,6 +75,8 @@ CASES = [
     # and of 128 x 128
     (3001, 160, 1032, 40, 6, "runs", F16, True, True),
     (3100, 33, 1000, 6, 11, "alternate", BF, True, False),
+    # copies of odd rows in a launch of their own
+    (4001, 1001, 72, 16, 3, "runs", BF, True, False),
 ]
 
 
