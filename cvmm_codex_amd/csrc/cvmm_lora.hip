@@ -394,6 +394,8 @@ hipError_t launch_lora(const LoraParams& q, int32_t op, void* ws, size_t ws_byte
   LoraParams p = q;
   p.n_out = p.N;
   p.rank_out = p.rank;
+  LoraPads pads{};
+  void* x_copy = nullptr;  // x's copy where it takes a launch of its own
   if (op != kF32 && !fast_ok(p, op)) {
     // copies of whole pieces, where there is room for them
     const bool weight = p.w != nullptr;
@@ -403,16 +405,13 @@ hipError_t launch_lora(const LoraParams& q, int32_t op, void* ws, size_t ws_byte
     constexpr size_t kMost = (size_t)1 << 34;
     if (c.x < kMost && c.w < kMost && c.a < kMost && c.b < kMost && ws_bytes >= own + c.total()) {
       char* at = (char*)ws + own;
-      LoraPads pads{};
       int64_t se = 0;
       if (p.K % 8 != 0 || p.x_ld % 8 != 0 || !al16(p.x)) {
         if (c.x <= kLoraPadRows) {
           int64_t unit = 1;
           add_pad(pads, p.x, se, p.x_ld, unit, 1, p.rows, p.K, at, false);
         } else {
-          const hipError_t e = launch_pad_rows(p.x, op, p.x_ld, p.rows, p.K, nullptr, 0, op, at, s);
-          if (e != hipSuccess) return e;
-          p.x = at;
+          p.x = x_copy = at;
           p.x_ld = pad8(p.K);
         }
       }
@@ -426,22 +425,31 @@ hipError_t launch_lora(const LoraParams& q, int32_t op, void* ws, size_t ws_byte
       at += c.a;
       if (p.N % 8 != 0 || p.rank % 8 != 0 || !pieces(p.b, p.b_se, p.b_sr, p.b_sn))
         add_pad(pads, p.b, p.b_se, p.b_sr, p.b_sn, p.n, p.rank, p.N, at);
-      if (pads.n > 0) {
-        hipLaunchKernelGGL(lora_pad_kernel, dim3(pads.of[pads.n - 1].end), dim3(256), 0, s, pads);
-        const hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
-      }
       p.K = pad8(p.K);
       p.N = pad8(p.N);
       p.rank = pad8(p.rank);
       p.h_ld = (p.rank + 31) / 32 * 32;
     }
   }
-  if (fast_ok(p, op)) return op == kBF16 ? launch_fast<bf16_t>(p, ws, s) : launch_fast<f16_t>(p, ws, s);
-  p.h = ws;
-  if (op == kBF16) return launch_general<bf16_t>(p, s);
-  if (op == kF16) return launch_general<f16_t>(p, s);
-  return launch_general<float>(p, s);
+  if (!fast_ok(p, op)) {
+    // (matrices past 32-bit offsets too, copied or not: the general kernels store up to N
+    // and the rank, so they get the call's own sizes and operands, and nothing is copied)
+    p = q;
+    p.h = ws;
+    if (op == kBF16) return launch_general<bf16_t>(p, s);
+    if (op == kF16) return launch_general<f16_t>(p, s);
+    return launch_general<float>(p, s);
+  }
+  if (x_copy != nullptr) {
+    const hipError_t e = launch_pad_rows(q.x, op, q.x_ld, q.rows, q.K, nullptr, 0, op, x_copy, s);
+    if (e != hipSuccess) return e;
+  }
+  if (pads.n > 0) {
+    hipLaunchKernelGGL(lora_pad_kernel, dim3(pads.of[pads.n - 1].end), dim3(256), 0, s, pads);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return op == kBF16 ? launch_fast<bf16_t>(p, ws, s) : launch_fast<f16_t>(p, ws, s);
 }
 
 // ---------------------------------------------------------------------------
