@@ -566,8 +566,7 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW, STAGES>::OCC)) voi
     __builtin_amdgcn_sched_barrier(0);
   });
 
-  // ---- what was left out: added to the rows it belongs to, a row at a time (its
-  // products are infinities or NaN, beside which the stored value does not count)
+  // ---- what was left out: added to the rows it belongs to, an element at a time
   if (__any(dropped)) {
     vm_wait<0>();  // the stores above
     for (int i = 0; i < MI * 16; ++i) {
@@ -582,7 +581,26 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW, STAGES>::OCC)) voi
           const float v = to_f32(b[r * p.b_sr + n * p.b_sn]);
           if (!isfinite(v)) sum += to_f32(h[r]) * v;
         }
-        if (!isfinite(sum)) reinterpret_cast<OpT*>(p.out)[row * p.out_ld + n] = from_f32<OpT>(sum);
+        if (isfinite(sum)) continue;
+        OpT* at = reinterpret_cast<OpT*>(p.out) + row * p.out_ld + n;
+        float rest = to_f32(*at);
+        // An infinity against the sum's may have come of the output's rounding alone; then
+        // the terms say whether one of them is infinite.
+        if (isinf(rest) && isinf(sum) && rest != sum) {
+          rest = p.base != nullptr ? load_as_f32(p.base, p.base_dtype, row * p.base_ld + n) : 0.f;
+          const OpT* x = reinterpret_cast<const OpT*>(p.x) + row * p.x_ld;
+          const OpT* w = reinterpret_cast<const OpT*>(p.w);
+          const int64_t K = w != nullptr ? p.K : 0;
+#pragma unroll 1
+          for (int64_t k = 0; k < K && isfinite(rest); ++k)
+            rest += to_f32(x[k]) * to_f32(w[k * p.w_sk + n * p.w_sn]);
+#pragma unroll 1
+          for (int32_t r = 0; r < rank && isfinite(rest); ++r) {
+            const float v = to_f32(b[r * p.b_sr + n * p.b_sn]);
+            if (isfinite(v)) rest += to_f32(h[r]) * v;
+          }
+        }
+        *at = from_f32<OpT>(rest + sum);
       }
     }
   }

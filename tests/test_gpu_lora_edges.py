@@ -65,3 +65,32 @@ def test_weights_past_32_bit_offsets(T, d_in, d_out, r, pitch):
     _within(out[:T * d_out].view(T, d_out)[:, at.cuda()], exp, bound)
     _within(inner[:r, :T], h.t(), hb.t())
     assert bool((out[T * d_out:] == 77.0).all()) and bool((inner[r:] == 77.0).all())
+
+
+# one per tile size of the fused product, with and without the shared weight, and the few rows' path
+@pytest.mark.parametrize("T,d_out,weight", [(200, 264, True), (777, 264, True), (3001, 1032, True), (12345, 1032, True),
+                                            (777, 264, False)])
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_infinities_beside_other_infinities(T, d_out, weight, dtype):
+    """A tile's rows of several adapters, some of whose B hold an infinity: what base and
+    projection hold beside it counts as it does in a sum."""
+    d_in, r, n = 64, 8, 3
+    t = _make(T, d_in, d_out, r, n, dtype, 3)
+    t["ids"] = torch.arange(T) % 4 - 1
+    t["x"], t["a"] = t["x"].abs(), t["a"].abs()   # inner rows above 0
+    t["weight"][:, 16:24] = -1000.0                # about -51000 a row; in fp16 base takes it past the type's range
+    b, base, ids = t["b"], t["base"], t["ids"]
+    b[1, 2, 8:24] = INF
+    b[2, 5, 10] = -INF
+    for i in range(T):
+        base[i, 8 + i // 4 % 3] = (NAN, -INF, INF)[i // 12 % 3]
+        base[i, 16 + i % 8] = -60000.0
+    x, a, bd, w, bs, idd = _dev(t, "x", "a", "b", "weight", "base", "ids")
+    y = C.cvmm_lora(x, idd, a, bd, weight=w if weight else None, base=bs).cpu()
+    exp, bound, _, _ = O.lora(t["x"], ids, t["a"], b, t["weight"] if weight else None, base, 1.0, dtype)
+    e = exp.to(dtype)
+    assert bool(e.isnan().any() and (e == INF).any() and (e == -INF).any())
+    for f in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert torch.equal(f(y), f(e)), f"{int((f(y) != f(e)).sum())} places"
+    at = e.isfinite() & bound.isfinite()
+    _within(y[at], exp[at], bound[at])
