@@ -1294,11 +1294,13 @@ def cvmm_lora(x: torch.Tensor, adapters: Union[torch.Tensor, CVMMSel], a: torch.
     and more in mixed order take a selection 2 to 6 times as fast as plain ids.
 
     The op type is the autocast dtype, or ``x``'s where autocast is off; operands are
-    rounded to it (base: taken in it or in fp32), ``scale * x @ a[i]`` is rounded
-    to it once, all sums are fp32 and the output is rounded once.  In fp16 those
-    inner values must stay below 65520.  An adapter's infinities and NaN reach its
-    own rows only.  Gradients flow to x, a, b and base; the adapters' are summed in a
-    fixed order; no second derivatives."""
+    rounded to it (base: taken in it or in fp32), all sums are fp32 and the output is
+    rounded once.  ``scale * x @ a[i]`` is rounded to the op type once in calls of more
+    than 256 rows (512 at ranks to 16) and where the gradient of ``b`` is asked for, and
+    its twin for the gradient of x alike; in fp16 those inner values must stay below
+    65520.  Smaller calls keep it in fp32.  An adapter's infinities and NaN reach its own
+    rows only.  Gradients flow to x, a, b and base; the adapters' are summed in a fixed
+    order; no second derivatives."""
     _require_device(x, "x")
     op = torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
     if op not in _DTYPE_IDS:

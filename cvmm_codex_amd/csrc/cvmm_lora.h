@@ -1,6 +1,6 @@
 // Low-rank adapters beside a shared projection (csrc/cvmm_lora*.hip):
 //   out[t] = base[t] + x[t] W + h[t] B_i,   h[t] = rnd_op(s_i x[t] A_i),   i = ids[t]
-// rows with an id outside [0, n) take the base and the projection alone.
+// (calls of few rows do not round h); rows with an id outside [0, n) take the base and the projection alone.
 #pragma once
 
 #include "cvmm_common.h"

@@ -8,7 +8,8 @@
 // zero: an infinity or a NaN of one request's adapter stays with its rows).
 // h is rounded to the op type, whose matrix instructions form h B_i: an error of
 // at most half a step of each of its values, beside the one of the output's own
-// rounding.  All sums are 32-bit.
+// rounding.  (Calls of few rows form h B_i of 32-bit values, cvmm_lora_rows.h.)  All
+// sums are 32-bit.
 #include "cvmm_common.h"
 #include "cvmm_internal.h"
 #include "cvmm_lora.h"

@@ -233,7 +233,7 @@ __global__ __launch_bounds__(256, RB <= 4 ? 3 : 1) void lora_inner_tile_kernel(c
 // ---------------------------------------------------------------------------
 // Calls of few rows, most of them with an adapter of their own: plain 32-bit
 // multiply-adds, each of a row's matrices read once and spread over many
-// workgroups.  First launch: shares of x A_i (here) beside shares of x W (the split
+// workgroups.  Nothing but the output is rounded.  First launch: shares of x A_i (here) beside shares of x W (the split
 // GEMM); second: their sums, then h B_i (lora_join_kernel).  Bound by launches and
 // the latency of one chain of loads each: 32 rows of 2048 -> 2048, rank 16, 64
 // adapters: 5.4 + 4.1 us, 12 MB, of which 2.4 would be bandwidth; one row of
@@ -317,7 +317,7 @@ __global__ __launch_bounds__(kLoraJoinThreads) void lora_join_kernel(const LoraP
       float s = 0.f;
 #pragma unroll 4
       for (int q = 0; q < sp.h_splits; ++q) s += sp.h_part[((int64_t)q * p.rows + row) * rank + r];
-      h[r] = to_f32(from_f32<OpT>(sc * s));
+      h[r] = sc * s;
     }
   }
   __syncthreads();

@@ -545,6 +545,8 @@ int cvmm_balance_loss_backward(const void* logits, int32_t logits_dtype, int64_t
  * Low-rank adapters of many requests beside a shared projection (no counterpart
  * in cvmm.py):
  *   out[t] = base[t] + x[t] W + h[t] B_i,  h[t] = rnd_op(s_i x[t] A_i),  i = ids[t]
+ * (h in fp32 up to 256 rows, or 512 at ranks to 16, where inner_t is NULL and the
+ * op type has 16 bits; copies of odd operands need their room for that).
  * x, W [d_in][d_out] (or NULL), A [n_adapters][d_in][rank], B [n_adapters]
  * [rank][d_out] in the op dtype with any element strides (rows of x, base and out
  * with unit column stride); base (or NULL) in the op dtype or fp32; s_i = scale,

@@ -94,3 +94,24 @@ def test_infinities_beside_other_infinities(T, d_out, weight, dtype):
         assert torch.equal(f(y), f(e)), f"{int((f(y) != f(e)).sum())} places"
     at = e.isfinite() & bound.isfinite()
     _within(y[at], exp[at], bound[at])
+
+
+@pytest.mark.parametrize("T,r,dtype", [(1, 16, BF), (40, 12, BF), (256, 64, F16), (500, 8, BF)])
+@pytest.mark.parametrize("weight", [True, False])
+def test_few_rows_hold_inner_rows_in_32_bits(T, r, dtype, weight):
+    """Calls of few rows round nothing but their output."""
+    t = _make(T, 320, 520, r, 7, dtype, 6)
+    x, ids, a, b, w = _dev(t, "x", "ids", "a", "b", "weight")
+    y = C.cvmm_lora(x, ids, a, b, weight=w if weight else None, scale=1.5)
+    exp, bound, _, _ = O.lora(t["x"], t["ids"], t["a"], t["b"], t["weight"] if weight else None, None, 1.5, F32, dtype)
+    _within(y, exp, bound)
+
+
+def test_few_rows_inner_values_past_half_precision():
+    t = _make(33, 64, 72, 8, 3, F16, 7)
+    t["b"] *= 2.0 ** -12
+    x, ids, a, b = _dev(t, "x", "ids", "a", "b")
+    y = C.cvmm_lora(x, ids, a, b, scale=2.0 ** 18)
+    exp, bound, h, _ = O.lora(t["x"], t["ids"], t["a"], t["b"], None, None, 2.0 ** 18, F32, F16)
+    assert float(h.abs().max()) > 65520 and float(exp.abs().max()) < 65000
+    _within(y, exp, bound)
