@@ -779,7 +779,8 @@ def cvmm_balance_loss(logits: torch.Tensor, sel: Union[torch.Tensor, CVMMSel], k
     group = max(logits.shape[-2] if per_sequence else T, 1)
     args = (logits, sel, mask, group, N.BALANCE_KINDS[kind], N.SCORES[scores], float(weight), float(z_weight))
     if _compiling():
-        return _ops.balance_loss(*args)[:3]
+        loss, terms, counts, _ = _ops.balance_loss(*args)
+        return loss, terms.detach(), counts   # (terms: for logging, as the eager function marks them)
     return tuple(N.host().balance_loss_apply(*args, _differentiated(logits)))
 
 
