@@ -1374,5 +1374,5 @@ def cvmm_lora(x: torch.Tensor, adapters: Union[torch.Tensor, CVMMSel], a: torch.
     if _compiling():
         if grad and order is None and ids.numel() > 0:
             _, order, _, offsets, _ = _ops.sort_routes(ids, n, 1)
-        return _ops.lora(x, a, b, base, ids, weight, scales, factor, order, offsets, op)[0]
+        return _ops.lora(x, a, b, base, ids, weight, scales, factor, order, offsets, op, grad and b.requires_grad)[0]
     return N.host().lora_apply(x, ids, a, b, weight, base, scales, factor, order, offsets, _DTYPE_IDS[op], grad)

@@ -394,22 +394,22 @@ balance_loss.register_autograd(_balance_backward, setup_context=_balance_setup)
 
 # ---------------------------------------------------------------------------
 # low-rank adapters (api.cvmm_lora): the output, and the inner rows that the
-# adapters' gradients read (made where a sorted order is given)
+# gradient of b reads (made where want_inner, in the sorted order)
 # ---------------------------------------------------------------------------
 @torch.library.custom_op(f"{NS}::lora", mutates_args=())
 def lora(x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, base: Optional[torch.Tensor], ids: torch.Tensor,
          weight: Optional[torch.Tensor], scales: Optional[torch.Tensor], scale: float,
-         order: Optional[torch.Tensor], offsets: Optional[torch.Tensor],
-         op_dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
-    out, inner = N.host().lora_forward(x, ids, a, b, weight, base, scales, scale, order, order is not None,
+         order: Optional[torch.Tensor], offsets: Optional[torch.Tensor], op_dtype: torch.dtype,
+         want_inner: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    out, inner = N.host().lora_forward(x, ids, a, b, weight, base, scales, scale, order, want_inner,
                                        N.dtype_id(op_dtype))
     return out.view(*x.shape[:-1], b.shape[2]), inner if inner is not None else _empty(x)
 
 
 @lora.register_fake
-def _(x, a, b, base, ids, weight, scales, scale, order, offsets, op_dtype):
+def _(x, a, b, base, ids, weight, scales, scale, order, offsets, op_dtype, want_inner):
     rows = ids.numel()
-    inner = (x.new_empty((a.shape[2], (rows + 7) // 8 * 8), dtype=op_dtype) if order is not None else _empty(x))
+    inner = x.new_empty((a.shape[2], (rows + 7) // 8 * 8), dtype=op_dtype) if want_inner else _empty(x)
     return x.new_empty((*x.shape[:-1], b.shape[2]), dtype=op_dtype), inner
 
 
@@ -431,7 +431,7 @@ def _(grad, x, a, b, ids, weight, scales, scale, order, offsets, inner, op_dtype
 
 
 def _lora_setup(ctx, inputs, output):
-    x, a, b, base, ids, weight, scales, scale, order, offsets, op_dtype = inputs
+    x, a, b, base, ids, weight, scales, scale, order, offsets, op_dtype, _ = inputs
     ctx.save_for_backward(x, a, b, ids, weight, scales, order, offsets, output[1])
     ctx.args = (scale, op_dtype, base.dtype if base is not None else None)
 
@@ -445,7 +445,7 @@ def _lora_backward(ctx, grad, _):
         g = [t if n else None for t, n in zip(lora_backward(grad, x, a, b, ids, weight, scales, scale, order, offsets,
                                                             inner, op_dtype, *need), need)]
     gb = grad.to(base_dtype) if base_dtype is not None and ctx.needs_input_grad[3] else None
-    return (*g, gb) + (None,) * 7
+    return (*g, gb) + (None,) * 8
 
 
 lora.register_autograd(_lora_backward, setup_context=_lora_setup)

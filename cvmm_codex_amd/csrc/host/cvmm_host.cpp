@@ -1395,6 +1395,8 @@ std::tuple<OptT, OptT, OptT> lora_backward(const Tensor& grad_output, const Tens
   lora_check_order(s, order, offsets, x);
   if ((need_a || need_b) && s.rows > 0 && (!order.has_value() || !offsets.has_value()))
     throw py::value_error("cvmm_lora: the adapters' gradients need a sorted selection");
+  if (need_b && s.rows > 0 && (!inner.has_value() || inner->numel() != s.rank * ((s.rows + 7) / 8 * 8)))
+    throw py::value_error("cvmm_lora: the gradient of b needs the forward's inner rows");
   c10::DeviceGuard guard(x.device());
   const int64_t stream = current_stream(x);
   const auto op = dtype_of(op_id);

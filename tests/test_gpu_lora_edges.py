@@ -115,3 +115,26 @@ def test_few_rows_inner_values_past_half_precision():
     exp, bound, h, _ = O.lora(t["x"], t["ids"], t["a"], t["b"], None, None, 2.0 ** 18, F32, F16)
     assert float(h.abs().max()) > 65520 and float(exp.abs().max()) < 65000
     _within(y, exp, bound)
+
+
+@pytest.mark.parametrize("wanted", ["nothing", "x"])
+def test_compiled_without_gradients_of_adapters(wanted):
+    """The same kernels, and so the same bits, as the eager call: no inner rows are made
+    for a gradient that nobody asks for."""
+    t = _make(200, 256, 192, 16, 5, BF, 4)
+    x, ids, a, b, w, grad = _dev(t, "x", "ids", "a", "b", "weight", "grad")
+
+    def f(x):
+        return C.cvmm_lora(x, C.cvmm_prepare_sel2(ids, route_input=True), a, b, weight=w, scale=1.25)
+
+    res = []
+    for fn in (f, torch.compile(f, backend="aot_eager", fullgraph=True)):
+        if wanted == "x":
+            leaf = x.detach().requires_grad_()
+            y = fn(leaf)
+            res.append((y, *torch.autograd.grad(y, leaf, grad)))
+        else:
+            with torch.no_grad():
+                res.append((fn(x),))
+    for e, c in zip(*res):
+        assert torch.equal(e, c)
