@@ -1369,10 +1369,11 @@ def cvmm_lora(x: torch.Tensor, adapters: Union[torch.Tensor, CVMMSel], a: torch.
             raise ValueError(f"cvmm_lora: adapters {tuple(ids.shape)} are not one id per row of x {tuple(x.shape)}")
     if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
         raise TypeError(f"cvmm_lora: adapters must hold ids, not {ids.dtype}")
-    if (a.requires_grad or b.requires_grad) and grad and n > 32767:
+    adapter_grads = grad and (a.requires_grad or b.requires_grad)
+    if adapter_grads and n > 32767:
         raise ValueError(f"cvmm_lora: gradients of at most 32767 adapters, not {n}")
     if _compiling():
-        if grad and order is None and ids.numel() > 0:
+        if adapter_grads and order is None and ids.numel() > 0:
             _, order, _, offsets, _ = _ops.sort_routes(ids, n, 1)
         return _ops.lora(x, a, b, base, ids, weight, scales, factor, order, offsets, op, grad and b.requires_grad)[0]
     return N.host().lora_apply(x, ids, a, b, weight, base, scales, factor, order, offsets, _DTYPE_IDS[op], grad)

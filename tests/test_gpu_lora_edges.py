@@ -138,3 +138,20 @@ def test_compiled_without_gradients_of_adapters(wanted):
                 res.append((fn(x),))
     for e, c in zip(*res):
         assert torch.equal(e, c)
+
+
+def test_compiled_gradient_of_rows_needs_no_sort():
+    """Only the adapters' gradients need one: more adapters than a sort takes."""
+    t = _make(70, 16, 24, 8, 32768, BF, 9)
+    x, ids, a, b, w, grad = _dev(t, "x", "ids", "a", "b", "weight", "grad")
+
+    def f(x):
+        return C.cvmm_lora(x, ids, a, b, weight=w)
+
+    res = []
+    for fn in (f, torch.compile(f, backend="aot_eager", fullgraph=True)):
+        leaf = x.detach().requires_grad_()
+        y = fn(leaf)
+        res.append((y, *torch.autograd.grad(y, leaf, grad)))
+    for e, c in zip(*res):
+        assert torch.equal(e, c)
