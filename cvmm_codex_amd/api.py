@@ -317,6 +317,7 @@ def _offsets_for(sel: torch.Tensor, n_experts: int) -> torch.Tensor:
 # copy (cvmm_copy_ids_count), and the sort skips that launch when cvmm()
 # brings the same count.
 _expert_guess: Dict[Tuple[int, int], int] = {}
+_MAX_SORTED = 32767   # expert counts that the sort takes
 
 
 class _Routing:
@@ -340,7 +341,7 @@ class _Routing:
         if self.counted is not None:   # one use: the sort turns the counts into prefixes
             ws = self.counted[1] if self.counted[0] == n_experts else None
             self.counted = None
-        if not _compiling():
+        if not _compiling() and 1 <= n_experts <= _MAX_SORTED:   # (the sort refuses others)
             if len(_expert_guess) > 64:
                 _expert_guess.clear()
             _expert_guess[(self.raw.numel(), self.k)] = n_experts
@@ -1345,7 +1346,7 @@ def cvmm_lora(x: torch.Tensor, adapters: Union[torch.Tensor, CVMMSel], a: torch.
             raise ValueError(f"cvmm_lora: the selection's {ids.numel()} routes are not the {x.numel() // d_in} rows of x")
         if ids.numel() > 0:
             r = adapters._routing
-            if not _compiling() and adapters._pending() and n not in r.by_e and n <= 32767:
+            if not _compiling() and adapters._pending() and n not in r.by_e and n <= _MAX_SORTED:
                 # a recorded selection: its sort (if still to be made) and the product in
                 # one host call
                 bufs = r.buffers.get(n)
@@ -1370,8 +1371,8 @@ def cvmm_lora(x: torch.Tensor, adapters: Union[torch.Tensor, CVMMSel], a: torch.
     if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
         raise TypeError(f"cvmm_lora: adapters must hold ids, not {ids.dtype}")
     adapter_grads = grad and (a.requires_grad or b.requires_grad)
-    if adapter_grads and n > 32767:
-        raise ValueError(f"cvmm_lora: gradients of at most 32767 adapters, not {n}")
+    if adapter_grads and n > _MAX_SORTED:
+        raise ValueError(f"cvmm_lora: gradients of at most {_MAX_SORTED} adapters, not {n}")
     if _compiling():
         if adapter_grads and order is None and ids.numel() > 0:
             _, order, _, offsets, _ = _ops.sort_routes(ids, n, 1)
