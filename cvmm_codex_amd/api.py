@@ -1292,8 +1292,9 @@ def cvmm_lora(x: torch.Tensor, adapters: Union[torch.Tensor, CVMMSel], a: torch.
     ``adapters`` may be a selection with one route per row of x
     (``cvmm_prepare_sel2(ids, route_input=True)``): the sort is then shared with the
     projections that use it; plain ids are sorted where the adapters' gradients are
-    asked for.  Rows of one adapter that stand together are fastest; some hundred rows
-    and more in mixed order take a selection 2 to 6 times as fast as plain ids.
+    asked for (those of at most 32767 adapters).  Rows of one adapter that stand
+    together are fastest; some hundred rows and more in mixed order take a selection 2
+    to 6 times as fast as plain ids.
 
     The op type is the autocast dtype, or ``x``'s where autocast is off; operands are
     rounded to it (base: taken in it or in fp32), all sums are fp32 and the output is
@@ -1344,9 +1345,9 @@ def cvmm_lora(x: torch.Tensor, adapters: Union[torch.Tensor, CVMMSel], a: torch.
         _require_device(ids, "adapters")
         if ids.numel() != x.numel() // d_in:
             raise ValueError(f"cvmm_lora: the selection's {ids.numel()} routes are not the {x.numel() // d_in} rows of x")
-        if ids.numel() > 0:
+        if ids.numel() > 0 and n <= _MAX_SORTED:   # (more adapters: the ids alone)
             r = adapters._routing
-            if not _compiling() and adapters._pending() and n not in r.by_e and n <= _MAX_SORTED:
+            if not _compiling() and adapters._pending() and n not in r.by_e:
                 # a recorded selection: its sort (if still to be made) and the product in
                 # one host call
                 bufs = r.buffers.get(n)

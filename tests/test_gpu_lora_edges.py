@@ -155,3 +155,35 @@ def test_compiled_gradient_of_rows_needs_no_sort():
         res.append((y, *torch.autograd.grad(y, leaf, grad)))
     for e, c in zip(*res):
         assert torch.equal(e, c)
+
+
+@pytest.mark.parametrize("how", ["new", "used", "compiled"])
+@pytest.mark.parametrize("wanted", ["nothing", "x"])
+def test_selection_beside_more_adapters_than_a_sort_takes(how, wanted):
+    """Its ids are used as plain ones are; the adapters' gradients are refused."""
+    t = _make(70, 16, 24, 8, 32768, BF, 5)
+    x, ids, a, b, w, grad = _dev(t, "x", "ids", "a", "b", "weight", "grad")
+
+    def call(fn):
+        if wanted == "nothing":
+            with torch.no_grad():
+                return (fn(x),)
+        leaf = x.detach().requires_grad_()
+        y = fn(leaf)
+        return (y, *torch.autograd.grad(y, leaf, grad))
+
+    exp = call(lambda x: C.cvmm_lora(x, ids, a, b, weight=w))
+    _within(exp[0], *O.lora(t["x"], t["ids"], t["a"], t["b"], t["weight"], None, 1.0, BF)[:2])
+    sel = C.cvmm_prepare_sel2(ids.view(70, 1), route_input=True)
+    if how == "used":
+        C.cvmm(torch.zeros(70, 1, 64, device="cuda", dtype=BF), sel, torch.zeros(8, 64, 64, device="cuda", dtype=BF))
+
+    def f(x):
+        s = C.cvmm_prepare_sel2(ids, route_input=True) if how == "compiled" else sel
+        return C.cvmm_lora(x, s, a, b, weight=w)
+
+    got = call(torch.compile(f, backend="aot_eager", fullgraph=True) if how == "compiled" else f)
+    for e, g in zip(exp, got):
+        assert torch.equal(e, g)
+    with pytest.raises(ValueError):
+        C.cvmm_lora(x, sel, a.requires_grad_(), b)
