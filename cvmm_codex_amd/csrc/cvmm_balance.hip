@@ -16,7 +16,7 @@
 // in bf16 are 4 MB, under a microsecond of the card's bandwidth.  So two
 // launches forward (chunks of tokens, then their sums in a fixed order) and one
 // backward.  Terms of a token are 32-bit; a chunk's sums
-// too (at most some hundred addends per lane); sums over chunks are 64-bit.
+// too (at most 256 addends per lane, then at most 64 lanes); sums over chunks are 64-bit.
 // Measured (chunks, sums, backward), us: 512 tokens of 16 experts 4.4, 6.2, 3.4; 16384 of
 // 128 in bf16 5.4, 9.6, 7.3; 32768 of 256 in 8 sequences 12.8, 8.5, 20.9 (the last
 // 34 MB at 1.6 TB/s: exponentials, 8 a lane, and coefficients beside them).
@@ -409,12 +409,15 @@ __global__ __launch_bounds__(kBalanceThreads) void balance_bwd_kernel(
 }
 
 // Tokens per chunk: two workgroups per CU, of whole passes (32768 tokens of 256 experts:
-// 20.8 us forward; one per CU 24.3, four 25; 16384 of 128: 15, one 14.5, four 20).
+// 20.8 us forward; one per CU 24.3, four 25; 16384 of 128: 15, one 14.5, four 20), but
+// at most 256 passes, whose 32-bit sums lose 256 half steps at most.
+constexpr int64_t kBalancePasses = 256;
 static int64_t balance_chunk_tokens(int64_t n_tokens, int64_t group_tokens, int32_t n_experts) {
   int64_t segs = 0;
   by_experts(n_experts, [&](auto lpt, auto) { segs = kBalanceThreads / decltype(lpt)::value; });
   int64_t tpc = ((n_tokens > 0 ? n_tokens : 1) + 511) / 512;
   tpc = (tpc + segs - 1) / segs * segs;
+  if (tpc > kBalancePasses * segs) tpc = kBalancePasses * segs;
   return tpc < group_tokens ? tpc : group_tokens;
 }
 

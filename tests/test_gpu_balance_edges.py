@@ -1,4 +1,6 @@
 """The balance loss: compiled calls, very many tokens."""
+import math
+
 import pytest
 import torch
 
@@ -23,3 +25,23 @@ def test_compiled_terms_have_no_gradient():
             torch.autograd.grad(terms.sum(), leaf)
         (grad,) = torch.autograd.grad(loss, leaf)
         assert bool(grad.any())
+
+
+def test_sums_of_very_many_tokens():
+    """Equal tokens, whose 32-bit sums lose most: each addition the same part of a step, the
+    same way.  A lane adds at most 256 of them, the workgroup 64 such sums (the additions'
+    errors, half a step each, add up at most); an exponential, its sum and quotient and the
+    result's rounding are within 16 more halves of a step."""
+    T = 1 << 27
+    c = -1.15625
+    logits = torch.tensor([c, 0.0], dtype=torch.bfloat16, device="cuda").repeat(T, 1)
+    sel = torch.zeros(T, 1, dtype=torch.int32, device="cuda")
+    loss, terms, counts = C.cvmm_balance_loss(logits, sel)
+    assert counts.tolist() == [T, 0]
+    exp = 2.0 / (1.0 + math.exp(-c))
+    assert abs(float(terms[0]) - exp) <= (256 + 64 + 16) * 2.0 ** -24 * exp
+    assert float(loss) == float(terms[0])
+    # sum of the exponentials: 2^-23 of 1.3 off, so its logarithm 2^-23 + half a step of
+    # 0.27, 10 half steps; twice that and a rounding in the square
+    z = math.log(1.0 + math.exp(c)) ** 2
+    assert abs(float(terms[1]) - z) <= (256 + 64 + 32) * 2.0 ** -24 * z
