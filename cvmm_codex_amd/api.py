@@ -320,12 +320,19 @@ _expert_guess: Dict[Tuple[int, int], int] = {}
 _MAX_SORTED = 32767   # expert counts that the sort takes
 
 
+def _version(t: torch.Tensor) -> Optional[int]:
+    """What tells whether a tensor was written since (compiled code and inference tensors
+    keep no count of it)."""
+    return None if _compiling() or t.is_inference() else t._version
+
+
 class _Routing:
     """One recorded selection; sorted on the device on first use, per expert count.
     `counted` = (expert count, sort workspace holding the ids' histogram for it)."""
 
     def __init__(self, raw_flat: torch.Tensor, top_k: int, counted=None):
         self.raw = raw_flat
+        self.version = _version(raw_flat)
         self.k = top_k
         self.by_e: Dict[int, Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]] = {}
         self.first_e: Optional[int] = None
@@ -333,6 +340,16 @@ class _Routing:
         # expert count -> the sort's two buffers (int32, int64), views of which
         # make a by_e entry where one is asked for
         self.buffers: Dict[int, Tuple[torch.Tensor, torch.Tensor]] = {}
+
+    def ids(self) -> torch.Tensor:
+        """The ids as recorded.  `raw` may be a tensor that the caller has too (a router's
+        output, cvmm_prepare_sel's argument); if that was written since, they are put
+        together again from the sort that was made with them."""
+        if self.version is not None and self.first_e is not None and _version(self.raw) != self.version:
+            ssel, perm = self.get(self.first_e)[:2]
+            self.raw = torch.empty_like(ssel).scatter_(0, perm, ssel)
+            self.version = _version(self.raw)
+        return self.raw
 
     def counts(self, n_experts: int) -> Optional[torch.Tensor]:
         """The sort workspace that holds the ids' histogram for this expert
@@ -360,8 +377,9 @@ class _Routing:
             hit = self.by_e[n_experts] = (ssel, perm, tok, offsets)
         if hit is None:
             ws = self.counts(n_experts)
-            hit = (_sort_routes_cast(self.raw, n_experts, self.k, cast, ws) if cast is not None
-                   else _sort_routes(self.raw, n_experts, self.k, ws))
+            raw = self.ids()
+            hit = (_sort_routes_cast(raw, n_experts, self.k, cast, ws) if cast is not None
+                   else _sort_routes(raw, n_experts, self.k, ws))
             self.by_e[n_experts] = hit
             if self.first_e is None:
                 self.first_e = n_experts
@@ -409,7 +427,7 @@ class CVMMSel:
             return CVMMSel._deferred(self._raw_shape_tensor(), self._routing, self._route_mode,
                                      self.reduction_weight)
         out = CVMMSel(self.raw_sel, self.sel, self.sel_index, self.out_index, self.reduction_weight)
-        out._sorted_for = self._sorted_for
+        out._sorted_for, out._routing = self._sorted_for, self._routing
         return out
 
     @classmethod
@@ -428,6 +446,13 @@ class CVMMSel:
         if self._raw_sel is None and self._raw_src is not None:
             return self._raw_src
         return self._raw_sel
+
+    def _ids(self) -> torch.Tensor:
+        """The ids in raw_sel's shape, of any integer type, as this library recorded them
+        (raw_sel itself where the sort is not its own)."""
+        if self._routing is not None and (self._sel is None or self._sorted_for is not None):
+            return self._routing.ids().view(self._raw_shape_tensor().shape)
+        return self._raw_shape_tensor()
 
     def _pending(self) -> bool:
         return self._routing is not None and self._sel is None
@@ -508,13 +533,14 @@ def cvmm_prepare_sel(sel: torch.Tensor, n_experts: int) -> CVMMSel:
     if not sel.is_cuda:
         raw, ssel, perm = _host_sel(sel)
         return CVMMSel(raw, ssel, perm, None)
-    ssel, perm, _, offsets = _Routing(sel.reshape(-1), 1).get(n_experts)
+    routing = _Routing(sel.reshape(-1), 1)
+    ssel, perm, _, offsets = routing.get(n_experts)
     s = ssel.view(sel.shape)
     s._cvmm_offsets = {n_experts: offsets}
     s._cvmm_i32 = ssel
     out = CVMMSel(None, s, perm, None)
     out._raw_src = sel
-    out._sorted_for = n_experts
+    out._sorted_for, out._routing = n_experts, routing
     return out
 
 
@@ -534,7 +560,8 @@ def cvmm_prepare_sel2(sel: Union[torch.Tensor, CVMMSel], w: Optional[torch.Tenso
         else:
             out = CVMMSel(None, sel.sel, sel.sel_index, sel.out_index, w)
         # raw_sel as the parent holds it: its int32 copy is made if it is read
-        out._raw_sel, out._raw_src, out._sorted_for = sel._raw_sel, sel._raw_src, sel._sorted_for
+        out._raw_sel, out._raw_src = sel._raw_sel, sel._raw_src
+        out._sorted_for, out._routing = sel._sorted_for, sel._routing
         return out
 
     n_per_batch = sel.shape[-1]
@@ -759,7 +786,7 @@ def cvmm_balance_loss(logits: torch.Tensor, sel: Union[torch.Tensor, CVMMSel], k
     if scores not in N.SCORES:
         raise ValueError(f"cvmm_balance_loss: scores must be 'softmax' or 'sigmoid', not {scores!r}")
     if isinstance(sel, CVMMSel):
-        sel = sel._raw_shape_tensor()
+        sel = sel._ids()
     _require_device(sel, "sel")
     if sel.is_floating_point() or sel.is_complex() or sel.dtype == torch.bool:
         raise TypeError(f"cvmm_balance_loss: sel must hold ids, not {sel.dtype}")
@@ -1252,7 +1279,7 @@ def cvmm_mx4(x: torch.Tensor, sel: Union[torch.Tensor, CVMMSel], keys: CVMMMx4,
         bufs = r.buffers.get(E)
         shape = [*rw.shape[:-1], d_out] if rw is not None else [*raw.shape, d_out]
         y, i32, i64 = N.host().mx4_apply_recorded(
-            x, rw, keys.codes, keys.scales, E, d_in, d_out, r.raw, r.k, r.counts(E) if bufs is None else None,
+            x, rw, keys.codes, keys.scales, E, d_in, d_out, r.ids(), r.k, r.counts(E) if bufs is None else None,
             *(bufs or (None, None)), sel._route_mode, _DTYPE_IDS[op], quantize_input, grad, shape)
         if bufs is None:
             r.keep(E, i32, i64)
@@ -1341,7 +1368,7 @@ def cvmm_lora(x: torch.Tensor, adapters: Union[torch.Tensor, CVMMSel], a: torch.
     if isinstance(adapters, CVMMSel):
         if adapters.reduction_weight is not None:
             raise ValueError("cvmm_lora: a selection with routing weights has no sum here")
-        ids = adapters._raw_shape_tensor()
+        ids = adapters._ids()
         _require_device(ids, "adapters")
         if ids.numel() != x.numel() // d_in:
             raise ValueError(f"cvmm_lora: the selection's {ids.numel()} routes are not the {x.numel() // d_in} rows of x")
@@ -1352,7 +1379,7 @@ def cvmm_lora(x: torch.Tensor, adapters: Union[torch.Tensor, CVMMSel], a: torch.
                 # one host call
                 bufs = r.buffers.get(n)
                 y, i32, i64 = N.host().lora_apply_recorded(
-                    x, r.raw, a, b, weight, base, scales, factor, r.k, r.counts(n) if bufs is None else None,
+                    x, r.ids(), a, b, weight, base, scales, factor, r.k, r.counts(n) if bufs is None else None,
                     *(bufs or (None, None)), _DTYPE_IDS[op], grad)
                 if bufs is None:
                     r.keep(n, i32, i64)

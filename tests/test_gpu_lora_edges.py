@@ -187,3 +187,40 @@ def test_selection_beside_more_adapters_than_a_sort_takes(how, wanted):
         assert torch.equal(e, g)
     with pytest.raises(ValueError):
         C.cvmm_lora(x, sel, a.requires_grad_(), b)
+
+
+@pytest.mark.parametrize("made", ["scored", "topk", "prepared"])
+@pytest.mark.parametrize("used", [False, True])
+@pytest.mark.parametrize("n", [16, 20])
+def test_ids_written_after_the_selection_was_made(made, used, n):
+    """A selection is the routing that was recorded, whatever the tensor of ids that came or
+    went with it holds by now: output, every gradient, counts."""
+    T, k, E = 90, 4, 16
+    g = torch.Generator().manual_seed(10)
+    logits = torch.randn(T, E, generator=g).cuda()
+    t = _make(T * k, 64, 72, 8, n, BF, 10)
+    grad = t["grad"].cuda().view(T, k, 72)
+    res = []
+    for write in (False, True):
+        if made == "scored":
+            _, ids, sel = C.cvmm_route_scored(logits, k)
+        elif made == "topk":
+            _, ids, sel = C.cvmm_route_topk(logits, k)
+        else:
+            ids = logits.topk(k).indices
+            ids[::5, 1] = -1
+            ids[::7, 2] = n
+            sel = C.cvmm_prepare_sel(ids, E)
+        if used:
+            C.cvmm(torch.zeros(T, k, 64, device="cuda", dtype=BF), C.cvmm_prepare_sel2(sel, route_input=True),
+                   torch.zeros(E, 64, 64, device="cuda", dtype=BF))
+        if write:
+            ids.copy_((ids * 7 + 3) % E)
+        x, a, b = (v.requires_grad_() for v in _dev(t, "x", "a", "b"))
+        with torch.no_grad():
+            quiet = C.cvmm_lora(x.view(T, k, 64), sel, a, b)
+        y = C.cvmm_lora(x.view(T, k, 64), C.cvmm_prepare_sel2(sel, route_input=True), a, b)
+        counts = C.cvmm_balance_loss(logits, sel)[2]
+        res.append((quiet, y, *torch.autograd.grad(y, [x, a, b], grad), counts))
+    for e, c in zip(*res):
+        assert torch.equal(e, c)
