@@ -26,6 +26,7 @@ FLAG_ROWS_SCALED = 64
 HOST_OVERLAP_BACKWARD = 1 << 48
 SCORES = {"softmax": 0, "sigmoid": 1}
 BALANCE_KINDS = {"load": 0, "entropy": 1}
+LORA_COPY_ALL, LORA_COPY_X, LORA_COPY_WEIGHT, LORA_COPY_A, LORA_COPY_B = 1, 2, 4, 8, 16
 CAST_T_INTERLEAVED = 1
 CAST_N_INTERLEAVED = 2
 TUNE_PANEL_TILES_PER_WG = 1

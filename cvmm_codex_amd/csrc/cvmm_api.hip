@@ -854,7 +854,7 @@ size_t cvmm_lora_workspace_bytes(int64_t rows, int32_t n_adapters, int64_t d_in,
   if (rows <= 0 || n_adapters <= 0 || d_in <= 0 || d_out <= 0 || rank <= 0 || rank > kLoraMaxRank ||
       !valid_dtype(op_dtype))
     return 0;
-  return lora_workspace_bytes(rows, n_adapters, d_in, d_out, rank, op_dtype, has_weight != 0, copied != 0);
+  return lora_workspace_bytes(rows, n_adapters, d_in, d_out, rank, op_dtype, has_weight != 0, copied);
 }
 
 int cvmm_lora(const void* x, int32_t op_dtype, int64_t rows, int64_t x_ld, const void* weight, int64_t w_si,

@@ -320,9 +320,9 @@ hipError_t launch_balance_loss_backward(const void* logits, int32_t dtype, int64
 struct LoraParams;
 struct LoraWgradParams;
 // `copied`: with room for copies of operands that are not made of aligned 16-byte
-// pieces; without it such calls run the general kernels.
+// pieces (CVMM_LORA_COPY_*); without it such calls run the general kernels.
 size_t lora_workspace_bytes(int64_t rows, int32_t n, int64_t K, int64_t N, int64_t rank, int32_t op_dtype,
-                            bool weight, bool copied);
+                            bool weight, int32_t copied);
 hipError_t launch_lora(const LoraParams& p, int32_t op_dtype, void* ws, size_t ws_bytes, hipStream_t stream);
 size_t lora_wgrad_workspace_bytes(int64_t rows, int32_t n, int64_t d_in, int64_t d_out, int64_t rank, bool copied);
 hipError_t launch_lora_wgrad(const LoraWgradParams& p, int32_t op_dtype, size_t ws_bytes, hipStream_t stream);

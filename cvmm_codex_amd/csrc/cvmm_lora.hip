@@ -14,6 +14,7 @@
 #include "cvmm_internal.h"
 #include "cvmm_lora.h"
 #include "cvmm_mfma.h"
+#include "../../include/cvmm_hip.h"
 
 namespace cvmm {
 
@@ -290,10 +291,21 @@ struct LoraCopies {
   size_t x, w, a, b;
   size_t total() const { return x + w + a + b; }
 };
-LoraCopies copies_bytes(int64_t rows, int64_t n, int64_t K, int64_t N, int64_t rank, bool weight) {
+// which: CVMM_LORA_COPY_* of the operands that are copied
+LoraCopies copies_bytes(int64_t rows, int64_t n, int64_t K, int64_t N, int64_t rank, int32_t which) {
   const size_t k8 = (size_t)pad8(K), n8 = (size_t)pad8(N), r8 = (size_t)pad8(rank);
-  return {align_up((size_t)rows * k8 * 2, 256), weight ? align_up(k8 * n8 * 2, 256) : 0,
-          align_up((size_t)n * k8 * r8 * 2, 256), align_up((size_t)n * r8 * n8 * 2, 256)};
+  auto room = [&](int32_t bit, size_t values) { return which & bit ? align_up(values * 2, 256) : 0; };
+  return {room(CVMM_LORA_COPY_X, (size_t)rows * k8), room(CVMM_LORA_COPY_WEIGHT, k8 * n8),
+          room(CVMM_LORA_COPY_A, (size_t)n * k8 * r8), room(CVMM_LORA_COPY_B, (size_t)n * r8 * n8)};
+}
+
+// The operands of a call that are not whole pieces, by their widths or by themselves.
+int32_t to_copy(const LoraParams& p) {
+  const bool k = p.K % 8 != 0, n = p.N % 8 != 0, r = p.rank % 8 != 0;
+  return (k || p.x_ld % 8 != 0 || !al16(p.x) ? CVMM_LORA_COPY_X : 0) |
+         (p.w != nullptr && (k || n || !pieces(p.w, 0, p.w_sk, p.w_sn)) ? CVMM_LORA_COPY_WEIGHT : 0) |
+         (k || r || !pieces(p.a, p.a_se, p.a_sk, p.a_sr) ? CVMM_LORA_COPY_A : 0) |
+         (n || r || !pieces(p.b, p.b_se, p.b_sr, p.b_sn) ? CVMM_LORA_COPY_B : 0);
 }
 
 // Matrices [n][d_i][d_j] of any strides in 16-bit values -> whole pieces, zeros in
@@ -378,7 +390,7 @@ hipError_t launch_fast(const LoraParams& q, void* ws, hipStream_t s) {
 }  // namespace
 
 size_t lora_workspace_bytes(int64_t rows, int32_t n, int64_t K, int64_t N, int64_t rank, int32_t op, bool weight,
-                            bool copied) {
+                            int32_t copied) {
   size_t own = h_bytes(rows, rank, op);
   if (op == kF32) return own;
   if (few_rows(rows, pad8(rank))) {
@@ -387,8 +399,8 @@ size_t lora_workspace_bytes(int64_t rows, int32_t n, int64_t K, int64_t N, int64
                        (weight ? (size_t)sp.splits * (size_t)rows * (size_t)sp.part_ld * 4 : 0);
     own = own > few ? own : few;
   }
-  own = align_up(own, 256);
-  return own + (copied ? copies_bytes(rows, n, K, N, rank, weight).total() : 0);
+  if (copied & CVMM_LORA_COPY_ALL) copied = ~0;
+  return align_up(own, 256) + copies_bytes(rows, n, K, N, rank, weight ? copied : copied & ~CVMM_LORA_COPY_WEIGHT).total();
 }
 
 hipError_t launch_lora(const LoraParams& q, int32_t op, void* ws, size_t ws_bytes, hipStream_t s) {
@@ -399,15 +411,15 @@ hipError_t launch_lora(const LoraParams& q, int32_t op, void* ws, size_t ws_byte
   void* x_copy = nullptr;  // x's copy where it takes a launch of its own
   if (op != kF32 && !fast_ok(p, op)) {
     // copies of whole pieces, where there is room for them
-    const bool weight = p.w != nullptr;
-    const size_t own = lora_workspace_bytes(p.rows, p.n, p.K, p.N, p.rank, op, weight, false);
-    const LoraCopies c = copies_bytes(p.rows, p.n, p.K, p.N, p.rank, weight);
+    const size_t own = lora_workspace_bytes(p.rows, p.n, p.K, p.N, p.rank, op, p.w != nullptr, 0);
+    const int32_t which = to_copy(p);
+    const LoraCopies c = copies_bytes(p.rows, p.n, p.K, p.N, p.rank, which);
     // (what the copies' grids and 32-bit indices hold)
     constexpr size_t kMost = (size_t)1 << 34;
     if (c.x < kMost && c.w < kMost && c.a < kMost && c.b < kMost && ws_bytes >= own + c.total()) {
       char* at = (char*)ws + own;
       int64_t se = 0;
-      if (p.K % 8 != 0 || p.x_ld % 8 != 0 || !al16(p.x)) {
+      if (which & CVMM_LORA_COPY_X) {
         if (c.x <= kLoraPadRows) {
           int64_t unit = 1;
           add_pad(pads, p.x, se, p.x_ld, unit, 1, p.rows, p.K, at, false);
@@ -418,14 +430,11 @@ hipError_t launch_lora(const LoraParams& q, int32_t op, void* ws, size_t ws_byte
       }
       at += c.x;
       se = 0;
-      if (weight && (p.K % 8 != 0 || p.N % 8 != 0 || !pieces(p.w, 0, p.w_sk, p.w_sn)))
-        add_pad(pads, p.w, se, p.w_sk, p.w_sn, 1, p.K, p.N, at);
+      if (which & CVMM_LORA_COPY_WEIGHT) add_pad(pads, p.w, se, p.w_sk, p.w_sn, 1, p.K, p.N, at);
       at += c.w;
-      if (p.K % 8 != 0 || p.rank % 8 != 0 || !pieces(p.a, p.a_se, p.a_sk, p.a_sr))
-        add_pad(pads, p.a, p.a_se, p.a_sk, p.a_sr, p.n, p.K, p.rank, at);
+      if (which & CVMM_LORA_COPY_A) add_pad(pads, p.a, p.a_se, p.a_sk, p.a_sr, p.n, p.K, p.rank, at);
       at += c.a;
-      if (p.N % 8 != 0 || p.rank % 8 != 0 || !pieces(p.b, p.b_se, p.b_sr, p.b_sn))
-        add_pad(pads, p.b, p.b_se, p.b_sr, p.b_sn, p.n, p.rank, p.N, at);
+      if (which & CVMM_LORA_COPY_B) add_pad(pads, p.b, p.b_se, p.b_sr, p.b_sn, p.n, p.rank, p.N, at);
       p.K = pad8(p.K);
       p.N = pad8(p.N);
       p.rank = pad8(p.rank);

@@ -1335,10 +1335,13 @@ std::tuple<OptT, OptT> lora_product(const Tensor& xf, const Tensor& ids, const T
   if (rows == 0) return {out, inner};
   if (base.has_value())
     bf = rows_of(base->scalar_type() == op || base->scalar_type() == at::kFloat ? *base : base->to(op), N);
-  const bool copied = !whole_pieces(xf) || !whole_pieces(a) || !whole_pieces(b) || (w.has_value() && !whole_pieces(*w)) ||
-                      K % 8 != 0 || N % 8 != 0 || rank % 8 != 0;
+  const bool ko = K % 8 != 0, no = N % 8 != 0, ro = rank % 8 != 0;
+  const int32_t copied = (ko || !whole_pieces(xf) ? CVMM_LORA_COPY_X : 0) |
+                         (w.has_value() && (ko || no || !whole_pieces(*w)) ? CVMM_LORA_COPY_WEIGHT : 0) |
+                         (ko || ro || !whole_pieces(a) ? CVMM_LORA_COPY_A : 0) |
+                         (no || ro || !whole_pieces(b) ? CVMM_LORA_COPY_B : 0);
   const size_t ws_bytes = cvmm_lora_workspace_bytes(rows, (int32_t)a.size(0), K, N, rank, od, w.has_value() ? 1 : 0,
-                                                    copied ? 1 : 0);
+                                                    copied);
   if (ws_bytes) ws = at::empty({(int64_t)ws_bytes}, opts(xf, at::kByte));
   check(cvmm_lora(ptr(xf), od, rows, xf.stride(0) < K ? K : xf.stride(0), ptr(w), w.has_value() ? w->stride(0) : 0,
                   w.has_value() ? w->stride(1) : 0, ptr(a), a.stride(0), a.stride(1), a.stride(2), ptr(b), b.stride(0),

@@ -569,7 +569,15 @@ int cvmm_balance_loss_backward(const void* logits, int32_t logits_dtype, int64_t
  *
  * copied of the workspace queries: room for copies of 16-bit operands that are not
  * made of aligned 16-byte pieces (widths, rank or strides no multiple of 8, or an
- * unaligned base address); without it such calls run slower, general kernels. */
+ * unaligned base address); without it such calls run slower, general kernels.
+ * cvmm_lora's takes a sum of those that are copied -- x and A where d_in, W where
+ * d_in or d_out, A and B where the rank, B where d_out is no multiple of 8, and each
+ * by its own strides and address -- or CVMM_LORA_COPY_ALL for room whichever they are. */
+#define CVMM_LORA_COPY_ALL 1
+#define CVMM_LORA_COPY_X 2
+#define CVMM_LORA_COPY_WEIGHT 4
+#define CVMM_LORA_COPY_A 8
+#define CVMM_LORA_COPY_B 16
 size_t cvmm_lora_workspace_bytes(int64_t rows, int32_t n_adapters, int64_t d_in, int64_t d_out, int64_t rank,
                                  int32_t op_dtype, int32_t has_weight, int32_t copied);
 int cvmm_lora(const void* x, int32_t op_dtype, int64_t rows, int64_t x_ld, const void* weight, int64_t w_si,

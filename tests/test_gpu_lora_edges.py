@@ -224,3 +224,20 @@ def test_ids_written_after_the_selection_was_made(made, used, n):
         res.append((quiet, y, *torch.autograd.grad(y, [x, a, b], grad), counts))
     for e, c in zip(*res):
         assert torch.equal(e, c)
+
+
+@pytest.mark.parametrize("odd", ["rank", "x", "weight", "a", "b", "d_in", "d_out"])
+def test_copies_have_their_room(odd):
+    """Few rows hold the inner rows in 32 bits, which the kernels of whole pieces do alone:
+    each operand that is none by itself or by its width is copied."""
+    d_in, d_out, r = 320 - (odd == "d_in"), 520 - (odd == "d_out"), 16 - (odd == "rank")
+    t = _make(40, d_in, d_out, r, 7, BF, 11)
+    x, ids, a, b, w = _dev(t, "x", "ids", "a", "b", "weight")
+
+    def shifted(v):
+        return torch.cat([v.flatten()[:1], v.flatten()])[1:].view(v.shape)
+
+    x, w, a, b = (shifted(v) if odd == name else v for name, v in (("x", x), ("weight", w), ("a", a), ("b", b)))
+    y = C.cvmm_lora(x, ids, a, b, weight=w, scale=1.5)
+    exp, bound, _, _ = O.lora(t["x"], t["ids"], t["a"], t["b"], t["weight"], None, 1.5, F32, BF)
+    _within(y, exp, bound)
