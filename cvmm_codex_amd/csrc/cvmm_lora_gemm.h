@@ -569,34 +569,40 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW, STAGES>::OCC)) voi
   // ---- what was left out: added to the rows it belongs to, an element at a time
   if (__any(dropped)) {
     vm_wait<0>();  // the stores above
+    // (The arguments are read again here: with those that only this part takes in registers
+    // from the start the largest tile's prologue spilled scalars, and 16384 rows of
+    // 2048 -> 2048 at rank 64 took 3-5 us more a call, of 152; so 1-3.)
+    using Args = const __attribute__((address_space(4))) LoraParams;
+    Args* q = (Args*)__builtin_amdgcn_kernarg_segment_ptr();  // (p is the first argument)
+    asm volatile("" : "+s"(q));
     for (int i = 0; i < MI * 16; ++i) {
       const int64_t row = s_row[wm * MI * 16 + i];
       const int32_t a = s_id[wm * MI * 16 + i];
       if (a < 0) continue;
-      const OpT* h = reinterpret_cast<const OpT*>(p.h) + row * p.h_ld;
-      const OpT* b = reinterpret_cast<const OpT*>(p.b) + a * p.b_se;
-      for (int64_t n = nw + lane; n < nw + NJ * 16 && n < p.n_out; n += 64) {
+      const OpT* h = reinterpret_cast<const OpT*>(q->h) + row * q->h_ld;
+      const OpT* b = reinterpret_cast<const OpT*>(q->b) + a * q->b_se;
+      for (int64_t n = nw + lane; n < nw + NJ * 16 && n < q->n_out; n += 64) {
         float sum = 0.f;
         for (int32_t r = 0; r < rank; ++r) {
-          const float v = to_f32(b[r * p.b_sr + n * p.b_sn]);
+          const float v = to_f32(b[r * q->b_sr + n * q->b_sn]);
           if (!isfinite(v)) sum += to_f32(h[r]) * v;
         }
         if (isfinite(sum)) continue;
-        OpT* at = reinterpret_cast<OpT*>(p.out) + row * p.out_ld + n;
+        OpT* at = reinterpret_cast<OpT*>(q->out) + row * q->out_ld + n;
         float rest = to_f32(*at);
         // An infinity against the sum's may have come of the output's rounding alone; then
         // the terms say whether one of them is infinite.
         if (isinf(rest) && isinf(sum) && rest != sum) {
-          rest = p.base != nullptr ? load_as_f32(p.base, p.base_dtype, row * p.base_ld + n) : 0.f;
-          const OpT* x = reinterpret_cast<const OpT*>(p.x) + row * p.x_ld;
-          const OpT* w = reinterpret_cast<const OpT*>(p.w);
-          const int64_t K = w != nullptr ? p.K : 0;
+          rest = q->base != nullptr ? load_as_f32(q->base, q->base_dtype, row * q->base_ld + n) : 0.f;
+          const OpT* x = reinterpret_cast<const OpT*>(q->x) + row * q->x_ld;
+          const OpT* w = reinterpret_cast<const OpT*>(q->w);
+          const int64_t K = w != nullptr ? q->K : 0;
 #pragma unroll 1
           for (int64_t k = 0; k < K && isfinite(rest); ++k)
-            rest += to_f32(x[k]) * to_f32(w[k * p.w_sk + n * p.w_sn]);
+            rest += to_f32(x[k]) * to_f32(w[k * q->w_sk + n * q->w_sn]);
 #pragma unroll 1
           for (int32_t r = 0; r < rank && isfinite(rest); ++r) {
-            const float v = to_f32(b[r * p.b_sr + n * p.b_sn]);
+            const float v = to_f32(b[r * q->b_sr + n * q->b_sn]);
             if (isfinite(v)) rest += to_f32(h[r]) * v;
           }
         }
