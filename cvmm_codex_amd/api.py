@@ -333,6 +333,7 @@ class _Routing:
     def __init__(self, raw_flat: torch.Tensor, top_k: int, counted=None):
         self.raw = raw_flat
         self.version = _version(raw_flat)
+        self.restored = False   # raw is no longer the tensor that was recorded
         self.k = top_k
         self.by_e: Dict[int, Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]] = {}
         self.first_e: Optional[int] = None
@@ -348,7 +349,7 @@ class _Routing:
         if self.version is not None and self.first_e is not None and _version(self.raw) != self.version:
             ssel, perm = self.get(self.first_e)[:2]
             self.raw = torch.empty_like(ssel).scatter_(0, perm, ssel)
-            self.version = _version(self.raw)
+            self.version, self.restored = _version(self.raw), True
         return self.raw
 
     def counts(self, n_experts: int) -> Optional[torch.Tensor]:
@@ -450,9 +451,12 @@ class CVMMSel:
     def _ids(self) -> torch.Tensor:
         """The ids in raw_sel's shape, of any integer type, as this library recorded them
         (raw_sel itself where the sort is not its own)."""
-        if self._routing is not None and (self._sel is None or self._sorted_for is not None):
-            return self._routing.ids().view(self._raw_shape_tensor().shape)
-        return self._raw_shape_tensor()
+        raw, r = self._raw_shape_tensor(), self._routing
+        if r is not None and (self._sel is None or self._sorted_for is not None):
+            ids = r.ids()
+            if r.restored:
+                return ids.view(raw.shape)
+        return raw
 
     def _pending(self) -> bool:
         return self._routing is not None and self._sel is None
@@ -539,7 +543,7 @@ def cvmm_prepare_sel(sel: torch.Tensor, n_experts: int) -> CVMMSel:
     s._cvmm_offsets = {n_experts: offsets}
     s._cvmm_i32 = ssel
     out = CVMMSel(None, s, perm, None)
-    out._raw_src = sel
+    out._raw_src = sel if sel.is_contiguous() else routing.raw.view(sel.shape)
     out._sorted_for, out._routing = n_experts, routing
     return out
 

@@ -189,7 +189,7 @@ def test_selection_beside_more_adapters_than_a_sort_takes(how, wanted):
         C.cvmm_lora(x, sel, a.requires_grad_(), b)
 
 
-@pytest.mark.parametrize("made", ["scored", "topk", "prepared"])
+@pytest.mark.parametrize("made", ["scored", "topk", "prepared", "prepared strided"])
 @pytest.mark.parametrize("used", [False, True])
 @pytest.mark.parametrize("n", [16, 20])
 def test_ids_written_after_the_selection_was_made(made, used, n):
@@ -208,6 +208,8 @@ def test_ids_written_after_the_selection_was_made(made, used, n):
             _, ids, sel = C.cvmm_route_topk(logits, k)
         else:
             ids = logits.topk(k).indices
+            if made.endswith("strided"):
+                ids = ids.t().contiguous().t()
             ids[::5, 1] = -1
             ids[::7, 2] = n
             sel = C.cvmm_prepare_sel(ids, E)
