@@ -18,8 +18,12 @@
 // backward.  Terms of a token are 32-bit; a chunk's sums
 // too (at most 256 addends per lane, then at most 64 lanes); sums over chunks are 64-bit.
 // Measured (chunks, sums, backward), us: 512 tokens of 16 experts 4.4, 6.2, 3.4; 16384 of
-// 128 in bf16 5.4, 9.6, 7.3; 32768 of 256 in 8 sequences 12.8, 8.5, 20.9 (the last
-// 34 MB at 1.6 TB/s: exponentials, 8 a lane, and coefficients beside them).
+// 128 in bf16 5.4, 9.6, 7.3; 32768 of 256 in 8 sequences 12.8, 7.9, 20.7.  The sums are
+// the latency of few workgroups (two of 16384 x 128) that walk all chunks.  The last
+// backward is 34 MB at 1.6 TB/s: a wave has two tokens and then ends, so that each waits
+// for its own loads (the logits, then 8 single words of coefficients), and issues 361
+// vector instructions for them where the forward's passes take 213; vector instructions
+// issue for about half of the time.
 #include <cmath>
 
 #include "cvmm_common.h"

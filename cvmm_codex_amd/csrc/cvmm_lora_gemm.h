@@ -22,7 +22,7 @@
 // element of the accumulators instead, 256 of them through branches, the compiler
 // spilled: 800 us against 130 for 16384 rows of 2048 -> 2048.)
 //
-// Measured, bf16: 16384 rows, 2048 -> 2048, rank 64: 121-129 us (146 GFLOP: 1.13-1.21
+// Measured, bf16: 16384 rows, 2048 -> 2048, rank 64: 121-135 us (146 GFLOP: 1.08-1.21
 // PFLOP/s; the library's product without adapters 113).  Bound by the matrix pipe,
 // busy for 60 % of the cycles: a further 2048 k cost 1.4 PFLOP/s, but each round of
 // tiles starts with an empty ring and ends with its CU's stores, 11 us together.

@@ -40,8 +40,9 @@ __device__ __forceinline__ uint4 keep_if(const uint4& v, bool keep) {
 // comes through LDS as [rank][k] rows, transposed on the way where it is stored
 // [k][rank].  Bound by reading x once; each workgroup reads its adapters whole,
 // from L2.  Measured: 16384 rows of 2048, rank 64: 29-32 us (67 MB at 2.2 TB/s: a
-// stage's A waits for its LDS turn); 8192 of 1024, rank 16: 11 (1.5 TB/s);
-// 16384 of 128: 10, the chain order, id, row, store.
+// stage's A waits for its LDS turn, and ranks 33-64 with k shared by two waves, in the
+// 168 registers that three workgroups a CU leave, spill 40 bytes a lane); 8192 of 1024,
+// rank 16: 11 (1.5 TB/s); 16384 of 128: 10, the chain order, id, row, store.
 // ---------------------------------------------------------------------------
 // Workgroups that share the adapters of a tile, in turns: nearly all tiles have one
 // or two (a request ends within), and a second one, taken after the first, made the
