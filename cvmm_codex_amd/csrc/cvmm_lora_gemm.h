@@ -590,21 +590,23 @@ __global__ __launch_bounds__(256, (LoraTile<MI, NJ, WMW, WNW, STAGES>::OCC)) voi
         if (isfinite(sum)) continue;
         OpT* at = reinterpret_cast<OpT*>(q->out) + row * q->out_ld + n;
         float rest = to_f32(*at);
-        // An infinity against the sum's may have come of the output's rounding alone; then
-        // the terms say whether one of them is infinite.
-        if (isinf(rest) && isinf(sum) && rest != sum) {
+        // An infinity against the sum's may have come of the output's rounding alone, and a
+        // NaN of an infinite inner value times the zero of what was left out; then the terms
+        // without those say what they are.
+        if (isinf(sum) && !isfinite(rest) && rest != sum) {
+          // (up to a NaN, or the other infinity, which makes one)
           rest = q->base != nullptr ? load_as_f32(q->base, q->base_dtype, row * q->base_ld + n) : 0.f;
+#pragma unroll 1
+          for (int32_t r = 0; r < rank && !isnan(rest + sum); ++r) {
+            const float v = to_f32(b[r * q->b_sr + n * q->b_sn]);
+            if (isfinite(v)) rest += to_f32(h[r]) * v;
+          }
           const OpT* x = reinterpret_cast<const OpT*>(q->x) + row * q->x_ld;
           const OpT* w = reinterpret_cast<const OpT*>(q->w);
           const int64_t K = w != nullptr ? q->K : 0;
 #pragma unroll 1
-          for (int64_t k = 0; k < K && isfinite(rest); ++k)
+          for (int64_t k = 0; k < K && !isnan(rest + sum); ++k)
             rest += to_f32(x[k]) * to_f32(w[k * q->w_sk + n * q->w_sn]);
-#pragma unroll 1
-          for (int32_t r = 0; r < rank && isfinite(rest); ++r) {
-            const float v = to_f32(b[r * q->b_sr + n * q->b_sn]);
-            if (isfinite(v)) rest += to_f32(h[r]) * v;
-          }
         }
         *at = from_f32<OpT>(rest + sum);
       }

@@ -243,3 +243,31 @@ def test_copies_have_their_room(odd):
     y = C.cvmm_lora(x, ids, a, b, weight=w, scale=1.5)
     exp, bound, _, _ = O.lora(t["x"], t["ids"], t["a"], t["b"], t["weight"], None, 1.5, F32, BF)
     _within(y, exp, bound)
+
+
+@pytest.mark.parametrize("T,d_out,weight", [(200, 264, True), (777, 264, True), (3001, 1032, True), (12345, 1032, True),
+                                            (777, 264, False)])
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_infinite_rows_beside_infinite_adapters(T, d_out, weight, dtype):
+    """Inner rows that are infinite themselves where B is: an infinity by the definition, as
+    in tiles of one adapter."""
+    d_in, r, n = 64, 8, 3
+    t = _make(T, d_in, d_out, r, n, dtype, 12)
+    t["ids"] = torch.arange(T) % 4 - 1
+    t["x"], t["a"], t["b"] = t["x"].abs(), t["a"].abs(), t["b"].abs()
+    t["weight"] = t["weight"].abs()
+    t["x"][1::5, 3] = INF
+    t["b"][1, 2, 8:24] = INF
+    t["b"][2, :, 20:30] = -INF
+    t["b"][2, 4, 40] = 0   # infinity times 0
+    t["base"][:, 9:12], t["base"][:, 21] = INF, -INF
+    t["weight"][5, 9], t["weight"][5, 10] = NAN, -INF
+    x, a, bd, w, bs, idd = _dev(t, "x", "a", "b", "weight", "base", "ids")
+    y = C.cvmm_lora(x, idd, a, bd, weight=w if weight else None, base=bs).cpu()
+    exp, bound, _, _ = O.lora(t["x"], t["ids"], t["a"], t["b"], t["weight"] if weight else None, t["base"], 1.0, dtype)
+    e = exp.to(dtype)
+    assert bool(e.isnan().any() and (e == INF).any() and (e == -INF).any())
+    for f in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert torch.equal(f(y), f(e)), f"{int((f(y) != f(e)).sum())} places"
+    at = e.isfinite() & bound.isfinite()
+    _within(y[at], exp[at], bound[at])
