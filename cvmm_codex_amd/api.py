@@ -488,6 +488,8 @@ class CVMMSel:
 # The dataclass fields above are served by properties: reading sel / sel_index
 # / out_index of a deferred selector runs its sort, raw_sel is made on demand.
 def _get_raw_sel(self):
+    if self._routing is not None and self._routing.counted is not None:
+        self._routing.counted = None   # the reader may write the ids: the sort counts them itself
     if self._raw_sel is None and self._raw_src is not None:
         src = self._raw_src
         self._raw_sel = src if src.dtype == torch.int32 else src.reshape(-1).to(torch.int32).view(src.shape)
