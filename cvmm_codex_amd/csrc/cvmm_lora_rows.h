@@ -219,7 +219,8 @@ __global__ __launch_bounds__(256, RB <= 4 ? 3 : 1) void lora_inner_tile_kernel(c
     const int64_t r = b * 16 + 4 * fq;
     union { uint2 u; OpT e[4]; } o;
 #pragma unroll
-    for (int v = 0; v < 4; ++v) o.e[v] = from_f32<OpT>(r + v < p.rank ? res[b][v] : 0.f);
+    // (an infinity of x times a copy's zeros would be NaN)
+    for (int v = 0; v < 4; ++v) o.e[v] = from_f32<OpT>(r + v < p.rank_out ? res[b][v] : 0.f);
     if (row >= 0 && r < p.h_ld) *reinterpret_cast<uint2*>(h + row * p.h_ld + r) = o.u;
     if (ht != nullptr && m0 + my < p.rows) {
 #pragma unroll
@@ -234,11 +235,11 @@ __global__ __launch_bounds__(256, RB <= 4 ? 3 : 1) void lora_inner_tile_kernel(c
 // ---------------------------------------------------------------------------
 // Calls of few rows, most of them with an adapter of their own: plain 32-bit
 // multiply-adds, each of a row's matrices read once and spread over many
-// workgroups.  Nothing but the output is rounded.  First launch: shares of x A_i (here) beside shares of x W (the split
-// GEMM); second: their sums, then h B_i (lora_join_kernel).  Bound by launches and
-// the latency of one chain of loads each: 32 rows of 2048 -> 2048, rank 16, 64
-// adapters: 5.4 + 4.1 us, 12 MB, of which 2.4 would be bandwidth; one row of
-// 1024 -> 1024: 4.8 + 4.0.
+// workgroups.  Nothing but the output is rounded.  First launch: shares of x A_i (here)
+// beside shares of x W (the split GEMM); second: their sums, then h B_i
+// (lora_join_kernel).  Bound by launches and the latency of one chain of loads each:
+// 32 rows of 2048 -> 2048, rank 16, 64 adapters: 5.6 + 4.0 us, 12 MB, of which 2.4
+// would be bandwidth; one row of 1024 -> 1024: 4.8 + 4.2.
 // ---------------------------------------------------------------------------
 constexpr int kLoraRowLds = 256 * 8 * 4;  // bytes of LDS that lora_inner_row uses
 
@@ -318,7 +319,7 @@ __global__ __launch_bounds__(kLoraJoinThreads) void lora_join_kernel(const LoraP
       float s = 0.f;
 #pragma unroll 4
       for (int q = 0; q < sp.h_splits; ++q) s += sp.h_part[((int64_t)q * p.rows + row) * rank + r];
-      h[r] = sc * s;
+      h[r] = r < p.rank_out ? sc * s : 0.f;  // (an infinity of x times a copy's zeros would be NaN)
     }
   }
   __syncthreads();

@@ -271,3 +271,21 @@ def test_infinite_rows_beside_infinite_adapters(T, d_out, weight, dtype):
         assert torch.equal(f(y), f(e)), f"{int((f(y) != f(e)).sum())} places"
     at = e.isfinite() & bound.isfinite()
     _within(y[at], exp[at], bound[at])
+
+
+@pytest.mark.parametrize("T", [40, 777, 3001])
+@pytest.mark.parametrize("r", [4, 12, 16])
+@pytest.mark.parametrize("weight", [True, False])
+def test_infinite_rows_at_ranks_that_are_padded(T, r, weight):
+    """The ranks that a copy adds are zeros, not the NaN of infinity times zero."""
+    t = _make(T, 64, 72, r, 3, BF, 13)
+    for name in ("x", "a", "b", "weight"):
+        t[name] = t[name].abs()
+    t["x"][1::3, 7] = INF
+    x, ids, a, b, w = _dev(t, "x", "ids", "a", "b", "weight")
+    y = C.cvmm_lora(x, ids, a, b, weight=w if weight else None).cpu()
+    exp, bound, _, _ = O.lora(t["x"], t["ids"], t["a"], t["b"], t["weight"] if weight else None, None, 1.0, BF)
+    assert bool((exp == INF).any()) and not bool(exp.isnan().any())
+    assert torch.equal(y == INF, exp == INF) and not bool(y.isnan().any())
+    at = exp.isfinite()
+    _within(y[at], exp[at], bound[at])
