@@ -309,7 +309,8 @@ __global__ __launch_bounds__(kBalanceSumThreads) void balance_sum_kernel(
         a = f * each / n;
       }
     }
-    coef[(int64_t)g * E + e0 + tid] = (float)(p.weight * a);
+    // (a weight of 0 passes no NaN of P on)
+    coef[(int64_t)g * E + e0 + tid] = p.weight != 0.0 ? (float)(p.weight * a) : 0.f;
     __hip_atomic_store(&w.group_c[(int64_t)g * E + e0 + tid], c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   term = block_sum(term, red_d);

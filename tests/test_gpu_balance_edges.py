@@ -45,3 +45,24 @@ def test_sums_of_very_many_tokens():
     # 0.27, 10 half steps; twice that and a rounding in the square
     z = math.log(1.0 + math.exp(c)) ** 2
     assert abs(float(terms[1]) - z) <= (256 + 64 + 32) * 2.0 ** -24 * z
+
+
+@pytest.mark.parametrize("kind", ["load", "entropy"])
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_balance_of_weight_0_passes_no_nan_on(kind, scores):
+    """With a weight of 0 the rows of finite logits have the gradient of z alone."""
+    g = torch.Generator().manual_seed(1)
+    logits = torch.randn(2, 30, 24, generator=g).cuda()
+    sel = torch.randint(0, 24, (2, 30, 2), generator=g).cuda()
+    logits[0, 7, 3] = float("nan")
+    leaf = logits.requires_grad_()
+    loss, terms, _ = C.cvmm_balance_loss(leaf, sel, kind=kind, scores=scores, per_sequence=True, weight=0.0, z_weight=0.5)
+    (grad,) = torch.autograd.grad(loss, leaf)
+    l = logits.detach().double().cpu()
+    exp = torch.logsumexp(l, -1, keepdim=True) * torch.softmax(l, -1) / 60
+    rows = torch.ones(2, 30, dtype=torch.bool)
+    rows[0, 7] = False
+    assert bool(grad[~rows].isnan().all())
+    # a logarithm, an exponential and their quotient to a few steps each, 24 addends
+    tol = 64 * 2.0 ** -24 * ((1 + torch.logsumexp(l, -1, keepdim=True).abs()) * torch.softmax(l, -1) / 60)
+    assert bool(((grad.cpu().double() - exp).abs() <= tol)[rows].all())
