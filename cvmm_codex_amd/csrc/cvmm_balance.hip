@@ -84,6 +84,8 @@ struct BalanceTerms {
   float soft[MAXV], p[MAXV];
   float lse;
   bool clamped;  // the sigmoids' sum is below 1e-20
+  // FORWARD: lse as it is for infinite logits too (their gradient is NaN either way).
+  template <bool FORWARD>
   __device__ __forceinline__ void make(const float (&l)[MAXV], bool sigmoid, bool want_z) {
     lse = 0.f;
     clamped = false;
@@ -102,6 +104,13 @@ struct BalanceTerms {
 #pragma unroll
       for (int v = 0; v < MAXV; ++v) soft[v] *= inv;
       lse = m + logf(s);
+      if (FORWARD && __any(s != s)) {  // a NaN in the row, or an infinite maximum: that is its logsumexp
+        float nan = 0.f;
+#pragma unroll
+        for (int v = 0; v < MAXV; ++v) nan = l[v] != l[v] ? 1.f : nan;
+        nan = seg_max<LPT>(nan);
+        lse = s != s && nan == 0.f ? m : lse;
+      }
     }
     if (sigmoid) {
       float s = 0.f;
@@ -185,7 +194,7 @@ __global__ __launch_bounds__(kBalanceThreads) void balance_chunk_kernel(
     float l[MAXV];
     balance_row<LT, LPT, MAXV, VEC>(logits + at * p.ld, li, E, l);
     BalanceTerms<LPT, MAXV> x;
-    x.make(l, p.sigmoid != 0, true);
+    x.template make<true>(l, p.sigmoid != 0, true);
 #pragma unroll
     for (int v = 0; v < MAXV; ++v) col[v] += live ? x.p[v] : 0.f;
     z += live ? x.lse * x.lse : 0.f;
@@ -371,7 +380,7 @@ __global__ __launch_bounds__(kBalanceThreads) void balance_bwd_kernel(
   const float b = coef[(int64_t)groups * E], g = *grad_loss;
   const bool live = p.mask == nullptr || p.mask[at];
   BalanceTerms<LPT, MAXV> x;
-  x.make(l, p.sigmoid != 0, b != 0.f);
+  x.template make<false>(l, p.sigmoid != 0, b != 0.f);
   float dot = 0.f;
 #pragma unroll
   for (int v = 0; v < MAXV; ++v) dot += balance_expert<LPT>(li, v) < E ? a[v] * x.p[v] : 0.f;

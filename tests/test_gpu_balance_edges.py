@@ -66,3 +66,20 @@ def test_balance_of_weight_0_passes_no_nan_on(kind, scores):
     # a logarithm, an exponential and their quotient to a few steps each, 24 addends
     tol = 64 * 2.0 ** -24 * ((1 + torch.logsumexp(l, -1, keepdim=True).abs()) * torch.softmax(l, -1) / 60)
     assert bool(((grad.cpu().double() - exp).abs() <= tol)[rows].all())
+
+
+@pytest.mark.parametrize("E", [8, 100, 300, 1024])
+def test_infinite_logits(E):
+    """logsumexp of a row is infinite where a logit is, NaN where one is NaN."""
+    g = torch.Generator().manual_seed(2)
+    for value, with_nan in ((math.inf, False), (-math.inf, False), (math.inf, True)):
+        logits = torch.randn(1, 20, E, generator=g)
+        logits[0, 5, E // 2] = value
+        if with_nan:
+            logits[0, 5, E - 1] = math.nan
+        sel = torch.randint(0, E, (1, 20, 2), generator=g)
+        _, terms, _ = C.cvmm_balance_loss(logits.cuda(), sel.cuda(), scores="sigmoid")
+        z = (torch.logsumexp(logits.double(), -1) ** 2).mean()
+        assert bool(terms[1].isnan()) == bool(z.isnan()) and bool(terms[1].isinf()) == bool(z.isinf())
+        if z.isfinite():   # 20 rows of a logarithm and a square, each to 32 steps
+            assert abs(float(terms[1]) - float(z)) <= 64 * 2.0 ** -24 * float(z)
