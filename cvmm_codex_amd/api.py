@@ -326,6 +326,12 @@ def _version(t: torch.Tensor) -> Optional[int]:
     return None if _compiling() or t.is_inference() else t._version
 
 
+def _recorded(ids: torch.Tensor) -> torch.Tensor:
+    """Flat ids of a selection that the caller has too: a copy in compiled code, where no
+    version tells of writes."""
+    return ids.reshape(-1).clone() if _compiling() else ids.reshape(-1)
+
+
 class _Routing:
     """One recorded selection; sorted on the device on first use, per expert count.
     `counted` = (expert count, sort workspace holding the ids' histogram for it)."""
@@ -346,10 +352,13 @@ class _Routing:
         """The ids as recorded.  `raw` may be a tensor that the caller has too (a router's
         output, cvmm_prepare_sel's argument); if that was written since, they are put
         together again from the sort that was made with them."""
-        if self.version is not None and self.first_e is not None and _version(self.raw) != self.version:
-            ssel, perm = self.get(self.first_e)[:2]
-            self.raw = torch.empty_like(ssel).scatter_(0, perm, ssel)
-            self.version, self.restored = _version(self.raw), True
+        if self.version is None or self.first_e is None or (not _compiling() and self.raw._version == self.version):
+            return self.raw
+        ssel, perm = self.get(self.first_e)[:2]
+        if _compiling():   # a selection made before, in every call: nothing tells there
+            return torch.empty_like(ssel).scatter(0, perm, ssel)
+        self.raw = torch.empty_like(ssel).scatter_(0, perm, ssel)
+        self.version, self.restored = _version(self.raw), True
         return self.raw
 
     def counts(self, n_experts: int) -> Optional[torch.Tensor]:
@@ -454,7 +463,7 @@ class CVMMSel:
         raw, r = self._raw_shape_tensor(), self._routing
         if r is not None and (self._sel is None or self._sorted_for is not None):
             ids = r.ids()
-            if r.restored:
+            if r.restored or _compiling():
                 return ids.view(raw.shape)
         return raw
 
@@ -539,7 +548,7 @@ def cvmm_prepare_sel(sel: torch.Tensor, n_experts: int) -> CVMMSel:
     if not sel.is_cuda:
         raw, ssel, perm = _host_sel(sel)
         return CVMMSel(raw, ssel, perm, None)
-    routing = _Routing(sel.reshape(-1), 1)
+    routing = _Routing(_recorded(sel), 1)
     ssel, perm, _, offsets = routing.get(n_experts)
     s = ssel.view(sel.shape)
     s._cvmm_offsets = {n_experts: offsets}
@@ -701,7 +710,7 @@ def cvmm_route_topk(logits: torch.Tensor, k: int, renormalize: bool = True):
         w, sel, ssel, perm, tok, offsets, route_pos = _apply(_RouteTopK, logits, k, renormalize)
         perm._cvmm_route_pos = route_pos
     sel = sel.view(*lead, k)
-    routing = _Routing(sel.reshape(-1), k)
+    routing = _Routing(_recorded(sel), k)
     routing.by_e[E] = (ssel, perm, tok, offsets)
     routing.first_e = E
     return w.view(*lead, k), sel, CVMMSel._deferred(sel, routing, False, None)
@@ -751,7 +760,7 @@ def cvmm_route_scored(logits: torch.Tensor, k: int, bias: Optional[torch.Tensor]
         w, sel, *sort = N.host().route_scored_apply(*args, _differentiated(logits))
     if len(lead) != 1:
         w, sel = w.view(*lead, k), sel.view(*lead, k)
-    routing = _Routing(sel.view(-1), k)
+    routing = _Routing(_recorded(sel), k)
     if _compiling():
         routing.by_e[E] = tuple(sort[:4])
         routing.first_e = E

@@ -289,3 +289,66 @@ def test_infinite_rows_at_ranks_that_are_padded(T, r, weight):
     assert torch.equal(y == INF, exp == INF) and not bool(y.isnan().any())
     at = exp.isfinite()
     _within(y[at], exp[at], bound[at])
+
+
+@pytest.mark.parametrize("written", [False, True])
+@pytest.mark.parametrize("made", ["scored", "prepared", "lazy"])
+def test_compiled_use_of_a_selection_made_before(made, written):
+    """The eager call's bits, gradients too, and the selection stays as it was; so with ids
+    that are written before the compiled call."""
+    T, k, E = 90, 4, 16
+    g = torch.Generator().manual_seed(14)
+    logits = torch.randn(T, E, generator=g).cuda()
+    t = _make(T * k, 64, 72, 8, E, BF, 14)
+    x, a, b, grad = _dev(t, "x", "a", "b", "grad")
+    ids = logits.topk(k).indices
+    if made == "scored":
+        _, ids, sel = C.cvmm_route_scored(logits, k)
+    elif made == "prepared":
+        sel = C.cvmm_prepare_sel(ids, E)
+    else:
+        sel = C.cvmm_prepare_sel2(ids, route_input=True)
+    raw = sel._routing.raw
+
+    def f(x, a, b):
+        return C.cvmm_lora(x.view(T, k, 64), sel, a, b)
+
+    res = []
+    for fn in (f, torch.compile(f, backend="aot_eager"), f):
+        if written and len(res) == 1:
+            ids.copy_((ids * 5 + 2) % E)
+        leaves = [v.detach().requires_grad_() for v in (x, a, b)]
+        y = fn(*leaves)
+        res.append((y, *torch.autograd.grad(y, leaves, grad.view(T, k, 72))))
+        with torch.no_grad():
+            res[-1] += (fn(x, a, b),)
+    for e, *others in zip(*res):
+        assert all(torch.equal(e, o) for o in others)
+    assert written or (sel._routing.raw is raw and not sel._routing.restored)
+
+
+@pytest.mark.parametrize("made", ["scored", "topk", "prepared"])
+def test_compiled_ids_written_after_the_selection_was_made(made):
+    T, k, E = 90, 4, 16
+    g = torch.Generator().manual_seed(15)
+    logits = torch.randn(T, E, generator=g).cuda()
+    t = _make(T * k, 64, 72, 8, E, BF, 15)
+    x, a, b = _dev(t, "x", "a", "b")
+
+    def f(x, write):
+        if made == "scored":
+            _, ids, sel = C.cvmm_route_scored(logits, k)
+        elif made == "topk":
+            _, ids, sel = C.cvmm_route_topk(logits, k)
+        else:
+            ids = logits.topk(k).indices
+            sel = C.cvmm_prepare_sel(ids, E)
+        if write:
+            ids.copy_((ids * 5 + 2) % E)
+        return C.cvmm_lora(x.view(T, k, 64), sel, a, b), C.cvmm_balance_loss(logits, sel)[2], ids
+
+    with torch.no_grad():
+        exp = f(x, False)
+        got = torch.compile(f, backend="aot_eager", fullgraph=True)(x, True)
+    assert torch.equal(exp[0], got[0]) and torch.equal(exp[1], got[1])
+    assert torch.equal(got[2], (exp[2] * 5 + 2) % E)
